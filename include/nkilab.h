@@ -322,6 +322,112 @@ int nkl_attention_allgather(const void* q, const void* k, const void* v, void* c
                             int64_t head_offset, void* workspace, size_t workspace_bytes, int64_t heads,
                             int64_t seq, int64_t head_dim, float scale, int dtype, void* stream);
 
+/* ---- decoding: attention over a paged cache, its pages, drafted tokens ------------- */
+
+/* The cache: k_cache and v_cache [layers, pages, kv_heads, page_size, head_dim], shared by
+ * all sequences. Row b of tables [batch, max_pages] lists the pages of slot b in order of
+ * position (-1: none), lens[b] is its number of cached positions and refs[p] the number of
+ * table entries naming page p (0: free). These arrays are int32 device memory and no call
+ * reads them on the host. An index in them that is out of range is skipped (its rows read
+ * as zeros and are not written), it never addresses memory outside the arrays. `*_strides`
+ * are host arrays in elements (NULL: dense in the order written); a row of head_dim is
+ * contiguous, and every stride a multiple of 16 bytes. Strides apply to k and v alike.
+ * The reference keeps no cache: none of these calls has a counterpart in it
+ * (nkilab/model.py:70-89 computes a whole prompt each time). */
+
+/* Most drafted tokens of one sequence. */
+#define NKL_MAX_DRAFTED 128
+
+/* Workspace of nkl_attention_tree on the current device; 256-byte aligned, no contents
+ * needed. It depends on the capacity of the tables, not on the lengths in them. */
+size_t nkl_attention_tree_workspace_size(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t page_size, int64_t max_pages, int dtype);
+
+/* Attention of `tokens` drafted tokens of each sequence over its cached positions and over
+ * each other, as a tree: out[b, i, h] = softmax(scale q k^T) v over the cached positions
+ * 0 .. lens[b] - 1, token i itself and its ancestors. q, out [batch, tokens, heads,
+ * head_dim] (out dense); k_new, v_new [batch, tokens, kv_heads, head_dim] are the drafted
+ * tokens' own, not yet in the cache; query head h uses kv head h / (heads / kv_heads).
+ * parents [batch, tokens]: an earlier token, -1 for a child of the last cached position,
+ * below -1 for an absent token, whose output is zero and which no token sees (a child of it,
+ * or of a token that is not earlier, counts as a child of the last cached position). NULL:
+ * each token's parent is the one before it (a prompt's chunk; tokens = 1 is plain decoding).
+ * One layer's caches: strides of q [batch, token, head], new [batch, token, head], cache
+ * [page, head, row]. head_dim a multiple of 8 up to 128, tokens <= NKL_MAX_DRAFTED, 16-byte
+ * aligned pointers. fp32 accumulation and softmax statistics; the output is rounded once,
+ * and the bf16 tensor-core kernel (head_dim 64 or 128, page_size a multiple of 8, at most
+ * 128 query heads per kv head) rounds the exponentials to bf16 for their product with v. */
+int nkl_attention_tree(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
+                       const int64_t* new_strides, const void* k_cache, const void* v_cache,
+                       const int64_t* cache_strides, const int32_t* tables, const int32_t* lens,
+                       const int32_t* parents, void* out, void* workspace, size_t workspace_bytes, int64_t batch,
+                       int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                       int64_t page_size, int64_t max_pages, float scale, int dtype, void* stream);
+
+/* Writes rows of k and v [layers, batch, tokens, kv_heads, head_dim] to the pages: row
+ * path[b, j] of sequence b, for j < count[b], goes to position lens[b] + j of every layer;
+ * lens_out = lens + count. path NULL: row j; count NULL: tokens. The pages have to be in
+ * the tables (nkl_cache_reserve) and belong to one slot alone: a row without a page is
+ * dropped. Strides: k and v [layer, batch, token, head], cache [layer, page, head, row]. */
+int nkl_cache_append(const void* k, const void* v, const int64_t* kv_strides, void* k_cache, void* v_cache,
+                     const int64_t* cache_strides, const int32_t* tables, const int32_t* lens, const int32_t* path,
+                     const int32_t* count, int32_t* lens_out, int64_t layers, int64_t batch, int64_t tokens,
+                     int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages,
+                     int dtype, void* stream);
+
+/* Free pages, lowest index first, for extra[b] more positions of each slot b, in order of
+ * b. All or nothing: with too few free pages, or rows too long for the tables, missing[0] > 0
+ * says how many lack and tables and refs come out as they went in. */
+size_t nkl_cache_reserve_workspace_size(int64_t batch);
+int nkl_cache_reserve(const int32_t* tables, const int32_t* lens, const int32_t* refs, const int32_t* extra,
+                      int32_t* tables_out, int32_t* refs_out, int32_t* missing, void* workspace,
+                      size_t workspace_bytes, int64_t batch, int64_t pages, int64_t page_size, int64_t max_pages,
+                      void* stream);
+
+/* Slot dst[f] becomes a copy of slot src[f]: it shares the full pages (their refs grow) and
+ * gets a free page of its own, lowest index first in order of f, into which the used rows of
+ * the last, partly filled page are copied in every layer; what dst held before is freed. All
+ * sources are read as they were before the call. A fork with a slot out of range, onto itself
+ * or into the dst of an earlier one is skipped. All or nothing, as nkl_cache_reserve. */
+size_t nkl_cache_fork_workspace_size(int64_t batch, int64_t forks);
+int nkl_cache_fork(void* k_cache, void* v_cache, const int64_t* cache_strides, const int32_t* tables,
+                   const int32_t* lens, const int32_t* refs, const int32_t* src, const int32_t* dst,
+                   int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* missing, void* workspace,
+                   size_t workspace_bytes, int64_t forks, int64_t layers, int64_t batch, int64_t kv_heads,
+                   int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages, int dtype, void* stream);
+
+/* Gives back the pages of the slots listed: their refs shrink, their rows become -1 and
+ * their lengths 0. Slots out of range are skipped, one listed twice is freed once. */
+int nkl_cache_free(const int32_t* tables, const int32_t* lens, const int32_t* refs, const int32_t* slots,
+                   int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int64_t n_slots, int64_t batch,
+                   int64_t pages, int64_t max_pages, void* stream);
+
+/* Moves the n pages in use to the indices 0 .. n - 1: those from n on, in order, into the
+ * free ones below n, in order; tables and refs follow. No page is read after it is written. */
+size_t nkl_cache_compact_workspace_size(int64_t pages);
+int nkl_cache_compact(void* k_cache, void* v_cache, const int64_t* cache_strides, const int32_t* tables,
+                      const int32_t* refs, int32_t* tables_out, int32_t* refs_out, void* workspace,
+                      size_t workspace_bytes, int64_t layers, int64_t batch, int64_t kv_heads, int64_t head_dim,
+                      int64_t pages, int64_t page_size, int64_t max_pages, int dtype, void* stream);
+
+/* Which drafted tokens the target accepts, and the token after them. probs [batch, drafted +
+ * 1, vocab]: row 0 follows the last cached token, row i + 1 drafted token i. uniforms [batch,
+ * drafted + 1] in [0, 1): number i tests token i, the last one draws the next token.
+ * With draft_probs [batch, drafted, vocab] the tokens are a chain and row i is what token i was
+ * drawn from: accepted while u q(x) < p(x), then max(p - q, 0) is drawn from. Without,
+ * they are a tree (parents as in nkl_attention_tree; NULL: a chain): a node's children are
+ * tried in order of index, accepted if u * (1 - mass of the rejected ones) < p(x), and what the
+ * rejected ones leave is drawn from. Either way the result is distributed as the target.
+ * A token outside the vocabulary is never accepted (in a chain it ends it). Probabilities and
+ * uniform numbers are taken as whole multiples of 2^-31 and summed as whole numbers, so the
+ * result does not depend on an order of summation. path [batch, drafted]: the accepted tokens'
+ * indices, then -1; count [batch]; token [batch]: the first x whose cumulative weight is
+ * over the last uniform number's share of their sum (weights that are all zero: p itself; -1 if
+ * that is zero too). drafted <= NKL_MAX_DRAFTED; dense arrays. */
+int nkl_verify_drafts(const void* probs, const void* draft_probs, const int32_t* tokens, const float* uniforms,
+                      const int32_t* parents, int32_t* path, int32_t* count, int32_t* token, int64_t batch,
+                      int64_t drafted, int64_t vocab, int dtype, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -72,11 +72,26 @@ SIGNATURES = {
     "nkl_ipc_free": (_int, [_p]),
     "nkl_attention_allgather": (_int, [_p, _p, _p, _p, _p, _int, _int, _i64, _i64, _p, _sz, _i64, _i64, _i64, _f, _int,
                                        _p]),
+    "nkl_attention_tree_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "nkl_attention_tree": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _i64,
+                                  _i64, _i64, _i64, _f, _int, _p]),
+    "nkl_cache_append": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                _i64, _int, _p]),
+    "nkl_cache_reserve_workspace_size": (_sz, [_i64]),
+    "nkl_cache_reserve": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _p]),
+    "nkl_cache_fork_workspace_size": (_sz, [_i64, _i64]),
+    "nkl_cache_fork": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _i64, _i64,
+                              _i64, _i64, _int, _p]),
+    "nkl_cache_free": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "nkl_cache_compact_workspace_size": (_sz, [_i64]),
+    "nkl_cache_compact": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p]),
+    "nkl_verify_drafts": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
     "nkl_attention_naive_workspace_size": (_sz, [_i64, _i64, _int]),
     "nkl_attention_naive": (_int, [_p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _f, _int, _p]),
 }
 
 ABI_VERSION = 1
+MAX_DRAFTED = 128  # NKL_MAX_DRAFTED
 SOFTMAX_UNFUSED_STATIC_BYTES = 16 * 1024 * 1024  # NKL_SOFTMAX_UNFUSED_STATIC_BYTES
 
 

@@ -23,7 +23,9 @@ from ._host import like_input as _like_input
 from ._host import to_device as _to_device
 from .kernels import attention as _attn
 
-__all__ = ["choose_blocks", "matmul", "softmax", "rmsnorm", "swiglu", "attention", "ATTENTION_VARIANTS"]
+__all__ = ["choose_blocks", "matmul", "softmax", "rmsnorm", "swiglu", "attention", "ATTENTION_VARIANTS",
+           "rope", "attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
+           "verify_drafts"]
 
 
 # --------------------------------------------------------------------------- matmul
@@ -145,3 +147,80 @@ def rope(x, base: float = 10000.0, pos_offset: int = 0):
     xd = _to_device(x).contiguous()
     o = torch.ops.nkilab.rope(xd, float(base), int(pos_offset))
     return _like_input(o, x)
+
+
+# --------------------------------------------------------------------------- decoding (extension)
+# Operations of a decoding loop on a paged key/value cache. The cache lives on the GPU, so
+# these take CUDA tensors only. Shapes: caches [pages, kv heads, page size, head_dim], with a
+# leading [layers] for the page operations where there are several; tables [B, M] int32, the
+# pages of each slot in order (-1: none); lens [B] int32, cached positions of each slot; refs
+# [pages] int32, how many table entries name each page. Nothing here reads them on the host
+# or waits for the GPU. nkilab.serving.PagedCache keeps them together.
+
+_decode = torch.ops.nkilab
+
+
+def _layers(*ts):
+    """Each tensor with its leading [layers] dimension."""
+    return tuple(t if t.dim() == 5 else t.unsqueeze(0) for t in ts)
+
+
+def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=None):
+    """Attention of T drafted tokens per sequence over its cached positions and, as a tree,
+    over each other. q: [B, T, H, d]; k, v: [B, T, Hkv, d], the drafted tokens' own, not yet
+    in the cache (views of a fused projection are read as they lie); returns [B, T, H, d].
+
+    parents [B, T] int32: each token's parent among the earlier ones, -1 for a child of the
+    last cached position, -2 for an absent token (its output is zero, none sees it). None:
+    each token follows the one before it, so T = 1 is plain decoding and T > 1 a chunk of a
+    prompt. At most 128 tokens; scale defaults to 1/sqrt(d). d: a multiple of 8 up to 128
+    (64 and 128 in bf16, with pages of a multiple of 8 positions, run on the tensor cores).
+    """
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    return _decode.attention_tree.default(q, k, v, k_cache, v_cache, tables, lens, parents, float(scale))
+
+
+def cache_append(k, v, k_cache, v_cache, tables, lens, path=None, count=None):
+    """Writes rows of k and v [(layers,) B, T, Hkv, d] to the pages at positions lens[b]
+    onward and returns the new lengths: row path[b, j] for j < count[b] (the accepted path
+    of drafted tokens), or all T rows in order. The pages come from cache_reserve; rows
+    without a page are dropped."""
+    return _decode.cache_append.default(*_layers(k, v, k_cache, v_cache), tables, lens, path, count)
+
+
+def cache_reserve(tables, lens, refs, extra, page_size):
+    """Pages for extra[b] more positions of each slot, lowest free index first. Returns
+    (tables, refs, missing): with too few free pages, or too narrow tables, missing [1] is
+    how many lack and nothing is given out."""
+    return _decode.cache_reserve.default(tables, lens, refs, extra, int(page_size))
+
+
+def cache_fork(k_cache, v_cache, tables, lens, refs, src, dst):
+    """Slot dst[f] becomes a copy of slot src[f]: full pages are shared, the last, partly
+    filled one is copied to a free page. Returns (tables, lens, refs, missing); with
+    missing [1] > 0 (too few free pages) nothing is forked."""
+    return _decode.cache_fork.default(*_layers(k_cache, v_cache), tables, lens, refs, src, dst)
+
+
+def cache_free(tables, lens, refs, slots):
+    """Gives back the pages of the slots listed. Returns (tables, lens, refs)."""
+    return _decode.cache_free.default(tables, lens, refs, slots)
+
+
+def cache_compact(k_cache, v_cache, tables, refs):
+    """Moves the pages in use to the lowest indices. Returns (tables, refs)."""
+    return _decode.cache_compact.default(*_layers(k_cache, v_cache), tables, refs)
+
+
+def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):
+    """Accepts drafted tokens against the target's probabilities and draws the next token, so
+    that the tokens are distributed as the target's. probs [B, T + 1, V]: row 0 after the last
+    cached token, row i + 1 after drafted token i; tokens [B, T] int32; uniforms [B, T + 1]
+    float32 in [0, 1). A chain with draft_probs [B, T, V] (what each token was drawn from), or
+    a tree with parents [B, T] (None: a chain) and no draft_probs.
+
+    Returns (path [B, T], the accepted tokens' indices and then -1; count [B]; token [B]).
+    Sums are whole numbers of 2^-31, so equal inputs give equal tokens on every launch.
+    """
+    return _decode.verify_drafts.default(probs, tokens, uniforms, parents, draft_probs)
