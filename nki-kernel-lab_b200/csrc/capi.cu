@@ -54,9 +54,12 @@ extern "C" int nkl_check_device(void* stream) {
   if (e != cudaSuccess) return nkl::fail(NKL_ERR_CUDA, "nkl_check_device: %s", cudaGetErrorString(e));
   const int g = nkl::gemm_read_and_clear_device_error();
   const int a = nkl::attention_read_and_clear_device_error();
-  if (g < 0 || a < 0) return nkl::fail(NKL_ERR_CUDA, "nkl_check_device: could not read the device flag");
-  if (g || a)
-    return nkl::fail(NKL_ERR_DEVICE, "nkl_check_device: kernel gave up waiting (gemm code %d, attention code %d)", g, a);
+  const int t = nkl::tree_read_and_clear_device_error();
+  if (g < 0 || a < 0 || t < 0) return nkl::fail(NKL_ERR_CUDA, "nkl_check_device: could not read the device flag");
+  if (g || a || t)
+    return nkl::fail(NKL_ERR_DEVICE,
+                     "nkl_check_device: kernel gave up waiting (gemm code %d, attention code %d, tree attention code %d)",
+                     g, a, t);
   return NKL_OK;
 }
 

@@ -46,6 +46,7 @@ int sm_count();
 // Device-failure flag readers, one per translation unit that waits on barriers.
 int gemm_read_and_clear_device_error();
 int attention_read_and_clear_device_error();
+int tree_read_and_clear_device_error();
 
 // ---------------------------------------------------------------- device helpers
 

@@ -12,8 +12,12 @@
 // lane x scores key x of a 32-key tile and then accumulates 4 columns. Key ranges split over
 // several blocks leave (max, sum, O) in the workspace; tree_combine_kernel joins them in order.
 #include <algorithm>
+#include <atomic>
 
+#include "attn_math.cuh"
 #include "common.cuh"
+#include "sm100.cuh"
+#include "tma_host.cuh"
 
 namespace nkl {
 namespace {
@@ -168,7 +172,21 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
       ps[warp * 4 + i][lane] = p;
     }
     __syncwarp();
-    if (lane < quads) {
+    if (lane < quads && !cached) {
+      // a drafted token that a row does not see leaves no trace in it, whatever its v holds
+      for (int x = 0; x < kKeys && key0 + x < a.tokens; ++x) {
+        const float4 v = *reinterpret_cast<const float4*>(&vs[x][lane * 4]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (!((seen[i][(key0 >> 5) & 3] >> x) & 1u)) continue;
+          const float pk = ps[warp * 4 + i][x];
+          o[i].x = fmaf(pk, v.x, o[i].x);
+          o[i].y = fmaf(pk, v.y, o[i].y);
+          o[i].z = fmaf(pk, v.z, o[i].z);
+          o[i].w = fmaf(pk, v.w, o[i].w);
+        }
+      }
+    } else if (lane < quads) {
       for (int x = 0; x < kKeys; x += 4) {
         float4 v[4];
 #pragma unroll
@@ -243,6 +261,12 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
     store4(static_cast<T*>(a.out) + at + lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
+}  // namespace
+
+#include "tree_attention_tc.cuh"
+
+namespace {
+
 // ------------------------------------------------------------------ host
 
 // Blocks that share a sequence's keys: enough of them to give every SM a few, each with at
@@ -265,6 +289,14 @@ bool tree_sizes_ok(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_head
 }
 
 }  // namespace
+
+int tree_read_and_clear_device_error() {
+  unsigned int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_tree_dev_error, sizeof(v)) != cudaSuccess) return -1;
+  if (v && cudaMemcpyToSymbol(g_tree_dev_error, &zero, sizeof(zero)) != cudaSuccess) return -1;
+  return (int)v;
+}
+
 }  // namespace nkl
 
 using namespace nkl;
@@ -275,8 +307,11 @@ extern "C" size_t nkl_attention_tree_workspace_size(int64_t batch, int64_t token
   if (!valid_dtype(dtype) || !tree_sizes_ok(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages) ||
       batch == 0 || tokens == 0)
     return 0;
+  // strides and the scale's sign, which are not known here, may still choose the CUDA-core kernel
+  const TcPlan p = tc_plan(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages, dtype);
   const int64_t row_blocks = (tokens * (heads / kv_heads) + kRows - 1) / kRows;
-  return split_bytes(split_count(batch, kv_heads, row_blocks, page_size * max_pages), batch, heads, tokens, head_dim);
+  return std::max(p.on ? p.bytes : 0, split_bytes(split_count(batch, kv_heads, row_blocks, page_size * max_pages),
+                                                  batch, heads, tokens, head_dim));
 }
 
 extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
@@ -322,6 +357,23 @@ extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const
   a.batch = (int)batch; a.tokens = (int)tokens; a.heads = (int)heads; a.kv_heads = (int)kv_heads;
   a.group = (int)(heads / kv_heads); a.d = (int)head_dim; a.pages = (int)pages; a.page = (int)page_size;
   a.max_pages = (int)max_pages; a.scale = scale;
+  const TcPlan p = tc_plan(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages, dtype);
+  bool tc = p.on && scale > 0.f && scale < INFINITY;  // the running maximum is one of scaled scores
+  for (int i = 0; i < 9; ++i) tc = tc && (n[i] == 1 || (s[i] > 0 && s[i] < (1LL << 38)));  // tensor map strides
+  if (tc) {
+    if (p.bytes) {
+      if (!workspace || workspace_bytes < p.bytes) return fail(NKL_ERR_ARG, "%s: workspace too small", op);
+      if (!is_aligned(workspace, 256)) return fail(NKL_ERR_ALIGN, "%s: workspace not 256-byte aligned", op);
+    }
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    cudaStream_t on = static_cast<cudaStream_t>(stream);
+    // a dimension of one position is never stepped over, but its stride still has to be a valid one
+    int64_t* const steps[9] = {&a.q_b, &a.q_t, &a.q_h, &a.n_b, &a.n_t, &a.n_h, &a.c_p, &a.c_h, &a.c_s};
+    for (int i = 0; i < 9; ++i)
+      if (n[i] == 1) *steps[i] = head_dim;
+    if (head_dim == 128) return p.nq == 1 ? tc_launch<128, 1>(a, p, ws, on) : tc_launch<128, 2>(a, p, ws, on);
+    return p.nq == 1 ? tc_launch<64, 1>(a, p, ws, on) : tc_launch<64, 2>(a, p, ws, on);
+  }
   a.row_blocks = (int)((tokens * a.group + kRows - 1) / kRows);
   a.splits = split_count(batch, kv_heads, a.row_blocks, page_size * max_pages);
   const size_t need = split_bytes(a.splits, batch, heads, tokens, head_dim);

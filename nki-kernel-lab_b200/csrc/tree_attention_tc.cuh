@@ -1,0 +1,878 @@
+// tree_attention_tc.cuh - tcgen05 kernel of the tree attention (bf16, head_dim 64 or 128);
+// included by tree_attention.cu.
+//
+// A segment is one (sequence, key/value head, block of query rows): its keys are the cached
+// tiles of 128 positions, the last of them partly filled, and one tile of drafted tokens. The
+// lengths are known on the GPU only, so the blocks share the work out there: all segments'
+// tiles form one row, of which block c takes tiles [c X, (c + 1) X). A segment that is cut
+// leaves (max, sum, O) per piece in the workspace, and tree_join_kernel joins the pieces in
+// order. Cuts near a segment's end move there, and short segments are not cut.
+//
+// Query rows of a tile: `tt` tokens times the G query heads of the key/value head (tt G <=
+// 128), fetched by one TMA box per 64 columns, so row r is token r / G, head r % G.
+//   warps 0-3, 4-7  softmax groups 0 and 1, one thread per row: scores from TMEM, mask, running
+//                   maximum and sum, exponentials rounded to bf16 back into TMEM over the scores
+//   warp 8          TMA: queries, and keys and values through one ring of tiles; the lanes look
+//                   up the pages of a tile and fetch one box each
+//   warp 9          tcgen05.mma, both products: S = Q K^T, O += P V (P from TMEM)
+//   TMEM            S / P of group 0, 1 [0, 128), [128, 256); O of group 0, 1 after them
+// NQ = 1 (rows fit one tile): the groups take the tiles of keys in turn, each with a maximum,
+// sum and O of its own, joined at the end of the segment's piece; while one exponentiates, the
+// tensor core fills the other's scores. NQ = 2: each group has its own tile of rows, and both
+// meet the same keys, which so cross shared memory's boundary once for 256 rows.
+//
+// The running maximum may lag behind by up to 2^8: O is rescaled only when a row's maximum
+// grows by more than that. P is then up to 2^8 instead of 1, with the same relative rounding.
+#pragma once
+
+namespace {
+
+using namespace sm100;
+
+__device__ unsigned int g_tree_dev_error = 0;
+
+constexpr int kTile = 128;
+constexpr int kTcThreads = 320;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kWhole = 4;        // segments of up to so many tiles are not cut
+// Sequences of up to so many cached positions have P in two bf16 parts, P V in two products: a
+// row that sees few keys does not average the roundings of P out (one part: up to 2^-8 of a
+// weight). The second product is hidden behind the loads there is time for; on long rows,
+// where 256 query rows keep the tensor core busy, it is not.
+constexpr int kFine = 1024;
+constexpr float kLag = 8.f;      // log2 of how far the running maximum may lag
+
+struct TcArgs {
+  const int *tables, *lens, *parents;
+  const bf16* v_new;
+  int64_t n_b, n_t, n_h;  // its strides
+  bf16* out;
+  int* ws_plan;    // [0] X, [1..] prefix sums of the sequences' tiles
+  float* ws_ml;    // [slot][NQ][2][128]
+  float4* ws_o;    // [slot][NQ][d / 4][128]
+  int batch, tokens, heads, kv_heads, group, pages, page, max_pages;
+  int tt;          // tokens per query tile
+  int row_blocks;  // blocks of NQ query tiles
+  int box;         // rows of a page fetched by one TMA box
+  int boxes_per_page, log_bpp;  // log_bpp < 0: no power of two
+  unsigned long long bpp_magic;  // ceil(2^36 / boxes_per_page)
+  float scale_log2;
+};
+
+__device__ __forceinline__ int tree_len(const TcArgs& a, int b) {
+  return (int)min((long long)max(a.lens[b], 0), (long long)a.max_pages * a.page);
+}
+__device__ __forceinline__ int tree_tiles(const TcArgs& a, int b) { return (tree_len(a, b) + kTile - 1) / kTile + 1; }
+
+// Where a cut at tile `off` of a segment of n tiles goes: 0 or n when it is near, or when the
+// segment is short.
+__device__ __forceinline__ int snap(int off, int n, int share) {
+  if (n <= kWhole) return 2 * off >= n ? n : 0;
+  const int near = min(max(share / 4, 1), 4);
+  if (off < near) return 0;
+  if (n - off < near) return n;
+  return off;
+}
+
+// One block's walk over its pieces of segments.
+struct Walk {
+  int b, hm, t, tiles, left;
+};
+struct Piece {
+  int b, kvh, mb, t0, n, tiles, len;
+};
+
+template <int D, int NQ>
+struct TreeSmem {
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kRing = (D == 128 ? 7 : 12) - NQ;
+  uint8_t q[NQ][kTileBytes];
+  uint8_t ring[kRing][kTileBytes];
+  uint64_t q_full, q_empty;
+  uint64_t full[kRing], empty[kRing];
+  uint64_t s_full[2], p_full[2], o_done[2], o_free[2];
+  uint64_t x_full;
+  uint64_t mma_done;
+  float xm[2][kTile], xl[2][kTile];  // NQ = 1: the groups' maxima and sums
+  int scan[kTcThreads / 32 + 2];
+  uint32_t bad[4];  // drafted tokens of the piece whose v holds infinities or NaN
+  int cut[2][3];  // this block's first tile and end: sequence, tile of the sequence, tiles before it
+  uint32_t tmem_base;
+  int abort;
+};
+
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort, &g_tree_dev_error, code) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+__device__ __forceinline__ bool next_piece(const TcArgs& a, Walk& w, Piece& p) {
+  if (w.left <= 0) return false;
+  p.b = w.b;
+  p.kvh = w.hm / a.row_blocks;
+  p.mb = w.hm - p.kvh * a.row_blocks;
+  p.t0 = w.t;
+  p.tiles = w.tiles;
+  p.n = min(w.tiles - w.t, w.left);
+  p.len = tree_len(a, w.b);
+  w.left -= p.n;
+  w.t = 0;
+  if (++w.hm == a.kv_heads * a.row_blocks) {
+    w.hm = 0;
+    ++w.b;
+    if (w.left > 0) w.tiles = tree_tiles(a, w.b);
+  }
+  return true;
+}
+
+// Inclusive scan and total over the block; two barriers.
+__device__ __forceinline__ int tree_scan(int v, int* scratch, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = inc;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kTcThreads / 32; ++w) {
+    const int x = scratch[w];
+    before += w < warp ? x : 0;
+    total += x;
+  }
+  return before + inc;
+}
+
+// This block's walk; block 0 leaves the prefix sums for the join.
+template <class Smem>
+__device__ __forceinline__ Walk tree_plan(const TcArgs& a, Smem& s, bool join) {
+  const int tid = threadIdx.x, hm = a.kv_heads * a.row_blocks;
+  int sum = 0, longest = 0, mine = 0, inc = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kTcThreads) {
+    const int b = b0 + tid;
+    mine = b < a.batch ? tree_tiles(a, b) : 0;
+    longest = max(longest, mine);
+    int t;
+    inc = sum + tree_scan(mine, s.scan, t);
+    sum += t;
+    if (join && blockIdx.x == 0 && b < a.batch) a.ws_plan[1 + b] = inc - mine;
+  }
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (tid == 0) s.cut[0][0] = 0;
+  __syncthreads();
+  if ((tid & 31) == 0) atomicMax(&s.cut[0][0], longest);
+  __syncthreads();
+  longest = s.cut[0][0];
+  const int total = sum * hm;
+  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, min(longest, kWhole));
+  if (join && blockIdx.x == 0 && tid == 0) a.ws_plan[0] = share;
+  __syncthreads();
+  if (tid < 2) s.cut[tid][0] = -1;
+  __syncthreads();
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kTcThreads) {
+    const int b = b0 + tid;
+    if (a.batch > kTcThreads) {  // else the values of the only round are still here
+      mine = b < a.batch ? tree_tiles(a, b) : 0;
+      int t;
+      inc = before + tree_scan(mine, s.scan, t);
+      before += t;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const long long at = (long long)(blockIdx.x + k) * share;
+      const long long lo = (long long)(inc - mine) * hm;
+      if (mine > 0 && at >= lo && at < (long long)inc * hm) {
+        s.cut[k][0] = b;
+        s.cut[k][1] = (int)(at - lo);
+        s.cut[k][2] = (int)lo;
+      }
+    }
+  }
+  __syncthreads();
+  Walk w = {0, 0, 0, 0, 0};
+  if (s.cut[0][0] < 0) return w;
+  int end = total;
+  if (s.cut[1][0] >= 0) {
+    const int n = tree_tiles(a, s.cut[1][0]), h = s.cut[1][1] / n;
+    end = s.cut[1][2] + h * n + snap(s.cut[1][1] - h * n, n, share);
+  }
+  w.b = s.cut[0][0];
+  w.tiles = tree_tiles(a, w.b);
+  w.hm = s.cut[0][1] / w.tiles;
+  w.t = snap(s.cut[0][1] - w.hm * w.tiles, w.tiles, share);
+  w.left = end - (s.cut[0][2] + w.hm * w.tiles + w.t);
+  if (w.t == w.tiles) {
+    w.t = 0;
+    if (++w.hm == hm) {
+      w.hm = 0;
+      ++w.b;
+      if (w.left > 0) w.tiles = tree_tiles(a, w.b);
+    }
+  }
+  return w;
+}
+
+// Position of V(t) among the 2 n tiles that a piece of n tiles takes from the ring:
+// K0 V0 K1 V1 ... (NQ = 2), K0 K1 V0 K2 V1 ... V(n-2) V(n-1) (NQ = 1).
+template <int NQ>
+__device__ __forceinline__ int v_at(int t, int n) {
+  if (NQ == 2) return 2 * t + 1;
+  return t == n - 1 ? 2 * n - 1 : 2 * t + 2;
+}
+
+template <int D, int NQ>
+__global__ void __launch_bounds__(kTcThreads, 1)
+tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kn,
+                         const __grid_constant__ CUtensorMap map_vn, const __grid_constant__ CUtensorMap map_kc,
+                         const __grid_constant__ CUtensorMap map_vc, const __grid_constant__ TcArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  if (smem_u32(smem_raw) & 1023u) {  // the swizzled tiles need a 1024-byte-aligned base
+    if (threadIdx.x == 0) atomicCAS(&g_tree_dev_error, 0u, 40u);
+    return;
+  }
+  pdl_launch_dependents();
+  using Smem = TreeSmem<D, NQ>;
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw);
+  constexpr int kRing = Smem::kRing;
+  constexpr uint32_t kTileBytes = Smem::kTileBytes;
+  constexpr uint32_t kTmemCols = 512;
+  constexpr uint32_t kOCol = 2 * kTile;  // O of group g at kOCol + g * D
+  constexpr uint32_t kIdescS = idesc_bf16_f32(kTile, kTile, false, false);
+  constexpr uint32_t kIdescPV = idesc_bf16_f32(kTile, D, false, true);
+  constexpr int kSub = D / 64;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&s.q_full, 1);
+    mbar_init(&s.q_empty, 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], kTile);
+      mbar_init(&s.o_done[i], 1);
+      mbar_init(&s.o_free[i], NQ == 1 ? 2 * kTile : kTile);
+    }
+    mbar_init(&s.x_full, 2 * kTile);
+    mbar_init(&s.mma_done, 1);
+    s.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kLoadWarp && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_kc);
+    tma_prefetch_desc(&map_vc);
+    tma_prefetch_desc(&map_kn);
+    tma_prefetch_desc(&map_vn);
+  }
+  if (warp == kMmaWarp) tmem_alloc(&s.tmem_base, kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  pdl_wait();
+  Walk w = tree_plan(a, s, a.ws_plan != nullptr);
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------ TMA
+    uint32_t rc = 0, uc = 0;
+    bool ok = true;
+    Piece p = {};
+    // Tile t of keys (or values) into the ring.
+    auto load = [&](const CUtensorMap* cached, const CUtensorMap* drafted, int t) -> bool {
+      const uint32_t st = rc % kRing, par = (rc / kRing) & 1u;
+      const bool old = t < p.tiles - 1;
+      int page = 0, slot = 0, boxes = 0;
+      if (old) {  // the box's page, looked up before the wait for a free tile
+        boxes = min(kTile, p.len - t * kTile);
+        boxes = (boxes + a.box - 1) / a.box;
+        if (lane < boxes) {
+          const uint32_t g = (uint32_t)(t * (kTile / a.box) + lane);
+          const uint32_t pi = a.log_bpp >= 0 ? g >> a.log_bpp : (uint32_t)((g * a.bpp_magic) >> 36);
+          slot = (int)(g - pi * a.boxes_per_page) * a.box;
+          page = a.tables[(int64_t)p.b * a.max_pages + pi];
+          if ((uint32_t)page >= (uint32_t)a.pages) page = a.pages;  // outside: read as zeros
+        }
+      }
+      if (!tree_wait(&s.empty[st], par ^ 1u, &s.abort, 11)) return false;
+      if (lane == 0) mbar_arrive_expect_tx(&s.full[st], old ? (uint32_t)(boxes * a.box * D * 2) : kTileBytes);
+      __syncwarp();
+      uint8_t* to = s.ring[st];
+      if (old) {
+        if (lane < boxes)
+          for (int c = 0; c < kSub; ++c)
+            tma_load_4d(to + c * (kTile * 128) + lane * a.box * 128, cached, &s.full[st], c * 64, slot, p.kvh, page);
+      } else if (lane < kSub) {
+        tma_load_4d(to + lane * (kTile * 128), drafted, &s.full[st], lane * 64, 0, p.kvh, p.b);
+      }
+      __syncwarp();
+      ++rc;
+      return true;
+    };
+    while (ok && next_piece(a, w, p)) {
+      const int t0 = p.t0, n = p.n;
+      if (!tree_wait(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&s.q_full, (uint32_t)(NQ * D * 2 * a.tt * a.group));
+        for (int i = 0; i < NQ; ++i)
+          for (int c = 0; c < kSub; ++c)
+            tma_load_4d(s.q[i] + c * (kTile * 128), &map_q, &s.q_full, c * 64, p.kvh * a.group,
+                        (p.mb * NQ + i) * a.tt, p.b);
+      }
+      __syncwarp();
+      ++uc;
+      ok = load(&map_kc, &map_kn, t0);
+      if constexpr (NQ == 1) {
+        if (ok && n > 1) ok = load(&map_kc, &map_kn, t0 + 1);
+        for (int t = 0; ok && t < n; ++t) {
+          ok = load(&map_vc, &map_vn, t0 + t);
+          if (ok && t + 2 < n) ok = load(&map_kc, &map_kn, t0 + t + 2);
+        }
+      } else {
+        for (int t = 0; ok && t < n; ++t) {
+          ok = load(&map_vc, &map_vn, t0 + t);
+          if (ok && t + 1 < n) ok = load(&map_kc, &map_kn, t0 + t + 1);
+        }
+      }
+    }
+    if (!ok && lane == 0) {  // let issued copies land before shared memory is released
+      const uint64_t begin = globaltimer();
+      if (uc > 0)
+        while (!mbar_try_wait(&s.q_full, (uc - 1) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
+      for (uint32_t i = rc > kRing ? rc - kRing : 0; i < rc; ++i)
+        while (!mbar_try_wait(&s.full[i % kRing], (i / kRing) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------ MMA
+    if (elect_one()) {
+      uint32_t rc = 0, uc = 0, gt = 0;
+      bool ok = true;
+      Piece p;
+      auto wait_full = [&](uint32_t i, int code) {
+        const bool y = mbar_wait(&s.full[i % kRing], (i / kRing) & 1u, &s.abort, &g_tree_dev_error, code);
+        tc_fence_after();
+        return y;
+      };
+      auto issue_s = [&](int g, int qi, uint32_t i) {  // scores of group g from Q tile qi and ring tile i
+        const uint64_t qd = smem_desc_sw128(smem_u32(s.q[qi]), 16, 1024);
+        const uint64_t kd = smem_desc_sw128(smem_u32(s.ring[i % kRing]), 16, 1024);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (uint32_t)(((kk >> 2) * (kTile * 128) + (kk & 3) * 32) >> 4);
+          mma_bf16_ss(tmem + (uint32_t)(g * kTile), qd + off, kd + off, kIdescS, kk > 0 ? 1u : 0u);
+        }
+        mma_commit(&s.s_full[g]);
+      };
+      auto issue_pv = [&](int g, uint32_t i, bool add, bool two) {  // O of group g (+)= P V
+        const uint64_t vd = smem_desc_sw128(smem_u32(s.ring[i % kRing]), kTile * 128, 1024);
+        if (two) {
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            mma_bf16_ts(tmem + kOCol + (uint32_t)(g * D), tmem + (uint32_t)(g * kTile + kTile / 2 + kk * 8),
+                        vd + (uint32_t)(kk * 128), kIdescPV, (add || kk > 0) ? 1u : 0u);
+          add = true;
+        }
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk)
+          mma_bf16_ts(tmem + kOCol + (uint32_t)(g * D), tmem + (uint32_t)(g * kTile + kk * 8),
+                      vd + (uint32_t)(kk * 128), kIdescPV, (add || kk > 0) ? 1u : 0u);
+        mma_commit(&s.o_done[g]);
+      };
+      while (ok && next_piece(a, w, p)) {
+        const int n = p.n;
+        if (!mbar_wait(&s.q_full, uc & 1u, &s.abort, &g_tree_dev_error, 20)) { ok = false; break; }
+        tc_fence_after();
+        if constexpr (NQ == 1) {
+          for (int t = 0; ok && t < n && t < 2; ++t) {
+            if (!(ok = wait_full(rc, 21))) break;
+            issue_s((gt + t) & 1, 0, rc);
+            mma_commit(&s.empty[rc % kRing]);
+            ++rc;
+          }
+          if (ok && n <= 2) mma_commit(&s.q_empty);
+          for (int t = 0; ok && t < n; ++t) {
+            const uint32_t G = gt + (uint32_t)t;
+            const int g = G & 1;
+            if (!(ok = wait_full(rc, 22))) break;
+            if (t == 0 && !(ok = mbar_wait(&s.o_free[0], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23))) break;
+            if (!(ok = mbar_wait(&s.p_full[g], (G >> 1) & 1u, &s.abort, &g_tree_dev_error, 24))) break;
+            tc_fence_after();
+            issue_pv(g, rc, t >= 2, p.len <= kFine);
+            mma_commit(&s.empty[rc % kRing]);
+            ++rc;
+            if (t + 2 < n) {  // the scores after next, behind the product that reads their place
+              if (!(ok = wait_full(rc, 25))) break;
+              issue_s(g, 0, rc);
+              mma_commit(&s.empty[rc % kRing]);
+              ++rc;
+              if (t + 3 == n) mma_commit(&s.q_empty);
+            }
+          }
+        } else {
+          if (!(ok = wait_full(rc, 21))) break;
+          issue_s(0, 0, rc);
+          issue_s(1, 1, rc);
+          mma_commit(&s.empty[rc % kRing]);
+          ++rc;
+          if (n == 1) mma_commit(&s.q_empty);
+          for (int t = 0; ok && t < n; ++t) {
+            const uint32_t G = gt + (uint32_t)t;
+            if (!(ok = wait_full(rc, 22))) break;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (t == 0 && !(ok = mbar_wait(&s.o_free[g], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23))) break;
+              if (!(ok = mbar_wait(&s.p_full[g], G & 1u, &s.abort, &g_tree_dev_error, 24))) break;
+              tc_fence_after();
+              issue_pv(g, rc, t > 0, p.len <= kFine);
+              if (g == 1) mma_commit(&s.empty[rc % kRing]);
+              if (t + 1 < n) {
+                if (g == 0 && !(ok = wait_full(rc + 1, 25))) break;
+                issue_s(g, g, rc + 1);
+                if (g == 1) {
+                  mma_commit(&s.empty[(rc + 1) % kRing]);
+                  if (t + 2 == n) mma_commit(&s.q_empty);
+                }
+              }
+            }
+            rc += t + 1 < n ? 2 : 1;
+          }
+        }
+        if (!ok) break;
+        gt += (uint32_t)n;
+        ++uc;
+      }
+      // Every MMA issued by this thread has completed once mma_done flips.
+      mma_commit(&s.mma_done);
+      const uint64_t begin = globaltimer();
+      while (!mbar_try_wait(&s.mma_done, 0) && globaltimer() - begin < kWaitTimeoutNs) {}
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------ softmax groups
+    const int g = warp >> 2, qd = warp & 3;
+    const int r = qd * 32 + lane;  // row of the query tile == TMEM lane
+    const uint32_t lane_off = (uint32_t)(qd * 32) << 16;
+    const uint32_t s_addr = tmem + lane_off + (uint32_t)(g * kTile);
+    const uint32_t o_addr = tmem + lane_off + kOCol;
+    uint32_t rc = 0, gt = 0, uc = 0;
+    bool ok = true;
+    Piece p;
+    while (ok && next_piece(a, w, p)) {
+      const int n = p.n;
+      const int tok0 = (p.mb * NQ + (NQ == 1 ? 0 : g)) * a.tt;
+      const int rows = max(min(a.tt, a.tokens - tok0), 0) * a.group;
+      const bool busy = qd * 32 < rows;  // a warp without query rows only keeps the barriers going
+      const int token = tok0 + r / a.group;
+      uint32_t seen[4] = {0u, 0u, 0u, 0u};
+      float m = -INFINITY, l = 0.f;
+      bool any = false;  // this group has had a tile of this piece
+      for (int t = 0; t < n; ++t) {
+        const uint32_t G = gt + (uint32_t)t;
+        if (NQ == 1 && (int)(G & 1u) != g) continue;
+        const uint32_t use = NQ == 1 ? G >> 1 : G;  // how often the group's buffers were used before
+        const int tile = p.t0 + t;
+        const bool old = tile < p.tiles - 1;
+        const int valid = old ? min(kTile, p.len - tile * kTile) : kTile;
+        if (!old && r < rows) ancestor_bits(a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr, token, seen);
+        if (!tree_wait(&s.s_full[g], use & 1u, &s.abort, 31)) { ok = false; break; }
+        tc_fence_after();
+        if (busy) {
+          uint32_t v[kTile];
+#pragma unroll
+          for (int c = 0; c < kTile; c += 32) tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[c]));
+          tmem_wait_ld();
+          reg_fence<kTile>(v);
+          if (!old) {
+#pragma unroll
+            for (int c = 0; c < kTile; ++c)
+              if (!((seen[c >> 5] >> (c & 31)) & 1u)) v[c] = 0xff800000u;
+          } else if (valid < kTile) {
+#pragma unroll
+            for (int c = 0; c < kTile; ++c)
+              if (c >= valid) v[c] = 0xff800000u;
+          }
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < kTile; c += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx4[k] = max3f(mx4[k], __uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1]));
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+          float factor = 1.f;
+          if (m == -INFINITY) {
+            m = mx;  // nothing seen before: O and l are zero
+          } else if (mx > m + kLag) {
+            factor = fast_exp2(m - mx);
+            m = mx;
+          }
+          f32x2 rs[2];
+          const float neg_m = m == -INFINITY ? 0.f : -m;
+          if (p.len <= kFine) {
+            uint32_t hi[kTile / 2], lo[kTile / 2];
+            exp_pack_two<kTile, 2>(v, hi, lo, a.scale_log2, neg_m, rs);
+            tmem_st32(s_addr, hi);
+            tmem_st32(s_addr + 32, hi + 32);
+            tmem_st32(s_addr + 64, lo);
+            tmem_st32(s_addr + 96, lo + 32);
+          } else {
+            exp_pack_rounded<kTile, 2>(v, a.scale_log2, neg_m, rs);
+            tmem_st32(s_addr, v);
+            tmem_st32(s_addr + 32, v + 32);
+          }
+          l = l * factor + ((f2_lo(rs[0]) + f2_hi(rs[0])) + (f2_lo(rs[1]) + f2_hi(rs[1])));
+          if (any && __any_sync(0xffffffffu, factor != 1.f)) {
+            // O *= factor; it must hold every product before this one
+            if (!tree_wait(&s.o_done[g], (use - 1) & 1u, &s.abort, 32)) { ok = false; break; }
+            tc_fence_after();
+            tmem_wait_st();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + (uint32_t)(g * D + c), o);
+              tmem_wait_ld();
+              reg_fence<32>(o);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+              tmem_st32(o_addr + (uint32_t)(g * D + c), o);
+            }
+          }
+          tmem_wait_st();
+        }
+        if (!old && (NQ == 1 || g == 0)) {
+          // A product with P = 0 has to leave no trace of a drafted token's v, whatever it
+          // holds: the rows of absent tokens are cleared, and infinities and NaN of present
+          // ones are cleared and put back at the end for the rows that see them. With two
+          // query tiles the first group does it for both: the second group's product is
+          // issued after the first one's.
+          const uint32_t i = rc + (uint32_t)v_at<NQ>(t, n);
+          if (uc > 0 && !tree_wait(&s.o_free[0], (uc - 1) & 1u, &s.abort, 38)) { ok = false; break; }
+          if (NQ == 2 && uc > 0 && !tree_wait(&s.o_free[1], (uc - 1) & 1u, &s.abort, 39)) { ok = false; break; }
+          if (!tree_wait(&s.full[i % kRing], (i / kRing) & 1u, &s.abort, 33)) { ok = false; break; }
+          uint8_t* row_v = s.ring[i % kRing] + r * 128;
+          const bool absent = a.parents && r < a.tokens && a.parents[(int64_t)p.b * a.tokens + r] < -1;
+          bool bad = false;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c) {
+            uint4* at = reinterpret_cast<uint4*>(row_v + (c / 8) * (kTile * 128) + ((c ^ r) & 7) * 16);
+            uint4 x = *at;
+            uint32_t* word = reinterpret_cast<uint32_t*>(&x);
+            bool change = absent;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (absent) {
+                word[k] = 0u;
+              } else {
+                const bool lo = (word[k] & 0x7f80u) == 0x7f80u, hi = (word[k] & 0x7f800000u) == 0x7f800000u;
+                if (lo) word[k] &= 0xffff0000u;
+                if (hi) word[k] &= 0x0000ffffu;
+                bad |= lo || hi;
+                change |= lo || hi;
+              }
+            }
+            if (change) *at = x;
+          }
+          const uint32_t word = __ballot_sync(0xffffffffu, bad);
+          if (lane == 0) s.bad[qd] = word;
+          fence_proxy_async_smem();
+        }
+        if (valid < kTile && (NQ == 1 || g == 0)) {
+          // Rows of V past the sequence's end hold whatever the page or the ring held before:
+          // they are cleared too.
+          const uint32_t i = rc + (uint32_t)v_at<NQ>(t, n);
+          if (!tree_wait(&s.full[i % kRing], (i / kRing) & 1u, &s.abort, 33)) { ok = false; break; }
+          uint8_t* tile_v = s.ring[i % kRing];
+          for (int x = valid * 8 + r; x < kTile * 8; x += kTile)
+#pragma unroll
+            for (int c = 0; c < kSub; ++c)
+              *reinterpret_cast<uint4*>(tile_v + c * (kTile * 128) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        mbar_arrive(&s.p_full[g]);
+        any = true;
+      }
+      if (!ok) break;
+      // ---------------- end of the piece: O / l, or the piece's (max, sum, O)
+      const bool cut = !(p.t0 == 0 && n == p.tiles);
+      const int slot = 2 * (int)blockIdx.x + (p.t0 == 0 ? 1 : 0);
+      if (NQ == 1 && p.t0 + n == p.tiles && r < rows && (int)((gt + (uint32_t)n - 1) & 1u) != g)
+        ancestor_bits(a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr, token, seen);  // the other group had the drafted tile
+      const bool here = (seen[0] | seen[1] | seen[2] | seen[3]) != 0u;
+      const uint32_t last = gt + (uint32_t)n - 1;
+      const int64_t row_at =
+          (((int64_t)p.b * a.tokens + token) * a.heads + p.kvh * a.group + r % a.group) * D;
+      float w0 = 1.f, w1 = 0.f;
+      bool use0 = true, use1 = false;
+      int c0 = 0, c1 = D;
+      if constexpr (NQ == 1) {
+        // both groups' results: this one writes half of the columns
+        if (uc > 0 && !tree_wait(&s.o_free[0], (uc - 1) & 1u, &s.abort, 34)) { ok = false; break; }
+        s.xm[g][r] = m;
+        s.xl[g][r] = l;
+        mbar_arrive(&s.x_full);
+        const uint32_t other = last - 1;  // the last tile of the other parity, if the piece has one
+        if (!tree_wait(&s.o_done[last & 1], (last >> 1) & 1u, &s.abort, 35)) { ok = false; break; }
+        if (n > 1 && !tree_wait(&s.o_done[other & 1], (other >> 1) & 1u, &s.abort, 36)) { ok = false; break; }
+        if (!tree_wait(&s.x_full, uc & 1u, &s.abort, 37)) { ok = false; break; }
+        use0 = n > 1 || (last & 1u) == 0u;
+        use1 = n > 1 || (last & 1u) == 1u;
+        const float m0 = use0 ? s.xm[0][r] : -INFINITY, m1 = use1 ? s.xm[1][r] : -INFINITY;
+        m = fmaxf(m0, m1);
+        w0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m);
+        w1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - m);
+        l = (use0 ? s.xl[0][r] * w0 : 0.f) + (use1 ? s.xl[1][r] * w1 : 0.f);
+        c0 = g * (D / 2);
+        c1 = c0 + D / 2;
+      } else {
+        if (!tree_wait(&s.o_done[g], last & 1u, &s.abort, 35)) { ok = false; break; }
+      }
+      tc_fence_after();
+      const float inv = cut ? 1.f : here ? 1.f / l : 0.f;
+      uint32_t sees_bad[4] = {0u, 0u, 0u, 0u};  // drafted tokens that bring infinities or NaN to this row
+      if (p.t0 + n == p.tiles) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sees_bad[k] = r < rows ? seen[k] & s.bad[k] : 0u;
+      }
+      if (busy) {
+        const int ti = NQ == 1 ? 0 : g;
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 32) {
+          uint32_t o[32];
+          if constexpr (NQ == 1) {
+            uint32_t x[32];
+            tmem_ld32(o_addr + (uint32_t)c, o);
+            tmem_ld32(o_addr + (uint32_t)(D + c), x);
+            tmem_wait_ld();
+            reg_fence<32>(o);
+            reg_fence<32>(x);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {  // an unused group's O is not read as a number
+              const float y0 = use0 ? __uint_as_float(o[k]) * w0 : 0.f;
+              const float y1 = use1 ? __uint_as_float(x[k]) * w1 : 0.f;
+              o[k] = __float_as_uint((y0 + y1) * inv);
+            }
+          } else {
+            tmem_ld32(o_addr + (uint32_t)(g * D + c), o);
+            tmem_wait_ld();
+            reg_fence<32>(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+          }
+          if ((sees_bad[0] | sees_bad[1] | sees_bad[2] | sees_bad[3]) != 0u) {
+            for (int j = 0; j < a.tokens; ++j) {
+              const uint32_t bits = j < 32 ? sees_bad[0] : j < 64 ? sees_bad[1] : j < 96 ? sees_bad[2] : sees_bad[3];
+              if (!((bits >> (j & 31)) & 1u)) continue;
+              const bf16* vj = a.v_new + p.b * a.n_b + j * a.n_t + p.kvh * a.n_h + c;
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const float x = __bfloat162float(vj[k]);
+                if (!(fabsf(x) < INFINITY)) o[k] = __float_as_uint(__uint_as_float(o[k]) + x);
+              }
+            }
+          }
+          if (r < rows) {
+            if (cut) {
+              float4* to = a.ws_o + ((int64_t)(slot * NQ + ti) * (D / 4) + c / 4) * kTile + r;
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                to[k * kTile] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                            __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint4 packed = pack16<bf16>(reinterpret_cast<const float*>(o) + 8 * k);
+                if (!here) packed = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(a.out + row_at + c + 8 * k) = packed;
+              }
+            }
+          }
+        }
+        if (cut && r < rows && (NQ == 2 || g == 0)) {
+          float* to = a.ws_ml + (int64_t)(slot * NQ + ti) * 2 * kTile + r;
+          to[0] = m;
+          to[kTile] = l;
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&s.o_free[NQ == 1 ? 0 : g]);
+      rc += 2 * (uint32_t)n;
+      gt += (uint32_t)n;
+      ++uc;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the pieces of the segments that were cut: out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p,
+// in order of the pieces. A block takes 8 rows of a segment, a thread 4 columns of one row.
+template <int D, int NQ>
+__global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant__ TcArgs a) {
+  pdl_enter();
+  const int b = blockIdx.z, hm = blockIdx.y, hms = a.kv_heads * a.row_blocks;
+  const int kvh = hm / a.row_blocks, mb = hm - kvh * a.row_blocks;
+  const int share = a.ws_plan[0], n = tree_tiles(a, b);
+  const long long first = (long long)a.ws_plan[1 + b] * hms + (long long)hm * n;
+  // cuts strictly inside the segment belong to blocks lo .. hi, in a row
+  int lo = (int)(first / share) + 1, hi = (int)((first + n - 1) / share);
+  while (lo <= hi) {
+    const int off = (int)((long long)lo * share - first), at = snap(off, n, share);
+    if (at > 0 && at < n) break;
+    ++lo;
+  }
+  while (lo <= hi) {
+    const int off = (int)((long long)hi * share - first), at = snap(off, n, share);
+    if (at > 0 && at < n) break;
+    --hi;
+  }
+  if (lo > hi) return;
+  const int x = blockIdx.x * 8 + (threadIdx.x & 7), c4 = threadIdx.x >> 3;
+  const int ti = x / kTile, r = x - ti * kTile;
+  const int token = (mb * NQ + ti) * a.tt + r / a.group;
+  if (r >= a.tt * a.group || token >= a.tokens) return;
+  const int pieces = hi - lo + 2;  // piece 0 is the end of block lo - 1, piece i the beginning of block lo - 1 + i
+  auto slot = [&](int i) { return (int64_t)((i == 0 ? 2 * (lo - 1) + 1 : 2 * (lo - 1 + i)) * NQ + ti); };
+  float m = -INFINITY;
+  for (int i = 0; i < pieces; ++i) m = fmaxf(m, __ldcg(a.ws_ml + slot(i) * 2 * kTile + r));
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) {
+    const float mi = __ldcg(a.ws_ml + slot(i) * 2 * kTile + r), li = __ldcg(a.ws_ml + slot(i) * 2 * kTile + kTile + r);
+    const float4 v = __ldcg(a.ws_o + (slot(i) * (D / 4) + c4) * kTile + r);
+    if (mi == -INFINITY) continue;  // nothing of this piece is visible
+    const float wi = fast_exp2(mi - m);
+    l = fmaf(wi, li, l);
+    o.x = fmaf(wi, v.x, o.x);
+    o.y = fmaf(wi, v.y, o.y);
+    o.z = fmaf(wi, v.z, o.z);
+    o.w = fmaf(wi, v.w, o.w);
+  }
+  const bool here = !a.parents || a.parents[(int64_t)b * a.tokens + token] >= -1;
+  const float inv = here ? 1.f / l : 0.f;
+  if (!here) o = make_float4(0.f, 0.f, 0.f, 0.f);
+  store4(a.out + (((int64_t)b * a.tokens + token) * a.heads + kvh * a.group + r % a.group) * D + c4 * 4,
+         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+}
+
+// ------------------------------------------------------------------ host
+
+struct TcPlan {
+  bool on;          // the tensor-core kernel takes this call
+  int nq, tt, row_blocks, box, grid;
+  bool join;        // segments may be cut
+  size_t ml_off, o_off, bytes;
+};
+
+// The call's sizes and types (not its strides and pointers) decide; measured against the
+// CUDA-core kernel in the file's head.
+TcPlan tc_plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t d, int64_t page,
+               int64_t max_pages, int dtype) {
+  TcPlan p = {};
+  const int64_t group = heads / kv_heads;
+  if (dtype != NKL_BFLOAT16 || (d != 64 && d != 128) || group > kTile || page % 8 != 0) return p;
+  p.box = 8;
+  while (p.box < kTile && page % (2 * p.box) == 0) p.box *= 2;
+  if (page / p.box > 256) return p;  // the division by boxes per page is exact up to there
+  p.tt = (int)(kTile / group);
+  const int64_t q_tiles = (tokens + p.tt - 1) / p.tt;
+  p.nq = q_tiles > 1 ? 2 : 1;
+  p.row_blocks = (int)((q_tiles + p.nq - 1) / p.nq);
+  const int64_t seg_tiles = (page * max_pages + kTile - 1) / kTile + 1;
+  const int64_t segments = batch * kv_heads * p.row_blocks;
+  if (segments * seg_tiles > 0x7fffffffLL / 2 || kv_heads * p.row_blocks > 65535) return p;
+  p.on = true;
+  p.join = seg_tiles > kWhole;
+  p.grid = (int)std::min<int64_t>(sm_count(), p.join ? segments * seg_tiles : segments);
+  if (p.join) {
+    const size_t slots = 2 * (size_t)p.grid * p.nq;
+    p.ml_off = ((size_t)(batch + 1) * 4 + 255) & ~size_t(255);
+    p.o_off = p.ml_off + slots * 2 * kTile * 4;
+    p.bytes = p.o_off + slots * kTile * d * 4;
+  }
+  return p;
+}
+
+template <int D, int NQ>
+int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_t st) {
+  const char* op = "nkl_attention_tree";
+  CUtensorMap mq, mkn, mvn, mkc, mvc;
+  {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)g.heads, (uint64_t)g.tokens, (uint64_t)g.batch};
+    const uint64_t strides[3] = {(uint64_t)g.q_h * 2, (uint64_t)g.q_t * 2, (uint64_t)g.q_b * 2};
+    const uint32_t box[4] = {64, (uint32_t)g.group, (uint32_t)p.tt, 1};
+    if (int rc = make_tensor_map_bf16(&mq, g.q, 4, dims, strides, box, op)) return rc;
+  }
+  {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)g.tokens, (uint64_t)g.kv_heads, (uint64_t)g.batch};
+    const uint64_t strides[3] = {(uint64_t)g.n_t * 2, (uint64_t)g.n_h * 2, (uint64_t)g.n_b * 2};
+    const uint32_t box[4] = {64, kTile, 1, 1};
+    if (int rc = make_tensor_map_bf16(&mkn, g.k_new, 4, dims, strides, box, op)) return rc;
+    if (int rc = make_tensor_map_bf16(&mvn, g.v_new, 4, dims, strides, box, op)) return rc;
+  }
+  {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)g.page, (uint64_t)g.kv_heads, (uint64_t)g.pages};
+    const uint64_t strides[3] = {(uint64_t)g.c_s * 2, (uint64_t)g.c_h * 2, (uint64_t)g.c_p * 2};
+    const uint32_t box[4] = {64, (uint32_t)p.box, 1, 1};
+    if (int rc = make_tensor_map_bf16(&mkc, g.k_cache, 4, dims, strides, box, op)) return rc;
+    if (int rc = make_tensor_map_bf16(&mvc, g.v_cache, 4, dims, strides, box, op)) return rc;
+  }
+  TcArgs a = {};
+  a.tables = g.tables;
+  a.lens = g.lens;
+  a.parents = g.parents;
+  a.v_new = static_cast<const bf16*>(g.v_new);
+  a.n_b = g.n_b;
+  a.n_t = g.n_t;
+  a.n_h = g.n_h;
+  a.out = static_cast<bf16*>(g.out);
+  if (p.join) {
+    a.ws_plan = reinterpret_cast<int*>(ws);
+    a.ws_ml = reinterpret_cast<float*>(ws + p.ml_off);
+    a.ws_o = reinterpret_cast<float4*>(ws + p.o_off);
+  }
+  a.batch = g.batch; a.tokens = g.tokens; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.group;
+  a.pages = g.pages; a.page = g.page; a.max_pages = g.max_pages;
+  a.tt = p.tt; a.row_blocks = p.row_blocks; a.box = p.box;
+  a.boxes_per_page = g.page / p.box;
+  a.log_bpp = -1;
+  for (int i = 0; i < 9; ++i)
+    if (a.boxes_per_page == 1 << i) a.log_bpp = i;
+  a.bpp_magic = ((1ull << 36) + a.boxes_per_page - 1) / a.boxes_per_page;
+  a.scale_log2 = g.scale * kLog2e;
+  constexpr size_t smem = sizeof(TreeSmem<D, NQ>);
+  static_assert(smem <= 232448, "shared memory of a block");
+  static std::atomic<bool> set[64] = {};  // per device: the smem attribute is set (idempotent)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(tree_attention_tc_kernel<D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+  }
+  int rc = launch_pdl(tree_attention_tc_kernel<D, NQ>, dim3((unsigned)p.grid), dim3(kTcThreads), smem, st, op, mq, mkn,
+                      mvn, mkc, mvc, a);
+  if (rc || !p.join) return rc;
+  const int rows = std::min<int>(NQ == 1 ? p.tt * g.group : NQ * kTile, NQ == 1 ? g.tokens * g.group : NQ * kTile);
+  return launch_pdl(tree_join_kernel<D, NQ>,
+                    dim3((unsigned)((rows + 7) / 8), (unsigned)(g.kv_heads * p.row_blocks), (unsigned)g.batch),
+                    dim3(2 * D), 0, st, op, a);
+}
+
+}  // namespace

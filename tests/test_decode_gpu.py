@@ -188,6 +188,35 @@ def test_attention_extreme_scores():
                     *attention_64(q, k, v, kc, vc, tables, lens, parents, 128 ** -0.5))
 
 
+@pytest.mark.parametrize("dtype,H", [(BF, 4), (BF, 40), (F32, 4)])
+def test_attention_infinities_of_unseen_tokens(dtype, H):
+    """Infinities and NaN in the k and v of absent tokens, and of tokens on other branches, leave
+    no trace; a token's own show in its row and its descendants'."""
+    q, k, v, kc, vc, tables, lens = setup_attention(2, 9, H, 2, 64, 16, [300, 0], dtype)
+    parents = [[-1, 0, 0, 2, -1, -2, 4, 3, -2], [-1, -1, 1, 2, 3, -2, -2, 1, 7]]
+    k, v = k.clone(), v.clone()
+    k[0, 5], v[0, 5] = float("nan"), float("nan")  # absent
+    v[0, 8] = float("inf")
+    v[1, 5], k[1, 6] = float("-inf"), float("inf")
+    clean = [t.clone() for t in (k, v)]
+    v[0, 2, 0, 3], v[0, 2, 1, 60] = float("inf"), float("nan")  # seen by 2, 3 and 7
+    v[1, 0, 0, :] = float("-inf")  # a leaf
+    x = (q, k, v, kc, vc, tables, lens)
+    for ks in (k, clean[0]):
+        ks[0, 5], ks[1, 6] = 0, 0  # the statement in 64 bits never looks at them, but copies
+    want, mag = attention_64(q, *clean, kc, vc, tables, lens, i32(parents), 1 / 8)
+    k[0, 5], k[1, 6] = float("nan"), float("inf")
+    got = ops.attention_tree(*x, i32(parents))
+    shows = torch.zeros(2, 9, H, 64, dtype=torch.bool)
+    shows[0, [2, 3, 7], :H // 2, 3] = True
+    shows[0, [2, 3, 7], H // 2:, 60] = True
+    shows[1, 0, :H // 2] = True
+    shows = shows.to(DEV)
+    assert not torch.isfinite(got[shows]).any()
+    assert (got[0, [2, 3, 7], :H // 2, 3] == float("inf")).all() and got[0, [2, 3, 7], H // 2:, 60].isnan().all()
+    check_attention(torch.where(shows, 0, got), torch.where(shows.cpu(), 0, want), mag)
+
+
 @pytest.mark.parametrize("dtype,T", [(BF, 1), (BF, 70), (F32, 3)])
 def test_attention_growing_maxima(dtype, T):
     """Every later key scores higher: the running maximum grows in every tile."""
