@@ -4,16 +4,17 @@
 // A segment is one (sequence, key/value head, block of query rows): its keys are the cached
 // tiles of 128 positions, the last of them partly filled, and one tile of drafted tokens. The
 // lengths are known on the GPU only, so the blocks share the work out there: all segments'
-// tiles form one row, of which block c takes tiles [c X, (c + 1) X). A segment that is cut
-// leaves (max, sum, O) per piece in the workspace, and tree_join_kernel joins the pieces in
-// order. Cuts near a segment's end move there, and short segments are not cut.
+// tiles, and kExtra more for what a segment costs besides, form one row, of which block c takes
+// [c X, (c + 1) X). A segment that is cut leaves (max, sum, O) per piece in the workspace, and
+// tree_join_kernel joins the pieces in order. Cuts near a segment's end move there, and short
+// segments are not cut.
 //
 // Query rows of a tile: `tt` tokens times the G query heads of the key/value head (tt G <=
 // 128), fetched by one TMA box per 64 columns, so row r is token r / G, head r % G.
 //   warps 0-3, 4-7  softmax groups 0 and 1, one thread per row: scores from TMEM, mask, running
 //                   maximum and sum, exponentials rounded to bf16 back into TMEM over the scores
-//   warp 8          TMA: queries, and keys and values through one ring of tiles; the lanes look
-//                   up the pages of a tile and fetch one box each
+//   warps 8, 10     TMA: queries and keys, values, each through a ring of tiles; the lanes look
+//                   up the pages, a box of rows of one page each
 //   warp 9          tcgen05.mma, both products: S = Q K^T, O += P V (P from TMEM)
 //   TMEM            S / P of group 0, 1 [0, 128), [128, 256); O of group 0, 1 after them
 // NQ = 1 (rows fit one tile): the groups take the tiles of keys in turn, each with a maximum,
@@ -32,9 +33,10 @@ using namespace sm100;
 __device__ unsigned int g_tree_dev_error = 0;
 
 constexpr int kTile = 128;
-constexpr int kTcThreads = 320;
-constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kTcThreads = 352;
+constexpr int kKeyWarp = 8, kMmaWarp = 9, kValueWarp = 10;
 constexpr int kWhole = 4;        // segments of up to so many tiles are not cut
+constexpr int kExtra = 1;        // a segment's beginning and end, in tiles
 // Sequences of up to so many cached positions have P in two bf16 parts, P V in two products: a
 // row that sees few keys does not average the roundings of P out (one part: up to 2^-8 of a
 // weight). The second product is hidden behind the loads there is time for; on long rows,
@@ -51,6 +53,7 @@ struct TcArgs {
   float* ws_ml;    // [slot][NQ][2][128]
   float4* ws_o;    // [slot][NQ][d / 4][128]
   int batch, tokens, heads, kv_heads, group, pages, page, max_pages;
+  int capacity;    // positions that a row of the tables holds
   int tt;          // tokens per query tile
   int row_blocks;  // blocks of NQ query tiles
   int box;         // rows of a page fetched by one TMA box
@@ -60,13 +63,14 @@ struct TcArgs {
 };
 
 __device__ __forceinline__ int tree_len(const TcArgs& a, int b) {
-  return (int)min((long long)max(a.lens[b], 0), (long long)a.max_pages * a.page);
+  return min(max(a.lens[b], 0), a.capacity);
 }
 __device__ __forceinline__ int tree_tiles(const TcArgs& a, int b) { return (tree_len(a, b) + kTile - 1) / kTile + 1; }
 
-// Where a cut at tile `off` of a segment of n tiles goes: 0 or n when it is near, or when the
-// segment is short.
-__device__ __forceinline__ int snap(int off, int n, int share) {
+// Where a cut goes that falls `off` into a segment of n tiles (and kExtra before them): to a
+// tile, or to 0 or n when that is near or the segment is short.
+__device__ __forceinline__ int cut_at(int off, int n, int share) {
+  off = max(off - kExtra, 0);
   if (n <= kWhole) return 2 * off >= n ? n : 0;
   const int near = min(max(share / 4, 1), 4);
   if (off < near) return 0;
@@ -74,9 +78,9 @@ __device__ __forceinline__ int snap(int off, int n, int share) {
   return off;
 }
 
-// One block's walk over its pieces of segments.
+// One block's walk over its pieces of segments: the place it has come to and its end.
 struct Walk {
-  int b, hm, t, tiles, left;
+  int b, hm, t, tiles, end_b, end_hm, end_t;
 };
 struct Piece {
   int b, kvh, mb, t0, n, tiles, len;
@@ -85,146 +89,120 @@ struct Piece {
 template <int D, int NQ>
 struct TreeSmem {
   static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kRing = (D == 128 ? 7 : 12) - NQ;
+  static constexpr int kRingK = D == 128 ? 3 : 5;
+  static constexpr int kRingV = (D == 128 ? 4 : 6) - NQ;
   uint8_t q[NQ][kTileBytes];
-  uint8_t ring[kRing][kTileBytes];
+  uint8_t k[kRingK][kTileBytes];
+  uint8_t v[kRingV][kTileBytes];
   uint64_t q_full, q_empty;
-  uint64_t full[kRing], empty[kRing];
+  uint64_t k_full[kRingK], k_empty[kRingK];
+  uint64_t v_full[kRingV], v_empty[kRingV];
   uint64_t s_full[2], p_full[2], o_done[2], o_free[2];
   uint64_t x_full;
   uint64_t mma_done;
   float xm[2][kTile], xl[2][kTile];  // NQ = 1: the groups' maxima and sums
-  int scan[kTcThreads / 32 + 2];
   uint32_t bad[4];  // drafted tokens of the piece whose v holds infinities or NaN
-  int cut[2][3];  // this block's first tile and end: sequence, tile of the sequence, tiles before it
   uint32_t tmem_base;
   int abort;
 };
 
 __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   int ok = 1;
   if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort, &g_tree_dev_error, code) ? 1 : 0;
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
 __device__ __forceinline__ bool next_piece(const TcArgs& a, Walk& w, Piece& p) {
-  if (w.left <= 0) return false;
+  const bool last = w.b == w.end_b && w.hm == w.end_hm;
+  if (last ? w.t >= w.end_t : w.b >= w.end_b && (w.b > w.end_b || w.hm > w.end_hm)) return false;
   p.b = w.b;
-  p.kvh = w.hm / a.row_blocks;
+  p.kvh = a.row_blocks == 1 ? w.hm : w.hm / a.row_blocks;
   p.mb = w.hm - p.kvh * a.row_blocks;
   p.t0 = w.t;
   p.tiles = w.tiles;
-  p.n = min(w.tiles - w.t, w.left);
+  p.n = (last ? w.end_t : w.tiles) - w.t;
   p.len = tree_len(a, w.b);
-  w.left -= p.n;
   w.t = 0;
-  if (++w.hm == a.kv_heads * a.row_blocks) {
+  if (last) {
+    w.t = w.end_t;
+  } else if (++w.hm == a.kv_heads * a.row_blocks) {
     w.hm = 0;
-    ++w.b;
-    if (w.left > 0) w.tiles = tree_tiles(a, w.b);
+    if (++w.b < a.batch) w.tiles = tree_tiles(a, w.b);
   }
   return true;
 }
 
-// Inclusive scan and total over the block; two barriers.
-__device__ __forceinline__ int tree_scan(int v, int* scratch, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc = v;
+// This block's walk, computed by each warp for itself (a lane takes consecutive sequences);
+// block 0 leaves the prefix sums for the join.
+__device__ __forceinline__ Walk tree_plan(const TcArgs& a, bool leave) {
+  const int lane = threadIdx.x & 31, hms = a.kv_heads * a.row_blocks;
+  const int per = (a.batch + 31) >> 5, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
+  int sum = 0, longest = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int t = tree_tiles(a, b) + kExtra;
+    sum += t;
+    longest = max(longest, t);
+  }
+  int inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += x;
   }
-  __syncthreads();
-  if (lane == 31) scratch[warp] = inc;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kTcThreads / 32; ++w) {
-    const int x = scratch[w];
-    before += w < warp ? x : 0;
-    total += x;
-  }
-  return before + inc;
-}
-
-// This block's walk; block 0 leaves the prefix sums for the join.
-template <class Smem>
-__device__ __forceinline__ Walk tree_plan(const TcArgs& a, Smem& s, bool join) {
-  const int tid = threadIdx.x, hm = a.kv_heads * a.row_blocks;
-  int sum = 0, longest = 0, mine = 0, inc = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kTcThreads) {
-    const int b = b0 + tid;
-    mine = b < a.batch ? tree_tiles(a, b) : 0;
-    longest = max(longest, mine);
-    int t;
-    inc = sum + tree_scan(mine, s.scan, t);
-    sum += t;
-    if (join && blockIdx.x == 0 && b < a.batch) a.ws_plan[1 + b] = inc - mine;
-  }
   longest = __reduce_max_sync(0xffffffffu, longest);
-  if (tid == 0) s.cut[0][0] = 0;
-  __syncthreads();
-  if ((tid & 31) == 0) atomicMax(&s.cut[0][0], longest);
-  __syncthreads();
-  longest = s.cut[0][0];
-  const int total = sum * hm;
-  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, min(longest, kWhole));
-  if (join && blockIdx.x == 0 && tid == 0) a.ws_plan[0] = share;
-  __syncthreads();
-  if (tid < 2) s.cut[tid][0] = -1;
-  __syncthreads();
-  int before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kTcThreads) {
-    const int b = b0 + tid;
-    if (a.batch > kTcThreads) {  // else the values of the only round are still here
-      mine = b < a.batch ? tree_tiles(a, b) : 0;
-      int t;
-      inc = before + tree_scan(mine, s.scan, t);
-      before += t;
+  const int total = __shfl_sync(0xffffffffu, inc, 31) * hms;
+  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, min(longest, kWhole + kExtra));
+  if (leave) {
+    if (lane == 0) a.ws_plan[0] = share;
+    int before = inc - sum;
+    for (int b = b0; b < b1; ++b) {
+      a.ws_plan[1 + b] = before;
+      before += tree_tiles(a, b) + kExtra;
     }
+  }
+  Walk w;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const long long at = (long long)(blockIdx.x + k) * share;
-      const long long lo = (long long)(inc - mine) * hm;
-      if (mine > 0 && at >= lo && at < (long long)inc * hm) {
-        s.cut[k][0] = b;
-        s.cut[k][1] = (int)(at - lo);
-        s.cut[k][2] = (int)lo;
+  for (int k = 0; k < 2; ++k) {  // where this block's range begins and ends
+    const int at = ((int)blockIdx.x + k) * share;
+    int b = 0, n = 0, lo = (inc - sum) * hms;
+    const bool mine = at >= lo && at < inc * hms;
+    if (mine) {
+      for (b = b0;; ++b) {
+        n = tree_tiles(a, b);
+        if (at < lo + (n + kExtra) * hms) break;
+        lo += (n + kExtra) * hms;
       }
     }
-  }
-  __syncthreads();
-  Walk w = {0, 0, 0, 0, 0};
-  if (s.cut[0][0] < 0) return w;
-  int end = total;
-  if (s.cut[1][0] >= 0) {
-    const int n = tree_tiles(a, s.cut[1][0]), h = s.cut[1][1] / n;
-    end = s.cut[1][2] + h * n + snap(s.cut[1][1] - h * n, n, share);
-  }
-  w.b = s.cut[0][0];
-  w.tiles = tree_tiles(a, w.b);
-  w.hm = s.cut[0][1] / w.tiles;
-  w.t = snap(s.cut[0][1] - w.hm * w.tiles, w.tiles, share);
-  w.left = end - (s.cut[0][2] + w.hm * w.tiles + w.t);
-  if (w.t == w.tiles) {
-    w.t = 0;
-    if (++w.hm == hm) {
-      w.hm = 0;
-      ++w.b;
-      if (w.left > 0) w.tiles = tree_tiles(a, w.b);
+    const unsigned who = __ballot_sync(0xffffffffu, mine);
+    const int src = who ? __ffs(who) - 1 : 0;
+    b = who ? __shfl_sync(0xffffffffu, b, src) : a.batch;
+    n = __shfl_sync(0xffffffffu, n, src);
+    lo = __shfl_sync(0xffffffffu, lo, src);
+    int hm = 0, t = 0;
+    if (who) {
+      hm = (at - lo) / (n + kExtra);
+      t = cut_at(at - lo - hm * (n + kExtra), n, share);
+      if (t == n) {
+        t = 0;
+        if (++hm == hms) {
+          hm = 0;
+          if (++b < a.batch) n = tree_tiles(a, b);
+        }
+      }
+    }
+    if (k == 0) {
+      w.b = b;
+      w.hm = hm;
+      w.t = t;
+      w.tiles = n;
+    } else {
+      w.end_b = b;
+      w.end_hm = hm;
+      w.end_t = t;
     }
   }
   return w;
-}
-
-// Position of V(t) among the 2 n tiles that a piece of n tiles takes from the ring:
-// K0 V0 K1 V1 ... (NQ = 2), K0 K1 V0 K2 V1 ... V(n-2) V(n-1) (NQ = 1).
-template <int NQ>
-__device__ __forceinline__ int v_at(int t, int n) {
-  if (NQ == 2) return 2 * t + 1;
-  return t == n - 1 ? 2 * n - 1 : 2 * t + 2;
 }
 
 template <int D, int NQ>
@@ -240,7 +218,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   pdl_launch_dependents();
   using Smem = TreeSmem<D, NQ>;
   Smem& s = *reinterpret_cast<Smem*>(smem_raw);
-  constexpr int kRing = Smem::kRing;
+  constexpr int kRingK = Smem::kRingK, kRingV = Smem::kRingV;
   constexpr uint32_t kTileBytes = Smem::kTileBytes;
   constexpr uint32_t kTmemCols = 512;
   constexpr uint32_t kOCol = 2 * kTile;  // O of group g at kOCol + g * D
@@ -252,9 +230,13 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, 1);
     mbar_init(&s.q_empty, 1);
-    for (int i = 0; i < kRing; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < kRingK; ++i) {
+      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.k_empty[i], 1);
+    }
+    for (int i = 0; i < kRingV; ++i) {
+      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
@@ -267,11 +249,13 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     s.abort = 0;
     fence_barrier_init();
   }
-  if (warp == kLoadWarp && lane == 0) {
+  if (warp == kKeyWarp && lane == 0) {
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_kc);
-    tma_prefetch_desc(&map_vc);
     tma_prefetch_desc(&map_kn);
+  }
+  if (warp == kValueWarp && lane == 0) {
+    tma_prefetch_desc(&map_vc);
     tma_prefetch_desc(&map_vn);
   }
   if (warp == kMmaWarp) tmem_alloc(&s.tmem_base, kTmemCols);
@@ -280,92 +264,105 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
   pdl_wait();
-  Walk w = tree_plan(a, s, a.ws_plan != nullptr);
+  Walk w = tree_plan(a, a.ws_plan != nullptr && blockIdx.x == 0 && warp == 0);
 
-  if (warp == kLoadWarp) {
+  if (warp == kKeyWarp || warp == kValueWarp) {
     // ------------------------------------------------ TMA
-    uint32_t rc = 0, uc = 0;
+    const bool keys = warp == kKeyWarp;
+    const CUtensorMap* const cached = keys ? &map_kc : &map_vc;
+    const CUtensorMap* const drafted = keys ? &map_kn : &map_vn;
+    uint8_t* const ring = keys ? s.k[0] : s.v[0];
+    uint64_t* const full = keys ? s.k_full : s.v_full;
+    uint64_t* const empty = keys ? s.k_empty : s.v_empty;
+    const uint32_t depth = keys ? kRingK : kRingV;
+    const int per_tile = kTile / a.box;
+    uint32_t st = 0, par = 0, loads = 0, uc = 0;
     bool ok = true;
     Piece p = {};
-    // Tile t of keys (or values) into the ring.
-    auto load = [&](const CUtensorMap* cached, const CUtensorMap* drafted, int t) -> bool {
-      const uint32_t st = rc % kRing, par = (rc / kRing) & 1u;
-      const bool old = t < p.tiles - 1;
-      int page = 0, slot = 0, boxes = 0;
-      if (old) {  // the box's page, looked up before the wait for a free tile
-        boxes = min(kTile, p.len - t * kTile);
-        boxes = (boxes + a.box - 1) / a.box;
-        if (lane < boxes) {
-          const uint32_t g = (uint32_t)(t * (kTile / a.box) + lane);
-          const uint32_t pi = a.log_bpp >= 0 ? g >> a.log_bpp : (uint32_t)((g * a.bpp_magic) >> 36);
-          slot = (int)(g - pi * a.boxes_per_page) * a.box;
-          page = a.tables[(int64_t)p.b * a.max_pages + pi];
-          if ((uint32_t)page >= (uint32_t)a.pages) page = a.pages;  // outside: read as zeros
-        }
+    // page and first row in it of a box of the piece's sequence
+    auto look_up = [&](int box, int& page, int& slot) {
+      page = slot = 0;
+      if (box * a.box < p.len) {
+        const int pi = a.log_bpp >= 0 ? box >> a.log_bpp : (int)(((uint32_t)box * a.bpp_magic) >> 36);
+        slot = (box - pi * a.boxes_per_page) * a.box;
+        page = a.tables[(int64_t)p.b * a.max_pages + pi];
+        if ((uint32_t)page >= (uint32_t)a.pages) page = a.pages;  // outside: read as zeros
       }
-      if (!tree_wait(&s.empty[st], par ^ 1u, &s.abort, 11)) return false;
-      if (lane == 0) mbar_arrive_expect_tx(&s.full[st], old ? (uint32_t)(boxes * a.box * D * 2) : kTileBytes);
-      __syncwarp();
-      uint8_t* to = s.ring[st];
-      if (old) {
-        if (lane < boxes)
-          for (int c = 0; c < kSub; ++c)
-            tma_load_4d(to + c * (kTile * 128) + lane * a.box * 128, cached, &s.full[st], c * 64, slot, p.kvh, page);
-      } else if (lane < kSub) {
-        tma_load_4d(to + lane * (kTile * 128), drafted, &s.full[st], lane * 64, 0, p.kvh, p.b);
-      }
-      __syncwarp();
-      ++rc;
-      return true;
     };
     while (ok && next_piece(a, w, p)) {
-      const int t0 = p.t0, n = p.n;
-      if (!tree_wait(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&s.q_full, (uint32_t)(NQ * D * 2 * a.tt * a.group));
-        for (int i = 0; i < NQ; ++i)
-          for (int c = 0; c < kSub; ++c)
-            tma_load_4d(s.q[i] + c * (kTile * 128), &map_q, &s.q_full, c * 64, p.kvh * a.group,
-                        (p.mb * NQ + i) * a.tt, p.b);
+      // 32 boxes in a row, one to a lane, and the 32 after them
+      int first = p.t0 * per_tile, page, slot, next_page, next_slot;
+      look_up(first + lane, page, slot);
+      look_up(first + 32 + lane, next_page, next_slot);
+      if (keys) {
+        if (!tree_wait(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&s.q_full, (uint32_t)(NQ * D * 2 * a.tt * a.group));
+#pragma unroll
+          for (int i = 0; i < NQ * kSub; ++i)
+            tma_load_4d(s.q[i / kSub] + (i % kSub) * (kTile * 128), &map_q, &s.q_full, (i % kSub) * 64,
+                        p.kvh * a.group, (p.mb * NQ + i / kSub) * a.tt, p.b);
+        }
+        __syncwarp();
       }
-      __syncwarp();
       ++uc;
-      ok = load(&map_kc, &map_kn, t0);
-      if constexpr (NQ == 1) {
-        if (ok && n > 1) ok = load(&map_kc, &map_kn, t0 + 1);
-        for (int t = 0; ok && t < n; ++t) {
-          ok = load(&map_vc, &map_vn, t0 + t);
-          if (ok && t + 2 < n) ok = load(&map_kc, &map_kn, t0 + t + 2);
+      for (int t = p.t0; t < p.t0 + p.n; ++t) {
+        const bool old = t < p.tiles - 1;
+        const int boxes = old ? (min(kTile, p.len - t * kTile) + a.box - 1) / a.box : 0;
+        const int at = t * per_tile - first;
+        if (!tree_wait(&empty[st], par ^ 1u, &s.abort, 11)) { ok = false; break; }
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], old ? (uint32_t)(boxes * a.box * D * 2) : kTileBytes);
+        uint8_t* const to = ring + st * kTileBytes;
+        if (old) {
+          for (int i = 0; i < boxes; ++i) {
+            const int pg = __shfl_sync(0xffffffffu, page, at + i), sl = __shfl_sync(0xffffffffu, slot, at + i);
+            if (lane == 0) {
+#pragma unroll
+              for (int c = 0; c < kSub; ++c)
+                tma_load_4d(to + c * (kTile * 128) + i * a.box * 128, cached, &full[st], c * 64, sl, p.kvh, pg);
+            }
+          }
+        } else if (lane == 0) {
+#pragma unroll
+          for (int c = 0; c < kSub; ++c)
+            tma_load_4d(to + c * (kTile * 128), drafted, &full[st], c * 64, 0, p.kvh, p.b);
         }
-      } else {
-        for (int t = 0; ok && t < n; ++t) {
-          ok = load(&map_vc, &map_vn, t0 + t);
-          if (ok && t + 1 < n) ok = load(&map_kc, &map_kn, t0 + t + 1);
+        __syncwarp();
+        if (at + per_tile == 32) {
+          first += 32;
+          page = next_page;
+          slot = next_slot;
+          look_up(first + 32 + lane, next_page, next_slot);
         }
+        ++loads;
+        if (++st == depth) { st = 0; par ^= 1u; }
       }
     }
     if (!ok && lane == 0) {  // let issued copies land before shared memory is released
       const uint64_t begin = globaltimer();
-      if (uc > 0)
+      if (keys && uc > 0)
         while (!mbar_try_wait(&s.q_full, (uc - 1) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
-      for (uint32_t i = rc > kRing ? rc - kRing : 0; i < rc; ++i)
-        while (!mbar_try_wait(&s.full[i % kRing], (i / kRing) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
+      for (uint32_t i = loads > depth ? loads - depth : 0; i < loads; ++i)
+        while (!mbar_try_wait(&full[i % depth], (i / depth) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------ MMA
     if (elect_one()) {
-      uint32_t rc = 0, uc = 0, gt = 0;
+      uint32_t uc = 0, gt = 0;
       bool ok = true;
       Piece p;
-      auto wait_full = [&](uint32_t i, int code) {
-        const bool y = mbar_wait(&s.full[i % kRing], (i / kRing) & 1u, &s.abort, &g_tree_dev_error, code);
+      auto wait_k = [&](uint32_t i) {
+        const bool y = mbar_wait(&s.k_full[i % kRingK], (i / kRingK) & 1u, &s.abort, &g_tree_dev_error, 21);
         tc_fence_after();
         return y;
       };
-      auto issue_s = [&](int g, int qi, uint32_t i) {  // scores of group g from Q tile qi and ring tile i
+      auto wait_v = [&](uint32_t i) {
+        return mbar_wait(&s.v_full[i % kRingV], (i / kRingV) & 1u, &s.abort, &g_tree_dev_error, 22);
+      };
+      auto issue_s = [&](int g, int qi, uint32_t i) {  // scores of group g from Q tile qi and key tile i
         const uint64_t qd = smem_desc_sw128(smem_u32(s.q[qi]), 16, 1024);
-        const uint64_t kd = smem_desc_sw128(smem_u32(s.ring[i % kRing]), 16, 1024);
+        const uint64_t kd = smem_desc_sw128(smem_u32(s.k[i % kRingK]), 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (uint32_t)(((kk >> 2) * (kTile * 128) + (kk & 3) * 32) >> 4);
@@ -373,78 +370,78 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         mma_commit(&s.s_full[g]);
       };
-      auto issue_pv = [&](int g, uint32_t i, bool add, bool two) {  // O of group g (+)= P V
-        const uint64_t vd = smem_desc_sw128(smem_u32(s.ring[i % kRing]), kTile * 128, 1024);
+      // O of group g (+)= P V: the exponentials of 32 keys take 16 of the 32 columns that their
+      // scores had, their second parts the other 16
+      auto issue_pv = [&](int g, uint32_t i, bool add, bool two) {
+        const uint64_t vd = smem_desc_sw128(smem_u32(s.v[i % kRingV]), kTile * 128, 1024);
+        const uint32_t o = tmem + kOCol + (uint32_t)(g * D), pc = tmem + (uint32_t)(g * kTile);
         if (two) {
 #pragma unroll
           for (int kk = 0; kk < kTile / 16; ++kk)
-            mma_bf16_ts(tmem + kOCol + (uint32_t)(g * D), tmem + (uint32_t)(g * kTile + kTile / 2 + kk * 8),
-                        vd + (uint32_t)(kk * 128), kIdescPV, (add || kk > 0) ? 1u : 0u);
+            mma_bf16_ts(o, pc + (uint32_t)((kk >> 1) * 32 + 16 + (kk & 1) * 8), vd + (uint32_t)(kk * 128), kIdescPV,
+                        (add || kk > 0) ? 1u : 0u);
           add = true;
         }
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk)
-          mma_bf16_ts(tmem + kOCol + (uint32_t)(g * D), tmem + (uint32_t)(g * kTile + kk * 8),
-                      vd + (uint32_t)(kk * 128), kIdescPV, (add || kk > 0) ? 1u : 0u);
+          mma_bf16_ts(o, pc + (uint32_t)((kk >> 1) * 32 + (kk & 1) * 8), vd + (uint32_t)(kk * 128), kIdescPV,
+                      (add || kk > 0) ? 1u : 0u);
         mma_commit(&s.o_done[g]);
       };
       while (ok && next_piece(a, w, p)) {
         const int n = p.n;
+        const bool two = p.len <= kFine;
         if (!mbar_wait(&s.q_full, uc & 1u, &s.abort, &g_tree_dev_error, 20)) { ok = false; break; }
         tc_fence_after();
         if constexpr (NQ == 1) {
-          for (int t = 0; ok && t < n && t < 2; ++t) {
-            if (!(ok = wait_full(rc, 21))) break;
-            issue_s((gt + t) & 1, 0, rc);
-            mma_commit(&s.empty[rc % kRing]);
-            ++rc;
+          for (int t = 0; t < n && t < 2; ++t) {
+            const uint32_t G = gt + (uint32_t)t;
+            if (!(ok = wait_k(G))) break;
+            issue_s(G & 1, 0, G);
+            mma_commit(&s.k_empty[G % kRingK]);
           }
           if (ok && n <= 2) mma_commit(&s.q_empty);
           for (int t = 0; ok && t < n; ++t) {
             const uint32_t G = gt + (uint32_t)t;
             const int g = G & 1;
-            if (!(ok = wait_full(rc, 22))) break;
+            if (!(ok = wait_v(G))) break;
             if (t == 0 && !(ok = mbar_wait(&s.o_free[0], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23))) break;
             if (!(ok = mbar_wait(&s.p_full[g], (G >> 1) & 1u, &s.abort, &g_tree_dev_error, 24))) break;
             tc_fence_after();
-            issue_pv(g, rc, t >= 2, p.len <= kFine);
-            mma_commit(&s.empty[rc % kRing]);
-            ++rc;
+            issue_pv(g, G, t >= 2, two);
+            mma_commit(&s.v_empty[G % kRingV]);
             if (t + 2 < n) {  // the scores after next, behind the product that reads their place
-              if (!(ok = wait_full(rc, 25))) break;
-              issue_s(g, 0, rc);
-              mma_commit(&s.empty[rc % kRing]);
-              ++rc;
+              if (!(ok = wait_k(G + 2))) break;
+              issue_s(g, 0, G + 2);
+              mma_commit(&s.k_empty[(G + 2) % kRingK]);
               if (t + 3 == n) mma_commit(&s.q_empty);
             }
           }
         } else {
-          if (!(ok = wait_full(rc, 21))) break;
-          issue_s(0, 0, rc);
-          issue_s(1, 1, rc);
-          mma_commit(&s.empty[rc % kRing]);
-          ++rc;
+          if (!(ok = wait_k(gt))) break;
+          issue_s(0, 0, gt);
+          issue_s(1, 1, gt);
+          mma_commit(&s.k_empty[gt % kRingK]);
           if (n == 1) mma_commit(&s.q_empty);
           for (int t = 0; ok && t < n; ++t) {
             const uint32_t G = gt + (uint32_t)t;
-            if (!(ok = wait_full(rc, 22))) break;
+            if (!(ok = wait_v(G))) break;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               if (t == 0 && !(ok = mbar_wait(&s.o_free[g], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23))) break;
               if (!(ok = mbar_wait(&s.p_full[g], G & 1u, &s.abort, &g_tree_dev_error, 24))) break;
               tc_fence_after();
-              issue_pv(g, rc, t > 0, p.len <= kFine);
-              if (g == 1) mma_commit(&s.empty[rc % kRing]);
+              issue_pv(g, G, t > 0, two);
+              if (g == 1) mma_commit(&s.v_empty[G % kRingV]);
               if (t + 1 < n) {
-                if (g == 0 && !(ok = wait_full(rc + 1, 25))) break;
-                issue_s(g, g, rc + 1);
+                if (g == 0 && !(ok = wait_k(G + 1))) break;
+                issue_s(g, g, G + 1);
                 if (g == 1) {
-                  mma_commit(&s.empty[(rc + 1) % kRing]);
+                  mma_commit(&s.k_empty[(G + 1) % kRingK]);
                   if (t + 2 == n) mma_commit(&s.q_empty);
                 }
               }
             }
-            rc += t + 1 < n ? 2 : 1;
           }
         }
         if (!ok) break;
@@ -464,7 +461,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t lane_off = (uint32_t)(qd * 32) << 16;
     const uint32_t s_addr = tmem + lane_off + (uint32_t)(g * kTile);
     const uint32_t o_addr = tmem + lane_off + kOCol;
-    uint32_t rc = 0, gt = 0, uc = 0;
+    uint32_t gt = 0, uc = 0;
     bool ok = true;
     Piece p;
     while (ok && next_piece(a, w, p)) {
@@ -487,27 +484,42 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         if (!tree_wait(&s.s_full[g], use & 1u, &s.abort, 31)) { ok = false; break; }
         tc_fence_after();
         if (busy) {
-          uint32_t v[kTile];
+          // Loops over 64 columns keep the code short: its first pass is fetched from L2, and
+          // that is what a short call waits for.
+          if (valid < kTile || !old) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {  // scores that the row does not see
+              const int left = valid - 32 * c;
+              const uint32_t keep = old ? (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u)
+                                        : c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+              uint32_t v[32];
+              tmem_ld32(s_addr + 32 * c, v);
+              tmem_wait_ld();
+              reg_fence<32>(v);
 #pragma unroll
-          for (int c = 0; c < kTile; c += 32) tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[c]));
-          tmem_wait_ld();
-          reg_fence<kTile>(v);
-          if (!old) {
-#pragma unroll
-            for (int c = 0; c < kTile; ++c)
-              if (!((seen[c >> 5] >> (c & 31)) & 1u)) v[c] = 0xff800000u;
-          } else if (valid < kTile) {
-#pragma unroll
-            for (int c = 0; c < kTile; ++c)
-              if (c >= valid) v[c] = 0xff800000u;
+              for (int k = 0; k < 32; ++k)
+                if (!((keep >> k) & 1u)) v[k] = 0xff800000u;
+              tmem_st32(s_addr + 32 * c, v);
+            }
+            tmem_wait_st();
           }
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 64) {
+            uint32_t v[64];
+            tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+            tmem_ld32(s_addr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+            tmem_wait_ld();
+            reg_fence<64>(v);
+            float x[4] = {mx, mx, mx, mx};
 #pragma unroll
-          for (int c = 0; c < kTile; c += 8)
+            for (int k = 0; k < 64; k += 8)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mx4[k] = max3f(mx4[k], __uint_as_float(v[c + 2 * k]), __uint_as_float(v[c + 2 * k + 1]));
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+              for (int j = 0; j < 4; ++j)
+                x[j] = max3f(x[j], __uint_as_float(v[k + 2 * j]), __uint_as_float(v[k + 2 * j + 1]));
+            mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          }
+          mx *= a.scale_log2;
           float factor = 1.f;
           if (m == -INFINITY) {
             m = mx;  // nothing seen before: O and l are zero
@@ -515,21 +527,32 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             factor = fast_exp2(m - mx);
             m = mx;
           }
-          f32x2 rs[2];
           const float neg_m = m == -INFINITY ? 0.f : -m;
-          if (p.len <= kFine) {
-            uint32_t hi[kTile / 2], lo[kTile / 2];
-            exp_pack_two<kTile, 2>(v, hi, lo, a.scale_log2, neg_m, rs);
-            tmem_st32(s_addr, hi);
-            tmem_st32(s_addr + 32, hi + 32);
-            tmem_st32(s_addr + 64, lo);
-            tmem_st32(s_addr + 96, lo + 32);
-          } else {
-            exp_pack_rounded<kTile, 2>(v, a.scale_log2, neg_m, rs);
-            tmem_st32(s_addr, v);
-            tmem_st32(s_addr + 32, v + 32);
+          l *= factor;
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 64) {
+            uint32_t v[64];
+            f32x2 rs[2];
+            tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+            tmem_ld32(s_addr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+            tmem_wait_ld();
+            reg_fence<64>(v);
+            if (p.len <= kFine) {
+              uint32_t x[2][32];  // of 32 keys each: 16 words of first parts, 16 of second ones
+              f32x2 r2[2];
+              exp_pack_two<32, 2>(v, x[0], x[0] + 16, a.scale_log2, neg_m, rs);
+              exp_pack_two<32, 2>(v + 32, x[1], x[1] + 16, a.scale_log2, neg_m, r2);
+              rs[0] = f2_add(rs[0], r2[0]);
+              rs[1] = f2_add(rs[1], r2[1]);
+              tmem_st32(s_addr + c, x[0]);
+              tmem_st32(s_addr + c + 32, x[1]);
+            } else {
+              exp_pack_rounded<64, 2>(v, a.scale_log2, neg_m, rs);
+              tmem_st16(s_addr + c, *reinterpret_cast<const uint32_t(*)[16]>(&v[0]));
+              tmem_st16(s_addr + c + 32, *reinterpret_cast<const uint32_t(*)[16]>(&v[16]));
+            }
+            l += (f2_lo(rs[0]) + f2_hi(rs[0])) + (f2_lo(rs[1]) + f2_hi(rs[1]));
           }
-          l = l * factor + ((f2_lo(rs[0]) + f2_hi(rs[0])) + (f2_lo(rs[1]) + f2_hi(rs[1])));
           if (any && __any_sync(0xffffffffu, factor != 1.f)) {
             // O *= factor; it must hold every product before this one
             if (!tree_wait(&s.o_done[g], (use - 1) & 1u, &s.abort, 32)) { ok = false; break; }
@@ -548,20 +571,19 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
           tmem_wait_st();
         }
-        if (!old && (NQ == 1 || g == 0)) {
+        if (!old && (NQ == 1 || g == 0) && qd * 32 < a.tokens) {
           // A product with P = 0 has to leave no trace of a drafted token's v, whatever it
           // holds: the rows of absent tokens are cleared, and infinities and NaN of present
           // ones are cleared and put back at the end for the rows that see them. With two
           // query tiles the first group does it for both: the second group's product is
           // issued after the first one's.
-          const uint32_t i = rc + (uint32_t)v_at<NQ>(t, n);
           if (uc > 0 && !tree_wait(&s.o_free[0], (uc - 1) & 1u, &s.abort, 38)) { ok = false; break; }
           if (NQ == 2 && uc > 0 && !tree_wait(&s.o_free[1], (uc - 1) & 1u, &s.abort, 39)) { ok = false; break; }
-          if (!tree_wait(&s.full[i % kRing], (i / kRing) & 1u, &s.abort, 33)) { ok = false; break; }
-          uint8_t* row_v = s.ring[i % kRing] + r * 128;
+          if (!tree_wait(&s.v_full[G % kRingV], (G / kRingV) & 1u, &s.abort, 33)) { ok = false; break; }
+          uint8_t* row_v = s.v[G % kRingV] + r * 128;
           const bool absent = a.parents && r < a.tokens && a.parents[(int64_t)p.b * a.tokens + r] < -1;
           bool bad = false;
-#pragma unroll
+#pragma unroll 4
           for (int c = 0; c < D / 8; ++c) {
             uint4* at = reinterpret_cast<uint4*>(row_v + (c / 8) * (kTile * 128) + ((c ^ r) & 7) * 16);
             uint4 x = *at;
@@ -588,9 +610,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         if (valid < kTile && (NQ == 1 || g == 0)) {
           // Rows of V past the sequence's end hold whatever the page or the ring held before:
           // they are cleared too.
-          const uint32_t i = rc + (uint32_t)v_at<NQ>(t, n);
-          if (!tree_wait(&s.full[i % kRing], (i / kRing) & 1u, &s.abort, 33)) { ok = false; break; }
-          uint8_t* tile_v = s.ring[i % kRing];
+          if (!tree_wait(&s.v_full[G % kRingV], (G / kRingV) & 1u, &s.abort, 33)) { ok = false; break; }
+          uint8_t* tile_v = s.v[G % kRingV];
           for (int x = valid * 8 + r; x < kTile * 8; x += kTile)
 #pragma unroll
             for (int c = 0; c < kSub; ++c)
@@ -620,9 +641,13 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         s.xm[g][r] = m;
         s.xl[g][r] = l;
         mbar_arrive(&s.x_full);
-        const uint32_t other = last - 1;  // the last tile of the other parity, if the piece has one
-        if (!tree_wait(&s.o_done[last & 1], (last >> 1) & 1u, &s.abort, 35)) { ok = false; break; }
-        if (n > 1 && !tree_wait(&s.o_done[other & 1], (other >> 1) & 1u, &s.abort, 36)) { ok = false; break; }
+        // This group's last product first: with it all products before it are complete, so the
+        // other group's barrier is at most one phase short of the one waited for (a parity says
+        // nothing about a phase two ahead).
+        const uint32_t own = (last & 1u) == (uint32_t)g ? last : last - 1;
+        const uint32_t other = own == last ? last - 1 : last;
+        if ((n > 1 || own == last) && !tree_wait(&s.o_done[g], (own >> 1) & 1u, &s.abort, 35)) { ok = false; break; }
+        if ((n > 1 || other == last) && !tree_wait(&s.o_done[g ^ 1], (other >> 1) & 1u, &s.abort, 36)) { ok = false; break; }
         if (!tree_wait(&s.x_full, uc & 1u, &s.abort, 37)) { ok = false; break; }
         use0 = n > 1 || (last & 1u) == 0u;
         use1 = n > 1 || (last & 1u) == 1u;
@@ -705,7 +730,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       tc_fence_before();
       mbar_arrive(&s.o_free[NQ == 1 ? 0 : g]);
-      rc += 2 * (uint32_t)n;
       gt += (uint32_t)n;
       ++uc;
     }
@@ -727,16 +751,16 @@ __global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant_
   const int b = blockIdx.z, hm = blockIdx.y, hms = a.kv_heads * a.row_blocks;
   const int kvh = hm / a.row_blocks, mb = hm - kvh * a.row_blocks;
   const int share = a.ws_plan[0], n = tree_tiles(a, b);
-  const long long first = (long long)a.ws_plan[1 + b] * hms + (long long)hm * n;
+  const long long first = (long long)a.ws_plan[1 + b] * hms + (long long)hm * (n + kExtra);
   // cuts strictly inside the segment belong to blocks lo .. hi, in a row
-  int lo = (int)(first / share) + 1, hi = (int)((first + n - 1) / share);
+  int lo = (int)(first / share) + 1, hi = (int)((first + n + kExtra - 1) / share);
   while (lo <= hi) {
-    const int off = (int)((long long)lo * share - first), at = snap(off, n, share);
+    const int off = (int)((long long)lo * share - first), at = cut_at(off, n, share);
     if (at > 0 && at < n) break;
     ++lo;
   }
   while (lo <= hi) {
-    const int off = (int)((long long)hi * share - first), at = snap(off, n, share);
+    const int off = (int)((long long)hi * share - first), at = cut_at(off, n, share);
     if (at > 0 && at < n) break;
     --hi;
   }
@@ -793,9 +817,9 @@ TcPlan tc_plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, i
   const int64_t q_tiles = (tokens + p.tt - 1) / p.tt;
   p.nq = q_tiles > 1 ? 2 : 1;
   p.row_blocks = (int)((q_tiles + p.nq - 1) / p.nq);
-  const int64_t seg_tiles = (page * max_pages + kTile - 1) / kTile + 1;
+  const int64_t seg_tiles = (page * max_pages + kTile - 1) / kTile + 1;  // at most
   const int64_t segments = batch * kv_heads * p.row_blocks;
-  if (segments * seg_tiles > 0x7fffffffLL / 2 || kv_heads * p.row_blocks > 65535) return p;
+  if (segments * (seg_tiles + kExtra) > 0x7fffffffLL / 4 || kv_heads * p.row_blocks > 65535) return p;
   p.on = true;
   p.join = seg_tiles > kWhole;
   p.grid = (int)std::min<int64_t>(sm_count(), p.join ? segments * seg_tiles : segments);
@@ -847,7 +871,7 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
     a.ws_o = reinterpret_cast<float4*>(ws + p.o_off);
   }
   a.batch = g.batch; a.tokens = g.tokens; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.group;
-  a.pages = g.pages; a.page = g.page; a.max_pages = g.max_pages;
+  a.pages = g.pages; a.page = g.page; a.max_pages = g.max_pages; a.capacity = g.max_pages * g.page;
   a.tt = p.tt; a.row_blocks = p.row_blocks; a.box = p.box;
   a.boxes_per_page = g.page / p.box;
   a.log_bpp = -1;
