@@ -2,7 +2,8 @@
 // included by tree_attention.cu.
 //
 // A segment is one (sequence, key/value head, block of query rows): its keys are the cached
-// tiles of 128 positions, the last of them partly filled, and one tile of drafted tokens. The
+// tiles of 128 positions, the last of them partly filled, and the drafted tokens, which go into
+// what is left of that last tile if they are few, else into a tile of their own. The
 // lengths are known on the GPU only, so the blocks share the work out there: all segments'
 // tiles, and kExtra more for what a segment costs besides, form one row, of which block c takes
 // [c X, (c + 1) X). A segment that is cut leaves (max, sum, O) per piece in the workspace, and
@@ -15,6 +16,8 @@
 //                   maximum and sum, exponentials rounded to bf16 back into TMEM over the scores
 //   warps 8, 10     TMA: queries and keys, values, each through a ring of tiles; the lanes look
 //                   up the pages, a box of rows of one page each
+//   warp 11         mends tiles that hold more or less than cached rows: drafted tokens put behind
+//                   the last cached row, rows past the end cleared
 //   warp 9          tcgen05.mma, both products: S = Q K^T, O += P V (P from TMEM)
 //   TMEM            S / P of group 0, 1 [0, 128), [128, 256); O of group 0, 1 after them
 // NQ = 1 (rows fit one tile): the groups take the tiles of keys in turn, each with a maximum,
@@ -33,8 +36,9 @@ using namespace sm100;
 __device__ unsigned int g_tree_dev_error = 0;
 
 constexpr int kTile = 128;
-constexpr int kTcThreads = 352;
-constexpr int kKeyWarp = 8, kMmaWarp = 9, kValueWarp = 10;
+constexpr int kTcThreads = 384;
+constexpr int kKeyWarp = 8, kMmaWarp = 9, kValueWarp = 10, kMendWarp = 11;
+constexpr int kFewDrafts = 16;   // so many drafted tokens can share the last cached tile
 constexpr int kWhole = 4;        // segments of up to so many tiles are not cut
 constexpr int kExtra = 1;        // a segment's beginning and end, in tiles
 // Sequences of up to so many cached positions have P in two bf16 parts, P V in two products: a
@@ -46,7 +50,7 @@ constexpr float kLag = 8.f;      // log2 of how far the running maximum may lag
 
 struct TcArgs {
   const int *tables, *lens, *parents;
-  const bf16* v_new;
+  const bf16 *k_new, *v_new;
   int64_t n_b, n_t, n_h;  // its strides
   bf16* out;
   int* ws_plan;    // [0] X, [1..] prefix sums of the sequences' tiles
@@ -57,6 +61,7 @@ struct TcArgs {
   int tt;          // tokens per query tile
   int row_blocks;  // blocks of NQ query tiles
   int box;         // rows of a page fetched by one TMA box
+  int log_bpt;     // log2 of the boxes of a tile
   int boxes_per_page, log_bpp;  // log_bpp < 0: no power of two
   unsigned long long bpp_magic;  // ceil(2^36 / boxes_per_page)
   float scale_log2;
@@ -65,7 +70,15 @@ struct TcArgs {
 __device__ __forceinline__ int tree_len(const TcArgs& a, int b) {
   return min(max(a.lens[b], 0), a.capacity);
 }
-__device__ __forceinline__ int tree_tiles(const TcArgs& a, int b) { return (tree_len(a, b) + kTile - 1) / kTile + 1; }
+// Whether the drafted tokens share the last cached tile of a sequence of this length.
+__device__ __forceinline__ bool tree_shares(const TcArgs& a, int len) {
+  const int rest = len % kTile;
+  return rest != 0 && a.tokens <= kFewDrafts && rest + a.tokens <= kTile;
+}
+__device__ __forceinline__ int tree_tiles(const TcArgs& a, int b) {
+  const int len = tree_len(a, b);
+  return (len + kTile - 1) / kTile + (tree_shares(a, len) ? 0 : 1);
+}
 
 // Where a cut goes that falls `off` into a segment of n tiles (and kExtra before them): to a
 // tile, or to 0 or n when that is near or the segment is short.
@@ -84,6 +97,7 @@ struct Walk {
 };
 struct Piece {
   int b, kvh, mb, t0, n, tiles, len;
+  bool shares;  // the drafted tokens are in the last cached tile
 };
 
 template <int D, int NQ>
@@ -95,13 +109,15 @@ struct TreeSmem {
   uint8_t k[kRingK][kTileBytes];
   uint8_t v[kRingV][kTileBytes];
   uint64_t q_full, q_empty;
-  uint64_t k_full[kRingK], k_empty[kRingK];
-  uint64_t v_full[kRingV], v_empty[kRingV];
+  uint64_t k_full[kRingK], k_empty[kRingK], k_land[kRingK];  // land: the copies of a tile that is mended before it is full
+  uint64_t v_full[kRingV], v_empty[kRingV], v_land[kRingV];
   uint64_t s_full[2], p_full[2], o_done[2], o_free[2];
   uint64_t x_full;
   uint64_t mma_done;
   float xm[2][kTile], xl[2][kTile];  // NQ = 1: the groups' maxima and sums
-  uint32_t bad[4];  // drafted tokens of the piece whose v holds infinities or NaN
+  // Drafted tokens whose v holds infinities or NaN, of the last pieces: products wait for the
+  // end of the piece before, so the mending warp is at most kRingV pieces ahead of a reader.
+  uint32_t bad[8][4];
   uint32_t tmem_base;
   int abort;
 };
@@ -123,6 +139,7 @@ __device__ __forceinline__ bool next_piece(const TcArgs& a, Walk& w, Piece& p) {
   p.tiles = w.tiles;
   p.n = (last ? w.end_t : w.tiles) - w.t;
   p.len = tree_len(a, w.b);
+  p.shares = tree_shares(a, p.len);
   w.t = 0;
   if (last) {
     w.t = w.end_t;
@@ -161,47 +178,39 @@ __device__ __forceinline__ Walk tree_plan(const TcArgs& a, bool leave) {
       before += tree_tiles(a, b) + kExtra;
     }
   }
-  Walk w;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {  // where this block's range begins and ends
-    const int at = ((int)blockIdx.x + k) * share;
-    int b = 0, n = 0, lo = (inc - sum) * hms;
-    const bool mine = at >= lo && at < inc * hms;
-    if (mine) {
-      for (b = b0;; ++b) {
-        n = tree_tiles(a, b);
-        if (at < lo + (n + kExtra) * hms) break;
-        lo += (n + kExtra) * hms;
-      }
+  // Where this block's range begins (even lanes) and ends (odd lanes): the lane whose sequences
+  // hold the place, the sequence among them, the segment of the sequence, the tile of the segment.
+  const int from = (int)blockIdx.x * share, at = from + (lane & 1) * share;
+  const unsigned beyond0 = __ballot_sync(0xffffffffu, inc * hms > from);
+  const unsigned beyond1 = __ballot_sync(0xffffffffu, inc * hms > from + share);
+  const unsigned beyond = (lane & 1) ? beyond1 : beyond0;
+  const int src = beyond ? __ffs(beyond) - 1 : 0;
+  int lo = __shfl_sync(0xffffffffu, inc - sum, src) * hms;
+  int b = a.batch, hm = 0, t = 0, n = 0;
+  if (beyond) {
+    for (b = src * per;; ++b) {
+      n = tree_tiles(a, b);
+      if (at < lo + (n + kExtra) * hms) break;
+      lo += (n + kExtra) * hms;
     }
-    const unsigned who = __ballot_sync(0xffffffffu, mine);
-    const int src = who ? __ffs(who) - 1 : 0;
-    b = who ? __shfl_sync(0xffffffffu, b, src) : a.batch;
-    n = __shfl_sync(0xffffffffu, n, src);
-    lo = __shfl_sync(0xffffffffu, lo, src);
-    int hm = 0, t = 0;
-    if (who) {
-      hm = (at - lo) / (n + kExtra);
-      t = cut_at(at - lo - hm * (n + kExtra), n, share);
-      if (t == n) {
-        t = 0;
-        if (++hm == hms) {
-          hm = 0;
-          if (++b < a.batch) n = tree_tiles(a, b);
-        }
+    hm = (at - lo) / (n + kExtra);
+    t = cut_at(at - lo - hm * (n + kExtra), n, share);
+    if (t == n) {
+      t = 0;
+      if (++hm == hms) {
+        hm = 0;
+        if (++b < a.batch) n = tree_tiles(a, b);
       }
-    }
-    if (k == 0) {
-      w.b = b;
-      w.hm = hm;
-      w.t = t;
-      w.tiles = n;
-    } else {
-      w.end_b = b;
-      w.end_hm = hm;
-      w.end_t = t;
     }
   }
+  Walk w;
+  w.b = __shfl_sync(0xffffffffu, b, 0);
+  w.hm = __shfl_sync(0xffffffffu, hm, 0);
+  w.t = __shfl_sync(0xffffffffu, t, 0);
+  w.tiles = __shfl_sync(0xffffffffu, n, 0);
+  w.end_b = __shfl_sync(0xffffffffu, b, 1);
+  w.end_hm = __shfl_sync(0xffffffffu, hm, 1);
+  w.end_t = __shfl_sync(0xffffffffu, t, 1);
   return w;
 }
 
@@ -233,10 +242,12 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     for (int i = 0; i < kRingK; ++i) {
       mbar_init(&s.k_full[i], 1);
       mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.k_land[i], 1);
     }
     for (int i = 0; i < kRingV; ++i) {
       mbar_init(&s.v_full[i], 1);
       mbar_init(&s.v_empty[i], 1);
+      mbar_init(&s.v_land[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
@@ -274,9 +285,11 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     uint8_t* const ring = keys ? s.k[0] : s.v[0];
     uint64_t* const full = keys ? s.k_full : s.v_full;
     uint64_t* const empty = keys ? s.k_empty : s.v_empty;
+    uint64_t* const land = keys ? s.k_land : s.v_land;
     const uint32_t depth = keys ? kRingK : kRingV;
-    const int per_tile = kTile / a.box;
-    uint32_t st = 0, par = 0, loads = 0, uc = 0;
+    const int per_tile = 1 << a.log_bpt;
+    uint32_t st = 0, par = 0, uc = 0;
+    uint32_t used = 0u, landed = 0u, land_par = 0u;  // per ring place: loaded, last load to be mended, parity of `land`
     bool ok = true;
     Piece p = {};
     // page and first row in it of a box of the piece's sequence
@@ -293,7 +306,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       // 32 boxes in a row, one to a lane, and the 32 after them
       int first = p.t0 * per_tile, page, slot, next_page, next_slot;
       look_up(first + lane, page, slot);
-      look_up(first + 32 + lane, next_page, next_slot);
       if (keys) {
         if (!tree_wait(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
         if (lane == 0) {
@@ -306,12 +318,18 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         __syncwarp();
       }
       ++uc;
+      look_up(first + 32 + lane, next_page, next_slot);
       for (int t = p.t0; t < p.t0 + p.n; ++t) {
-        const bool old = t < p.tiles - 1;
+        const bool old = t * kTile < p.len;
         const int boxes = old ? (min(kTile, p.len - t * kTile) + a.box - 1) / a.box : 0;
         const int at = t * per_tile - first;
         if (!tree_wait(&empty[st], par ^ 1u, &s.abort, 11)) { ok = false; break; }
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], old ? (uint32_t)(boxes * a.box * D * 2) : kTileBytes);
+        const bool mend = keys ? p.shares && t == p.tiles - 1 : (t + 1) * kTile > p.len;
+        uint64_t* const bar = mend ? &land[st] : &full[st];
+        used |= 1u << st;
+        landed = mend ? landed | 1u << st : landed & ~(1u << st);
+        land_par ^= mend ? 1u << st : 0u;
+        if (lane == 0) mbar_arrive_expect_tx(bar, old ? (uint32_t)(boxes * a.box * D * 2) : kTileBytes);
         uint8_t* const to = ring + st * kTileBytes;
         if (old) {
           for (int i = 0; i < boxes; ++i) {
@@ -319,13 +337,13 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (lane == 0) {
 #pragma unroll
               for (int c = 0; c < kSub; ++c)
-                tma_load_4d(to + c * (kTile * 128) + i * a.box * 128, cached, &full[st], c * 64, sl, p.kvh, pg);
+                tma_load_4d(to + c * (kTile * 128) + i * a.box * 128, cached, bar, c * 64, sl, p.kvh, pg);
             }
           }
         } else if (lane == 0) {
 #pragma unroll
           for (int c = 0; c < kSub; ++c)
-            tma_load_4d(to + c * (kTile * 128), drafted, &full[st], c * 64, 0, p.kvh, p.b);
+            tma_load_4d(to + c * (kTile * 128), drafted, bar, c * 64, 0, p.kvh, p.b);
         }
         __syncwarp();
         if (at + per_tile == 32) {
@@ -334,7 +352,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           slot = next_slot;
           look_up(first + 32 + lane, next_page, next_slot);
         }
-        ++loads;
         if (++st == depth) { st = 0; par ^= 1u; }
       }
     }
@@ -342,8 +359,12 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const uint64_t begin = globaltimer();
       if (keys && uc > 0)
         while (!mbar_try_wait(&s.q_full, (uc - 1) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
-      for (uint32_t i = loads > depth ? loads - depth : 0; i < loads; ++i)
-        while (!mbar_try_wait(&full[i % depth], (i / depth) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
+      for (uint32_t i = 0; i < depth; ++i) {  // the last load of each place: this round's below st, the last round's from st on
+        if (!((used >> i) & 1u)) continue;
+        uint64_t* const bar = (landed >> i) & 1u ? &land[i] : &full[i];
+        const uint32_t phase = (landed >> i) & 1u ? ((land_par >> i) & 1u) ^ 1u : i < st ? par : par ^ 1u;
+        while (!mbar_try_wait(bar, phase) && globaltimer() - begin < kWaitTimeoutNs) {}
+      }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
@@ -351,7 +372,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (elect_one()) {
       uint32_t uc = 0, gt = 0;
       bool ok = true;
-      Piece p;
+      Piece p = {};
       auto wait_k = [&](uint32_t i) {
         const bool y = mbar_wait(&s.k_full[i % kRingK], (i / kRingK) & 1u, &s.abort, &g_tree_dev_error, 21);
         tc_fence_after();
@@ -454,6 +475,133 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       while (!mbar_try_wait(&s.mma_done, 0) && globaltimer() - begin < kWaitTimeoutNs) {}
     }
     __syncwarp();
+  } else if (warp == kMendWarp) {
+    // ------------------------------------------------ tiles that are not 128 cached rows
+    uint32_t gt = 0, uc = 0, k_par = 0u, v_par = 0u;  // per ring place: parity of `land`
+    bool ok = true;
+    Piece p;
+    auto chunk = [&](uint8_t* tile, int row, int c) {  // 16 bytes of a row, where the swizzle puts them
+      return reinterpret_cast<uint4*>(tile + (c / 8) * (kTile * 128) + row * 128 + ((c ^ row) & 7) * 16);
+    };
+    // An exponent of all ones among the 8 values: its half's top bit comes out set.
+    auto not_finite = [](const uint4& y) {
+      return (((y.x & 0x7f807f80u) + 0x00800080u) | ((y.y & 0x7f807f80u) + 0x00800080u) |
+              ((y.z & 0x7f807f80u) + 0x00800080u) | ((y.w & 0x7f807f80u) + 0x00800080u)) & 0x80008000u;
+    };
+    auto clear_not_finite = [](uint32_t& x) {
+      const uint32_t hit = ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+      if (hit & 0x8000u) x &= 0xffff0000u;
+      if (hit & 0x80000000u) x &= 0x0000ffffu;
+    };
+    while (ok && next_piece(a, w, p)) {
+      const int* const parents = a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr;
+      for (int tile = max(p.t0, p.len / kTile); tile < p.t0 + p.n; ++tile) {  // the last one or two of the segment
+        const uint32_t G = gt + (uint32_t)(tile - p.t0);
+        const int rest = p.len - tile * kTile;  // cached rows; none: the drafted tokens' own tile
+        const int ki = G % kRingK, vi = G % kRingV;
+        uint8_t* const kt = s.k[ki];
+        uint8_t* const vt = s.v[vi];
+        const uint32_t v_phase = (v_par >> vi) & 1u;
+        v_par ^= 1u << vi;
+        const bool drafts = tile == p.tiles - 1;
+        uint32_t gone[4] = {0u, 0u, 0u, 0u};  // absent tokens
+        if (drafts && parents)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            gone[k] = __ballot_sync(0xffffffffu, 32 * k + lane < a.tokens && parents[32 * k + lane] < -1);
+        // The products with P = 0 have to leave no trace of a drafted token's v, whatever it
+        // holds: absent tokens' rows are cleared, and infinities and NaN of the others are
+        // cleared and put back at the end for the rows that see them.
+        uint32_t bad[4] = {0u, 0u, 0u, 0u};
+        constexpr int kPer = kFewDrafts * (D / 8) / 32;
+        if (drafts && p.shares) {
+          uint4 kx[kPer], vx[kPer];
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int x = i * 32 + lane, row = x / (D / 8);
+            kx[i] = vx[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (row < a.tokens) {
+              const int64_t at = p.b * a.n_b + row * a.n_t + p.kvh * a.n_h + (x % (D / 8)) * 8;
+              kx[i] = *reinterpret_cast<const uint4*>(a.k_new + at);
+              vx[i] = *reinterpret_cast<const uint4*>(a.v_new + at);
+            }
+          }
+          if (!tree_wait(&s.k_land[ki], (k_par >> ki) & 1u, &s.abort, 41)) { ok = false; break; }
+          k_par ^= 1u << ki;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int x = i * 32 + lane, row = x / (D / 8);
+            if (row < a.tokens) *chunk(kt, rest + row, x % (D / 8)) = kx[i];
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.k_full[ki]);
+          if (!tree_wait(&s.v_land[vi], v_phase, &s.abort, 42)) { ok = false; break; }
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int x = i * 32 + lane, row = x / (D / 8);
+            if (row < a.tokens) {
+              if ((gone[0] >> row) & 1u) vx[i] = make_uint4(0u, 0u, 0u, 0u);
+              if (not_finite(vx[i])) {
+                bad[0] |= 1u << row;
+                clear_not_finite(vx[i].x);
+                clear_not_finite(vx[i].y);
+                clear_not_finite(vx[i].z);
+                clear_not_finite(vx[i].w);
+              }
+              *chunk(vt, rest + row, x % (D / 8)) = vx[i];
+            }
+          }
+          bad[0] = __reduce_or_sync(0xffffffffu, bad[0]);
+        } else {
+          if (!tree_wait(&s.v_land[vi], v_phase, &s.abort, 43)) { ok = false; break; }
+          if (drafts) {
+            uint32_t any_bad = 0u;
+#pragma unroll 4
+            for (int x = lane; x < a.tokens * (D / 8); x += 32) {
+              const int row = x / (D / 8);
+              const uint32_t g4 = row < 32 ? gone[0] : row < 64 ? gone[1] : row < 96 ? gone[2] : gone[3];
+              uint4* const at = chunk(vt, row, x % (D / 8));
+              if ((g4 >> (row & 31)) & 1u) *at = make_uint4(0u, 0u, 0u, 0u);
+              else any_bad |= not_finite(*at);
+            }
+            __syncwarp();
+            if (__any_sync(0xffffffffu, any_bad != 0u)) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                bool mine = false;
+#pragma unroll 1
+                for (int c = 0; c < D / 8; ++c) {
+                  uint4* const at = chunk(vt, 32 * k + lane, c);
+                  uint4 y = *at;
+                  if (!not_finite(y)) continue;
+                  mine = true;
+                  clear_not_finite(y.x);
+                  clear_not_finite(y.y);
+                  clear_not_finite(y.z);
+                  clear_not_finite(y.w);
+                  *at = y;
+                }
+                bad[k] = __ballot_sync(0xffffffffu, mine);
+              }
+            }
+          }
+        }
+        if (rest > 0) {  // rows past the end hold whatever the page or the ring held before
+#pragma unroll 4
+          for (int x = (rest + (drafts ? a.tokens : 0)) * 8 + lane; x < kTile * 8; x += 32)
+#pragma unroll
+            for (int c = 0; c < kSub; ++c)
+              *reinterpret_cast<uint4*>(vt + c * (kTile * 128) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        if (drafts && lane < 4) s.bad[uc & 7][lane] = lane == 0 ? bad[0] : lane == 1 ? bad[1] : lane == 2 ? bad[2] : bad[3];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.v_full[vi]);
+      }
+      gt += (uint32_t)p.n;
+      ++uc;
+    }
   } else {
     // ------------------------------------------------ softmax groups
     const int g = warp >> 2, qd = warp & 3;
@@ -478,46 +626,51 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         if (NQ == 1 && (int)(G & 1u) != g) continue;
         const uint32_t use = NQ == 1 ? G >> 1 : G;  // how often the group's buffers were used before
         const int tile = p.t0 + t;
-        const bool old = tile < p.tiles - 1;
-        const int valid = old ? min(kTile, p.len - tile * kTile) : kTile;
-        if (!old && r < rows) ancestor_bits(a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr, token, seen);
+        const int rest = p.len - tile * kTile;  // cached keys of the tile
+        const bool drafts = tile == p.tiles - 1;
+        if (drafts && r < rows) ancestor_bits(a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr, token, seen);
         if (!tree_wait(&s.s_full[g], use & 1u, &s.abort, 31)) { ok = false; break; }
         tc_fence_after();
         if (busy) {
           // Loops over 64 columns keep the code short: its first pass is fetched from L2, and
           // that is what a short call waits for.
-          if (valid < kTile || !old) {
+          float mx = -INFINITY;
+          if (rest < kTile) {
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {  // scores that the row does not see
-              const int left = valid - 32 * c;
-              const uint32_t keep = old ? (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u)
-                                        : c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+            for (int c = 0; c < 4; ++c) {  // with the scores that the row does not see masked
+              const int left = rest - 32 * c;
+              uint32_t keep = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+              if (rest <= 0) keep = c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+              else if (left < 32 && left > -32) keep |= left >= 0 ? seen[0] << left : seen[0] >> -left;
               uint32_t v[32];
               tmem_ld32(s_addr + 32 * c, v);
               tmem_wait_ld();
               reg_fence<32>(v);
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (!((keep >> k) & 1u)) v[k] = 0xff800000u;
+              for (int k = 0; k < 32; k += 2) {
+                v[k] = (keep >> k) & 1u ? v[k] : 0xff800000u;
+                v[k + 1] = (keep >> (k + 1)) & 1u ? v[k + 1] : 0xff800000u;
+                mx = max3f(mx, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+              }
               tmem_st32(s_addr + 32 * c, v);
             }
             tmem_wait_st();
-          }
-          float mx = -INFINITY;
+          } else {
 #pragma unroll 1
-          for (int c = 0; c < kTile; c += 64) {
-            uint32_t v[64];
-            tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-            tmem_ld32(s_addr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-            tmem_wait_ld();
-            reg_fence<64>(v);
-            float x[4] = {mx, mx, mx, mx};
+            for (int c = 0; c < kTile; c += 64) {
+              uint32_t v[64];
+              tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+              tmem_ld32(s_addr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+              tmem_wait_ld();
+              reg_fence<64>(v);
+              float x[4] = {mx, mx, mx, mx};
 #pragma unroll
-            for (int k = 0; k < 64; k += 8)
+              for (int k = 0; k < 64; k += 8)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                x[j] = max3f(x[j], __uint_as_float(v[k + 2 * j]), __uint_as_float(v[k + 2 * j + 1]));
-            mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                for (int j = 0; j < 4; ++j)
+                  x[j] = max3f(x[j], __uint_as_float(v[k + 2 * j]), __uint_as_float(v[k + 2 * j + 1]));
+              mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            }
           }
           mx *= a.scale_log2;
           float factor = 1.f;
@@ -571,53 +724,6 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
           tmem_wait_st();
         }
-        if (!old && (NQ == 1 || g == 0) && qd * 32 < a.tokens) {
-          // A product with P = 0 has to leave no trace of a drafted token's v, whatever it
-          // holds: the rows of absent tokens are cleared, and infinities and NaN of present
-          // ones are cleared and put back at the end for the rows that see them. With two
-          // query tiles the first group does it for both: the second group's product is
-          // issued after the first one's.
-          if (uc > 0 && !tree_wait(&s.o_free[0], (uc - 1) & 1u, &s.abort, 38)) { ok = false; break; }
-          if (NQ == 2 && uc > 0 && !tree_wait(&s.o_free[1], (uc - 1) & 1u, &s.abort, 39)) { ok = false; break; }
-          if (!tree_wait(&s.v_full[G % kRingV], (G / kRingV) & 1u, &s.abort, 33)) { ok = false; break; }
-          uint8_t* row_v = s.v[G % kRingV] + r * 128;
-          const bool absent = a.parents && r < a.tokens && a.parents[(int64_t)p.b * a.tokens + r] < -1;
-          bool bad = false;
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            uint4* at = reinterpret_cast<uint4*>(row_v + (c / 8) * (kTile * 128) + ((c ^ r) & 7) * 16);
-            uint4 x = *at;
-            uint32_t* word = reinterpret_cast<uint32_t*>(&x);
-            bool change = absent;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (absent) {
-                word[k] = 0u;
-              } else {
-                const bool lo = (word[k] & 0x7f80u) == 0x7f80u, hi = (word[k] & 0x7f800000u) == 0x7f800000u;
-                if (lo) word[k] &= 0xffff0000u;
-                if (hi) word[k] &= 0x0000ffffu;
-                bad |= lo || hi;
-                change |= lo || hi;
-              }
-            }
-            if (change) *at = x;
-          }
-          const uint32_t word = __ballot_sync(0xffffffffu, bad);
-          if (lane == 0) s.bad[qd] = word;
-          fence_proxy_async_smem();
-        }
-        if (valid < kTile && (NQ == 1 || g == 0)) {
-          // Rows of V past the sequence's end hold whatever the page or the ring held before:
-          // they are cleared too.
-          if (!tree_wait(&s.v_full[G % kRingV], (G / kRingV) & 1u, &s.abort, 33)) { ok = false; break; }
-          uint8_t* tile_v = s.v[G % kRingV];
-          for (int x = valid * 8 + r; x < kTile * 8; x += kTile)
-#pragma unroll
-            for (int c = 0; c < kSub; ++c)
-              *reinterpret_cast<uint4*>(tile_v + c * (kTile * 128) + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_smem();
-        }
         tc_fence_before();
         mbar_arrive(&s.p_full[g]);
         any = true;
@@ -666,7 +772,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       uint32_t sees_bad[4] = {0u, 0u, 0u, 0u};  // drafted tokens that bring infinities or NaN to this row
       if (p.t0 + n == p.tiles) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sees_bad[k] = r < rows ? seen[k] & s.bad[k] : 0u;
+        for (int k = 0; k < 4; ++k) sees_bad[k] = r < rows ? seen[k] & s.bad[uc & 7][k] : 0u;
       }
       if (busy) {
         const int ti = NQ == 1 ? 0 : g;
@@ -860,6 +966,7 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
   a.tables = g.tables;
   a.lens = g.lens;
   a.parents = g.parents;
+  a.k_new = static_cast<const bf16*>(g.k_new);
   a.v_new = static_cast<const bf16*>(g.v_new);
   a.n_b = g.n_b;
   a.n_t = g.n_t;
@@ -874,6 +981,8 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
   a.pages = g.pages; a.page = g.page; a.max_pages = g.max_pages; a.capacity = g.max_pages * g.page;
   a.tt = p.tt; a.row_blocks = p.row_blocks; a.box = p.box;
   a.boxes_per_page = g.page / p.box;
+  a.log_bpt = 0;
+  while (p.box << a.log_bpt < kTile) ++a.log_bpt;
   a.log_bpp = -1;
   for (int i = 0; i < 9; ++i)
     if (a.boxes_per_page == 1 << i) a.log_bpp = i;
