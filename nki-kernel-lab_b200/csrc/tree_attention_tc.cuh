@@ -21,9 +21,10 @@
 //   warp 9          tcgen05.mma, both products: S = Q K^T, O += P V (P from TMEM)
 //   TMEM            S / P of group 0, 1 [0, 128), [128, 256); O of group 0, 1 after them
 // NQ = 1 (rows fit one tile): the groups take the tiles of keys in turn, each with a maximum,
-// sum and O of its own, joined at the end of the segment's piece; while one exponentiates, the
-// tensor core fills the other's scores. NQ = 2: each group has its own tile of rows, and both
-// meet the same keys, which so cross shared memory's boundary once for 256 rows.
+// sum and O of its own, joined at the end of the segment's piece. NQ = 2: each group has its own
+// tile of rows, and both meet the same keys, which so cross shared memory's boundary once for
+// 256 rows. P of a tile is handed over in two halves of 64 keys, so that the first half's product
+// with V runs while the second half is exponentiated.
 //
 // The running maximum may lag behind by up to 2^8: O is rescaled only when a row's maximum
 // grows by more than that. P is then up to 2^8 instead of 1, with the same relative rounding.
@@ -40,7 +41,8 @@ constexpr int kTcThreads = 384;
 constexpr int kKeyWarp = 8, kMmaWarp = 9, kValueWarp = 10, kMendWarp = 11;
 constexpr int kFewDrafts = 16;   // so many drafted tokens can share the last cached tile
 constexpr int kWhole = 4;        // segments of up to so many tiles are not cut
-constexpr int kExtra = 1;        // a segment's beginning and end, in tiles
+constexpr int kMaxPieces = 192;  // of one segment: at most one for each block and one more
+constexpr int kExtra = 3;        // a segment's beginning and end, in tiles
 // Sequences of up to so many cached positions have P in two bf16 parts, P V in two products: a
 // row that sees few keys does not average the roundings of P out (one part: up to 2^-8 of a
 // weight). The second product is hidden behind the loads there is time for; on long rows,
@@ -111,7 +113,8 @@ struct TreeSmem {
   uint64_t q_full, q_empty;
   uint64_t k_full[kRingK], k_empty[kRingK], k_land[kRingK];  // land: the copies of a tile that is mended before it is full
   uint64_t v_full[kRingV], v_empty[kRingV], v_land[kRingV];
-  uint64_t s_full[2], p_full[2], o_done[2], o_free[2];
+  uint64_t s_full[2], p_full[2][2], o_done[2][2];  // [group][half of the tile]
+  uint64_t o_free[2];
   uint64_t x_full;
   uint64_t mma_done;
   float xm[2][kTile], xl[2][kTile];  // NQ = 1: the groups' maxima and sums
@@ -251,8 +254,10 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], kTile);
-      mbar_init(&s.o_done[i], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s.p_full[i][h], kTile);
+        mbar_init(&s.o_done[i][h], 1);
+      }
       mbar_init(&s.o_free[i], NQ == 1 ? 2 * kTile : kTile);
     }
     mbar_init(&s.x_full, 2 * kTile);
@@ -371,19 +376,28 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // ------------------------------------------------ MMA
     if (elect_one()) {
       uint32_t uc = 0, gt = 0;
+      uint32_t kt = 0, k_par = 0, vt = 0, v_par = 0;  // the rings' next places
       bool ok = true;
       Piece p = {};
-      auto wait_k = [&](uint32_t i) {
-        const bool y = mbar_wait(&s.k_full[i % kRingK], (i / kRingK) & 1u, &s.abort, &g_tree_dev_error, 21);
+      constexpr uint32_t kStep = kTileBytes >> 4;  // from one place of a ring to the next, in a descriptor
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(s.q[0]), 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(smem_u32(s.k[0]), 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(smem_u32(s.v[0]), kTile * 128, 1024);
+      auto wait_k = [&]() {
+        const bool y = mbar_wait(&s.k_full[kt], k_par, &s.abort, &g_tree_dev_error, 21);
         tc_fence_after();
         return y;
       };
-      auto wait_v = [&](uint32_t i) {
-        return mbar_wait(&s.v_full[i % kRingV], (i / kRingV) & 1u, &s.abort, &g_tree_dev_error, 22);
+      auto free_k = [&]() {
+        mma_commit(&s.k_empty[kt]);
+        if (++kt == kRingK) { kt = 0; k_par ^= 1u; }
       };
-      auto issue_s = [&](int g, int qi, uint32_t i) {  // scores of group g from Q tile qi and key tile i
-        const uint64_t qd = smem_desc_sw128(smem_u32(s.q[qi]), 16, 1024);
-        const uint64_t kd = smem_desc_sw128(smem_u32(s.k[i % kRingK]), 16, 1024);
+      auto free_v = [&]() {
+        mma_commit(&s.v_empty[vt]);
+        if (++vt == kRingV) { vt = 0; v_par ^= 1u; }
+      };
+      auto issue_s = [&](int g, int qi) {  // scores of group g: Q tile qi, the next key tile
+        const uint64_t qd = q_desc + (uint32_t)qi * kStep, kd = k_desc + kt * kStep;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = (uint32_t)(((kk >> 2) * (kTile * 128) + (kk & 3) * 32) >> 4);
@@ -391,79 +405,59 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         mma_commit(&s.s_full[g]);
       };
-      // O of group g (+)= P V: the exponentials of 32 keys take 16 of the 32 columns that their
-      // scores had, their second parts the other 16
-      auto issue_pv = [&](int g, uint32_t i, bool add, bool two) {
-        const uint64_t vd = smem_desc_sw128(smem_u32(s.v[i % kRingV]), kTile * 128, 1024);
-        const uint32_t o = tmem + kOCol + (uint32_t)(g * D), pc = tmem + (uint32_t)(g * kTile);
+      // O of group g (+)= P V over half h of the next value tile: the exponentials of 32 keys
+      // take 16 of the 32 columns that their scores had, their second parts the other 16.
+      auto issue_pv = [&](int g, int h, bool add, bool two) {
+        const uint64_t vd = v_desc + vt * kStep + (uint32_t)(h * (kTile / 2 * 128) >> 4);
+        const uint32_t o = tmem + kOCol + (uint32_t)(g * D), pc = tmem + (uint32_t)(g * kTile + h * (kTile / 2));
         if (two) {
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
+          for (int kk = 0; kk < kTile / 32; ++kk)
             mma_bf16_ts(o, pc + (uint32_t)((kk >> 1) * 32 + 16 + (kk & 1) * 8), vd + (uint32_t)(kk * 128), kIdescPV,
                         (add || kk > 0) ? 1u : 0u);
           add = true;
         }
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
+        for (int kk = 0; kk < kTile / 32; ++kk)
           mma_bf16_ts(o, pc + (uint32_t)((kk >> 1) * 32 + (kk & 1) * 8), vd + (uint32_t)(kk * 128), kIdescPV,
                       (add || kk > 0) ? 1u : 0u);
-        mma_commit(&s.o_done[g]);
+        mma_commit(&s.o_done[g][h]);
       };
       while (ok && next_piece(a, w, p)) {
         const int n = p.n;
         const bool two = p.len <= kFine;
         if (!mbar_wait(&s.q_full, uc & 1u, &s.abort, &g_tree_dev_error, 20)) { ok = false; break; }
         tc_fence_after();
-        if constexpr (NQ == 1) {
-          for (int t = 0; t < n && t < 2; ++t) {
+        // t = -2 .. n - 1 (NQ = 1), -1 .. n - 1 (NQ = 2): P V of tile t, and the scores of the tile
+        // whose place that frees
+        constexpr int kAhead = NQ == 1 ? 2 : 1;
+#pragma unroll 1
+        for (int t = -kAhead; ok && t < n; ++t) {
+          const bool more = t + kAhead < n;
+          if (t >= 0 && !(ok = mbar_wait(&s.v_full[vt], v_par, &s.abort, &g_tree_dev_error, 22))) break;
+#pragma unroll 1
+          for (int i = 0; i < NQ; ++i) {
             const uint32_t G = gt + (uint32_t)t;
-            if (!(ok = wait_k(G))) break;
-            issue_s(G & 1, 0, G);
-            mma_commit(&s.k_empty[G % kRingK]);
-          }
-          if (ok && n <= 2) mma_commit(&s.q_empty);
-          for (int t = 0; ok && t < n; ++t) {
-            const uint32_t G = gt + (uint32_t)t;
-            const int g = G & 1;
-            if (!(ok = wait_v(G))) break;
-            if (t == 0 && !(ok = mbar_wait(&s.o_free[0], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23))) break;
-            if (!(ok = mbar_wait(&s.p_full[g], (G >> 1) & 1u, &s.abort, &g_tree_dev_error, 24))) break;
-            tc_fence_after();
-            issue_pv(g, G, t >= 2, two);
-            mma_commit(&s.v_empty[G % kRingV]);
-            if (t + 2 < n) {  // the scores after next, behind the product that reads their place
-              if (!(ok = wait_k(G + 2))) break;
-              issue_s(g, 0, G + 2);
-              mma_commit(&s.k_empty[(G + 2) % kRingK]);
-              if (t + 3 == n) mma_commit(&s.q_empty);
-            }
-          }
-        } else {
-          if (!(ok = wait_k(gt))) break;
-          issue_s(0, 0, gt);
-          issue_s(1, 1, gt);
-          mma_commit(&s.k_empty[gt % kRingK]);
-          if (n == 1) mma_commit(&s.q_empty);
-          for (int t = 0; ok && t < n; ++t) {
-            const uint32_t G = gt + (uint32_t)t;
-            if (!(ok = wait_v(G))) break;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              if (t == 0 && !(ok = mbar_wait(&s.o_free[g], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23))) break;
-              if (!(ok = mbar_wait(&s.p_full[g], G & 1u, &s.abort, &g_tree_dev_error, 24))) break;
+            const int g = NQ == 1 ? (int)(G & 1u) : i;
+            const uint32_t use = NQ == 1 ? G >> 1 : G;
+            if (t == 0 &&
+                !(ok = mbar_wait(&s.o_free[i], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23)))
+              break;
+            for (int h = 0; t >= 0 && h < 2; ++h) {
+              if (!(ok = mbar_wait(&s.p_full[g][h], use & 1u, &s.abort, &g_tree_dev_error, 24))) break;
               tc_fence_after();
-              issue_pv(g, G, t > 0, two);
-              if (g == 1) mma_commit(&s.v_empty[G % kRingV]);
-              if (t + 1 < n) {
-                if (g == 0 && !(ok = wait_k(G + 1))) break;
-                issue_s(g, g, G + 1);
-                if (g == 1) {
-                  mma_commit(&s.k_empty[(G + 1) % kRingK]);
-                  if (t + 2 == n) mma_commit(&s.q_empty);
-                }
-              }
+              issue_pv(g, h, t >= kAhead || h > 0, two);
+            }
+            if (!ok) break;
+            if (more) {
+              if (i == 0 && !(ok = wait_k())) break;
+              issue_s(g, NQ == 1 ? 0 : i);
             }
           }
+          if (!ok) break;
+          if (t >= 0) free_v();
+          if (more) free_k();
+          if (t + kAhead == n - 1) mma_commit(&s.q_empty);
         }
         if (!ok) break;
         gt += (uint32_t)n;
@@ -631,101 +625,83 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         if (drafts && r < rows) ancestor_bits(a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr, token, seen);
         if (!tree_wait(&s.s_full[g], use & 1u, &s.abort, 31)) { ok = false; break; }
         tc_fence_after();
-        if (busy) {
-          // Loops over 64 columns keep the code short: its first pass is fetched from L2, and
-          // that is what a short call waits for.
-          float mx = -INFINITY;
-          if (rest < kTile) {
+        // A loop and not straight code for the halves: the code's first pass is fetched from L2,
+        // and that is what a short call waits for.
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {  // with the scores that the row does not see masked
-              const int left = rest - 32 * c;
-              uint32_t keep = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
-              if (rest <= 0) keep = c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
-              else if (left < 32 && left > -32) keep |= left >= 0 ? seen[0] << left : seen[0] >> -left;
-              uint32_t v[32];
-              tmem_ld32(s_addr + 32 * c, v);
-              tmem_wait_ld();
-              reg_fence<32>(v);
-#pragma unroll
-              for (int k = 0; k < 32; k += 2) {
-                v[k] = (keep >> k) & 1u ? v[k] : 0xff800000u;
-                v[k + 1] = (keep >> (k + 1)) & 1u ? v[k + 1] : 0xff800000u;
-                mx = max3f(mx, __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
-              }
-              tmem_st32(s_addr + 32 * c, v);
-            }
-            tmem_wait_st();
-          } else {
-#pragma unroll 1
-            for (int c = 0; c < kTile; c += 64) {
-              uint32_t v[64];
-              tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-              tmem_ld32(s_addr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-              tmem_wait_ld();
-              reg_fence<64>(v);
-              float x[4] = {mx, mx, mx, mx};
-#pragma unroll
-              for (int k = 0; k < 64; k += 8)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  x[j] = max3f(x[j], __uint_as_float(v[k + 2 * j]), __uint_as_float(v[k + 2 * j + 1]));
-              mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            }
-          }
-          mx *= a.scale_log2;
-          float factor = 1.f;
-          if (m == -INFINITY) {
-            m = mx;  // nothing seen before: O and l are zero
-          } else if (mx > m + kLag) {
-            factor = fast_exp2(m - mx);
-            m = mx;
-          }
-          const float neg_m = m == -INFINITY ? 0.f : -m;
-          l *= factor;
-#pragma unroll 1
-          for (int c = 0; c < kTile; c += 64) {
+        for (int h = 0; h < 2; ++h) {
+          if (busy) {
+            const uint32_t half = s_addr + (uint32_t)(h * (kTile / 2));
             uint32_t v[64];
-            f32x2 rs[2];
-            tmem_ld32(s_addr + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-            tmem_ld32(s_addr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+            tmem_ld32(half, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+            tmem_ld32(half + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
             tmem_wait_ld();
             reg_fence<64>(v);
+            const int left = rest - 64 * h;  // cached keys of this half
+            if (left < 64) {
+              uint32_t keep[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int x = left - 32 * c;
+                keep[c] = x >= 32 ? 0xffffffffu : x > 0 ? (1u << x) - 1u : 0u;
+                if (rest <= 0) keep[c] = h == 0 ? seen[c] : seen[2 + c];
+                else if (x < 32 && x > -32) keep[c] |= x >= 0 ? seen[0] << x : seen[0] >> -x;
+              }
+#pragma unroll
+              for (int k = 0; k < 64; ++k) v[k] = (keep[k >> 5] >> (k & 31)) & 1u ? v[k] : 0xff800000u;
+            }
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int k = 0; k < 64; k += 8)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                x[j] = max3f(x[j], __uint_as_float(v[k + 2 * j]), __uint_as_float(v[k + 2 * j + 1]));
+            const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
+            float factor = 1.f;
+            if (m == -INFINITY) {
+              m = mx;  // nothing seen before: O and l are zero
+            } else if (mx > m + kLag) {
+              factor = fast_exp2(m - mx);
+              m = mx;
+            }
+            const float neg_m = m == -INFINITY ? 0.f : -m;
+            f32x2 rs[2];
             if (p.len <= kFine) {
-              uint32_t x[2][32];  // of 32 keys each: 16 words of first parts, 16 of second ones
+              uint32_t y[2][32];  // of 32 keys each: 16 words of first parts, 16 of second ones
               f32x2 r2[2];
-              exp_pack_two<32, 2>(v, x[0], x[0] + 16, a.scale_log2, neg_m, rs);
-              exp_pack_two<32, 2>(v + 32, x[1], x[1] + 16, a.scale_log2, neg_m, r2);
+              exp_pack_two<32, 2>(v, y[0], y[0] + 16, a.scale_log2, neg_m, rs);
+              exp_pack_two<32, 2>(v + 32, y[1], y[1] + 16, a.scale_log2, neg_m, r2);
               rs[0] = f2_add(rs[0], r2[0]);
               rs[1] = f2_add(rs[1], r2[1]);
-              tmem_st32(s_addr + c, x[0]);
-              tmem_st32(s_addr + c + 32, x[1]);
+              tmem_st32(half, y[0]);
+              tmem_st32(half + 32, y[1]);
             } else {
               exp_pack_rounded<64, 2>(v, a.scale_log2, neg_m, rs);
-              tmem_st16(s_addr + c, *reinterpret_cast<const uint32_t(*)[16]>(&v[0]));
-              tmem_st16(s_addr + c + 32, *reinterpret_cast<const uint32_t(*)[16]>(&v[16]));
+              tmem_st16(half, *reinterpret_cast<const uint32_t(*)[16]>(&v[0]));
+              tmem_st16(half + 32, *reinterpret_cast<const uint32_t(*)[16]>(&v[16]));
             }
-            l += (f2_lo(rs[0]) + f2_hi(rs[0])) + (f2_lo(rs[1]) + f2_hi(rs[1]));
-          }
-          if (any && __any_sync(0xffffffffu, factor != 1.f)) {
-            // O *= factor; it must hold every product before this one
-            if (!tree_wait(&s.o_done[g], (use - 1) & 1u, &s.abort, 32)) { ok = false; break; }
-            tc_fence_after();
-            tmem_wait_st();
+            l = l * factor + ((f2_lo(rs[0]) + f2_hi(rs[0])) + (f2_lo(rs[1]) + f2_hi(rs[1])));
+            if ((any || h > 0) && __any_sync(0xffffffffu, factor != 1.f)) {
+              // O *= factor; it must hold every product before this one
+              if (!tree_wait(&s.o_done[g][h ^ 1], (h ? use : use - 1) & 1u, &s.abort, 32)) { ok = false; break; }
+              tc_fence_after();
+              tmem_wait_st();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + (uint32_t)(g * D + c), o);
-              tmem_wait_ld();
-              reg_fence<32>(o);
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + (uint32_t)(g * D + c), o);
+                tmem_wait_ld();
+                reg_fence<32>(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-              tmem_st32(o_addr + (uint32_t)(g * D + c), o);
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                tmem_st32(o_addr + (uint32_t)(g * D + c), o);
+              }
             }
+            tmem_wait_st();
           }
-          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&s.p_full[g][h]);
         }
-        tc_fence_before();
-        mbar_arrive(&s.p_full[g]);
+        if (!ok) break;
         any = true;
       }
       if (!ok) break;
@@ -752,8 +728,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         // nothing about a phase two ahead).
         const uint32_t own = (last & 1u) == (uint32_t)g ? last : last - 1;
         const uint32_t other = own == last ? last - 1 : last;
-        if ((n > 1 || own == last) && !tree_wait(&s.o_done[g], (own >> 1) & 1u, &s.abort, 35)) { ok = false; break; }
-        if ((n > 1 || other == last) && !tree_wait(&s.o_done[g ^ 1], (other >> 1) & 1u, &s.abort, 36)) { ok = false; break; }
+        if ((n > 1 || own == last) && !tree_wait(&s.o_done[g][1], (own >> 1) & 1u, &s.abort, 35)) { ok = false; break; }
+        if ((n > 1 || other == last) && !tree_wait(&s.o_done[g ^ 1][1], (other >> 1) & 1u, &s.abort, 36)) { ok = false; break; }
         if (!tree_wait(&s.x_full, uc & 1u, &s.abort, 37)) { ok = false; break; }
         use0 = n > 1 || (last & 1u) == 0u;
         use1 = n > 1 || (last & 1u) == 1u;
@@ -765,7 +741,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         c0 = g * (D / 2);
         c1 = c0 + D / 2;
       } else {
-        if (!tree_wait(&s.o_done[g], last & 1u, &s.abort, 35)) { ok = false; break; }
+        if (!tree_wait(&s.o_done[g][1], last & 1u, &s.abort, 35)) { ok = false; break; }
       }
       tc_fence_after();
       const float inv = cut ? 1.f : here ? 1.f / l : 0.f;
@@ -871,30 +847,51 @@ __global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant_
     --hi;
   }
   if (lo > hi) return;
-  const int x = blockIdx.x * 8 + (threadIdx.x & 7), c4 = threadIdx.x >> 3;
-  const int ti = x / kTile, r = x - ti * kTile;
+  const int pieces = hi - lo + 2;  // piece 0 is the end of block lo - 1, piece i the beginning of block lo - 1 + i
+  const int x0 = blockIdx.x * 8;   // the block's rows, all of one query tile
+  const int ti = x0 / kTile, r0 = x0 - ti * kTile;
+  auto slot = [&](int i) { return (int64_t)((i == 0 ? 2 * (lo - 1) + 1 : 2 * (lo - 1 + i)) * NQ + ti); };
+  // The pieces' weights 2^(m_p - m) for the 8 rows, and 1 / sum_p 2^(m_p - m) l_p.
+  __shared__ float weight[kMaxPieces][8];
+  __shared__ float inverse[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int y = warp; y < 8; y += 2 * D / 32) {
+    const int r = r0 + y;
+    float m = -INFINITY, l = 0.f, mi[kMaxPieces / 32];
+#pragma unroll
+    for (int k = 0; k < kMaxPieces / 32; ++k) {
+      const int i = k * 32 + lane;
+      mi[k] = i < pieces ? __ldcg(a.ws_ml + slot(i) * 2 * kTile + r) : -INFINITY;
+      m = fmaxf(m, mi[k]);
+    }
+    m = warp_max(m);
+#pragma unroll
+    for (int k = 0; k < kMaxPieces / 32; ++k) {
+      const int i = k * 32 + lane;
+      if (i >= pieces) continue;
+      const float wi = mi[k] == -INFINITY ? 0.f : fast_exp2(mi[k] - m);  // 0: nothing of the piece is visible
+      weight[i][y] = wi;
+      l += wi == 0.f ? 0.f : wi * __ldcg(a.ws_ml + slot(i) * 2 * kTile + kTile + r);
+    }
+    l = warp_sum(l);
+    if (lane == 0) inverse[y] = 1.f / l;
+  }
+  __syncthreads();
+  const int r = r0 + (threadIdx.x & 7), c4 = threadIdx.x >> 3;
   const int token = (mb * NQ + ti) * a.tt + r / a.group;
   if (r >= a.tt * a.group || token >= a.tokens) return;
-  const int pieces = hi - lo + 2;  // piece 0 is the end of block lo - 1, piece i the beginning of block lo - 1 + i
-  auto slot = [&](int i) { return (int64_t)((i == 0 ? 2 * (lo - 1) + 1 : 2 * (lo - 1 + i)) * NQ + ti); };
-  float m = -INFINITY;
-  for (int i = 0; i < pieces; ++i) m = fmaxf(m, __ldcg(a.ws_ml + slot(i) * 2 * kTile + r));
-  float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
   for (int i = 0; i < pieces; ++i) {
-    const float mi = __ldcg(a.ws_ml + slot(i) * 2 * kTile + r), li = __ldcg(a.ws_ml + slot(i) * 2 * kTile + kTile + r);
     const float4 v = __ldcg(a.ws_o + (slot(i) * (D / 4) + c4) * kTile + r);
-    if (mi == -INFINITY) continue;  // nothing of this piece is visible
-    const float wi = fast_exp2(mi - m);
-    l = fmaf(wi, li, l);
-    o.x = fmaf(wi, v.x, o.x);
-    o.y = fmaf(wi, v.y, o.y);
-    o.z = fmaf(wi, v.z, o.z);
-    o.w = fmaf(wi, v.w, o.w);
+    const float wi = weight[i][threadIdx.x & 7];
+    o.x = wi == 0.f ? o.x : fmaf(wi, v.x, o.x);
+    o.y = wi == 0.f ? o.y : fmaf(wi, v.y, o.y);
+    o.z = wi == 0.f ? o.z : fmaf(wi, v.z, o.z);
+    o.w = wi == 0.f ? o.w : fmaf(wi, v.w, o.w);
   }
   const bool here = !a.parents || a.parents[(int64_t)b * a.tokens + token] >= -1;
-  const float inv = here ? 1.f / l : 0.f;
+  const float inv = here ? inverse[threadIdx.x & 7] : 0.f;
   if (!here) o = make_float4(0.f, 0.f, 0.f, 0.f);
   store4(a.out + (((int64_t)b * a.tokens + token) * a.heads + kvh * a.group + r % a.group) * D + c4 * 4,
          make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -928,7 +925,7 @@ TcPlan tc_plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, i
   if (segments * (seg_tiles + kExtra) > 0x7fffffffLL / 4 || kv_heads * p.row_blocks > 65535) return p;
   p.on = true;
   p.join = seg_tiles > kWhole;
-  p.grid = (int)std::min<int64_t>(sm_count(), p.join ? segments * seg_tiles : segments);
+  p.grid = (int)std::min<int64_t>(std::min(sm_count(), kMaxPieces - 1), p.join ? segments * seg_tiles : segments);
   if (p.join) {
     const size_t slots = 2 * (size_t)p.grid * p.nq;
     p.ml_off = ((size_t)(batch + 1) * 4 + 255) & ~size_t(255);
