@@ -18,8 +18,7 @@ There is no CPU implementation: a CPU tensor is an error, never a fallback.
 """
 from __future__ import annotations
 
-import ctypes
-import functools
+import os
 
 import torch
 
@@ -334,284 +333,29 @@ def _(q, k, v, out, scale):
 
 # --------------------------------------------------------------------------- decoding
 # Attention of drafted tokens over a paged cache, the cache's page operations, and the
-# verification of drafted tokens. A decoding loop makes these calls once per layer or step on
-# little data, so they are registered by schema (a call costs a few microseconds of host time
-# less than a custom_op's).
+# verification of drafted tokens: registered in C++ (csrc/torch_ops.cpp), because a decoding
+# loop makes these calls on little data and the host's time bounds it.
 
-_LIB = torch.library.Library("nkilab", "FRAGMENT")
-_Strides3 = ctypes.c_int64 * 3
-_Strides4 = ctypes.c_int64 * 4
-
-
-def _op(schema: str, fake):
-    """Registers the decorated function as a CUDA op of the nkilab namespace."""
-    name = schema.split("(")[0]
-
-    def add(fn):
-        _LIB.define(schema)
-        _LIB.impl(name, fn, "CUDA")
-        torch.library.register_fake("nkilab::" + name, fake, lib=_LIB)
-        return fn
-
-    return add
+TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libnkilab_torch.so")
+if not os.path.exists(TORCH_LIB_PATH):
+    raise ImportError(f"libnkilab_torch.so is not built at {TORCH_LIB_PATH}; build it with `make -C nki-kernel-lab_b200`")
+torch.ops.load_library(TORCH_LIB_PATH)
 
 
-def _ints(dev: torch.device, shape: tuple, **arrays) -> None:
-    """Each array (None allowed) is a dense int32 tensor of this shape on the device."""
-    for name, t in arrays.items():
-        if t is None:
-            continue
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32, got {t.dtype}")
-        if t.device != dev:
-            raise RuntimeError(f"{name} is on {t.device}, not on {dev}")
-        if t.shape != shape:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        if not t.is_contiguous():
-            raise RuntimeError(f"{name} must be contiguous")
+def _like(*ts):
+    out = tuple(t.new_empty(t.shape) for t in ts)
+    return out if len(out) > 1 else out[0]
 
 
-def _rows16(t: torch.Tensor) -> bool:
-    """Whether t's rows are contiguous and 16-byte aligned, so that a kernel can read it as it lies."""
-    per = 16 // t.element_size()
-    st = t.stride()
-    return st[-1] == 1 and t.data_ptr() % 16 == 0 and not any(s % per for s in st[:-1])
-
-
-def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dims: int):
-    if k_cache.dim() != dims or k_cache.shape != v_cache.shape:
-        raise ValueError(f"caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)}: need equal shapes of {dims} dimensions")
-    if k_cache.dtype != v_cache.dtype or k_cache.device != v_cache.device:
-        raise TypeError("k and v caches differ in dtype or device")
-    if k_cache.stride() != v_cache.stride() or k_cache.stride(-1) != 1:
-        raise RuntimeError("caches need equal strides and contiguous rows")
-    return k_cache.device, dtype_code(k_cache)
-
-
-def _stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
-
-
-class _on:
-    """torch.cuda.device(dev) for the case that it changes something; most calls are already there."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, dev):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-@functools.lru_cache(maxsize=1024)
-def _tree_workspace_bytes(device: int, *sizes) -> int:
-    return N.lib.nkl_attention_tree_workspace_size(*sizes)
-
-
-@_op("attention_tree(Tensor q, Tensor k, Tensor v, Tensor k_cache, Tensor v_cache, Tensor tables, Tensor lens, "
-     "Tensor? parents, float scale) -> Tensor",
-     lambda q, k, v, k_cache, v_cache, tables, lens, parents, scale: q.new_empty(q.shape))
-def _attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents, scale):
-    dev, dt = _caches(k_cache, v_cache, 4)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: need [B, T, heads, head_dim]")
-    B, T, H, d = q.shape
-    P, Hkv, page, dc = k_cache.shape
-    if k.shape != (B, T, Hkv, d) or dc != d or H % Hkv:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, cache {tuple(k_cache.shape)}: sizes do not match, "
-                         "or the cache's heads do not divide q's")
-    for t in (q, k, v):
-        if t.dtype != k_cache.dtype:
-            raise TypeError(f"mixed dtypes: {t.dtype} vs {k_cache.dtype}")
-        if t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {t.device} vs {dev}")
-    if T > N.MAX_DRAFTED:
-        raise ValueError(f"{T} drafted tokens, at most {N.MAX_DRAFTED} are taken")
-    if tables.dim() != 2 or tables.shape[1] < 1:
-        raise ValueError(f"tables {tuple(tables.shape)}: need [B, pages of a slot]")
-    M = tables.shape[1]
-    _ints(dev, (B, M), tables=tables)
-    _ints(dev, (B,), lens=lens)
-    _ints(dev, (B, T), parents=parents)
-    if not _rows16(q):
-        q = q.contiguous()
-    if k.stride() != v.stride() or not _rows16(k) or not _rows16(v):
-        k, v = k.contiguous(), v.contiguous()
-    out = torch.empty((B, T, H, d), dtype=q.dtype, device=dev)
-    with _on(dev):
-        st = _stream(dev)
-        nbytes = _tree_workspace_bytes(dev.index, B, T, H, Hkv, d, page, M, dt)
-        ws = _attention_workspace(dev, st, nbytes).data_ptr() if nbytes else None
-        N.call("nkl_attention_tree", q.data_ptr(), _Strides3(*q.stride()[:3]), k.data_ptr(), v.data_ptr(),
-               _Strides3(*k.stride()[:3]), k_cache.data_ptr(), v_cache.data_ptr(), _Strides3(*k_cache.stride()[:3]),
-               tables.data_ptr(), lens.data_ptr(), None if parents is None else parents.data_ptr(), out.data_ptr(), ws,
-               nbytes, B, T, H, Hkv, d, P, page, M, scale, dt, st)
-    return out
-
-
-@_op("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor lens, "
-     "Tensor? path, Tensor? count) -> Tensor",
-     lambda k, v, k_cache, v_cache, tables, lens, path, count: lens.new_empty(lens.shape))
-def _cache_append(k, v, k_cache, v_cache, tables, lens, path, count):
-    dev, dt = _caches(k_cache, v_cache, 5)
-    L, P, Hkv, page, d = k_cache.shape
-    if k.dim() != 5 or k.shape != v.shape or k.shape[0] != L or k.shape[3:] != (Hkv, d):
-        raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)}, cache {tuple(k_cache.shape)}: need rows "
-                         "[layers, B, T, kv heads, head_dim]")
-    _, B, T, _, _ = k.shape
-    for t in (k, v):
-        if t.dtype != k_cache.dtype:
-            raise TypeError(f"mixed dtypes: {t.dtype} vs {k_cache.dtype}")
-        if t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {t.device} vs {dev}")
-    if tables.dim() != 2 or tables.shape[1] < 1:
-        raise ValueError(f"tables {tuple(tables.shape)}: need [B, pages of a slot]")
-    M = tables.shape[1]
-    _ints(dev, (B, M), tables=tables)
-    _ints(dev, (B,), lens=lens, count=count)
-    _ints(dev, (B, T), path=path)
-    if k.stride() != v.stride() or not _rows16(k) or not _rows16(v):
-        k, v = k.contiguous(), v.contiguous()
-    lens_out = torch.empty_like(lens)
-    with _on(dev):
-        N.call("nkl_cache_append", k.data_ptr(), v.data_ptr(), _Strides4(*k.stride()[:4]), k_cache.data_ptr(),
-               v_cache.data_ptr(), _Strides4(*k_cache.stride()[:4]), tables.data_ptr(), lens.data_ptr(),
-               None if path is None else path.data_ptr(), None if count is None else count.data_ptr(),
-               lens_out.data_ptr(), L, B, T, Hkv, d, P, page, M, dt, _stream(dev))
-    return lens_out
-
-
-def _table(tables: torch.Tensor, lens, refs: torch.Tensor):
-    """Device and sizes (B, M, P) of a cache's tables, lengths and counts."""
-    dev = tables.device
-    if tables.dim() != 2 or refs.dim() != 1 or tables.shape[1] < 1 or refs.shape[0] < 1:
-        raise ValueError(f"tables {tuple(tables.shape)}, refs {tuple(refs.shape)}: need [B, pages of a slot] and [pages]")
-    B, M = tables.shape
-    P = refs.shape[0]
-    _ints(dev, (B, M), tables=tables)
-    _ints(dev, (B,), lens=lens)
-    _ints(dev, (P,), refs=refs)
-    return dev, B, M, P
-
-
-@_op("cache_reserve(Tensor tables, Tensor lens, Tensor refs, Tensor extra, int page_size) -> (Tensor, Tensor, Tensor)",
-     lambda tables, lens, refs, extra, page_size: (tables.new_empty(tables.shape), refs.new_empty(refs.shape),
-                                                   refs.new_empty(1)))
-def _cache_reserve(tables, lens, refs, extra, page_size):
-    dev, B, M, P = _table(tables, lens, refs)
-    _ints(dev, (B,), extra=extra)
-    tables_out, refs_out = torch.empty_like(tables), torch.empty_like(refs)
-    missing = torch.empty(1, dtype=torch.int32, device=dev)
-    with _on(dev):
-        st = _stream(dev)
-        nbytes = N.lib.nkl_cache_reserve_workspace_size(B)
-        ws = _attention_workspace(dev, st, nbytes).data_ptr() if nbytes else None
-        N.call("nkl_cache_reserve", tables.data_ptr(), lens.data_ptr(), refs.data_ptr(), extra.data_ptr(),
-               tables_out.data_ptr(), refs_out.data_ptr(), missing.data_ptr(), ws, nbytes, B, P, page_size, M, st)
-    return tables_out, refs_out, missing
-
-
-@_op("cache_fork(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor lens, Tensor refs, Tensor src, Tensor dst) "
-     "-> (Tensor, Tensor, Tensor, Tensor)",
-     lambda k_cache, v_cache, tables, lens, refs, src, dst: (tables.new_empty(tables.shape), lens.new_empty(lens.shape),
-                                                             refs.new_empty(refs.shape), refs.new_empty(1)))
-def _cache_fork(k_cache, v_cache, tables, lens, refs, src, dst):
-    dc, dt = _caches(k_cache, v_cache, 5)
-    dev, B, M, P = _table(tables, lens, refs)
-    L, Pc, Hkv, page, d = k_cache.shape
-    if Pc != P:
-        raise ValueError(f"the cache has {Pc} pages, refs {P}")
-    if dc != dev:
-        raise RuntimeError(f"tensors on different devices: {dc} vs {dev}")
-    if src.dim() != 1:
-        raise ValueError(f"src {tuple(src.shape)}: need one dimension")
-    F = src.shape[0]
-    _ints(dev, (F,), src=src, dst=dst)
-    tables_out, lens_out, refs_out = torch.empty_like(tables), torch.empty_like(lens), torch.empty_like(refs)
-    missing = torch.empty(1, dtype=torch.int32, device=dev)
-    with _on(dev):
-        st = _stream(dev)
-        nbytes = N.lib.nkl_cache_fork_workspace_size(B, F)
-        ws = _attention_workspace(dev, st, nbytes).data_ptr() if nbytes else None
-        N.call("nkl_cache_fork", k_cache.data_ptr(), v_cache.data_ptr(), _Strides4(*k_cache.stride()[:4]),
-               tables.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(),
-               tables_out.data_ptr(), lens_out.data_ptr(), refs_out.data_ptr(), missing.data_ptr(), ws, nbytes, F, L, B,
-               Hkv, d, P, page, M, dt, st)
-    return tables_out, lens_out, refs_out, missing
-
-
-@_op("cache_free(Tensor tables, Tensor lens, Tensor refs, Tensor slots) -> (Tensor, Tensor, Tensor)",
-     lambda tables, lens, refs, slots: (tables.new_empty(tables.shape), lens.new_empty(lens.shape),
-                                        refs.new_empty(refs.shape)))
-def _cache_free(tables, lens, refs, slots):
-    dev, B, M, P = _table(tables, lens, refs)
-    if slots.dim() != 1:
-        raise ValueError(f"slots {tuple(slots.shape)}: need one dimension")
-    _ints(dev, tuple(slots.shape), slots=slots)
-    tables_out, lens_out, refs_out = torch.empty_like(tables), torch.empty_like(lens), torch.empty_like(refs)
-    with _on(dev):
-        N.call("nkl_cache_free", tables.data_ptr(), lens.data_ptr(), refs.data_ptr(), slots.data_ptr(),
-               tables_out.data_ptr(), lens_out.data_ptr(), refs_out.data_ptr(), slots.shape[0], B, P, M, _stream(dev))
-    return tables_out, lens_out, refs_out
-
-
-@_op("cache_compact(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor refs) -> (Tensor, Tensor)",
-     lambda k_cache, v_cache, tables, refs: (tables.new_empty(tables.shape), refs.new_empty(refs.shape)))
-def _cache_compact(k_cache, v_cache, tables, refs):
-    dc, dt = _caches(k_cache, v_cache, 5)
-    dev, B, M, P = _table(tables, None, refs)
-    L, Pc, Hkv, page, d = k_cache.shape
-    if Pc != P:
-        raise ValueError(f"the cache has {Pc} pages, refs {P}")
-    if dc != dev:
-        raise RuntimeError(f"tensors on different devices: {dc} vs {dev}")
-    tables_out, refs_out = torch.empty_like(tables), torch.empty_like(refs)
-    with _on(dev):
-        st = _stream(dev)
-        nbytes = N.lib.nkl_cache_compact_workspace_size(P)
-        ws = _attention_workspace(dev, st, nbytes).data_ptr()
-        N.call("nkl_cache_compact", k_cache.data_ptr(), v_cache.data_ptr(), _Strides4(*k_cache.stride()[:4]),
-               tables.data_ptr(), refs.data_ptr(), tables_out.data_ptr(), refs_out.data_ptr(), ws, nbytes, L, B, Hkv, d,
-               P, page, M, dt, st)
-    return tables_out, refs_out
-
-
-@_op("verify_drafts(Tensor probs, Tensor tokens, Tensor uniforms, Tensor? parents, Tensor? draft_probs) "
-     "-> (Tensor, Tensor, Tensor)",
-     lambda probs, tokens, uniforms, parents, draft_probs: (tokens.new_empty(tokens.shape),
-                                                            tokens.new_empty(tokens.shape[0]),
-                                                            tokens.new_empty(tokens.shape[0])))
-def _verify_drafts(probs, tokens, uniforms, parents, draft_probs):
-    dev, dt = probs.device, dtype_code(probs)
-    if tokens.dim() != 2 or probs.dim() != 3 or probs.shape[:2] != (tokens.shape[0], tokens.shape[1] + 1):
-        raise ValueError(f"probs {tuple(probs.shape)}, tokens {tuple(tokens.shape)}: need [B, T + 1, vocabulary] and [B, T]")
-    B, T = tokens.shape
-    V = probs.shape[2]
-    if parents is not None and draft_probs is not None:
-        raise ValueError("draft probabilities go with a chain, not with a tree")
-    if T > N.MAX_DRAFTED:
-        raise ValueError(f"{T} drafted tokens, at most {N.MAX_DRAFTED} are taken")
-    _ints(dev, (B, T), tokens=tokens, parents=parents)
-    if uniforms.dtype != torch.float32 or uniforms.shape != (B, T + 1) or uniforms.device != dev:
-        raise ValueError(f"uniforms: need float32 {(B, T + 1)} on {dev}, got {uniforms.dtype} {tuple(uniforms.shape)} on "
-                         f"{uniforms.device}")
-    if draft_probs is not None and (draft_probs.shape != (B, T, V) or draft_probs.dtype != probs.dtype
-                                    or draft_probs.device != dev):
-        raise ValueError(f"draft_probs: need {probs.dtype} {(B, T, V)} on {dev}, got {draft_probs.dtype} "
-                         f"{tuple(draft_probs.shape)} on {draft_probs.device}")
-    probs, uniforms = probs.contiguous(), uniforms.contiguous()
-    if draft_probs is not None:
-        draft_probs = draft_probs.contiguous()
-    path = torch.empty_like(tokens)
-    count, token = tokens.new_empty(B), tokens.new_empty(B)
-    with _on(dev):
-        N.call("nkl_verify_drafts", probs.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
-               tokens.data_ptr(), uniforms.data_ptr(), None if parents is None else parents.data_ptr(), path.data_ptr(),
-               count.data_ptr(), token.data_ptr(), B, T, V, dt, _stream(dev))
-    return path, count, token
+torch.library.register_fake("nkilab::attention_tree",
+                            lambda q, k, v, k_cache, v_cache, tables, lens, parents, scale: q.new_empty(q.shape))
+torch.library.register_fake("nkilab::cache_append",
+                            lambda k, v, k_cache, v_cache, tables, lens, path, count: _like(lens))
+torch.library.register_fake("nkilab::cache_reserve",
+                            lambda tables, lens, refs, extra, page_size: _like(tables, refs, refs[:1]))
+torch.library.register_fake("nkilab::cache_fork",
+                            lambda k_cache, v_cache, tables, lens, refs, src, dst: _like(tables, lens, refs, refs[:1]))
+torch.library.register_fake("nkilab::cache_free", lambda tables, lens, refs, slots: _like(tables, lens, refs))
+torch.library.register_fake("nkilab::cache_compact", lambda k_cache, v_cache, tables, refs: _like(tables, refs))
+torch.library.register_fake("nkilab::verify_drafts", lambda probs, tokens, uniforms, parents, draft_probs:
+                            (_like(tokens), tokens.new_empty(tokens.shape[0]), tokens.new_empty(tokens.shape[0])))

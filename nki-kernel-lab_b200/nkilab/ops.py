@@ -14,9 +14,11 @@ There is no CPU fallback: on a machine without a GPU every op raises.
 from __future__ import annotations
 
 import math
+import re
 
 import torch
 
+from . import _native
 from . import _torch_ops  # noqa: F401  (registers torch.ops.nkilab.*)
 from ._host import dtype_of as _dtype_of
 from ._host import like_input as _like_input
@@ -157,7 +159,25 @@ def rope(x, base: float = 10000.0, pos_offset: int = 0):
 # [pages] int32, how many table entries name each page. Nothing here reads them on the host
 # or waits for the GPU. nkilab.serving.PagedCache keeps them together.
 
-_decode = torch.ops.nkilab
+def _decode(name: str):
+    """torch.ops.nkilab.<name>, with a refusal of the C ABI raised as NklError."""
+    op = getattr(torch.ops.nkilab, name).default
+
+    def call(*args):
+        try:
+            return op(*args)
+        except RuntimeError as e:
+            m = re.match(r"(nkl_\w+) failed \((\d+)\): ([^\n]*)", str(e))
+            if type(e) is not RuntimeError or m is None:
+                raise
+            raise _native.NklError(m[1], int(m[2]), m[3]) from None
+
+    return call
+
+
+_attention_tree, _cache_append, _cache_reserve, _cache_fork, _cache_free, _cache_compact, _verify_drafts = map(
+    _decode, ("attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
+              "verify_drafts"))
 
 
 def _layers(*ts):
@@ -178,7 +198,7 @@ def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    return _decode.attention_tree.default(q, k, v, k_cache, v_cache, tables, lens, parents, float(scale))
+    return _attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents, float(scale))
 
 
 def cache_append(k, v, k_cache, v_cache, tables, lens, path=None, count=None):
@@ -186,31 +206,31 @@ def cache_append(k, v, k_cache, v_cache, tables, lens, path=None, count=None):
     onward and returns the new lengths: row path[b, j] for j < count[b] (the accepted path
     of drafted tokens), or all T rows in order. The pages come from cache_reserve; rows
     without a page are dropped."""
-    return _decode.cache_append.default(*_layers(k, v, k_cache, v_cache), tables, lens, path, count)
+    return _cache_append(*_layers(k, v, k_cache, v_cache), tables, lens, path, count)
 
 
 def cache_reserve(tables, lens, refs, extra, page_size):
     """Pages for extra[b] more positions of each slot, lowest free index first. Returns
     (tables, refs, missing): with too few free pages, or too narrow tables, missing [1] is
     how many lack and nothing is given out."""
-    return _decode.cache_reserve.default(tables, lens, refs, extra, int(page_size))
+    return _cache_reserve(tables, lens, refs, extra, int(page_size))
 
 
 def cache_fork(k_cache, v_cache, tables, lens, refs, src, dst):
     """Slot dst[f] becomes a copy of slot src[f]: full pages are shared, the last, partly
     filled one is copied to a free page. Returns (tables, lens, refs, missing); with
     missing [1] > 0 (too few free pages) nothing is forked."""
-    return _decode.cache_fork.default(*_layers(k_cache, v_cache), tables, lens, refs, src, dst)
+    return _cache_fork(*_layers(k_cache, v_cache), tables, lens, refs, src, dst)
 
 
 def cache_free(tables, lens, refs, slots):
     """Gives back the pages of the slots listed. Returns (tables, lens, refs)."""
-    return _decode.cache_free.default(tables, lens, refs, slots)
+    return _cache_free(tables, lens, refs, slots)
 
 
 def cache_compact(k_cache, v_cache, tables, refs):
     """Moves the pages in use to the lowest indices. Returns (tables, refs)."""
-    return _decode.cache_compact.default(*_layers(k_cache, v_cache), tables, refs)
+    return _cache_compact(*_layers(k_cache, v_cache), tables, refs)
 
 
 def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):
@@ -223,4 +243,4 @@ def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):
     Returns (path [B, T], the accepted tokens' indices and then -1; count [B]; token [B]).
     Sums are whole numbers of 2^-31, so equal inputs give equal tokens on every launch.
     """
-    return _decode.verify_drafts.default(probs, tokens, uniforms, parents, draft_probs)
+    return _verify_drafts(probs, tokens, uniforms, parents, draft_probs)
