@@ -16,6 +16,13 @@
 // down; an fp32 softmax row is itself no better than 2^-24 of its largest value), sums are
 // 64 bit. Sums of whole numbers do not depend on their order, so the drawn token is the same
 // for every launch shape, which a cumulative sum in fp32 is not.
+//
+// A cluster of blocks takes one sequence. Each block walks for itself (some hundred values,
+// from L2); then each warp sums a contiguous part of the one row (with q: two) that the next
+// token is drawn from, the blocks exchange their sums through shared memory, and the warp in
+// whose part the drawn place lies reads that part once more, from L2. So each of those rows is
+// read from HBM once, which is what bounds a batch; a single sequence is bound by the chain of
+// three dependent reads and the exchange.
 #include "common.cuh"
 
 namespace nkl {
@@ -43,92 +50,155 @@ struct VerifyArgs {
   int batch, drafted, vocab;
 };
 
-__device__ __forceinline__ unsigned long long warp_sum64(unsigned long long v) {
+typedef unsigned long long u64;
+
+__device__ __forceinline__ u64 warp_sum64(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// One block per sequence.
-template <typename T>
+// Weights of N elements x0 .. x0 + N - 1 of a row, less those of q; 0 from the row's end on.
+// VEC: rows are 16-byte aligned and whole vectors long.
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void load_row(const T* p, int x0, int end, uint32_t (&w)[N]) {
+  static_assert(N == Vec16<T>::N, "one vector");
+  if constexpr (VEC) {
+    Vec16<T> v;
+    v.raw = x0 < end ? *reinterpret_cast<const uint4*>(p + x0) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = whole(v.get(e));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = x0 + e < end ? whole(to_f32(p[x0 + e])) : 0u;
+  }
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Stores to the same shared variable of another block of the cluster.
+__device__ __forceinline__ void store_remote(u64* p, uint32_t rank, u64 v) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+constexpr int kMaxCluster = 8;
+
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_constant__ VerifyArgs a) {
+  constexpr int VE = Vec16<T>::N;
   __shared__ int s_token[kMaxDrafted], s_parent[kMaxDrafted], s_next[kMaxDrafted + 1];
-  __shared__ uint32_t s_mass[kMaxDrafted];
-  __shared__ int s_last, s_count;
-  __shared__ unsigned long long s_sum[kVerifyWarps], s_all[kVerifyWarps];
+  __shared__ uint32_t s_mass[kMaxDrafted], s_left[kMaxDrafted];
+  __shared__ int s_last;
+  __shared__ u64 s_sum[kVerifyWarps], s_all[kVerifyWarps];
+  __shared__ u64 s_blocks[kMaxCluster][2];  // the cluster's sums and sums of whole rows
   pdl_enter();
-  const int b = blockIdx.x, n = a.drafted, V = a.vocab;
+  const int blocks = (int)cluster_size(), rank = (int)cluster_rank();
+  const int b = blockIdx.x / blocks, n = a.drafted, V = a.vocab;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const T* probs = static_cast<const T*>(a.probs) + (int64_t)b * (n + 1) * V;
   const T* draft = a.draft ? static_cast<const T*>(a.draft) + (int64_t)b * n * V : nullptr;
   const float* u = a.uniforms + (int64_t)b * (n + 1);
 
   // each drafted token's mass in its parent's row; parent -2 marks one that cannot be accepted
-  for (int i = tid; i < n; i += kVerifyThreads) {
-    const int x = a.tokens[(int64_t)b * n + i];
-    int up = a.parents ? a.parents[(int64_t)b * n + i] : i - 1;
-    if (up >= i) up = -1;
+  u64 my_u = 0;
+  if (tid < n) {
+    const int x = a.tokens[(int64_t)b * n + tid];
+    int up = a.parents ? a.parents[(int64_t)b * n + tid] : tid - 1;
+    if (up >= tid) up = -1;
     if (x < 0 || x >= V || up < -1) up = -2;
-    s_token[i] = x;
-    s_parent[i] = up;
-    s_mass[i] = up >= -1 ? whole(to_f32(probs[(int64_t)(up + 1) * V + x])) : 0u;
+    my_u = whole_u(u[tid]);
+    s_token[tid] = x;
+    s_parent[tid] = up;
+    s_mass[tid] = up >= -1 ? whole(to_f32(probs[(int64_t)(up + 1) * V + x])) : 0u;
+    // what the chain's test compares with; the tree's is found below
+    s_left[tid] = draft ? (up >= -1 ? whole(to_f32(draft[(int64_t)tid * V + x])) : 0u) : (uint32_t)kOne;
   }
-  for (int i = tid; i <= n; i += kVerifyThreads) s_next[i] = 0x7fffffff;
+  if (tid <= n) s_next[tid] = 0x7fffffff;
+  const u64 last_u = whole_u(u[n]);
   __syncthreads();
-  // s_next[node + 1]: the node's first child that is accepted when the walk stands there
-  for (int i = tid; i < n; i += kVerifyThreads) {
-    const int up = s_parent[i], x = s_token[i];
-    if (up < -1) continue;
-    unsigned long long left = kOne, mass = s_mass[i];
-    if (draft) {
-      left = whole(to_f32(draft[(int64_t)i * V + x]));
-    } else {
-      for (int j = 0; j < i; ++j) {
-        if (s_parent[j] != up) continue;
-        if (s_token[j] == x) mass = 0;  // a token already rejected
-        bool again = false;
-        for (int k = 0; k < j; ++k) again |= s_parent[k] == up && s_token[k] == s_token[j];
-        if (!again) left -= min((unsigned long long)s_mass[j], left);
-      }
+  if (!draft && a.parents) {
+    // a token that an earlier brother has had already has no mass left
+    for (int i = warp; i < n; i += kVerifyWarps) {
+      const int up = s_parent[i], x = s_token[i];
+      bool again = false;
+      for (int j = lane; j < i; j += 32) again |= s_parent[j] == up && s_token[j] == x;
+      if (__any_sync(0xffffffffu, again) && lane == 0) s_mass[i] = 0u;  // read by no one before the barrier
     }
-    if (whole_u(u[i]) * left < mass * kOne) atomicMin(&s_next[up + 1], i);
+    __syncthreads();
+    // the mass that the brothers before a token leave, if they are rejected
+    for (int i = warp; i < n; i += kVerifyWarps) {
+      const int up = s_parent[i];
+      u64 out = 0;
+      for (int j = lane; j < i; j += 32) out += s_parent[j] == up ? s_mass[j] : 0u;
+      out = warp_sum64(out);
+      if (lane == 0) s_left[i] = (uint32_t)(kOne - min(out, kOne));
+    }
+    __syncthreads();
   }
+  // s_next[node + 1]: the node's first child that is accepted when the walk stands there
+  if (tid < n && s_parent[tid] >= -1 && my_u * s_left[tid] < s_mass[tid] * kOne) atomicMin(&s_next[s_parent[tid] + 1], tid);
   __syncthreads();
   if (tid == 0) {
     int at = -1, c = 0;
-    for (int i; (i = s_next[at + 1]) != 0x7fffffff; at = i) a.path[(int64_t)b * n + c++] = i;
+    for (int i; (i = s_next[at + 1]) != 0x7fffffff; at = i, ++c)
+      if (rank == 0) a.path[(int64_t)b * n + c] = i;
     s_last = at;
-    s_count = c;
-    a.count[b] = c;
+    if (rank == 0) {
+      a.count[b] = c;
+      for (; c < n; ++c) a.path[(int64_t)b * n + c] = -1;
+    }
   }
   __syncthreads();
   const int last = s_last;
-  for (int i = s_count + tid; i < n; i += kVerifyThreads) a.path[(int64_t)b * n + i] = -1;
 
   // the next token's weights: row p of the last accepted token, less q or the rejected tokens
   const T* p = probs + (int64_t)(last + 1) * V;
   const T* q = draft && last + 1 < n && s_parent[last + 1] >= -1 ? draft + (int64_t)(last + 1) * V : nullptr;
-  const int per_warp = ((V + kVerifyWarps - 1) / kVerifyWarps + 31) & ~31;
-  const int lo = min(warp * per_warp, V), hi = min(lo + per_warp, V);
-  unsigned long long sum = 0, all = 0;
-  for (int x = lo + lane; x < hi; x += 32) {
-    const uint32_t pw = whole(to_f32(p[x]));
-    all += pw;
-    if (q) {
-      const uint32_t qw = whole(to_f32(q[x]));
-      sum += pw > qw ? pw - qw : 0u;
+  const int step = 32 * VE, parts = blocks * kVerifyWarps;
+  const int per_warp = (V + parts * step - 1) / (parts * step) * step;
+  const int64_t begin = (int64_t)(rank * kVerifyWarps + warp) * per_warp;
+  const int lo = (int)min(begin, (int64_t)V), hi = min(lo + per_warp, V);
+  u64 sum = 0, all = 0;
+  if (q) {
+#pragma unroll 4
+    for (int x = lo + lane * VE; x < hi; x += step) {
+      uint32_t pw[VE], qw[VE];
+      load_row<T, VEC>(p, x, hi, pw);
+      load_row<T, VEC>(q, x, hi, qw);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        all += pw[e];
+        sum += pw[e] > qw[e] ? pw[e] - qw[e] : 0u;
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (int x = lo + lane * VE; x < hi; x += step) {
+      uint32_t pw[VE];
+      load_row<T, VEC>(p, x, hi, pw);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) all += pw[e];
     }
   }
   all = warp_sum64(all);
   sum = q ? warp_sum64(sum) : all;
   if (!draft) {
-    unsigned long long out = 0;
-    for (int i = lane; i < n; i += 32) {
-      if (s_parent[i] != last || s_token[i] < lo || s_token[i] >= hi) continue;
-      bool again = false;
-      for (int k = 0; k < i; ++k) again |= s_parent[k] == last && s_token[k] == s_token[i];
-      if (!again) out += s_mass[i];
-    }
+    u64 out = 0;
+    for (int i = lane; i < n; i += 32)
+      if (s_parent[i] == last && s_token[i] >= lo && s_token[i] < hi) out += s_mass[i];
     sum -= warp_sum64(out);
   }
   if (lane == 0) {
@@ -136,56 +206,112 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     s_all[warp] = all;
   }
   __syncthreads();
-  unsigned long long total = 0, whole_row = 0;
-  for (int w = 0; w < kVerifyWarps; ++w) {
-    total += s_sum[w];
-    whole_row += s_all[w];
+  if (warp == 0) {  // the block's sums to every block
+    const u64 x = warp_sum64(lane < kVerifyWarps ? s_sum[lane] : 0), y = warp_sum64(lane < kVerifyWarps ? s_all[lane] : 0);
+    if (lane < blocks) {
+      store_remote(&s_blocks[rank][0], lane, x);
+      store_remote(&s_blocks[rank][1], lane, y);
+    }
+  }
+  cluster_sync();
+  u64 total = 0, total_all = 0;
+  for (int r = 0; r < blocks; ++r) {
+    total += s_blocks[r][0];
+    total_all += s_blocks[r][1];
   }
   const bool plain = total == 0;  // nothing left: the row itself
-  if (plain) total = whole_row;
+  if (plain) total = total_all;
   if (total == 0) {
-    if (tid == 0) a.token[b] = -1;
+    if (rank == 0 && tid == 0) a.token[b] = -1;
     return;
   }
-  const unsigned long long ul = whole_u(u[n]);
-  const unsigned long long t = (total >> 31) * ul + (((total & (kOne - 1)) * ul) >> 31);
-  unsigned long long before = 0;
-  int w = 0;
-  for (; w < kVerifyWarps; ++w) {
-    const unsigned long long s = plain ? s_all[w] : s_sum[w];
-    if (before + s > t) break;
-    before += s;
-  }
-  if (w != warp) return;
-  for (int x0 = lo; x0 < hi; x0 += 32) {
-    const int x = x0 + lane;
-    unsigned long long v = 0;
-    if (x < hi) {
-      uint32_t pw = whole(to_f32(p[x]));
-      if (!plain) {
-        if (q) {
-          const uint32_t qw = whole(to_f32(q[x]));
-          pw = pw > qw ? pw - qw : 0u;
-        } else if (!draft) {
-          for (int i = 0; i < n; ++i)
-            if (s_parent[i] == last && s_token[i] == x) pw = 0;
-        }
-      }
-      v = pw;
-    }
-    unsigned long long inc = v;
+  const u64 t = (total >> 31) * last_u + (((total & (kOne - 1)) * last_u) >> 31);
+  u64 before = 0;
+  for (int r = 0; r < rank; ++r) before += s_blocks[r][plain];
+  if (t < before || t >= before + s_blocks[rank][plain]) return;  // another block has it
+  for (int w = 0; w < warp; ++w) before += plain ? s_all[w] : s_sum[w];
+  if (t < before || t >= before + (plain ? s_all[warp] : s_sum[warp])) return;  // another warp
+  // this warp's part again, element by element
+  constexpr int kBatch = 4;
+  for (int x0 = lo; x0 < hi; x0 += kBatch * step) {
+    uint32_t w[kBatch][VE];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
+    for (int i = 0; i < kBatch; ++i) {
+      const int x = x0 + i * step + lane * VE;
+      load_row<T, VEC>(p, x, hi, w[i]);
+      if (q && !plain) {
+        uint32_t qw[VE];
+        load_row<T, VEC>(q, x, hi, qw);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) w[i][e] = w[i][e] > qw[e] ? w[i][e] - qw[e] : 0u;
+      }
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + inc > t);
-    if (hit) {
-      if (lane == 0) a.token[b] = x0 + __ffs(hit) - 1;
-      return;
+    if (!draft && !plain) {
+      for (int j = 0; j < n; ++j) {
+        if (s_parent[j] != last) continue;
+        const int off = s_token[j] - x0 - lane * VE;  // place of a rejected token among the lane's elements
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) w[i][e] = off == i * step + e ? 0u : w[i][e];
+      }
     }
-    before += __shfl_sync(0xffffffffu, inc, 31);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      u64 mine = 0;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) mine += w[i][e];
+      u64 inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > t);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) {
+          u64 at = before + inc - mine;
+          int e = 0;
+#pragma unroll
+          for (int k = 0; k < VE; ++k) {
+            at += w[i][k];
+            if (at <= t) e = k + 1;
+          }
+          a.token[b] = x0 + i * step + lane * VE + e;
+        }
+        return;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
   }
+}
+
+template <typename T>
+int launch_verify(const VerifyArgs& a, cudaStream_t st) {
+  // Blocks per sequence: up to eight, as long as all fit the GPU at once (two to an SM by their
+  // registers) and a warp's part still has a step of its own.
+  int blocks = kMaxCluster;
+  while (blocks > 1 && ((int64_t)a.batch * blocks > 2LL * sm_count() ||
+                        (int64_t)blocks * kVerifyWarps * 32 * Vec16<T>::N > 2LL * a.vocab))
+    blocks /= 2;
+  const bool vec = a.vocab % Vec16<T>::N == 0 && is_aligned(a.probs, 16) && (!a.draft || is_aligned(a.draft, 16));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.batch * blocks));
+  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)blocks, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = vec ? cudaLaunchKernelEx(&cfg, verify_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, verify_kernel<T, false>, a);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(NKL_ERR_CUDA, "nkl_verify_drafts: %s", cudaGetErrorString(e));
+  }
+  return NKL_OK;
 }
 
 }  // namespace
@@ -199,7 +325,7 @@ extern "C" int nkl_verify_drafts(const void* probs, const void* draft_probs, con
                                  void* stream) {
   const char* op = "nkl_verify_drafts";
   if (!valid_dtype(dtype)) return fail(NKL_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
-  if (batch < 0 || batch > 0x7fffffffLL || vocab < 1 || vocab > (1LL << 30))
+  if (batch < 0 || batch > (1LL << 27) || vocab < 1 || vocab > (1LL << 30))
     return fail(NKL_ERR_SHAPE, "%s: batch %lld or vocabulary %lld out of range", op, (long long)batch, (long long)vocab);
   if (drafted < 0 || drafted > kMaxDrafted)
     return fail(NKL_ERR_SHAPE, "%s: %lld drafted tokens, at most %d are taken", op, (long long)drafted, kMaxDrafted);
@@ -213,7 +339,5 @@ extern "C" int nkl_verify_drafts(const void* probs, const void* draft_probs, con
                   count, token,       (int)batch, (int)drafted, (int)vocab};
   if (drafted == 0) a.draft = nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == NKL_FLOAT32)
-    return launch_pdl(verify_kernel<float>, dim3((unsigned)batch), dim3(kVerifyThreads), 0, st, op, a);
-  return launch_pdl(verify_kernel<bf16>, dim3((unsigned)batch), dim3(kVerifyThreads), 0, st, op, a);
+  return dtype == NKL_FLOAT32 ? launch_verify<float>(a, st) : launch_verify<bf16>(a, st);
 }
