@@ -9,8 +9,9 @@
 //
 // CUDA-core kernel (fp32, and bf16 layouts that the tensor-core kernel does not take): a block
 // owns 16 query rows of one key/value head and one range of the keys; each warp has 4 rows,
-// lane x scores key x of a 32-key tile and then accumulates 4 columns. Key ranges split over
-// several blocks leave (max, sum, O) in the workspace; tree_combine_kernel joins them in order.
+// lane x scores key x of a 32-key tile and then accumulates 4 columns; two tiles are on their
+// way (cp.async) while one is worked on. Key ranges split over several blocks leave (max, sum, O)
+// in the workspace; tree_combine_kernel joins them in order.
 #include <algorithm>
 #include <atomic>
 
@@ -77,32 +78,78 @@ __device__ __forceinline__ void store4(bf16* p, float4 v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
 }
 
+// 16 bytes from global to shared memory, zeros where `from` is null.
+__device__ __forceinline__ void copy16_async(void* to, const void* from, const void* any) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to), size = from ? 16u : 0u;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from ? from : any), "r"(size) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Shared memory: queries in fp32, and two tiles of keys and values as they come; a key row is
+// 16 bytes longer than its data, so that 32 lanes reading a row each do not collide.
+template <typename T>
+size_t tree_smem(int d) {
+  return (size_t)kRows * d * 4 + 2 * (size_t)kKeys * (2 * d * sizeof(T) + 16);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
-  __shared__ __align__(16) float qs[kRows][kMaxDim];
-  __shared__ __align__(16) float ks[kKeys][kMaxDim + 4];
-  __shared__ __align__(16) float vs[kKeys][kMaxDim];
+  constexpr int VE = Vec16<T>::N;
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float ps[kRows][kKeys];
-  __shared__ int64_t base[kKeys];
   pdl_enter();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int split = blockIdx.x / a.row_blocks, r0 = (blockIdx.x % a.row_blocks) * kRows;
   const int kvh = blockIdx.y, b = blockIdx.z;
-  const int rows = a.tokens * a.group, quads = a.d / 4;
+  const int rows = a.tokens * a.group, quads = a.d / 4, chunks = a.d / VE, pitch = a.d + VE;
+  float* const qs = reinterpret_cast<float*>(smem);
+  T* const ring = reinterpret_cast<T*>(smem + (size_t)kRows * a.d * 4);
+  const int stage_size = kKeys * (pitch + a.d);
   const int n = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
   // this block's tiles: a share of the cached ones, and the drafted ones in the last split
   const int tiles = (n + kKeys - 1) / kKeys;
   const int per = (tiles + a.splits - 1) / a.splits;
   const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
-  const int new_tiles = split == a.splits - 1 ? (a.tokens + kKeys - 1) / kKeys : 0;
+  const int end = t1 + (split == a.splits - 1 ? (a.tokens + kKeys - 1) / kKeys : 0);
+
+  const float per_row = 1.f / (float)chunks;
+  auto fetch = [&](int t) {  // tile t into its place of the ring
+    if (t < end) {
+      const bool cached = t < t1;
+      const int key0 = (cached ? t : t - t1) * kKeys;
+      const T* const kp = static_cast<const T*>(cached ? a.k_cache : a.k_new);
+      const T* const vp = static_cast<const T*>(cached ? a.v_cache : a.v_new);
+      T* const ks = ring + (t & 1) * stage_size;
+      T* const vs = ks + kKeys * pitch;
+      for (int i = tid; i < kKeys * chunks; i += kThreads) {
+        const int r = (int)(((float)i + 0.5f) * per_row), c = (i - r * chunks) * VE, key = key0 + r;  // r = i / chunks
+        int64_t at = -1;
+        if (!cached) {
+          if (key < a.tokens) at = b * a.n_b + key * a.n_t + kvh * a.n_h + c;
+        } else if (key < n) {
+          const int pi = key / a.page, p = a.tables[(int64_t)b * a.max_pages + pi];
+          if (p >= 0 && p < a.pages) at = p * a.c_p + kvh * a.c_h + (key - pi * a.page) * a.c_s + c;
+        }
+        copy16_async(ks + r * pitch + c, at >= 0 ? kp + at : nullptr, kp);
+        copy16_async(vs + r * a.d + c, at >= 0 ? vp + at : nullptr, vp);
+      }
+    }
+    copies_commit();  // also where there is nothing: the count of groups goes on
+  };
+  fetch(t0);
+  fetch(t0 + 1);
 
   const T* q = static_cast<const T*>(a.q) + b * a.q_b;
   for (int i = tid; i < kRows * quads; i += kThreads) {
     const int r = i / quads, c = (i - r * quads) * 4, row = r0 + r;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row < rows) x = load4<T>(q + (row / a.group) * a.q_t + (kvh * a.group + row % a.group) * a.q_h + c);
-    *reinterpret_cast<float4*>(&qs[r][c]) = x;
+    *reinterpret_cast<float4*>(qs + r * a.d + c) = x;
   }
+  const int* const parents = a.parents ? a.parents + (int64_t)b * a.tokens : nullptr;
   uint32_t seen[4][4];  // drafted tokens visible to each of the warp's rows
   bool here[4];
   float m[4], l[4];
@@ -110,57 +157,40 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = r0 + warp * 4 + i;
+    const int token = row / a.group;
+    here[i] = row < rows && (!parents || parents[token] >= -1);
     seen[i][0] = seen[i][1] = seen[i][2] = seen[i][3] = 0u;
-    if (row < rows) ancestor_bits(a.parents ? a.parents + (int64_t)b * a.tokens : nullptr, row / a.group, seen[i]);
-    here[i] = (seen[i][0] | seen[i][1] | seen[i][2] | seen[i][3]) != 0u;
+    if (here[i] && end > t1) ancestor_bits(parents, token, seen[i]);
     m[i] = -INFINITY;
     l[i] = 0.f;
     o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  // With head_dim up to 64 the warp's halves take the columns twice, for every second key each.
+  const bool halves = quads <= 16;
+  const int col = (halves ? lane & 15 : lane) * 4, key_of = halves ? lane >> 4 : 0, key_step = halves ? 2 : 1;
 
-  for (int t = t0; t < t1 + new_tiles; ++t) {
+  for (int t = t0; t < end; ++t) {
     const bool cached = t < t1;
     const int key0 = (cached ? t : t - t1) * kKeys;
-    __syncthreads();
-    if (tid < kKeys) {
-      int64_t at = -1;
-      const int key = key0 + tid;
-      if (!cached) {
-        if (key < a.tokens) at = b * a.n_b + key * a.n_t + kvh * a.n_h;
-      } else if (key < n) {
-        const int p = a.tables[(int64_t)b * a.max_pages + key / a.page];
-        if (p >= 0 && p < a.pages) at = p * a.c_p + kvh * a.c_h + (key % a.page) * a.c_s;
-      }
-      base[tid] = at;
-    }
-    __syncthreads();
-    const T* kp = static_cast<const T*>(cached ? a.k_cache : a.k_new);
-    const T* vp = static_cast<const T*>(cached ? a.v_cache : a.v_new);
-    for (int i = tid; i < kKeys * quads; i += kThreads) {
-      const int r = i / quads, c = (i - r * quads) * 4;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-      if (base[r] >= 0) {
-        x = load4<T>(kp + base[r] + c);
-        y = load4<T>(vp + base[r] + c);
-      }
-      *reinterpret_cast<float4*>(&ks[r][c]) = x;
-      *reinterpret_cast<float4*>(&vs[r][c]) = y;
-    }
+    const T* const ks = ring + (t & 1) * stage_size;
+    const T* const vs = ks + kKeys * pitch;
+    copies_wait<1>();
     __syncthreads();
     float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int c = 0; c < a.d; c += 4) {
-      const float4 kx = *reinterpret_cast<const float4*>(&ks[lane][c]);
+      const float4 kx = load4<T>(ks + lane * pitch + c);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 qx = *reinterpret_cast<const float4*>(&qs[warp * 4 + i][c]);
+        const float4 qx = *reinterpret_cast<const float4*>(qs + (warp * 4 + i) * a.d + c);
         s[i] = fmaf(qx.x, kx.x, fmaf(qx.y, kx.y, fmaf(qx.z, kx.z, fmaf(qx.w, kx.w, s[i]))));
       }
     }
+    const int word = (key0 >> 5) & 3;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      bool sees = here[i];
-      if (cached) sees &= key0 + lane < n;
-      else sees &= (seen[i][(key0 >> 5) & 3] >> lane) & 1u;
+      const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
+      const bool sees = here[i] && (cached ? key0 + lane < n : ((drafts >> lane) & 1u) != 0u);
       const float x = sees ? s[i] * a.scale : -INFINITY;
       const float top = fmaxf(m[i], warp_max(x));
       const float ref = top == -INFINITY ? 0.f : top;  // nothing seen so far
@@ -172,53 +202,58 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
       ps[warp * 4 + i][lane] = p;
     }
     __syncwarp();
-    if (lane < quads && !cached) {
-      // a drafted token that a row does not see leaves no trace in it, whatever its v holds
-      for (int x = 0; x < kKeys && key0 + x < a.tokens; ++x) {
-        const float4 v = *reinterpret_cast<const float4*>(&vs[x][lane * 4]);
+    if (col < a.d && cached) {
+#pragma unroll 4
+      for (int x = key_of; x < kKeys; x += key_step) {
+        const float4 v = load4<T>(vs + x * a.d + col);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (!((seen[i][(key0 >> 5) & 3] >> x) & 1u)) continue;
-          const float pk = ps[warp * 4 + i][x];
-          o[i].x = fmaf(pk, v.x, o[i].x);
-          o[i].y = fmaf(pk, v.y, o[i].y);
-          o[i].z = fmaf(pk, v.z, o[i].z);
-          o[i].w = fmaf(pk, v.w, o[i].w);
+          const float p = ps[warp * 4 + i][x];
+          o[i].x = fmaf(p, v.x, o[i].x);
+          o[i].y = fmaf(p, v.y, o[i].y);
+          o[i].z = fmaf(p, v.z, o[i].z);
+          o[i].w = fmaf(p, v.w, o[i].w);
         }
       }
-    } else if (lane < quads) {
-      for (int x = 0; x < kKeys; x += 4) {
-        float4 v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float4*>(&vs[x + k][lane * 4]);
+    } else if (col < a.d) {
+      // a drafted token that a row does not see leaves no trace in it, whatever its v holds
+      for (int x = key_of; x < kKeys && key0 + x < a.tokens; x += key_step) {
+        const float4 v = load4<T>(vs + x * a.d + col);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 p = *reinterpret_cast<const float4*>(&ps[warp * 4 + i][x]);
-          const float pk[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            o[i].x = fmaf(pk[k], v[k].x, o[i].x);
-            o[i].y = fmaf(pk[k], v[k].y, o[i].y);
-            o[i].z = fmaf(pk[k], v[k].z, o[i].z);
-            o[i].w = fmaf(pk[k], v[k].w, o[i].w);
-          }
+          const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
+          if (!((drafts >> x) & 1u)) continue;
+          const float p = ps[warp * 4 + i][x];
+          o[i].x = fmaf(p, v.x, o[i].x);
+          o[i].y = fmaf(p, v.y, o[i].y);
+          o[i].z = fmaf(p, v.z, o[i].z);
+          o[i].w = fmaf(p, v.w, o[i].w);
         }
       }
     }
+    __syncthreads();  // every warp is through with this tile's place
+    fetch(t + 2);
   }
+  copies_wait<0>();
 
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    if (halves) {
+      o[i].x += __shfl_xor_sync(0xffffffffu, o[i].x, 16);
+      o[i].y += __shfl_xor_sync(0xffffffffu, o[i].y, 16);
+      o[i].z += __shfl_xor_sync(0xffffffffu, o[i].z, 16);
+      o[i].w += __shfl_xor_sync(0xffffffffu, o[i].w, 16);
+    }
     const int row = r0 + warp * 4 + i;
     if (row >= rows) continue;
     if (a.splits == 1) {
       const float inv = here[i] ? 1.f / l[i] : 0.f;  // an absent token's row is zero
       const int64_t at = (((int64_t)b * a.tokens + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d;
-      if (lane < quads)
-        store4(static_cast<T*>(a.out) + at + lane * 4, make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv));
+      if (key_of == 0 && col < a.d)
+        store4(static_cast<T*>(a.out) + at + col, make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv));
     } else {
       const int64_t at = (((int64_t)split * a.batch + b) * a.kv_heads + kvh) * rows + row;
-      if (lane < quads) store4(a.ws_o + at * a.d + lane * 4, o[i]);
+      if (key_of == 0 && col < a.d) store4(a.ws_o + at * a.d + col, o[i]);
       if (lane == 0) {
         a.ws_ml[2 * at] = m[i];
         a.ws_ml[2 * at + 1] = l[i];
@@ -227,35 +262,43 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
   }
 }
 
+constexpr int kMaxSplits = 256;
+
 // Joins the splits of each row, in split order: one warp per row, lane = 4 columns.
 template <typename T>
 __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
+  __shared__ float weight[4][kMaxSplits];
   pdl_enter();
-  const int rows = a.tokens * a.group, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), all = (int64_t)a.batch * a.kv_heads * rows;
+  const int rows = a.tokens * a.group, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * 4 + warp, all = (int64_t)a.batch * a.kv_heads * rows;
   if (row >= all) return;
   const int r = (int)(row % rows), kvh = (int)(row / rows % a.kv_heads), b = (int)(row / rows / a.kv_heads);
-  float m = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, a.ws_ml[2 * (s * all + row)]);
+  const float2* const ml = reinterpret_cast<const float2*>(a.ws_ml) + row;
+  float m = -INFINITY, l = 0.f;
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[s * all].x);
   m = warp_max(m);
-  float l = 0.f;
+  for (int s = lane; s < a.splits; s += 32) {
+    const float2 x = ml[s * all];
+    const float w = x.x == -INFINITY ? 0.f : expf(x.x - m);
+    weight[warp][s] = w;
+    l = fmaf(w, x.y, l);
+  }
+  l = warp_sum(l);
+  __syncwarp();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (m != -INFINITY) {
+  if (lane * 4 < a.d) {
+    const float* const po = a.ws_o + row * a.d + lane * 4;
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) {
-      const int64_t at = s * all + row;
-      const float w = expf(a.ws_ml[2 * at] - m);
-      if (w == 0.f) continue;
-      l = fmaf(w, a.ws_ml[2 * at + 1], l);
-      if (lane * 4 < a.d) {
-        const float4 x = load4<float>(a.ws_o + at * a.d + lane * 4);
-        o.x = fmaf(w, x.x, o.x);
-        o.y = fmaf(w, x.y, o.y);
-        o.z = fmaf(w, x.z, o.z);
-        o.w = fmaf(w, x.w, o.w);
-      }
+      const float w = weight[warp][s];
+      const float4 x = load4<float>(po + s * all * a.d);
+      o.x = fmaf(w, x.x, o.x);
+      o.y = fmaf(w, x.y, o.y);
+      o.z = fmaf(w, x.z, o.z);
+      o.w = fmaf(w, x.w, o.w);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l > 0.f ? 1.f / l : 0.f;  // 0: an absent token
   const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + kvh * a.group + r % a.group) * a.d;
   if (lane * 4 < a.d)
     store4(static_cast<T*>(a.out) + at + lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
@@ -269,12 +312,25 @@ namespace {
 
 // ------------------------------------------------------------------ host
 
-// Blocks that share a sequence's keys: enough of them to give every SM a few, each with at
-// least 64 keys of the longest sequence that the tables can hold.
+// Blocks that share a sequence's keys: up to four for each SM, each with at least 64 keys, the
+// two tiles it has on their way at once, of the longest sequence that the tables can hold.
 int split_count(int64_t batch, int64_t kv_heads, int64_t row_blocks, int64_t capacity) {
   const int64_t blocks = batch * kv_heads * row_blocks;
-  const int64_t want = (3 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (capacity + 63) / 64, 256}));
+  const int64_t want = (4 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (capacity + 63) / 64, kMaxSplits}));
+}
+
+// Allows a kernel more than 48 KB of shared memory, once per device.
+template <typename K>
+int allow_smem(K* kernel, size_t bytes, const char* op) {
+  static std::atomic<bool> set[64] = {};  // idempotent
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && set[dev].load(std::memory_order_acquire)) return NKL_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+  return NKL_OK;
 }
 
 size_t split_bytes(int64_t splits, int64_t batch, int64_t heads, int64_t tokens, int64_t d) {
@@ -385,8 +441,13 @@ extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)(a.splits * a.row_blocks), (unsigned)kv_heads, (unsigned)batch);
-  int rc = dtype == NKL_FLOAT32 ? launch_pdl(tree_attention_kernel<float>, grid, dim3(kThreads), 0, st, op, a)
-                                : launch_pdl(tree_attention_kernel<bf16>, grid, dim3(kThreads), 0, st, op, a);
+  int rc;
+  if (dtype == NKL_FLOAT32) {
+    rc = allow_smem(tree_attention_kernel<float>, tree_smem<float>(kMaxDim), op);
+    if (!rc) rc = launch_pdl(tree_attention_kernel<float>, grid, dim3(kThreads), tree_smem<float>((int)head_dim), st, op, a);
+  } else {
+    rc = launch_pdl(tree_attention_kernel<bf16>, grid, dim3(kThreads), tree_smem<bf16>((int)head_dim), st, op, a);
+  }
   if (rc || a.splits == 1) return rc;
   const int64_t rows = batch * heads * tokens;
   const dim3 join((unsigned)((rows + 3) / 4));
