@@ -55,11 +55,13 @@ extern "C" int nkl_check_device(void* stream) {
   const int g = nkl::gemm_read_and_clear_device_error();
   const int a = nkl::attention_read_and_clear_device_error();
   const int t = nkl::tree_read_and_clear_device_error();
-  if (g < 0 || a < 0 || t < 0) return nkl::fail(NKL_ERR_CUDA, "nkl_check_device: could not read the device flag");
-  if (g || a || t)
+  const int k = nkl::cache_read_and_clear_device_error();
+  if (g < 0 || a < 0 || t < 0 || k < 0) return nkl::fail(NKL_ERR_CUDA, "nkl_check_device: could not read the device flag");
+  if (g || a || t || k)
     return nkl::fail(NKL_ERR_DEVICE,
-                     "nkl_check_device: kernel gave up waiting (gemm code %d, attention code %d, tree attention code %d)",
-                     g, a, t);
+                     "nkl_check_device: kernel gave up waiting (gemm code %d, attention code %d, tree attention code %d, "
+                     "cache code %d)",
+                     g, a, t, k);
   return NKL_OK;
 }
 

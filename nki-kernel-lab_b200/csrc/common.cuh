@@ -47,6 +47,7 @@ int sm_count();
 int gemm_read_and_clear_device_error();
 int attention_read_and_clear_device_error();
 int tree_read_and_clear_device_error();
+int cache_read_and_clear_device_error();
 
 // ---------------------------------------------------------------- device helpers
 
@@ -129,6 +130,11 @@ __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Barrier over the cluster's blocks: what they wrote to memory before it is seen after it.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // Ask L2 to fetch [p, p + bytes) (p 16-byte aligned, bytes a multiple of 16). Issued
 // before pdl_wait it overlaps a kernel's first HBM reads with the previous kernel's

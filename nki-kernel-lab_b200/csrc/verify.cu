@@ -90,10 +90,6 @@ __device__ __forceinline__ void store_remote(u64* p, uint32_t rank, u64 v) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 constexpr int kMaxCluster = 8;
 
 template <typename T, bool VEC>
