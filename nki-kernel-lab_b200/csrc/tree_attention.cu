@@ -7,11 +7,17 @@
 // Query heads share key/value heads (G = heads / kv_heads), so the T * G query rows of a
 // key/value head meet each key together: the cache is read once per G * T rows.
 //
-// CUDA-core kernel (fp32, and bf16 layouts that the tensor-core kernel does not take): a block
-// owns 16 query rows of one key/value head and one range of the keys; each warp has 4 rows,
-// lane x scores key x of a 32-key tile and then accumulates 4 columns; two tiles are on their
-// way (cp.async) while one is worked on. Key ranges split over several blocks leave (max, sum, O)
-// in the workspace; tree_combine_kernel joins them in order.
+// fp32, and bf16 layouts that the tcgen05 kernel does not take: a block owns 16 query rows of
+// one key/value head and one range of the keys, in tiles of 32, two of them on their way
+// (cp.async) while one is worked on. Each of its four warps takes 8 keys of every tile, with a
+// maximum, sum and O of its own, and multiplies with mma.sync m16n8k8 in tf32, a tile of rows as
+// high as the block's. Values are split as x = hi + lo, both tf32, and three of the four products
+// summed (lo lo is 2^-22 of the result): fp32's accuracy at an eighth of the instructions
+// that fp32 multiply-adds took (that kernel spent 5500 cycles on a tile, this one about 1500),
+// which is what bound it. bf16 values are tf32 values: there lo is zero and only P is split. The
+// products of one tile are summed in the tensor core, the tiles in fp32 registers: an accumulator
+// that ran through long rows would gather the tensor core's roundings. Key ranges split over
+// several blocks leave (max, sum, O) in the workspace; tree_combine_kernel joins them in order.
 #include <algorithm>
 #include <atomic>
 
@@ -63,15 +69,6 @@ __device__ __forceinline__ void ancestor_bits(const int* parents, int i, uint32_
   }
 }
 
-template <typename T> __device__ __forceinline__ float4 load4(const T* p);
-template <> __device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
-template <> __device__ __forceinline__ float4 load4<bf16>(const bf16* p) {
-  const uint2 r = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void store4(bf16* p, float4 v) {
   __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
@@ -88,26 +85,52 @@ template <int N> __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Shared memory: queries in fp32, and two tiles of keys and values as they come; a key row is
-// 16 bytes longer than its data, so that 32 lanes reading a row each do not collide.
-template <typename T>
-size_t tree_smem(int d) {
-  return (size_t)kRows * d * 4 + 2 * (size_t)kKeys * (2 * d * sizeof(T) + 16);
+// x = hi + lo, hi rounded to tf32 and lo exact (its low bits are dropped by the product).
+struct Split {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Split split_tf32(float x) {
+  uint32_t hi;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  return {hi, __float_as_uint(x - __uint_as_float(hi))};
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Shared memory: the queries' hi and lo parts, and two tiles of keys and values. Rows are 16
+// bytes longer than their data, so that the lanes of a fragment load do not collide. The ring
+// is reused for the warps' results.
 template <typename T>
+struct TreeShared {
+  int pitch, stage;
+  size_t q_bytes, bytes;
+  __host__ __device__ explicit TreeShared(int d) {
+    pitch = d + 16 / (int)sizeof(T);
+    stage = 2 * kKeys * pitch;  // elements of a tile's keys and values
+    q_bytes = (size_t)kRows * (d + 4) * 8;
+    const size_t ring = 2 * (size_t)stage * sizeof(T), results = 4 * (size_t)kRows * (d + 2) * 4;
+    bytes = q_bytes + (ring > results ? ring : results);
+  }
+};
+
+// ND: 8 columns each, of head_dim up to 8 ND.
+template <typename T, int ND>
 __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
   constexpr int VE = Vec16<T>::N;
+  constexpr bool kExact = sizeof(T) == 2;  // q, k and v are tf32 values as they are
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ __align__(16) float ps[kRows][kKeys];
   pdl_enter();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;  // a fragment's row and column of this lane
   const int split = blockIdx.x / a.row_blocks, r0 = (blockIdx.x % a.row_blocks) * kRows;
   const int kvh = blockIdx.y, b = blockIdx.z;
-  const int rows = a.tokens * a.group, quads = a.d / 4, chunks = a.d / VE, pitch = a.d + VE;
-  float* const qs = reinterpret_cast<float*>(smem);
-  T* const ring = reinterpret_cast<T*>(smem + (size_t)kRows * a.d * 4);
-  const int stage_size = kKeys * (pitch + a.d);
+  const int rows = a.tokens * a.group, nd = a.d / 8, chunks = a.d / VE, q_pitch = a.d + 4;
+  const TreeShared<T> lay(a.d);
+  float2* const qs = reinterpret_cast<float2*>(smem);  // (hi, lo)
+  T* const ring = reinterpret_cast<T*>(smem + lay.q_bytes);
   const int n = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
   // this block's tiles: a share of the cached ones, and the drafted ones in the last split
   const int tiles = (n + kKeys - 1) / kKeys;
@@ -115,148 +138,236 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
   const int t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
   const int end = t1 + (split == a.splits - 1 ? (a.tokens + kKeys - 1) / kKeys : 0);
 
+  // Where the 32 rows of a tile lie (one thread looks one up), and their copies.
+  __shared__ int64_t place[2][kKeys];
+  auto look_up = [&](int t, int r) -> int64_t {
+    const bool cached = t < t1;
+    const int key = (cached ? t : t - t1) * kKeys + r;
+    if (t >= end) return -1;
+    if (!cached) return key < a.tokens ? b * a.n_b + key * a.n_t + kvh * a.n_h : -1;
+    if (key >= n) return -1;
+    const int pi = key / a.page, p = a.tables[(int64_t)b * a.max_pages + pi];
+    return p >= 0 && p < a.pages ? p * a.c_p + kvh * a.c_h + (key - pi * a.page) * a.c_s : -1;
+  };
   const float per_row = 1.f / (float)chunks;
   auto fetch = [&](int t) {  // tile t into its place of the ring
     if (t < end) {
       const bool cached = t < t1;
-      const int key0 = (cached ? t : t - t1) * kKeys;
       const T* const kp = static_cast<const T*>(cached ? a.k_cache : a.k_new);
       const T* const vp = static_cast<const T*>(cached ? a.v_cache : a.v_new);
-      T* const ks = ring + (t & 1) * stage_size;
-      T* const vs = ks + kKeys * pitch;
+      T* const ks = ring + (t & 1) * lay.stage;
+      T* const vs = ks + kKeys * lay.pitch;
+#pragma unroll 4
       for (int i = tid; i < kKeys * chunks; i += kThreads) {
-        const int r = (int)(((float)i + 0.5f) * per_row), c = (i - r * chunks) * VE, key = key0 + r;  // r = i / chunks
-        int64_t at = -1;
-        if (!cached) {
-          if (key < a.tokens) at = b * a.n_b + key * a.n_t + kvh * a.n_h + c;
-        } else if (key < n) {
-          const int pi = key / a.page, p = a.tables[(int64_t)b * a.max_pages + pi];
-          if (p >= 0 && p < a.pages) at = p * a.c_p + kvh * a.c_h + (key - pi * a.page) * a.c_s + c;
-        }
-        copy16_async(ks + r * pitch + c, at >= 0 ? kp + at : nullptr, kp);
-        copy16_async(vs + r * a.d + c, at >= 0 ? vp + at : nullptr, vp);
+        const int r = (int)(((float)i + 0.5f) * per_row), c = (i - r * chunks) * VE;  // r = i / chunks
+        const int64_t at = place[t & 1][r];
+        copy16_async(ks + r * lay.pitch + c, at >= 0 ? kp + at + c : nullptr, kp);
+        copy16_async(vs + r * lay.pitch + c, at >= 0 ? vp + at + c : nullptr, vp);
       }
     }
     copies_commit();  // also where there is nothing: the count of groups goes on
   };
+  if (tid < 2 * kKeys) place[(t0 + (tid >> 5)) & 1][lane] = look_up(t0 + (tid >> 5), lane);
+  const T* q = static_cast<const T*>(a.q) + b * a.q_b;
+  for (int i = tid; i < kRows * chunks; i += kThreads) {
+    const int r = (int)(((float)i + 0.5f) * per_row), c = (i - r * chunks) * VE, row = r0 + r, token = row / a.group;
+    Vec16<T> x;
+    x.raw = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows)
+      x.raw = *reinterpret_cast<const uint4*>(q + token * a.q_t + (kvh * a.group + row - token * a.group) * a.q_h + c);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const Split s = split_tf32(x.get(e));
+      qs[r * q_pitch + c + e] = make_float2(__uint_as_float(s.hi), __uint_as_float(s.lo));
+    }
+  }
+  __syncthreads();
   fetch(t0);
   fetch(t0 + 1);
 
-  const T* q = static_cast<const T*>(a.q) + b * a.q_b;
-  for (int i = tid; i < kRows * quads; i += kThreads) {
-    const int r = i / quads, c = (i - r * quads) * 4, row = r0 + r;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < rows) x = load4<T>(q + (row / a.group) * a.q_t + (kvh * a.group + row % a.group) * a.q_h + c);
-    *reinterpret_cast<float4*>(qs + r * a.d + c) = x;
-  }
+  // the lane's two rows, g and g + 8
   const int* const parents = a.parents ? a.parents + (int64_t)b * a.tokens : nullptr;
-  uint32_t seen[4][4];  // drafted tokens visible to each of the warp's rows
-  bool here[4];
-  float m[4], l[4];
-  float4 o[4];
+  uint32_t seen[2][4];  // drafted tokens visible to them
+  bool here[2];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + warp * 4 + i;
-    const int token = row / a.group;
+  for (int i = 0; i < 2; ++i) {
+    const int row = r0 + g + 8 * i, token = row / a.group;
     here[i] = row < rows && (!parents || parents[token] >= -1);
     seen[i][0] = seen[i][1] = seen[i][2] = seen[i][3] = 0u;
     if (here[i] && end > t1) ancestor_bits(parents, token, seen[i]);
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  // With head_dim up to 64 the warp's halves take the columns twice, for every second key each.
-  const bool halves = quads <= 16;
-  const int col = (halves ? lane & 15 : lane) * 4, key_of = halves ? lane >> 4 : 0, key_step = halves ? 2 : 1;
+  float o[ND][4];
+#pragma unroll
+  for (int j = 0; j < ND; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
   for (int t = t0; t < end; ++t) {
     const bool cached = t < t1;
     const int key0 = (cached ? t : t - t1) * kKeys;
-    const T* const ks = ring + (t & 1) * stage_size;
-    const T* const vs = ks + kKeys * pitch;
+    const T* const ks = ring + (t & 1) * lay.stage + (warp * 8) * lay.pitch;  // this warp's 8 keys
+    const T* const vs = ks + kKeys * lay.pitch;
+    const int64_t next = warp == 0 ? look_up(t + 2, lane) : 0;
     copies_wait<1>();
     __syncthreads();
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    // scores: c[0], c[1] of row g, keys 2 t4 and 2 t4 + 1; c[2], c[3] of row g + 8. The three
+    // products have sums of their own, so that they do not wait for one another.
+    float c[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int c = 0; c < a.d; c += 4) {
-      const float4 kx = load4<T>(ks + lane * pitch + c);
+    for (int s = 0; s < nd; ++s) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // (g, t4), (g + 8, t4), (g, t4 + 4), (g + 8, t4 + 4)
+        const float2 x = qs[(g + 8 * (i & 1)) * q_pitch + 8 * s + t4 + 4 * (i >> 1)];
+        hi[i] = __float_as_uint(x.x);
+        lo[i] = __float_as_uint(x.y);
+      }
+      const float k0 = to_f32(ks[g * lay.pitch + 8 * s + t4]), k1 = to_f32(ks[g * lay.pitch + 8 * s + t4 + 4]);
+      if constexpr (kExact) {
+        mma_tf32(c, hi, __float_as_uint(k0), __float_as_uint(k1));
+      } else {
+        const Split x = split_tf32(k0), y = split_tf32(k1);
+        mma_tf32(c1, lo, x.hi, y.hi);
+        mma_tf32(c2, hi, x.lo, y.lo);
+        mma_tf32(c, hi, x.hi, y.hi);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] += c1[i] + c2[i];
+    const int word = (key0 >> 5) & 3;
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
+      float x[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int key = warp * 8 + 2 * t4 + j;
+        const bool sees = here[i] && (cached ? key0 + key < n : ((drafts >> key) & 1u) != 0u);
+        x[j] = sees ? c[2 * i + j] * a.scale : -INFINITY;
+      }
+      float top = fmaxf(x[0], x[1]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(top, m[i]);
+      const float ref = top == -INFINITY ? 0.f : top;  // nothing seen so far
+      const float keep = expf(m[i] - ref);
+      p[2 * i] = x[0] == -INFINITY ? 0.f : expf(x[0] - ref);
+      p[2 * i + 1] = x[1] == -INFINITY ? 0.f : expf(x[1] - ref);
+      l[i] = l[i] * keep + (p[2 * i] + p[2 * i + 1]);  // this lane's keys; the four lanes' sums meet at the end
+      m[i] = top;
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        o[j][2 * i] *= keep;
+        o[j][2 * i + 1] *= keep;
+      }
+    }
+    if (cached) {
+      // P as the first operand: the columns t4 and t4 + 4 of a fragment stand for the keys 2 t4
+      // and 2 t4 + 1, so the scores' registers are in place and V's rows are taken in that order
+      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float4 qx = *reinterpret_cast<const float4*>(qs + (warp * 4 + i) * a.d + c);
-        s[i] = fmaf(qx.x, kx.x, fmaf(qx.y, kx.y, fmaf(qx.z, kx.z, fmaf(qx.w, kx.w, s[i]))));
+        const Split x = split_tf32(p[2 * (i & 1) + (i >> 1)]);
+        hi[i] = x.hi;
+        lo[i] = x.lo;
       }
-    }
-    const int word = (key0 >> 5) & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
-      const bool sees = here[i] && (cached ? key0 + lane < n : ((drafts >> lane) & 1u) != 0u);
-      const float x = sees ? s[i] * a.scale : -INFINITY;
-      const float top = fmaxf(m[i], warp_max(x));
-      const float ref = top == -INFINITY ? 0.f : top;  // nothing seen so far
-      const float p = sees ? expf(x - ref) : 0.f;
-      const float keep = expf(m[i] - ref);
-      l[i] = l[i] * keep + warp_sum(p);
-      o[i].x *= keep; o[i].y *= keep; o[i].z *= keep; o[i].w *= keep;
-      m[i] = top;
-      ps[warp * 4 + i][lane] = p;
-    }
-    __syncwarp();
-    if (col < a.d && cached) {
-#pragma unroll 4
-      for (int x = key_of; x < kKeys; x += key_step) {
-        const float4 v = load4<T>(vs + x * a.d + col);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = ps[warp * 4 + i][x];
-          o[i].x = fmaf(p, v.x, o[i].x);
-          o[i].y = fmaf(p, v.y, o[i].y);
-          o[i].z = fmaf(p, v.z, o[i].z);
-          o[i].w = fmaf(p, v.w, o[i].w);
+      for (int j = 0; j < ND; ++j) {
+        if (j >= nd) break;
+        const float v0 = to_f32(vs[(2 * t4) * lay.pitch + 8 * j + g]), v1 = to_f32(vs[(2 * t4 + 1) * lay.pitch + 8 * j + g]);
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (kExact) {
+          mma_tf32(y, lo, __float_as_uint(v0), __float_as_uint(v1));
+          mma_tf32(y, hi, __float_as_uint(v0), __float_as_uint(v1));
+        } else {
+          const Split s0 = split_tf32(v0), s1 = split_tf32(v1);
+          mma_tf32(y, lo, s0.hi, s1.hi);
+          mma_tf32(y, hi, s0.lo, s1.lo);
+          mma_tf32(y, hi, s0.hi, s1.hi);
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[j][k] += y[k];
       }
-    } else if (col < a.d) {
+    } else {
       // a drafted token that a row does not see leaves no trace in it, whatever its v holds
-      for (int x = key_of; x < kKeys && key0 + x < a.tokens; x += key_step) {
-        const float4 v = load4<T>(vs + x * a.d + col);
+#pragma unroll 1
+      for (int x = 0; x < 8 && key0 + warp * 8 + x < a.tokens; ++x) {
+        const int from = (lane & ~3) | (x >> 1);  // the lane that has this key's P of the row
+        float w[2];
+        bool sees[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
+          const float w0 = __shfl_sync(0xffffffffu, p[2 * i], from), w1 = __shfl_sync(0xffffffffu, p[2 * i + 1], from);
           const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
-          if (!((drafts >> x) & 1u)) continue;
-          const float p = ps[warp * 4 + i][x];
-          o[i].x = fmaf(p, v.x, o[i].x);
-          o[i].y = fmaf(p, v.y, o[i].y);
-          o[i].z = fmaf(p, v.z, o[i].z);
-          o[i].w = fmaf(p, v.w, o[i].w);
+          w[i] = x & 1 ? w1 : w0;
+          sees[i] = (drafts >> (warp * 8 + x)) & 1u;
+        }
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          if (j >= nd) break;
+          const float v0 = to_f32(vs[x * lay.pitch + 8 * j + 2 * t4]), v1 = to_f32(vs[x * lay.pitch + 8 * j + 2 * t4 + 1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            o[j][2 * i] = sees[i] ? fmaf(w[i], v0, o[j][2 * i]) : o[j][2 * i];
+            o[j][2 * i + 1] = sees[i] ? fmaf(w[i], v1, o[j][2 * i + 1]) : o[j][2 * i + 1];
+          }
         }
       }
     }
+    if (warp == 0) place[t & 1][lane] = next;
     __syncthreads();  // every warp is through with this tile's place
     fetch(t + 2);
   }
   copies_wait<0>();
+  __syncthreads();
 
+  // the four warps' (max, sum, O) through shared memory, in their order
+  float* const ro = reinterpret_cast<float*>(ring);                // [warp][row][d]
+  float* const rml = ro + (size_t)4 * kRows * a.d;                 // [warp][row][2]
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (halves) {
-      o[i].x += __shfl_xor_sync(0xffffffffu, o[i].x, 16);
-      o[i].y += __shfl_xor_sync(0xffffffffu, o[i].y, 16);
-      o[i].z += __shfl_xor_sync(0xffffffffu, o[i].z, 16);
-      o[i].w += __shfl_xor_sync(0xffffffffu, o[i].w, 16);
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    const int r = warp * kRows + g + 8 * i;
+    if (t4 == 0) {
+      rml[2 * r] = m[i];
+      rml[2 * r + 1] = l[i];
     }
-    const int row = r0 + warp * 4 + i;
-    if (row >= rows) continue;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+      if (j < nd) *reinterpret_cast<float2*>(ro + (size_t)r * a.d + 8 * j + 2 * t4) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
+  }
+  __syncthreads();
+  const int quads = a.d / 4;
+  for (int i = tid; i < kRows * quads; i += kThreads) {
+    const int r = i / quads, c = (i - r * quads) * 4, row = r0 + r;
+    if (row >= rows) break;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, rml[2 * (w * kRows + r)]);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = rml[2 * (w * kRows + r)];
+      if (mw == -INFINITY) continue;
+      const float f = expf(mw - top);
+      const float4 y = *reinterpret_cast<const float4*>(ro + (size_t)(w * kRows + r) * a.d + c);
+      sum = fmaf(f, rml[2 * (w * kRows + r) + 1], sum);
+      x.x = fmaf(f, y.x, x.x);
+      x.y = fmaf(f, y.y, x.y);
+      x.z = fmaf(f, y.z, x.z);
+      x.w = fmaf(f, y.w, x.w);
+    }
     if (a.splits == 1) {
-      const float inv = here[i] ? 1.f / l[i] : 0.f;  // an absent token's row is zero
-      const int64_t at = (((int64_t)b * a.tokens + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d;
-      if (key_of == 0 && col < a.d)
-        store4(static_cast<T*>(a.out) + at + col, make_float4(o[i].x * inv, o[i].y * inv, o[i].z * inv, o[i].w * inv));
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;  // 0: an absent token
+      const int64_t at = (((int64_t)b * a.tokens + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d + c;
+      store4(static_cast<T*>(a.out) + at, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
     } else {
       const int64_t at = (((int64_t)split * a.batch + b) * a.kv_heads + kvh) * rows + row;
-      if (key_of == 0 && col < a.d) store4(a.ws_o + at * a.d + col, o[i]);
-      if (lane == 0) {
-        a.ws_ml[2 * at] = m[i];
-        a.ws_ml[2 * at + 1] = l[i];
+      store4(a.ws_o + at * a.d + c, x);
+      if (c == 0) {
+        a.ws_ml[2 * at] = top;
+        a.ws_ml[2 * at + 1] = sum;
       }
     }
   }
@@ -264,44 +375,77 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
 
 constexpr int kMaxSplits = 256;
 
-// Joins the splits of each row, in split order: one warp per row, lane = 4 columns.
-template <typename T>
+// Joins the splits of each row: WARPS warps take them in turn (and half warps, with head_dim
+// up to 64, every second one of these), so that a row of many splits is one round of loads; the
+// partial sums are added in a fixed order.
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
-  __shared__ float weight[4][kMaxSplits];
+  constexpr int kRowsHere = 4 / WARPS;
+  __shared__ float weight[kRowsHere][kMaxSplits];
+  __shared__ float4 part[4][32];
   pdl_enter();
   const int rows = a.tokens * a.group, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * 4 + warp, all = (int64_t)a.batch * a.kv_heads * rows;
-  if (row >= all) return;
-  const int r = (int)(row % rows), kvh = (int)(row / rows % a.kv_heads), b = (int)(row / rows / a.kv_heads);
+  const int mine = warp / WARPS, wi = warp % WARPS;  // this warp's row of the block's, and its share of it
+  const int64_t all = (int64_t)a.batch * a.kv_heads * rows, row = min((int64_t)blockIdx.x * kRowsHere + mine, all - 1);
   const float2* const ml = reinterpret_cast<const float2*>(a.ws_ml) + row;
+  constexpr int kPer = kMaxSplits / 32;
+  float2 x[kPer];
   float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[s * all].x);
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int s = k * 32 + lane;
+    x[k] = s < a.splits ? ml[s * all] : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, x[k].x);
+  }
   m = warp_max(m);
-  for (int s = lane; s < a.splits; s += 32) {
-    const float2 x = ml[s * all];
-    const float w = x.x == -INFINITY ? 0.f : expf(x.x - m);
-    weight[warp][s] = w;
-    l = fmaf(w, x.y, l);
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const float w = x[k].x == -INFINITY ? 0.f : expf(x[k].x - m);
+    if (wi == 0) weight[mine][k * 32 + lane] = w;
+    l = fmaf(w, x[k].y, l);
   }
   l = warp_sum(l);
-  __syncwarp();
+  __syncthreads();
+  const bool halves = a.d <= 64;
+  const int c = (halves ? lane & 15 : lane) * 4;
+  const int first = halves ? wi * 2 + (lane >> 4) : wi, step = halves ? 2 * WARPS : WARPS;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (lane * 4 < a.d) {
-    const float* const po = a.ws_o + row * a.d + lane * 4;
+  if (c < a.d) {
+    const float* const po = a.ws_o + row * a.d + c;
 #pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) {
-      const float w = weight[warp][s];
-      const float4 x = load4<float>(po + s * all * a.d);
-      o.x = fmaf(w, x.x, o.x);
-      o.y = fmaf(w, x.y, o.y);
-      o.z = fmaf(w, x.z, o.z);
-      o.w = fmaf(w, x.w, o.w);
+    for (int s = first; s < a.splits; s += step) {
+      const float w = weight[mine][s];
+      const float4 y = *reinterpret_cast<const float4*>(po + s * all * a.d);
+      o.x = fmaf(w, y.x, o.x);
+      o.y = fmaf(w, y.y, o.y);
+      o.z = fmaf(w, y.z, o.z);
+      o.w = fmaf(w, y.w, o.w);
     }
   }
+  if (halves) {
+    o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
+    o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
+    o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
+    o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
+  }
+  if (WARPS > 1) {
+    part[warp][lane] = o;
+    __syncthreads();
+    if (wi != 0) return;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) {
+      const float4 y = part[warp + w][lane];
+      o.x += y.x;
+      o.y += y.y;
+      o.z += y.z;
+      o.w += y.w;
+    }
+  }
+  if ((int64_t)blockIdx.x * kRowsHere + mine >= all || c >= a.d || (halves && lane >= 16)) return;
+  const int r = (int)(row % rows), kvh = (int)(row / rows % a.kv_heads), b = (int)(row / rows / a.kv_heads);
   const float inv = l > 0.f ? 1.f / l : 0.f;  // 0: an absent token
-  const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + kvh * a.group + r % a.group) * a.d;
-  if (lane * 4 < a.d)
-    store4(static_cast<T*>(a.out) + at + lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+  const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + kvh * a.group + r % a.group) * a.d + c;
+  store4(static_cast<T*>(a.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 }  // namespace
@@ -312,25 +456,27 @@ namespace {
 
 // ------------------------------------------------------------------ host
 
-// Blocks that share a sequence's keys: up to four for each SM, each with at least 64 keys, the
+// Blocks that share a sequence's keys: up to five for each SM, each with at least 64 keys, the
 // two tiles it has on their way at once, of the longest sequence that the tables can hold.
 int split_count(int64_t batch, int64_t kv_heads, int64_t row_blocks, int64_t capacity) {
   const int64_t blocks = batch * kv_heads * row_blocks;
-  const int64_t want = (4 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1);
+  const int64_t want = (5 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1);
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, (capacity + 63) / 64, kMaxSplits}));
 }
 
-// Allows a kernel more than 48 KB of shared memory, once per device.
-template <typename K>
-int allow_smem(K* kernel, size_t bytes, const char* op) {
-  static std::atomic<bool> set[64] = {};  // idempotent
+template <typename T, int ND>
+int launch_split(const TreeArgs& a, dim3 grid, cudaStream_t st) {
+  const char* op = "nkl_attention_tree";
+  static std::atomic<bool> set[64] = {};  // per device: more than 48 KB of shared memory allowed (idempotent)
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && set[dev].load(std::memory_order_acquire)) return NKL_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
-  if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
-  return NKL_OK;
+  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, ND>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)TreeShared<T>(8 * ND).bytes);
+    if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+  }
+  return launch_pdl(tree_attention_kernel<T, ND>, grid, dim3(kThreads), TreeShared<T>(a.d).bytes, st, op, a);
 }
 
 size_t split_bytes(int64_t splits, int64_t batch, int64_t heads, int64_t tokens, int64_t d) {
@@ -442,15 +588,16 @@ extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid((unsigned)(a.splits * a.row_blocks), (unsigned)kv_heads, (unsigned)batch);
   int rc;
-  if (dtype == NKL_FLOAT32) {
-    rc = allow_smem(tree_attention_kernel<float>, tree_smem<float>(kMaxDim), op);
-    if (!rc) rc = launch_pdl(tree_attention_kernel<float>, grid, dim3(kThreads), tree_smem<float>((int)head_dim), st, op, a);
-  } else {
-    rc = launch_pdl(tree_attention_kernel<bf16>, grid, dim3(kThreads), tree_smem<bf16>((int)head_dim), st, op, a);
-  }
+  if (dtype == NKL_FLOAT32)
+    rc = head_dim <= 64 ? launch_split<float, 8>(a, grid, st) : launch_split<float, 16>(a, grid, st);
+  else
+    rc = head_dim <= 64 ? launch_split<bf16, 8>(a, grid, st) : launch_split<bf16, 16>(a, grid, st);
   if (rc || a.splits == 1) return rc;
   const int64_t rows = batch * heads * tokens;
-  const dim3 join((unsigned)((rows + 3) / 4));
-  return dtype == NKL_FLOAT32 ? launch_pdl(tree_combine_kernel<float>, join, dim3(128), 0, st, op, a)
-                              : launch_pdl(tree_combine_kernel<bf16>, join, dim3(128), 0, st, op, a);
+  auto join = [&](auto* kernel, int per_block) {
+    return launch_pdl(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(128), 0, st, op, a);
+  };
+  if (a.splits > 8)
+    return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 4>, 1) : join(tree_combine_kernel<bf16, 4>, 1);
+  return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 1>, 4) : join(tree_combine_kernel<bf16, 1>, 4);
 }
