@@ -55,7 +55,7 @@ struct TcArgs {
   const bf16 *k_new, *v_new;
   int64_t n_b, n_t, n_h;  // its strides
   bf16* out;
-  int* ws_plan;    // [0] X, [1..] prefix sums of the sequences' tiles
+  int4* ws_start;  // [block]: where it starts, for the join: sequence, head and row block, tile
   float* ws_ml;    // [slot][NQ][2][128]
   float4* ws_o;    // [slot][NQ][d / 4][128]
   int batch, tokens, heads, kv_heads, group, pages, page, max_pages;
@@ -153,9 +153,8 @@ __device__ __forceinline__ bool next_piece(const TcArgs& a, Walk& w, Piece& p) {
   return true;
 }
 
-// This block's walk, computed by each warp for itself (a lane takes consecutive sequences);
-// block 0 leaves the prefix sums for the join.
-__device__ __forceinline__ Walk tree_plan(const TcArgs& a, bool leave) {
+// This block's walk, computed by each warp for itself (a lane takes consecutive sequences).
+__device__ __forceinline__ Walk tree_plan(const TcArgs& a) {
   const int lane = threadIdx.x & 31, hms = a.kv_heads * a.row_blocks;
   const int per = (a.batch + 31) >> 5, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
   int sum = 0, longest = 0;
@@ -173,14 +172,6 @@ __device__ __forceinline__ Walk tree_plan(const TcArgs& a, bool leave) {
   longest = __reduce_max_sync(0xffffffffu, longest);
   const int total = __shfl_sync(0xffffffffu, inc, 31) * hms;
   const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, min(longest, kWhole + kExtra));
-  if (leave) {
-    if (lane == 0) a.ws_plan[0] = share;
-    int before = inc - sum;
-    for (int b = b0; b < b1; ++b) {
-      a.ws_plan[1 + b] = before;
-      before += tree_tiles(a, b) + kExtra;
-    }
-  }
   // Where this block's range begins (even lanes) and ends (odd lanes): the lane whose sequences
   // hold the place, the sequence among them, the segment of the sequence, the tile of the segment.
   const int from = (int)blockIdx.x * share, at = from + (lane & 1) * share;
@@ -280,7 +271,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
   pdl_wait();
-  Walk w = tree_plan(a, a.ws_plan != nullptr && blockIdx.x == 0 && warp == 0);
+  Walk w = tree_plan(a);
+  if (a.ws_start && threadIdx.x == 0) a.ws_start[blockIdx.x] = make_int4(w.b, w.hm, w.t, 0);
 
   if (warp == kKeyWarp || warp == kValueWarp) {
     // ------------------------------------------------ TMA
@@ -826,29 +818,26 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 }
 
 // Joins the pieces of the segments that were cut: out = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p,
-// in order of the pieces. A block takes 8 rows of a segment, a thread 4 columns of one row.
+// in order of the pieces. blockIdx.y: a block of the attention kernel that begins inside a
+// segment, the first one that does; blockIdx.x: 8 rows of the segment, a thread 4 columns of one row.
 template <int D, int NQ>
-__global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant__ TcArgs a) {
+__global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant__ TcArgs a, int blocks) {
+  __shared__ int stop;  // the first later block that does not begin inside the segment
   pdl_enter();
-  const int b = blockIdx.z, hm = blockIdx.y, hms = a.kv_heads * a.row_blocks;
-  const int kvh = hm / a.row_blocks, mb = hm - kvh * a.row_blocks;
-  const int share = a.ws_plan[0], n = tree_tiles(a, b);
-  const long long first = (long long)a.ws_plan[1 + b] * hms + (long long)hm * (n + kExtra);
-  // cuts strictly inside the segment belong to blocks lo .. hi, in a row
-  int lo = (int)(first / share) + 1, hi = (int)((first + n + kExtra - 1) / share);
-  while (lo <= hi) {
-    const int off = (int)((long long)lo * share - first), at = cut_at(off, n, share);
-    if (at > 0 && at < n) break;
-    ++lo;
+  const int c = blockIdx.y + 1;
+  if (threadIdx.x == 0) stop = blocks;
+  const int4 at = a.ws_start[c], before = a.ws_start[c - 1];
+  __syncthreads();
+  if (at.z == 0 || (before.x == at.x && before.y == at.y && before.z > 0)) return;
+  for (int i = c + 1 + threadIdx.x; i < blocks; i += 2 * D) {
+    const int4 x = a.ws_start[i];
+    if (x.x != at.x || x.y != at.y || x.z == 0) atomicMin(&stop, i);
   }
-  while (lo <= hi) {
-    const int off = (int)((long long)hi * share - first), at = cut_at(off, n, share);
-    if (at > 0 && at < n) break;
-    --hi;
-  }
-  if (lo > hi) return;
-  const int pieces = hi - lo + 2;  // piece 0 is the end of block lo - 1, piece i the beginning of block lo - 1 + i
-  const int x0 = blockIdx.x * 8;   // the block's rows, all of one query tile
+  __syncthreads();
+  const int b = at.x, hm = at.y, lo = c;
+  const int kvh = a.row_blocks == 1 ? hm : hm / a.row_blocks, mb = hm - kvh * a.row_blocks;
+  const int pieces = stop - c + 1;  // piece 0 is the end of block c - 1, piece i the beginning of block c - 1 + i
+  const int x0 = blockIdx.x * 8;    // the block's rows, all of one query tile
   const int ti = x0 / kTile, r0 = x0 - ti * kTile;
   auto slot = [&](int i) { return (int64_t)((i == 0 ? 2 * (lo - 1) + 1 : 2 * (lo - 1 + i)) * NQ + ti); };
   // The pieces' weights 2^(m_p - m) for the 8 rows, and 1 / sum_p 2^(m_p - m) l_p.
@@ -928,7 +917,7 @@ TcPlan tc_plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, i
   p.grid = (int)std::min<int64_t>(std::min(sm_count(), kMaxPieces - 1), p.join ? segments * seg_tiles : segments);
   if (p.join) {
     const size_t slots = 2 * (size_t)p.grid * p.nq;
-    p.ml_off = ((size_t)(batch + 1) * 4 + 255) & ~size_t(255);
+    p.ml_off = ((size_t)p.grid * 16 + 255) & ~size_t(255);
     p.o_off = p.ml_off + slots * 2 * kTile * 4;
     p.bytes = p.o_off + slots * kTile * d * 4;
   }
@@ -970,7 +959,7 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
   a.n_h = g.n_h;
   a.out = static_cast<bf16*>(g.out);
   if (p.join) {
-    a.ws_plan = reinterpret_cast<int*>(ws);
+    a.ws_start = reinterpret_cast<int4*>(ws);
     a.ws_ml = reinterpret_cast<float*>(ws + p.ml_off);
     a.ws_o = reinterpret_cast<float4*>(ws + p.o_off);
   }
@@ -998,11 +987,10 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
   }
   int rc = launch_pdl(tree_attention_tc_kernel<D, NQ>, dim3((unsigned)p.grid), dim3(kTcThreads), smem, st, op, mq, mkn,
                       mvn, mkc, mvc, a);
-  if (rc || !p.join) return rc;
+  if (rc || !p.join || p.grid < 2) return rc;
   const int rows = std::min<int>(NQ == 1 ? p.tt * g.group : NQ * kTile, NQ == 1 ? g.tokens * g.group : NQ * kTile);
-  return launch_pdl(tree_join_kernel<D, NQ>,
-                    dim3((unsigned)((rows + 7) / 8), (unsigned)(g.kv_heads * p.row_blocks), (unsigned)g.batch),
-                    dim3(2 * D), 0, st, op, a);
+  return launch_pdl(tree_join_kernel<D, NQ>, dim3((unsigned)((rows + 7) / 8), (unsigned)(p.grid - 1)), dim3(2 * D), 0, st,
+                    op, a, p.grid);
 }
 
 }  // namespace
