@@ -7,7 +7,7 @@
 // types TypeError, tensors on the wrong device RuntimeError, a refusal of the C ABI a
 // RuntimeError that begins with the entry point's name (nkilab.ops makes it an NklError).
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -50,7 +50,11 @@ const int32_t* ints(const char* name, OptTensor t, c10::Device dev, at::IntArray
 
 int32_t* out_ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
 
-Tensor new_ints(at::IntArrayRef shape, c10::Device dev) { return at::empty(shape, at::dtype(at::kInt).device(dev)); }
+// Straight from the caching allocator, past the dispatcher.
+Tensor new_tensor(at::IntArrayRef shape, at::ScalarType type, c10::Device dev) {
+  return at::detail::empty_cuda(shape, type, dev, std::nullopt);
+}
+Tensor new_ints(at::IntArrayRef shape, c10::Device dev) { return new_tensor(shape, at::kInt, dev); }
 
 void same(const Tensor& t, const Tensor& ref) {
   TORCH_CHECK_TYPE(t.scalar_type() == ref.scalar_type(), "mixed dtypes: ", t.scalar_type(), " vs ", ref.scalar_type());
@@ -100,7 +104,7 @@ Table check_table(const Tensor& tables, OptTensor lens, const Tensor& refs) {
 // capture into a graph gets one of the graph's own pool, so graphs never share.
 void* workspace(c10::Device dev, cudaStream_t stream, size_t bytes, Tensor& hold) {
   if (bytes == 0) return nullptr;
-  const auto make = [&] { return at::empty({(int64_t)bytes}, at::dtype(at::kByte).device(dev)); };
+  const auto make = [&] { return new_tensor({(int64_t)bytes}, at::kByte, dev); };
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
     hold = make();
     return hold.data_ptr();
@@ -140,7 +144,7 @@ Tensor attention_tree(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   const auto [k, v] = rows_of(k_in, v_in);
   const c10::cuda::CUDAGuard guard(dev);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-  Tensor out = at::empty({B, T, H, d}, q.options().memory_format(at::MemoryFormat::Contiguous)), hold;
+  Tensor out = new_tensor({B, T, H, d}, q.scalar_type(), dev), hold;
   const size_t bytes = nkl_attention_tree_workspace_size(B, T, H, Hkv, d, page, M, dt);
   void* ws = workspace(dev, st, bytes, hold);
   check("nkl_attention_tree",

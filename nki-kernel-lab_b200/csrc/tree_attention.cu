@@ -19,6 +19,7 @@
 // that ran through long rows would gather the tensor core's roundings. Key ranges split over
 // several blocks leave (max, sum, O) in the workspace; tree_combine_kernel joins them in order.
 #include <algorithm>
+#include <cstddef>
 #include <atomic>
 
 #include "attn_math.cuh"

@@ -124,6 +124,13 @@ struct TreeSmem {
   uint32_t tmem_base;
   int abort;
 };
+template <int D, int NQ>
+constexpr bool tiles_aligned() {
+  using S = TreeSmem<D, NQ>;
+  return offsetof(S, k) % 1024 == 0 && offsetof(S, v) % 1024 == 0;
+}
+static_assert(tiles_aligned<128, 1>() && tiles_aligned<128, 2>() && tiles_aligned<64, 1>() && tiles_aligned<64, 2>(),
+              "swizzled tiles are 1024-byte aligned");
 
 __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
@@ -439,17 +446,26 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
               if (!(ok = mbar_wait(&s.p_full[g][h], use & 1u, &s.abort, &g_tree_dev_error, 24))) break;
               tc_fence_after();
               issue_pv(g, h, t >= kAhead || h > 0, two);
+              if (NQ == 2 && t == 0 && i == 0 && h == 0) {
+                // The second group starts half a tile behind the first, and stays there: the groups
+                // take turns at the special function unit and the tensor core.
+                issue_s(1, 1);
+                free_k();
+                if (n == 1) mma_commit(&s.q_empty);
+              }
             }
             if (!ok) break;
-            if (more) {
+            if (more && !(NQ == 2 && t < 0 && i == 1)) {
               if (i == 0 && !(ok = wait_k())) break;
               issue_s(g, NQ == 1 ? 0 : i);
             }
           }
           if (!ok) break;
           if (t >= 0) free_v();
-          if (more) free_k();
-          if (t + kAhead == n - 1) mma_commit(&s.q_empty);
+          if (more && !(NQ == 2 && t < 0)) {
+            free_k();
+            if (t + kAhead == n - 1) mma_commit(&s.q_empty);
+          }
         }
         if (!ok) break;
         gt += (uint32_t)n;

@@ -180,11 +180,6 @@ _attention_tree, _cache_append, _cache_reserve, _cache_fork, _cache_free, _cache
               "verify_drafts"))
 
 
-def _layers(*ts):
-    """Each tensor with its leading [layers] dimension."""
-    return tuple(t if t.dim() == 5 else t.unsqueeze(0) for t in ts)
-
-
 def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=None):
     """Attention of T drafted tokens per sequence over its cached positions and, as a tree,
     over each other. q: [B, T, H, d]; k, v: [B, T, Hkv, d], the drafted tokens' own, not yet
@@ -206,7 +201,9 @@ def cache_append(k, v, k_cache, v_cache, tables, lens, path=None, count=None):
     onward and returns the new lengths: row path[b, j] for j < count[b] (the accepted path
     of drafted tokens), or all T rows in order. The pages come from cache_reserve; rows
     without a page are dropped."""
-    return _cache_append(*_layers(k, v, k_cache, v_cache), tables, lens, path, count)
+    if k_cache.dim() == 4:  # one layer
+        k, v, k_cache, v_cache = (t.unsqueeze(0) for t in (k, v, k_cache, v_cache))
+    return _cache_append(k, v, k_cache, v_cache, tables, lens, path, count)
 
 
 def cache_reserve(tables, lens, refs, extra, page_size):
@@ -220,7 +217,9 @@ def cache_fork(k_cache, v_cache, tables, lens, refs, src, dst):
     """Slot dst[f] becomes a copy of slot src[f]: full pages are shared, the last, partly
     filled one is copied to a free page. Returns (tables, lens, refs, missing); with
     missing [1] > 0 (too few free pages) nothing is forked."""
-    return _cache_fork(*_layers(k_cache, v_cache), tables, lens, refs, src, dst)
+    if k_cache.dim() == 4:  # one layer
+        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
+    return _cache_fork(k_cache, v_cache, tables, lens, refs, src, dst)
 
 
 def cache_free(tables, lens, refs, slots):
@@ -230,7 +229,9 @@ def cache_free(tables, lens, refs, slots):
 
 def cache_compact(k_cache, v_cache, tables, refs):
     """Moves the pages in use to the lowest indices. Returns (tables, refs)."""
-    return _cache_compact(*_layers(k_cache, v_cache), tables, refs)
+    if k_cache.dim() == 4:  # one layer
+        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
+    return _cache_compact(k_cache, v_cache, tables, refs)
 
 
 def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):
