@@ -262,7 +262,17 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
         o[j][2 * i + 1] *= keep;
       }
     }
-    if (cached) {
+    // A drafted token that a row does not see leaves no trace in it, whatever its v holds: where
+    // this warp's eight rows of v hold infinities or NaN, 0 times them is not summed but left out.
+    bool finite = true;
+    if (!cached) {
+      for (int i = lane; i < 8 * a.d; i += 32) {
+        const int x = i / a.d;
+        finite &= fabsf(to_f32(vs[x * lay.pitch + i - x * a.d])) < INFINITY;
+      }
+      finite = __all_sync(0xffffffffu, finite);
+    }
+    if (finite) {
       // P as the first operand: the columns t4 and t4 + 4 of a fragment stand for the keys 2 t4
       // and 2 t4 + 1, so the scores' registers are in place and V's rows are taken in that order
       uint32_t hi[4], lo[4];
@@ -290,7 +300,6 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
         for (int k = 0; k < 4; ++k) o[j][k] += y[k];
       }
     } else {
-      // a drafted token that a row does not see leaves no trace in it, whatever its v holds
 #pragma unroll 1
       for (int x = 0; x < 8 && key0 + warp * 8 + x < a.tokens; ++x) {
         const int from = (lane & ~3) | (x >> 1);  // the lane that has this key's P of the row

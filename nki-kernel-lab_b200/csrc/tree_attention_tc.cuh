@@ -42,7 +42,8 @@ constexpr int kKeyWarp = 8, kMmaWarp = 9, kValueWarp = 10, kMendWarp = 11;
 constexpr int kFewDrafts = 16;   // so many drafted tokens can share the last cached tile
 constexpr int kWhole = 4;        // segments of up to so many tiles are not cut
 constexpr int kMaxPieces = 192;  // of one segment: at most one for each block and one more
-constexpr int kExtra = 3;        // a segment's beginning and end, in tiles
+constexpr int kLeast = 2;        // least share of a block, in tiles
+constexpr int kExtra = 4;        // a segment's beginning and end, in tiles
 // Sequences of up to so many cached positions have P in two bf16 parts, P V in two products: a
 // row that sees few keys does not average the roundings of P out (one part: up to 2^-8 of a
 // weight). The second product is hidden behind the loads there is time for; on long rows,
@@ -164,11 +165,10 @@ __device__ __forceinline__ bool next_piece(const TcArgs& a, Walk& w, Piece& p) {
 __device__ __forceinline__ Walk tree_plan(const TcArgs& a) {
   const int lane = threadIdx.x & 31, hms = a.kv_heads * a.row_blocks;
   const int per = (a.batch + 31) >> 5, b0 = min(lane * per, a.batch), b1 = min(b0 + per, a.batch);
-  int sum = 0, longest = 0;
+  int sum = 0;
   for (int b = b0; b < b1; ++b) {
     const int t = tree_tiles(a, b) + kExtra;
     sum += t;
-    longest = max(longest, t);
   }
   int inc = sum;
 #pragma unroll
@@ -176,9 +176,8 @@ __device__ __forceinline__ Walk tree_plan(const TcArgs& a) {
     const int x = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += x;
   }
-  longest = __reduce_max_sync(0xffffffffu, longest);
   const int total = __shfl_sync(0xffffffffu, inc, 31) * hms;
-  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, min(longest, kWhole + kExtra));
+  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kLeast);
   // Where this block's range begins (even lanes) and ends (odd lanes): the lane whose sequences
   // hold the place, the sequence among them, the segment of the sequence, the tile of the segment.
   const int from = (int)blockIdx.x * share, at = from + (lane & 1) * share;
