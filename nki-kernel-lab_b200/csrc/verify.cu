@@ -19,10 +19,16 @@
 //
 // A cluster of blocks takes one sequence. Each block walks for itself (some hundred values,
 // from L2); then each warp sums a contiguous part of the one row (with q: two) that the next
-// token is drawn from, the blocks exchange their sums through shared memory, and the warp in
-// whose part the drawn place lies reads that part once more, from L2. So each of those rows is
-// read from HBM once, which is what bounds a batch; a single sequence is bound by the chain of
-// three dependent reads and the exchange.
+// token is drawn from, the blocks exchange their sums through shared memory, and the block that
+// holds the drawn place reads the part of the warp where it lies once more, from L2, a step for
+// each of its warps. So each of those rows is read from HBM once.
+//
+// Measured, fp32, GPU time: 64 chains of 8 over 131072 (two rows each, 67 MB) 20.5 us, of which
+// 10.3 us by bytes; the rest is the chain launch -> tokens -> gathered probabilities -> first
+// vectors of the rows, and after them exchange -> part, which does not overlap the reading. With the
+// part read by its warp alone, four steps at a time, it was 26.1 us; with one block to a sequence
+// and one element a lane at a time 204 us. One tree of 24 over 32768 is that chain and no more:
+// 7.8 us, with one block 40 us.
 #include "common.cuh"
 
 namespace nkl {
@@ -225,60 +231,61 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   u64 before = 0;
   for (int r = 0; r < rank; ++r) before += s_blocks[r][plain];
   if (t < before || t >= before + s_blocks[rank][plain]) return;  // another block has it
-  for (int w = 0; w < warp; ++w) before += plain ? s_all[w] : s_sum[w];
-  if (t < before || t >= before + (plain ? s_all[warp] : s_sum[warp])) return;  // another warp
-  // this warp's part again, element by element
-  constexpr int kBatch = 4;
-  for (int x0 = lo; x0 < hi; x0 += kBatch * step) {
-    uint32_t w[kBatch][VE];
+  // the warp that has it, whose part the block's warps read again, a step each
+  int owner = 0;
+  for (; owner < kVerifyWarps - 1; ++owner) {
+    const u64 x = plain ? s_all[owner] : s_sum[owner];
+    if (t < before + x) break;
+    before += x;
+  }
+  __syncthreads();  // the sums' place is used again
+  const int64_t from = (int64_t)(rank * kVerifyWarps + owner) * per_warp;
+  const int part_lo = (int)min(from, (int64_t)V), part_hi = min(part_lo + per_warp, V);
+  for (int base = part_lo; base < part_hi; base += kVerifyWarps * step) {
+    const int x0 = base + warp * step + lane * VE;
+    uint32_t w[VE];
+    load_row<T, VEC>(p, x0, part_hi, w);
+    if (q && !plain) {
+      uint32_t qw[VE];
+      load_row<T, VEC>(q, x0, part_hi, qw);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int x = x0 + i * step + lane * VE;
-      load_row<T, VEC>(p, x, hi, w[i]);
-      if (q && !plain) {
-        uint32_t qw[VE];
-        load_row<T, VEC>(q, x, hi, qw);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) w[i][e] = w[i][e] > qw[e] ? w[i][e] - qw[e] : 0u;
-      }
+      for (int e = 0; e < VE; ++e) w[e] = w[e] > qw[e] ? w[e] - qw[e] : 0u;
     }
     if (!draft && !plain) {
       for (int j = 0; j < n; ++j) {
         if (s_parent[j] != last) continue;
-        const int off = s_token[j] - x0 - lane * VE;  // place of a rejected token among the lane's elements
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-          for (int e = 0; e < VE; ++e) w[i][e] = off == i * step + e ? 0u : w[i][e];
+        for (int e = 0; e < VE; ++e) w[e] = s_token[j] == x0 + e ? 0u : w[e];
       }
     }
+    u64 mine = 0;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      u64 mine = 0;
+    for (int e = 0; e < VE; ++e) mine += w[e];
+    u64 to = mine;  // the sum up to this lane
 #pragma unroll
-      for (int e = 0; e < VE; ++e) mine += w[i][e];
-      u64 inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + inc > t);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          u64 at = before + inc - mine;
-          int e = 0;
-#pragma unroll
-          for (int k = 0; k < VE; ++k) {
-            at += w[i][k];
-            if (at <= t) e = k + 1;
-          }
-          a.token[b] = x0 + i * step + lane * VE + e;
-        }
-        return;
-      }
-      before += __shfl_sync(0xffffffffu, inc, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += y;
     }
+    if (lane == 31) s_sum[warp] = to;
+    __syncthreads();
+    u64 at = before;
+    for (int k = 0; k < kVerifyWarps; ++k) {
+      if (k < warp) at += s_sum[k];
+      before += s_sum[k];
+    }
+    at += to - mine;
+    if (t >= at && t < at + mine) {  // one lane of the block at most
+      int e = 0;
+#pragma unroll
+      for (int k = 0; k < VE; ++k) {
+        at += w[k];
+        if (at <= t) e = k + 1;
+      }
+      a.token[b] = x0 + e;
+    }
+    if (t < before) return;
+    __syncthreads();
   }
 }
 
