@@ -520,7 +520,7 @@ extern "C" size_t nkl_attention_tree_workspace_size(int64_t batch, int64_t token
   if (!valid_dtype(dtype) || !tree_sizes_ok(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages) ||
       batch == 0 || tokens == 0)
     return 0;
-  // strides and the scale's sign, which are not known here, may still choose the CUDA-core kernel
+  // strides and the scale's sign, which are not known here, may still choose the other kernel
   const TcPlan p = tc_plan(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages, dtype);
   const int64_t row_blocks = (tokens * (heads / kv_heads) + kRows - 1) / kRows;
   return std::max(p.on ? p.bytes : 0, split_bytes(split_count(batch, kv_heads, row_blocks, page_size * max_pages),
@@ -608,6 +608,8 @@ extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const
   auto join = [&](auto* kernel, int per_block) {
     return launch_pdl(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(128), 0, st, op, a);
   };
+  // Four warps to a row where many splits meet: 5 sequences of up to 1999 positions 18.2 against 19.3 us,
+  // one of 8000 28.5 against 33.4; one where few do: 16 of 700, 33 tokens, 118 against 121 us.
   if (a.splits > 8)
     return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 4>, 1) : join(tree_combine_kernel<bf16, 4>, 1);
   return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 1>, 4) : join(tree_combine_kernel<bf16, 1>, 4);

@@ -291,10 +291,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
 
 template <typename T>
 int launch_verify(const VerifyArgs& a, cudaStream_t st) {
-  // Blocks per sequence: up to eight, as long as all fit the GPU at once (two to an SM by their
-  // registers) and a warp's part still has a step of its own.
+  // Blocks per sequence: up to eight, as long as there are no more than three for each SM (two
+  // fit at once) and a warp's part still has a step of its own. Measured over 131072, chains, with
+  // 1, 2, 4, 8 blocks: 4 sequences 24.4, 14.6, 10.0, 7.6 us; 32: 47, 27, 17, 13.7; 64: 50, 29, 20.7,
+  // 25.6; 100: 52, 33, 27, 34; 200: 57, 43, 43, 52; 400: 73, 71, 69, 85.
   int blocks = kMaxCluster;
-  while (blocks > 1 && ((int64_t)a.batch * blocks > 2LL * sm_count() ||
+  while (blocks > 1 && ((int64_t)a.batch * blocks > 3LL * sm_count() ||
                         (int64_t)blocks * kVerifyWarps * 32 * Vec16<T>::N > 2LL * a.vocab))
     blocks /= 2;
   const bool vec = a.vocab % Vec16<T>::N == 0 && is_aligned(a.probs, 16) && (!a.draft || is_aligned(a.draft, 16));
