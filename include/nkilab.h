@@ -356,7 +356,9 @@ size_t nkl_attention_tree_workspace_size(int64_t batch, int64_t tokens, int64_t 
  * [page, head, row]. head_dim a multiple of 8 up to 128, tokens <= NKL_MAX_DRAFTED, 16-byte
  * aligned pointers. fp32 accumulation and softmax statistics; the output is rounded once,
  * and the bf16 tensor-core kernel (head_dim 64 or 128, page_size a multiple of 8, at most
- * 128 query heads per kv head) rounds the exponentials to bf16 for their product with v. */
+ * 128 query heads per kv head) takes the exponentials in bf16 for their product with v: as a
+ * sum of two for sequences of up to 1024 cached positions, rounded to one, with the sum of
+ * the rounded ones below it, for longer ones. */
 int nkl_attention_tree(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
                        const int64_t* new_strides, const void* k_cache, const void* v_cache,
                        const int64_t* cache_strides, const int32_t* tables, const int32_t* lens,
@@ -368,7 +370,8 @@ int nkl_attention_tree(const void* q, const int64_t* q_strides, const void* k_ne
  * path[b, j] of sequence b, for j < count[b], goes to position lens[b] + j of every layer;
  * lens_out = lens + count. path NULL: row j; count NULL: tokens. The pages have to be in
  * the tables (nkl_cache_reserve) and belong to one slot alone: a row without a page is
- * dropped. Strides: k and v [layer, batch, token, head], cache [layer, page, head, row]. */
+ * dropped. At most 65535 sequences and 1 MB in a token's row of all heads. Strides: k and v
+ * [layer, batch, token, head], cache [layer, page, head, row]. */
 int nkl_cache_append(const void* k, const void* v, const int64_t* kv_strides, void* k_cache, void* v_cache,
                      const int64_t* cache_strides, const int32_t* tables, const int32_t* lens, const int32_t* path,
                      const int32_t* count, int32_t* lens_out, int64_t layers, int64_t batch, int64_t tokens,

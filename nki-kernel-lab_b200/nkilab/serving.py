@@ -130,8 +130,10 @@ def speculative_step(blocks: list[DecoderBlock], embedding: torch.Tensor, head: 
     tokens = torch.cat([last[:, None], drafts], 1).clamp(0, embedding.shape[0] - 1)
     if parents is None:
         tree = None
-    else:  # `last` is the root: the others move up by one, absent ones stay absent
-        up = torch.where(parents < -1, parents, parents + 1)
+    else:  # `last` is the root: the others move up by one, absent ones stay absent, and one whose
+        # parent is no earlier token follows `last`, as it does in the verification
+        late = parents >= torch.arange(parents.shape[1], device=parents.device)
+        up = torch.where(parents < -1, parents, (parents + 1).masked_fill(late, 0))
         tree = torch.cat([torch.full_like(parents[:, :1], -1), up], 1)
     y, k, v = decode(blocks, embedding[tokens.long()], cache, tree)
     path, count, token = ops.verify_drafts(probabilities(y, head), drafts, uniforms, parents, draft_probs)

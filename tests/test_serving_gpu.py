@@ -112,6 +112,28 @@ def test_speculative_steps_keep_what_was_accepted(tree):
         assert (y[b, 0].float() - want).abs().max() / want.abs().max() < BOUND[dtype]
 
 
+def test_a_draft_without_an_earlier_parent_follows_the_last_token():
+    """A parent that is the token itself or a later one counts as none, in every part of a step."""
+    blocks = blocks_of(2, torch.float32)
+    embedding, head = torch.randn(64, 256, device=DEV), torch.randn(256, 64, device=DEV) * 0.05
+    prompt = torch.randn(1, 9, 256, device=DEV)
+    drafts = torch.tensor([[3, 14, 15, 9, 26]], dtype=torch.int32, device=DEV)
+    last = torch.tensor([5], dtype=torch.int32, device=DEV)
+    uniforms = torch.tensor([[0.0] * 5 + [0.5]], device=DEV)  # a first child is always accepted
+    got = []
+    for parents in ([-1, 0, 1, -1, 3], [0, 0, 1, 4, 3]):
+        cache = PagedCache(2, 1, 4, 4, 64, page_size=8, dtype=torch.float32)
+        cache.reserve(20)
+        cache.append(*decode(blocks, prompt, cache)[1:])
+        tree = torch.tensor([parents], dtype=torch.int32, device=DEV)
+        out = speculative_step(blocks, embedding, head, cache, last, drafts, uniforms, tree)
+        pages = cache.k[:, cache.tables[0, :3].long()]  # [layers, 3, heads, page, head_dim]
+        got.append([*out, cache.lens, pages.transpose(2, 3).flatten(1, 2)[:, :int(cache.lens)]])
+    assert got[0][0].tolist() == [[0, 1, 2, -1, -1]]
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 def test_a_step_replays_from_a_graph():
     dtype, V, B = torch.bfloat16, 64, 2
     blocks = blocks_of(1, dtype)
