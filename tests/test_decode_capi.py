@@ -149,3 +149,29 @@ def test_wrappers_take_no_cpu_tensors():
         ops.verify_drafts(torch.ones(1, 2, 4), i, torch.zeros(1, 2))
     with pytest.raises(NotImplementedError):
         ops.cache_free(i, i[0], i[0], i[0])
+
+
+def test_shapes_without_a_gpu():
+    """The operators' shape functions: what a trace or an allocation ahead of the call sees."""
+    import torch
+
+    from nkilab import ops
+
+    def m(*shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    bf = torch.bfloat16
+    L, B, T, H, Hkv, d, P, page, M, V = 3, 2, 5, 8, 2, 64, 20, 16, 7, 50
+    cache = m(L, P, Hkv, page, d, dtype=bf)
+    tables, lens, refs = m(B, M), m(B), m(P)
+    out = ops.attention_tree(m(B, T, H, d, dtype=bf), m(B, T, Hkv, d, dtype=bf), m(B, T, Hkv, d, dtype=bf), cache[0], cache[0],
+                             tables, lens, m(B, T))
+    assert out.shape == (B, T, H, d) and out.dtype == bf
+    rows = m(L, B, T, Hkv, d, dtype=bf)
+    assert ops.cache_append(rows, rows, cache, cache, tables, lens).shape == (B,)
+    assert [t.shape for t in ops.cache_reserve(tables, lens, refs, m(B), page)] == [(B, M), (P,), (1,)]
+    assert [t.shape for t in ops.cache_fork(cache, cache, tables, lens, refs, m(1), m(1))] == [(B, M), (B,), (P,), (1,)]
+    assert [t.shape for t in ops.cache_free(tables, lens, refs, m(1))] == [(B, M), (B,), (P,)]
+    assert [t.shape for t in ops.cache_compact(cache, cache, tables, refs)] == [(B, M), (P,)]
+    got = ops.verify_drafts(m(B, T + 1, V, dtype=torch.float32), m(B, T), m(B, T + 1, dtype=torch.float32))
+    assert [t.shape for t in got] == [(B, T), (B,), (B,)] and all(t.dtype == torch.int32 for t in got)
