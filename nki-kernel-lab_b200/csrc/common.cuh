@@ -90,11 +90,14 @@ template <typename T> __device__ __forceinline__ uint4 pack16(const float* f) {
   return r;
 }
 
-// Streaming 16-byte global load that does not allocate in L1 (data is touched once).
+// Streaming 16-byte global load that does not allocate in L1 (data is touched once). Not an
+// .nc load: those are for memory that nothing writes while the kernel runs, and a kernel that
+// was launched early runs while the one before it still writes. After an l2_prefetch from before
+// the wait, .nc loads of the other die's memory gave the prefetched, old contents.
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
   return r;
 }
 
