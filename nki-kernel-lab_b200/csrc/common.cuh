@@ -93,7 +93,7 @@ template <typename T> __device__ __forceinline__ uint4 pack16(const float* f) {
 // Streaming 16-byte global load that does not allocate in L1 (data is touched once). Not an
 // .nc load: those are for memory that nothing writes while the kernel runs, and a kernel that
 // was launched early runs while the one before it still writes. After an l2_prefetch from before
-// the wait, .nc loads of the other die's memory gave the prefetched, old contents.
+// the wait, .nc loads gave the prefetched, old contents.
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 r;
   asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"

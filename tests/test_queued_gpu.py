@@ -60,3 +60,43 @@ def test_reads_what_the_kernel_before_wrote(name):
     torch.cuda.synchronize()
     for y in got:
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("name", ["matmul", "attention", "attention_tree"])
+def test_tiles_of_what_the_kernel_before_wrote(name):
+    """The same where the reader fetches tiles, the first of them asked for before it may read."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(16, 1024, 128, generator=g).to(DEV, BF)
+    w = (torch.randn(2048, 1024, generator=g) * 0.02).to(DEV, BF)
+    ones = torch.ones(2048, device=DEV, dtype=BF)
+    kc = torch.randn(16, 16, 64, 128, generator=g).to(DEV, BF)
+    tables, lens = torch.arange(16, device=DEV).int()[None], torch.tensor([1000], device=DEV).int()
+
+    def write():
+        return ops.rmsnorm(x.view(-1, 2048), ones) if name == "matmul" else ops.rope(x)
+
+    def read(h):
+        if name == "matmul":
+            return ops.matmul(h, w)
+        if name == "attention":
+            return ops.attention(h, h, h)
+        q = h.view(16, 16, 64, 128)[None, :, :, 0].transpose(1, 2)  # 16 tokens of 16 heads
+        return ops.attention_tree(q, q, q, kc, kc, tables, lens)
+
+    h = write()
+    torch.cuda.synchronize()
+    want = read(h)
+    torch.cuda.synchronize()
+    del h
+    busy = torch.randn(4096, 4096, device=DEV, dtype=BF)
+    got = []
+    for i in range(12):
+        if i % 6 == 0:
+            for _ in range(8):
+                busy @ busy
+        old = torch.full((x.numel(),), 7.0, device=DEV, dtype=BF)
+        del old
+        got.append(read(write()))
+    torch.cuda.synchronize()
+    for y in got:
+        assert torch.equal(y, want)
