@@ -467,14 +467,12 @@ namespace {
 
 // ------------------------------------------------------------------ host
 
-// Blocks that share a sequence's keys: up to three for each SM, each with at least one tile of
-// 32 keys, of the longest sequence that the tables can hold. Measured with 2, 3 and 5 for each SM,
-// fp32: 5 sequences of up to 1999, 7 tokens 21.0, 17.2, 18.2 us; one of 8000 24.8, 22.8, 28.3; 32 of 500,
-// 4 tokens 38.9, 38.9, 43.2; with at least two tiles instead of one, 4 heads over 300 13.4 against 11.3.
+// Blocks that share a sequence's keys: up to five for each SM, each with at least 64 keys, the
+// two tiles it has on their way at once, of the longest sequence that the tables can hold.
 int split_count(int64_t batch, int64_t kv_heads, int64_t row_blocks, int64_t capacity) {
   const int64_t blocks = batch * kv_heads * row_blocks;
-  const int64_t want = (3 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (capacity + kKeys - 1) / kKeys, kMaxSplits}));
+  const int64_t want = (5 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (capacity + 63) / 64, kMaxSplits}));
 }
 
 template <typename T, int ND>
@@ -610,8 +608,8 @@ extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const
   auto join = [&](auto* kernel, int per_block) {
     return launch_pdl(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(128), 0, st, op, a);
   };
-  // Four warps to a row where many splits meet: 5 sequences of up to 1999 positions 17.2 against 18.4 us,
-  // one of 8000 22.9 against 25.3; one where few do: 16 of 700, 33 tokens, 122 against 125 us.
+  // Four warps to a row where many splits meet: 5 sequences of up to 1999 positions 18.2 against 19.3 us,
+  // one of 8000 28.5 against 33.4; one where few do: 16 of 700, 33 tokens, 118 against 121 us.
   if (a.splits > 8)
     return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 4>, 1) : join(tree_combine_kernel<bf16, 4>, 1);
   return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 1>, 4) : join(tree_combine_kernel<bf16, 1>, 4);
