@@ -100,23 +100,43 @@ Table check_table(const Tensor& tables, OptTensor lens, const Tensor& refs) {
   return {dev, B, M, P, ints("tables", tables, dev, {B, M}), ints("lens", lens, dev, {B}), ints("refs", refs, dev, {P})};
 }
 
-// Workspaces: calls of one stream share one, grown on demand (they are ordered); a call under
-// capture into a graph gets one of the graph's own pool, so graphs never share.
-void* workspace(c10::Device dev, cudaStream_t stream, size_t bytes, Tensor& hold) {
-  if (bytes == 0) return nullptr;
-  const auto make = [&] { return new_tensor({(int64_t)bytes}, at::kByte, dev); };
+// A call's workspace, for as long as the object lives: until the call's last launch is queued.
+struct Workspace {
+  void* data = nullptr;
+  Tensor hold;
+  std::unique_lock<std::mutex> lock;
+};
+
+// Calls of one stream share one, grown on demand. A call of two launches hands values from one to
+// the next through it, and another host thread may queue on the same stream (the default one
+// is every thread's), so a call holds the stream's lock from here to its last launch: the stream
+// then runs whole calls one after another. A call under capture into a graph gets a workspace
+// of the graph's own pool, so graphs never share.
+Workspace workspace(c10::Device dev, cudaStream_t stream, size_t bytes) {
+  Workspace w;
+  if (bytes == 0) return w;
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
-    hold = make();
-    return hold.data_ptr();
+    w.hold = new_tensor({(int64_t)bytes}, at::kByte, dev);
+  } else {
+    struct Kept {
+      std::mutex mutex;
+      Tensor tensor;
+    };
+    static std::mutex mutex;
+    // never destroyed: the CUDA context may be gone before static destructors run
+    static auto* const all = new std::map<std::pair<int, cudaStream_t>, Kept>;
+    Kept* kept;
+    {
+      std::lock_guard<std::mutex> lock(mutex);
+      kept = &(*all)[{dev.index(), stream}];
+    }
+    w.lock = std::unique_lock<std::mutex>(kept->mutex);
+    if (!kept->tensor.defined() || (size_t)kept->tensor.numel() < bytes)
+      kept->tensor = new_tensor({(int64_t)bytes}, at::kByte, dev);
+    w.hold = kept->tensor;
   }
-  static std::mutex mutex;
-  // never destroyed: the CUDA context may be gone before static destructors run
-  static auto* const kept = new std::map<std::pair<int, cudaStream_t>, Tensor>;
-  std::lock_guard<std::mutex> lock(mutex);
-  Tensor& t = (*kept)[{dev.index(), stream}];
-  if (!t.defined() || (size_t)t.numel() < bytes) t = make();
-  hold = t;
-  return t.data_ptr();
+  w.data = w.hold.data_ptr();
+  return w;
 }
 
 Tensor attention_tree(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache,
@@ -144,13 +164,13 @@ Tensor attention_tree(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   const auto [k, v] = rows_of(k_in, v_in);
   const c10::cuda::CUDAGuard guard(dev);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-  Tensor out = new_tensor({B, T, H, d}, q.scalar_type(), dev), hold;
+  Tensor out = new_tensor({B, T, H, d}, q.scalar_type(), dev);
   const size_t bytes = nkl_attention_tree_workspace_size(B, T, H, Hkv, d, page, M, dt);
-  void* ws = workspace(dev, st, bytes, hold);
+  const Workspace ws = workspace(dev, st, bytes);
   check("nkl_attention_tree",
         nkl_attention_tree(q.data_ptr(), q.strides().data(), k.data_ptr(), v.data_ptr(), k.strides().data(),
                            k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), tb, ln, up, out.data_ptr(),
-                           ws, bytes, B, T, H, Hkv, d, P, page, M, (float)scale, dt, st));
+                           ws.data, bytes, B, T, H, Hkv, d, P, page, M, (float)scale, dt, st));
   return out;
 }
 
@@ -189,11 +209,11 @@ std::tuple<Tensor, Tensor, Tensor> cache_reserve(const Tensor& tables, const Ten
   const int32_t* ex = ints("extra", extra, t.dev, {t.B});
   const c10::cuda::CUDAGuard guard(t.dev);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(t.dev.index()).stream();
-  Tensor tables_out = new_ints({t.B, t.M}, t.dev), refs_out = new_ints({t.P}, t.dev), missing = new_ints({1}, t.dev), hold;
+  Tensor tables_out = new_ints({t.B, t.M}, t.dev), refs_out = new_ints({t.P}, t.dev), missing = new_ints({1}, t.dev);
   const size_t bytes = nkl_cache_reserve_workspace_size(t.B);
-  void* ws = workspace(t.dev, st, bytes, hold);
+  const Workspace ws = workspace(t.dev, st, bytes);
   check("nkl_cache_reserve", nkl_cache_reserve(t.tables, t.lens, t.refs, ex, out_ints(tables_out), out_ints(refs_out),
-                                               out_ints(missing), ws, bytes, t.B, t.P, page_size, t.M, st));
+                                               out_ints(missing), ws.data, bytes, t.B, t.P, page_size, t.M, st));
   return {tables_out, refs_out, missing};
 }
 
@@ -211,12 +231,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_cache, con
   const c10::cuda::CUDAGuard guard(t.dev);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(t.dev.index()).stream();
   Tensor tables_out = new_ints({t.B, t.M}, t.dev), lens_out = new_ints({t.B}, t.dev), refs_out = new_ints({t.P}, t.dev),
-         missing = new_ints({1}, t.dev), hold;
+         missing = new_ints({1}, t.dev);
   const size_t bytes = nkl_cache_fork_workspace_size(t.B, F);
-  void* ws = workspace(t.dev, st, bytes, hold);
+  const Workspace ws = workspace(t.dev, st, bytes);
   check("nkl_cache_fork",
         nkl_cache_fork(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), t.tables, t.lens, t.refs, from,
-                       to, out_ints(tables_out), out_ints(lens_out), out_ints(refs_out), out_ints(missing), ws, bytes, F,
+                       to, out_ints(tables_out), out_ints(lens_out), out_ints(refs_out), out_ints(missing), ws.data, bytes, F,
                        k_cache.size(0), t.B, k_cache.size(2), k_cache.size(4), t.P, k_cache.size(3), t.M, dt, st));
   return {tables_out, lens_out, refs_out, missing};
 }
@@ -242,12 +262,12 @@ std::tuple<Tensor, Tensor> cache_compact(const Tensor& k_cache, const Tensor& v_
   TORCH_CHECK(k_cache.device() == t.dev, "tensors on different devices: ", k_cache.device(), " vs ", t.dev);
   const c10::cuda::CUDAGuard guard(t.dev);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(t.dev.index()).stream();
-  Tensor tables_out = new_ints({t.B, t.M}, t.dev), refs_out = new_ints({t.P}, t.dev), hold;
+  Tensor tables_out = new_ints({t.B, t.M}, t.dev), refs_out = new_ints({t.P}, t.dev);
   const size_t bytes = nkl_cache_compact_workspace_size(t.P);
-  void* ws = workspace(t.dev, st, bytes, hold);
+  const Workspace ws = workspace(t.dev, st, bytes);
   check("nkl_cache_compact",
         nkl_cache_compact(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), t.tables, t.refs,
-                          out_ints(tables_out), out_ints(refs_out), ws, bytes, k_cache.size(0), t.B, k_cache.size(2),
+                          out_ints(tables_out), out_ints(refs_out), ws.data, bytes, k_cache.size(0), t.B, k_cache.size(2),
                           k_cache.size(4), t.P, k_cache.size(3), t.M, dt, st));
   return {tables_out, refs_out};
 }
