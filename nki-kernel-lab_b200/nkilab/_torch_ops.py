@@ -19,6 +19,7 @@ There is no CPU implementation: a CPU tensor is an error, never a fallback.
 from __future__ import annotations
 
 import os
+import threading
 
 import torch
 
@@ -237,15 +238,28 @@ def _(a, b):
     return a.new_empty((a.shape[0], b.shape[1]), dtype=torch.float32)
 
 
-# Split-KV workspaces of the bf16 attention kernel. Eager calls share one workspace per
-# (device, stream), grown on demand (the kernels need no initialised contents): calls on
-# one stream are ordered, so they can share it, and other streams get their own. A call
+# Split-KV workspaces of the bf16 attention kernel. A host thread's eager calls share one
+# workspace per (device, stream), grown on demand (the kernels need no initialised contents):
+# a thread's calls on one stream are ordered, so they can share it, and other streams get
+# their own. Not so the calls of two threads on one stream: a call is two launches, the second
+# reads what the first left in the workspace, and the other thread's can come between. A call
 # made while its stream is being captured into a CUDA graph takes a fresh workspace from
 # the caching allocator instead, which during capture hands out memory of the graph's
 # own pool: every graph then owns the workspaces it writes, two graphs can be replayed
 # concurrently, and replacing an outgrown eager workspace never frees memory a graph
 # still uses.
-_attention_ws: dict = {}
+class _PerThread(threading.local):
+    """A mapping that each thread has for itself."""
+
+    def __init__(self):
+        self.own: dict = {}
+        self.get, self.pop = self.own.get, self.own.pop
+
+    def __setitem__(self, key, value):
+        self.own[key] = value
+
+
+_attention_ws = _PerThread()
 
 
 def _attention_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:

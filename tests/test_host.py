@@ -113,3 +113,24 @@ def test_eager_attention_workspace_grows_per_stream():
     assert T._attention_workspace(dev, -54321, 64) is not big  # another stream: its own
     T._attention_ws.pop((dev.index, stream))
     T._attention_ws.pop((dev.index, -54321))
+
+
+def test_eager_attention_workspace_is_a_threads_own():
+    """Two threads on one stream: each has its own, for the launches of their calls interleave."""
+    import threading
+
+    import torch
+
+    from nkilab import _torch_ops as T
+
+    dev, stream, got = torch.device("cpu"), -24680, []
+
+    def work():
+        got.append([T._attention_workspace(dev, stream, 256) for _ in range(2)])
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    work()
+    T._attention_ws.pop((dev.index, stream))
+    assert got[0][0] is got[0][1] and got[1][0] is got[1][1] and got[0][0] is not got[1][0]

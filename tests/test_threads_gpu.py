@@ -66,7 +66,24 @@ def compact(seed, P):
     return call
 
 
+def prompt(seed, H, S, strided=False):
+    """Long prompts of few heads, whose key ranges are split over the SMs."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q, k, v = (torch.randn(H, S, 64, generator=g, device=DEV).to(BF) for _ in range(3))
+
+    def call():
+        if not strided:
+            return (ops.attention(q, k, v),)
+        out = torch.empty_like(q)
+        torch.ops.nkilab.attention_strided_(q, k, v, out, 0.125)
+        return (out,)
+
+    return call
+
+
 PAIRS = {
+    "attention": lambda: (prompt(11, 2, 2048), prompt(12, 3, 1408)),
+    "attention strided": lambda: (prompt(13, 2, 2048, True), prompt(14, 1, 4096)),
     "attention_tree bf16": lambda: (tree(1, BF, 1, [5000, 4000]), tree(2, BF, 40, [900, 3000, 77, 2500])),
     "attention_tree f32": lambda: (tree(3, torch.float32, 1, [3000]), tree(4, torch.float32, 5, [700, 2000, 1500])),
     "cache_fork": lambda: (fork(5, 900, 5000), fork(6, 2500, 6000)),
