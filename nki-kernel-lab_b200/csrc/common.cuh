@@ -139,6 +139,11 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Says that this block has started; cluster_wait_started then waits until every block of the
+// cluster has said so: their shared memory may not be written to before.
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait_started() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // Ask L2 to fetch [p, p + bytes) (p 16-byte aligned, bytes a multiple of 16). Issued
 // before pdl_wait it overlaps a kernel's first HBM reads with the previous kernel's
 // tail; a prefetch only warms L2, the point of coherence, so it is correct even while

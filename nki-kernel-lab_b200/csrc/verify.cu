@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   __shared__ int s_last;
   __shared__ u64 s_sum[kVerifyWarps], s_all[kVerifyWarps];
   __shared__ u64 s_blocks[kMaxCluster][2];  // the cluster's sums and sums of whole rows
+  cluster_started();
   pdl_enter();
   const int blocks = (int)cluster_size(), rank = (int)cluster_rank();
   const int b = blockIdx.x / blocks, n = a.drafted, V = a.vocab;
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     s_all[warp] = all;
   }
   __syncthreads();
+  cluster_wait_started();  // no wait by now: the row has been read since
   if (warp == 0) {  // the block's sums to every block
     const u64 x = warp_sum64(lane < kVerifyWarps ? s_sum[lane] : 0), y = warp_sum64(lane < kVerifyWarps ? s_all[lane] : 0);
     if (lane < blocks) {

@@ -728,6 +728,22 @@ def test_verify_views_and_repeats():
         assert torch.equal(x, y) and torch.equal(x, z)
 
 
+@pytest.mark.parametrize("B,V", [(55, 8192), (111, 4096), (200, 2048)])
+def test_verify_short_rows_over_several_blocks(B, V):
+    """Rows that each block of a cluster is through with at once, so that the blocks exchange their
+    sums as soon as they can; every launch gives the same."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    probs = torch.randn(B, 2, V, generator=g, device=DEV).softmax(-1)
+    tokens = torch.randint(0, V, (B, 1), generator=g, device=DEV)
+    u = torch.rand(B, 2, generator=g, device=DEV)
+    check_verify(probs, tokens.tolist(), u, None, None)
+    want = ops.verify_drafts(probs, tokens.int(), u)
+    got = [ops.verify_drafts(probs, tokens.int(), u) for _ in range(200)]
+    for out in got:
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("mode", ["ratio", "tree"])
 def test_verify_keeps_the_targets_distribution(mode):
     """The first token that comes out of a step (an accepted draft or the drawn one) is
