@@ -98,6 +98,15 @@ __device__ __forceinline__ Split split_tf32(float x) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
   return {hi, __float_as_uint(x - __uint_as_float(hi))};
 }
+// x = hi + lo for every x: where rounding would overflow, hi is cut off instead, and an infinity or
+// NaN is hi alone.
+__device__ __forceinline__ Split split_any(float x) {
+  const Split s = split_tf32(x);
+  if (fabsf(__uint_as_float(s.hi)) < INFINITY) return s;
+  if (!(fabsf(x) < INFINITY)) return {__float_as_uint(x + x), 0u};
+  const uint32_t hi = __float_as_uint(x) & 0xffffe000u;
+  return {hi, __float_as_uint(x - __uint_as_float(hi))};
+}
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -171,7 +180,6 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
     }
     copies_commit();  // also where there is nothing: the count of groups goes on
   };
-  if (tid < 2 * kKeys) place[(t0 + (tid >> 5)) & 1][lane] = look_up(t0 + (tid >> 5), lane);
   const T* q = static_cast<const T*>(a.q) + b * a.q_b;
   for (int i = tid; i < kRows * chunks; i += kThreads) {
     const int r = (int)(((float)i + 0.5f) * per_row), c = (i - r * chunks) * VE, row = r0 + r, token = row / a.group;
@@ -181,19 +189,15 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
       x.raw = *reinterpret_cast<const uint4*>(q + token * a.q_t + (kvh * a.group + row - token * a.group) * a.q_h + c);
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      const Split s = split_tf32(x.get(e));
+      const Split s = split_any(x.get(e));
       qs[r * q_pitch + c + e] = make_float2(__uint_as_float(s.hi), __uint_as_float(s.lo));
     }
   }
-  __syncthreads();
-  fetch(t0);
-  fetch(t0 + 1);
 
   // the lane's two rows, g and g + 8
   const int* const parents = a.parents ? a.parents + (int64_t)b * a.tokens : nullptr;
   uint32_t seen[2][4];  // drafted tokens visible to them
   bool here[2];
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = r0 + g + 8 * i, token = row / a.group;
@@ -201,136 +205,156 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
     seen[i][0] = seen[i][1] = seen[i][2] = seen[i][3] = 0u;
     if (here[i] && end > t1) ancestor_bits(parents, token, seen[i]);
   }
-  float o[ND][4];
+  float m[2], l[2], o[ND][4];
+  // A value that is infinite, NaN or rounds to infinity has parts whose products are no sum of its
+  // own (inf - inf, 0 inf), and 0 times it is no 0 for a row that does not see its key. All that
+  // leaves a sum that is not finite, so the tiles go through the tensor core unchecked, and a block
+  // with such a sum goes through them again in fp32, a key that a row does not see left out.
+  for (bool plain = false;; plain = true) {
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
 #pragma unroll
-  for (int j = 0; j < ND; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-
-  for (int t = t0; t < end; ++t) {
-    const bool cached = t < t1;
-    const int key0 = (cached ? t : t - t1) * kKeys;
-    const T* const ks = ring + (t & 1) * lay.stage + (warp * 8) * lay.pitch;  // this warp's 8 keys
-    const T* const vs = ks + kKeys * lay.pitch;
-    const int64_t next = warp == 0 ? look_up(t + 2, lane) : 0;
-    copies_wait<1>();
+    for (int j = 0; j < ND; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    if (tid < 2 * kKeys) place[(t0 + (tid >> 5)) & 1][lane] = look_up(t0 + (tid >> 5), lane);
     __syncthreads();
-    // scores: c[0], c[1] of row g, keys 2 t4 and 2 t4 + 1; c[2], c[3] of row g + 8. The three
-    // products have sums of their own, so that they do not wait for one another.
-    float c[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};
+    fetch(t0);
+    fetch(t0 + 1);
+    for (int t = t0; t < end; ++t) {
+      const bool cached = t < t1;
+      const int key0 = (cached ? t : t - t1) * kKeys;
+      const T* const ks = ring + (t & 1) * lay.stage + (warp * 8) * lay.pitch;  // this warp's 8 keys
+      const T* const vs = ks + kKeys * lay.pitch;
+      const int64_t next = warp == 0 ? look_up(t + 2, lane) : 0;
+      copies_wait<1>();
+      __syncthreads();
+      // scores: c[0], c[1] of row g, keys 2 t4 and 2 t4 + 1; c[2], c[3] of row g + 8. The three
+      // products have sums of their own, so that they do not wait for one another.
+      float c[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f}, c2[4] = {0.f, 0.f, 0.f, 0.f};
+      if (!plain) {
 #pragma unroll 4
-    for (int s = 0; s < nd; ++s) {
-      uint32_t hi[4], lo[4];
+        for (int s = 0; s < nd; ++s) {
+          uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // (g, t4), (g + 8, t4), (g, t4 + 4), (g + 8, t4 + 4)
-        const float2 x = qs[(g + 8 * (i & 1)) * q_pitch + 8 * s + t4 + 4 * (i >> 1)];
-        hi[i] = __float_as_uint(x.x);
-        lo[i] = __float_as_uint(x.y);
-      }
-      const float k0 = to_f32(ks[g * lay.pitch + 8 * s + t4]), k1 = to_f32(ks[g * lay.pitch + 8 * s + t4 + 4]);
-      if constexpr (kExact) {
-        mma_tf32(c, hi, __float_as_uint(k0), __float_as_uint(k1));
-      } else {
-        const Split x = split_tf32(k0), y = split_tf32(k1);
-        mma_tf32(c1, lo, x.hi, y.hi);
-        mma_tf32(c2, hi, x.lo, y.lo);
-        mma_tf32(c, hi, x.hi, y.hi);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] += c1[i] + c2[i];
-    const int word = (key0 >> 5) & 3;
-    float p[4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
-      float x[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int key = warp * 8 + 2 * t4 + j;
-        const bool sees = here[i] && (cached ? key0 + key < n : ((drafts >> key) & 1u) != 0u);
-        x[j] = sees ? c[2 * i + j] * a.scale : -INFINITY;
-      }
-      float top = fmaxf(x[0], x[1]);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top, m[i]);
-      const float ref = top == -INFINITY ? 0.f : top;  // nothing seen so far
-      const float keep = expf(m[i] - ref);
-      p[2 * i] = x[0] == -INFINITY ? 0.f : expf(x[0] - ref);
-      p[2 * i + 1] = x[1] == -INFINITY ? 0.f : expf(x[1] - ref);
-      l[i] = l[i] * keep + (p[2 * i] + p[2 * i + 1]);  // this lane's keys; the four lanes' sums meet at the end
-      m[i] = top;
-#pragma unroll
-      for (int j = 0; j < ND; ++j) {
-        o[j][2 * i] *= keep;
-        o[j][2 * i + 1] *= keep;
-      }
-    }
-    // A drafted token that a row does not see leaves no trace in it, whatever its v holds: where
-    // this warp's eight rows of v hold infinities or NaN, 0 times them is not summed but left out.
-    bool finite = true;
-    if (!cached) {
-      for (int x = 0; x < 8; ++x)
-        for (int c = lane; c < a.d; c += 32) finite &= fabsf(to_f32(vs[x * lay.pitch + c])) < INFINITY;
-      finite = __all_sync(0xffffffffu, finite);
-    }
-    if (finite) {
-      // P as the first operand: the columns t4 and t4 + 4 of a fragment stand for the keys 2 t4
-      // and 2 t4 + 1, so the scores' registers are in place and V's rows are taken in that order
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Split x = split_tf32(p[2 * (i & 1) + (i >> 1)]);
-        hi[i] = x.hi;
-        lo[i] = x.lo;
-      }
-#pragma unroll
-      for (int j = 0; j < ND; ++j) {
-        if (j >= nd) break;
-        const float v0 = to_f32(vs[(2 * t4) * lay.pitch + 8 * j + g]), v1 = to_f32(vs[(2 * t4 + 1) * lay.pitch + 8 * j + g]);
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (kExact) {
-          mma_tf32(y, lo, __float_as_uint(v0), __float_as_uint(v1));
-          mma_tf32(y, hi, __float_as_uint(v0), __float_as_uint(v1));
-        } else {
-          const Split s0 = split_tf32(v0), s1 = split_tf32(v1);
-          mma_tf32(y, lo, s0.hi, s1.hi);
-          mma_tf32(y, hi, s0.lo, s1.lo);
-          mma_tf32(y, hi, s0.hi, s1.hi);
+          for (int i = 0; i < 4; ++i) {  // (g, t4), (g + 8, t4), (g, t4 + 4), (g + 8, t4 + 4)
+            const float2 x = qs[(g + 8 * (i & 1)) * q_pitch + 8 * s + t4 + 4 * (i >> 1)];
+            hi[i] = __float_as_uint(x.x);
+            lo[i] = __float_as_uint(x.y);
+          }
+          const float k0 = to_f32(ks[g * lay.pitch + 8 * s + t4]), k1 = to_f32(ks[g * lay.pitch + 8 * s + t4 + 4]);
+          if constexpr (kExact) {
+            mma_tf32(c, hi, __float_as_uint(k0), __float_as_uint(k1));
+          } else {
+            const Split x = split_tf32(k0), y = split_tf32(k1);
+            mma_tf32(c1, lo, x.hi, y.hi);
+            mma_tf32(c2, hi, x.lo, y.lo);
+            mma_tf32(c, hi, x.hi, y.hi);
+          }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[j][k] += y[k];
-      }
-    } else {
+        for (int i = 0; i < 4; ++i) c[i] += c1[i] + c2[i];
+      } else {
 #pragma unroll 1
-      for (int x = 0; x < 8 && key0 + warp * 8 + x < a.tokens; ++x) {
-        const int from = (lane & ~3) | (x >> 1);  // the lane that has this key's P of the row
-        float w[2];
-        bool sees[2];
+        for (int e = 0; e < a.d; ++e) {
+          const float2 x = qs[g * q_pitch + e], y = qs[(g + 8) * q_pitch + e];
+          const float k0 = to_f32(ks[2 * t4 * lay.pitch + e]), k1 = to_f32(ks[(2 * t4 + 1) * lay.pitch + e]);
+          c[0] = fmaf(x.x + x.y, k0, c[0]);
+          c[1] = fmaf(x.x + x.y, k1, c[1]);
+          c[2] = fmaf(y.x + y.y, k0, c[2]);
+          c[3] = fmaf(y.x + y.y, k1, c[3]);
+        }
+      }
+      const int word = (key0 >> 5) & 3;
+      float p[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float w0 = __shfl_sync(0xffffffffu, p[2 * i], from), w1 = __shfl_sync(0xffffffffu, p[2 * i + 1], from);
-          const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
-          w[i] = x & 1 ? w1 : w0;
-          sees[i] = (drafts >> (warp * 8 + x)) & 1u;
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
+        float x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = warp * 8 + 2 * t4 + j;
+          const bool sees = here[i] && (cached ? key0 + key < n : ((drafts >> key) & 1u) != 0u);
+          x[j] = sees ? c[2 * i + j] * a.scale : -INFINITY;
+        }
+        float top = fmaxf(x[0], x[1]);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = fmaxf(top, m[i]);
+        const float ref = top == -INFINITY ? 0.f : top;  // nothing seen so far
+        const float keep = expf(m[i] - ref);
+        p[2 * i] = x[0] == -INFINITY ? 0.f : expf(x[0] - ref);
+        p[2 * i + 1] = x[1] == -INFINITY ? 0.f : expf(x[1] - ref);
+        l[i] = l[i] * keep + (p[2 * i] + p[2 * i + 1]);  // this lane's keys; the four lanes' sums meet at the end
+        m[i] = top;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          o[j][2 * i] *= keep;
+          o[j][2 * i + 1] *= keep;
+        }
+      }
+      if (!plain) {
+        // P as the first operand: the columns t4 and t4 + 4 of a fragment stand for the keys 2 t4
+        // and 2 t4 + 1, so the scores' registers are in place and V's rows are taken in that order
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const Split x = split_tf32(p[2 * (i & 1) + (i >> 1)]);
+          hi[i] = x.hi;
+          lo[i] = x.lo;
         }
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
           if (j >= nd) break;
-          const float v0 = to_f32(vs[x * lay.pitch + 8 * j + 2 * t4]), v1 = to_f32(vs[x * lay.pitch + 8 * j + 2 * t4 + 1]);
+          const float v0 = to_f32(vs[(2 * t4) * lay.pitch + 8 * j + g]), v1 = to_f32(vs[(2 * t4 + 1) * lay.pitch + 8 * j + g]);
+          float y[4] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (kExact) {
+            mma_tf32(y, lo, __float_as_uint(v0), __float_as_uint(v1));
+            mma_tf32(y, hi, __float_as_uint(v0), __float_as_uint(v1));
+          } else {
+            const Split s0 = split_tf32(v0), s1 = split_tf32(v1);
+            mma_tf32(y, lo, s0.hi, s1.hi);
+            mma_tf32(y, hi, s0.lo, s1.lo);
+            mma_tf32(y, hi, s0.hi, s1.hi);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[j][k] += y[k];
+        }
+      } else {
+#pragma unroll 1
+        for (int x = 0; x < 8 && key0 + warp * 8 + x < (cached ? n : a.tokens); ++x) {
+          const int from = (lane & ~3) | (x >> 1);  // the lane that has this key's P of the row
+          float w[2];
+          bool sees[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            o[j][2 * i] = sees[i] ? fmaf(w[i], v0, o[j][2 * i]) : o[j][2 * i];
-            o[j][2 * i + 1] = sees[i] ? fmaf(w[i], v1, o[j][2 * i + 1]) : o[j][2 * i + 1];
+            const float w0 = __shfl_sync(0xffffffffu, p[2 * i], from), w1 = __shfl_sync(0xffffffffu, p[2 * i + 1], from);
+            const uint32_t drafts = word == 0 ? seen[i][0] : word == 1 ? seen[i][1] : word == 2 ? seen[i][2] : seen[i][3];
+            w[i] = x & 1 ? w1 : w0;
+            sees[i] = here[i] && (cached || ((drafts >> (warp * 8 + x)) & 1u));
+          }
+#pragma unroll
+          for (int j = 0; j < ND; ++j) {
+            if (j >= nd) break;
+            const float v0 = to_f32(vs[x * lay.pitch + 8 * j + 2 * t4]), v1 = to_f32(vs[x * lay.pitch + 8 * j + 2 * t4 + 1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              o[j][2 * i] = sees[i] ? fmaf(w[i], v0, o[j][2 * i]) : o[j][2 * i];
+              o[j][2 * i + 1] = sees[i] ? fmaf(w[i], v1, o[j][2 * i + 1]) : o[j][2 * i + 1];
+            }
           }
         }
       }
+      if (warp == 0) place[t & 1][lane] = next;
+      __syncthreads();  // every warp is through with this tile's place
+      fetch(t + 2);
     }
-    if (warp == 0) place[t & 1][lane] = next;
-    __syncthreads();  // every warp is through with this tile's place
-    fetch(t + 2);
+    copies_wait<0>();
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) finite &= fabsf(o[j][k]) < INFINITY;
+    if (!__syncthreads_or(!finite) || plain) break;
   }
-  copies_wait<0>();
-  __syncthreads();
 
   // the four warps' (max, sum, O) through shared memory, in their order
   float* const ro = reinterpret_cast<float*>(ring);                // [warp][row][d]

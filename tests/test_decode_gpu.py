@@ -217,6 +217,48 @@ def test_attention_infinities_of_unseen_tokens(dtype, H):
     check_attention(torch.where(shows, 0, got), torch.where(shows.cpu(), 0, want), mag)
 
 
+def put(x, b, pos, head, col, k=None, v=None):
+    """Sets one element of a cached position's key or value."""
+    kc, vc, tables, page = x[3], x[4], x[5], x[3].shape[2]
+    at = int(tables[b, pos // page]), head, pos % page, col
+    for c, value in ((kc, k), (vc, v)):
+        if value is not None:
+            c[at] = value
+
+
+def check_with_infinities(got, want, mag):
+    """Infinities and NaN where the statement in 64 bits has them, the rest as ever."""
+    got, finite = got.cpu(), torch.isfinite(want)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[want.isinf()].double(), want[want.isinf()])
+    check_attention(torch.where(finite, got, 0), torch.where(finite, want, 0), torch.where(finite, mag, 0))
+
+
+INFINITIES = [(F32, 64, 16), (F32, 128, 24), (BF, 96, 16), (BF, 64, 17)]
+
+
+@pytest.mark.parametrize("T", [1, 9])
+@pytest.mark.parametrize("dtype,d,page", INFINITIES)
+def test_attention_infinities_in_the_cache(dtype, d, page, T):
+    """Infinities, NaN and the largest values in cached positions show as the formula has them: an
+    infinite value in its column, a key whose score is minus infinity not at all."""
+    inf, big = float("inf"), torch.finfo(dtype).max
+    x = list(setup_attention(4, T, 4, 2, d, page, [130, 700, 90, 300], dtype, seed=d))
+    q = x[0] = x[0].clone()
+    q[..., 0] = q[..., 0].abs() + 0.25
+    for pos, col, v in ((5, 3, inf), (120, 3, inf), (10, 7, inf), (90, 7, -inf), (2, 9, float("nan")), (129, 11, -inf)):
+        put(x, 0, pos, 0, col, v=v)
+    put(x, 0, 20, 0, 0, k=-inf)
+    put(x, 1, 699, 0, 0, k=-inf)
+    put(x, 1, 7, 1, 0, k=inf)  # the rows of this head are NaN
+    put(x, 1, 300, 0, d - 1, v=-inf)
+    for pos, col, v in ((3, 5, big), (4, 6, -big)):
+        put(x, 2, pos, 1, col, v=v)
+    put(x, 3, 4, 0, 1, k=big)
+    q[3, :, :2] *= 1e-37  # its score is of the size of 1
+    check_with_infinities(ops.attention_tree(*x, None), *attention_64(*x, None, 1 / math.sqrt(d)))
+
+
 @pytest.mark.parametrize("dtype,T", [(BF, 1), (BF, 70), (F32, 3)])
 def test_attention_growing_maxima(dtype, T):
     """Every later key scores higher: the running maximum grows in every tile."""
