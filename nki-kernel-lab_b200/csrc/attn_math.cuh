@@ -78,24 +78,27 @@ __device__ __forceinline__ void exp_pack_rounded(uint32_t* v, float scale_log2, 
   }
 }
 
-// exp_pack in two parts: hi the rounded exponentials, lo what the rounding left, itself
-// rounded (2^-16 of the exponential); the sum is over the exponentials in fp32.
+// exp_pack in two parts: hi the exponentials cut off to bf16, lo what that left, rounded (2^-16 of
+// the exponential); the sum is over the exponentials in fp32. Neither part is negative, and lo has
+// 2^-40 of the exponential added, so that it is zero only where that is: an infinity in V times
+// either part is that infinity, and no NaN (0 inf, inf - inf) comes of their sum.
 template <int N, int ACC>
 __device__ __forceinline__ void exp_pack_two(const uint32_t* v, uint32_t* hi, uint32_t* lo, float scale_log2,
                                              float neg_m, f32x2 (&rs)[ACC]) {
   const f32x2 k2 = f2_pack(scale_log2, scale_log2), m2 = f2_pack(neg_m, neg_m);
+  const f32x2 minus = f2_pack(-1.f, -1.f), little = f2_pack(0x1p-40f, 0x1p-40f);
 #pragma unroll
   for (int j = 0; j < ACC; ++j) rs[j] = 0ull;
 #pragma unroll
   for (int c = 0; c < N; c += 2) {
     const f32x2 x2 = f2_fma(f2_pack_bits(v[c], v[c + 1]), k2, m2);
-    const float p0 = fast_exp2(f2_lo(x2)), p1 = fast_exp2(f2_hi(x2));
-    rs[(c >> 1) % ACC] = f2_add(rs[(c >> 1) % ACC], f2_pack(p0, p1));
-    __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
-    const uint32_t h = *reinterpret_cast<uint32_t*>(&h2);
-    __nv_bfloat162 l2 = __floats2bfloat162_rn(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
+    const f32x2 p2 = f2_pack(fast_exp2(f2_lo(x2)), fast_exp2(f2_hi(x2)));
+    rs[(c >> 1) % ACC] = f2_add(rs[(c >> 1) % ACC], p2);
+    const uint32_t h = __byte_perm((uint32_t)p2, (uint32_t)(p2 >> 32), 0x7632);
+    const f32x2 l2 = f2_fma(p2, little, f2_fma(f2_pack_bits(h << 16, h & 0xffff0000u), minus, p2));
+    __nv_bfloat162 b2 = __floats2bfloat162_rn(f2_lo(l2), f2_hi(l2));
     hi[c >> 1] = h;
-    lo[c >> 1] = *reinterpret_cast<uint32_t*>(&l2);
+    lo[c >> 1] = *reinterpret_cast<uint32_t*>(&b2);
   }
 }
 
