@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float mw = rml[2 * (w * kRows + r)];
-      if (mw == -INFINITY) continue;
+      if (mw == -INFINITY && rml[2 * (w * kRows + r) + 1] == 0.f) continue;  // nothing seen (a sum of NaN: only NaN was)
       const float f = expf(mw - top);
       const float4 y = *reinterpret_cast<const float4*>(ro + (size_t)(w * kRows + r) * a.d + c);
       sum = fmaf(f, rml[2 * (w * kRows + r) + 1], sum);

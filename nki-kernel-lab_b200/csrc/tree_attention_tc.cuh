@@ -881,11 +881,13 @@ __global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int y = warp; y < 8; y += 2 * D / 32) {
     const int r = r0 + y;
-    float m = -INFINITY, l = 0.f, mi[kMaxPieces / 32];
+    float m = -INFINITY, l = 0.f, mi[kMaxPieces / 32], li[kMaxPieces / 32];
 #pragma unroll
     for (int k = 0; k < kMaxPieces / 32; ++k) {
       const int i = k * 32 + lane;
-      mi[k] = i < pieces ? __ldcg(a.ws_ml + slot(i) * 2 * kTile + r) : -INFINITY;
+      const float* const ml = a.ws_ml + slot(i) * 2 * kTile + r;
+      mi[k] = i < pieces ? __ldcg(ml) : -INFINITY;
+      li[k] = i < pieces ? __ldcg(ml + kTile) : 0.f;
       m = fmaxf(m, mi[k]);
     }
     m = warp_max(m);
@@ -893,9 +895,10 @@ __global__ void __launch_bounds__(2 * D) tree_join_kernel(const __grid_constant_
     for (int k = 0; k < kMaxPieces / 32; ++k) {
       const int i = k * 32 + lane;
       if (i >= pieces) continue;
-      const float wi = mi[k] == -INFINITY ? 0.f : fast_exp2(mi[k] - m);  // 0: nothing of the piece is visible
+      // without a maximum the sum is 0, or NaN where all that is visible of the piece scores NaN
+      const float wi = mi[k] == -INFINITY ? li[k] : fast_exp2(mi[k] - m);
       weight[i][y] = wi;
-      l += wi == 0.f ? 0.f : wi * __ldcg(a.ws_ml + slot(i) * 2 * kTile + kTile + r);
+      l += wi == 0.f ? 0.f : wi * li[k];
     }
     l = warp_sum(l);
     if (lane == 0) inverse[y] = 1.f / l;

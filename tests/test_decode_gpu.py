@@ -261,6 +261,23 @@ def test_attention_infinities_in_the_cache(dtype, d, page, T):
     check_with_infinities(ops.attention_tree(*x, None), *attention_64(*x, None, 1 / math.sqrt(d)))
 
 
+@pytest.mark.parametrize("T", [1, 70])
+@pytest.mark.parametrize("dtype,d,page", INFINITIES)
+def test_attention_nan_scores_alone(dtype, d, page, T):
+    """Keys that are all NaN, where the rest of the row is finite: in eight keys in a row, in the
+    first tiles of a long row (some of them a piece by themselves), in all that a token sees."""
+    x = list(setup_attention(3, T, 8, 8, d, page, [4096, 64, 0], dtype, seed=d + T))
+    for head in range(8):
+        for pos in range(128 * (head + 1)):
+            put(x, 0, pos, head, 0, k=float("nan"))
+    for pos in range(8, 16):
+        put(x, 1, pos, 1, 5, k=float("nan"))
+        put(x, 1, pos + 32, 1, 5, k=float("nan"))
+    x[1] = x[1].clone()
+    x[1][2, 0, 0] = float("nan")  # seen by every token after it
+    check_with_infinities(ops.attention_tree(*x, None), *attention_64(*x, None, 1 / math.sqrt(d)))
+
+
 @pytest.mark.parametrize("dtype,T", [(BF, 1), (BF, 70), (F32, 3)])
 def test_attention_growing_maxima(dtype, T):
     """Every later key scores higher: the running maximum grows in every tile."""
