@@ -71,6 +71,13 @@ bool rows16(const Tensor& t) {
   return true;
 }
 
+// t, or a copy of it whose rows are contiguous and that begins where a kernel can read it.
+Tensor readable(const Tensor& t) {
+  if (rows16(t)) return t;
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+
 int check_caches(const Tensor& k, const Tensor& v, int64_t dims) {
   TORCH_CHECK_VALUE(k.dim() == dims && k.sizes() == v.sizes(), "caches ", k.sizes(), " and ", v.sizes(),
                     ": need equal shapes of ", dims, " dimensions");
@@ -83,7 +90,7 @@ int check_caches(const Tensor& k, const Tensor& v, int64_t dims) {
 // Rows k and v as the kernels read them: equal strides, aligned rows.
 std::pair<Tensor, Tensor> rows_of(const Tensor& k, const Tensor& v) {
   if (k.strides() == v.strides() && rows16(k) && rows16(v)) return {k, v};
-  return {k.contiguous(), v.contiguous()};
+  return {readable(k.contiguous()), readable(v.contiguous())};
 }
 
 struct Table {
@@ -160,7 +167,7 @@ Tensor attention_tree(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   const int32_t* tb = ints("tables", tables, dev, {B, M});
   const int32_t* ln = ints("lens", lens, dev, {B});
   const int32_t* up = ints("parents", parents, dev, {B, T});
-  const Tensor q = rows16(q_in) ? q_in : q_in.contiguous();
+  const Tensor q = readable(q_in);
   const auto [k, v] = rows_of(k_in, v_in);
   const c10::cuda::CUDAGuard guard(dev);
   const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();

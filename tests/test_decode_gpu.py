@@ -179,6 +179,28 @@ def test_attention_layouts(dtype):
     check_attention(ops.attention_tree(odd, kt, v, kc, vc, tables, lens, None, 0.3), *want)
 
 
+def shifted(t):
+    """The same values, contiguous, one element past an aligned address."""
+    buf = torch.empty(t.numel() + 1, device=DEV, dtype=t.dtype)
+    buf[1:] = t.flatten()
+    return buf[1:].view(t.shape)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_unaligned_inputs(dtype):
+    """Contiguous tensors that begin anywhere are taken as their aligned copies are."""
+    q, k, v, kc, vc, tables, lens = setup_attention(2, 3, 8, 2, 64, 16, [90, 33], dtype, junk=0.0)
+    want = ops.attention_tree(q, k, v, kc, vc, tables, lens)
+    for a, b, c in ((shifted(q), k, v), (q, shifted(k), v), (q, k.contiguous(), shifted(v)), (shifted(q), shifted(k), shifted(v))):
+        assert torch.equal(ops.attention_tree(a, b, c, kc, vc, tables, lens), want)
+    lens = lens - 3
+    for a, b in ((shifted(k), shifted(v)), (k.contiguous(), shifted(v))):
+        got, want = (kc.clone(), vc.clone()), (kc.clone(), vc.clone())
+        ops.cache_append(a, b, *got, tables, lens)
+        ops.cache_append(k, v, *want, tables, lens)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_attention_extreme_scores():
     """Scores that leave one key, and lowest values in masked places."""
     q, k, v, kc, vc, tables, lens = setup_attention(2, 8, 4, 2, 128, 16, [300, 17], BF, junk=-3.3e38)
