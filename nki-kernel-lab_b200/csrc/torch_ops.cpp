@@ -11,6 +11,8 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <map>
@@ -313,6 +315,28 @@ std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& probs_in, const T
   return {path, count, token};
 }
 
+// The attention has no backward pass: with inputs that require a gradient, one through it raises.
+Tensor attention_tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_cache,
+                               const Tensor& v_cache, const Tensor& tables, const Tensor& lens, OptTensor parents,
+                               double scale) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("nkilab::attention_tree", "")
+                             .typed<decltype(attention_tree_autograd)>();
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(q, k, v, k_cache, v_cache, tables, lens, parents, scale);
+  }
+  if (torch::autograd::compute_requires_grad(q, k, v, k_cache, v_cache)) {
+    const std::shared_ptr<torch::autograd::Node> node(
+        new torch::autograd::NotImplemented("nkilab::attention_tree",
+                                            torch::autograd::collect_next_edges(q, k, v, k_cache, v_cache)),
+        torch::autograd::deleteNode);
+    torch::autograd::set_history(out, node);
+  }
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nkilab, m) {
@@ -338,3 +362,5 @@ TORCH_LIBRARY_IMPL(nkilab, CUDA, m) {
   m.impl("cache_compact", &cache_compact);
   m.impl("verify_drafts", &verify_drafts);
 }
+
+TORCH_LIBRARY_IMPL(nkilab, Autograd, m) { m.impl("attention_tree", &attention_tree_autograd); }

@@ -175,3 +175,26 @@ def test_shapes_without_a_gpu():
     assert [t.shape for t in ops.cache_compact(cache, cache, tables, refs)] == [(B, M), (P,)]
     got = ops.verify_drafts(m(B, T + 1, V, dtype=torch.float32), m(B, T), m(B, T + 1, dtype=torch.float32))
     assert [t.shape for t in got] == [(B, T), (B,), (B,)] and all(t.dtype == torch.int32 for t in got)
+
+
+def test_a_backward_pass_raises():
+    """The attention is for decoding: a gradient through it is refused, never left out."""
+    import torch
+
+    from nkilab import ops
+
+    def m(*shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    i = torch.int32
+    args = [m(1, 2, 4, 64), m(1, 2, 2, 64), m(1, 2, 2, 64), m(9, 2, 16, 64), m(9, 2, 16, 64)]
+    assert not ops.attention_tree(*args, m(1, 3, dtype=i), m(1, dtype=i)).requires_grad
+    for x in args:
+        x.requires_grad_()
+        out = ops.attention_tree(*args, m(1, 3, dtype=i), m(1, dtype=i))
+        assert out.requires_grad
+        with pytest.raises(RuntimeError, match="attention_tree"):
+            out.sum().backward()
+        with torch.no_grad():
+            assert not ops.attention_tree(*args, m(1, 3, dtype=i), m(1, dtype=i)).requires_grad
+        x.requires_grad_(False)
