@@ -51,7 +51,8 @@ class PagedCache:
 
     def reserve(self, extra) -> torch.Tensor:
         """Pages for `extra` more positions (one number, or one per slot). Returns `missing`
-        [1], on the GPU: over 0, the pages did not suffice and none was given out."""
+        [1], on the GPU: over 0, the pages did not suffice and none was given out, so that slots
+        may lack the pages of the tokens to come (append then drops what does not fit)."""
         if isinstance(extra, int):
             extra = torch.full_like(self.lens, extra)
         tables, refs, missing = ops.cache_reserve(self.tables, self.lens, self.refs, self._slots(extra), self.page_size)
@@ -59,8 +60,11 @@ class PagedCache:
         return self.missing
 
     def append(self, k, v, path=None, count=None) -> None:
-        """Keeps rows of k and v [layers, slots, T, kv_heads, head_dim]; see ops.cache_append."""
-        self._keep(lens=ops.cache_append(k, v, self.k, self.v, self.tables, self.lens, path, count))
+        """Keeps rows of k and v [layers, slots, T, kv_heads, head_dim]; see ops.cache_append. A slot
+        keeps what its pages hold: its length ends with them, and the rows after that are dropped."""
+        lens = ops.cache_append(k, v, self.k, self.v, self.tables, self.lens, path, count)
+        room = (self.tables >= 0).sum(1, dtype=torch.int32) * self.page_size
+        torch.minimum(lens, room, out=self.lens)
 
     def fork(self, src, dst) -> torch.Tensor:
         """Slots `dst` become copies of slots `src`; returns `missing` [1] as reserve does."""
@@ -121,7 +125,8 @@ def speculative_step(blocks: list[DecoderBlock], embedding: torch.Tensor, head: 
                      last: torch.Tensor, drafts: torch.Tensor, uniforms: torch.Tensor, parents=None, draft_probs=None):
     """One step of every slot: `last` [slots], its latest token (not in the cache yet), and
     `drafts` [slots, T] after it, T <= 127, go through the blocks as one tree; the accepted
-    ones are kept in the cache, for which pages have to be reserved (T + 1 positions).
+    ones are kept in the cache, for which pages have to be reserved (T + 1 positions; where that
+    left pages missing, a slot without the room loses accepted tokens: look at `missing` first).
 
     parents, draft_probs and uniforms [slots, T + 1] as in ops.verify_drafts; embedding
     [V, d_model], head [d_model, V]. Returns (path, count, token): the accepted drafts of each

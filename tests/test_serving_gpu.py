@@ -174,6 +174,29 @@ def test_a_step_replays_from_a_graph():
     assert torch.equal(a.lens, b.lens) and torch.equal(a.tables, b.tables)
 
 
+def test_a_length_ends_with_the_pages():
+    """After a reserve that failed, rows without a page are dropped and not counted: no later
+    attention reads positions that were never written."""
+    blocks = blocks_of(1, torch.float32)
+    x = torch.randn(2, 20, 256, device=DEV)
+    cache = PagedCache(1, 2, 4, 4, 64, page_size=8, dtype=torch.float32)
+    cache.k.fill_(float("nan"))
+    cache.v.fill_(float("nan"))
+    cache.reserve([8, 16])
+    assert cache.reserve(20).item() > 0
+    _, k, v = decode(blocks, x, cache)
+    cache.append(k, v)
+    assert cache.lens.tolist() == [8, 16]
+    path = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    cache.append(k[:, :, :3], v[:, :, :3], path, torch.tensor([3, 2], dtype=torch.int32, device=DEV))
+    assert cache.lens.tolist() == [8, 16]
+    assert cache.reserve([1, 0]).item() == 0  # the last free page, with whatever it holds
+    y, _, _ = decode(blocks, x[:, :1], cache)
+    for b, n in enumerate((8, 16)):
+        want = whole(blocks, torch.cat([x[b, :n], x[b, :1]]))[-1]
+        assert (y[b, 0] - want).abs().max() / want.abs().max() < BOUND[torch.float32]
+
+
 def test_refusals():
     with pytest.raises(ValueError):
         PagedCache(1, 0, 4, 4, 64)
