@@ -78,7 +78,7 @@ __device__ __forceinline__ void exp_pack_rounded(uint32_t* v, float scale_log2, 
   }
 }
 
-// exp_pack in two parts: hi the exponentials cut off to bf16, lo what that left, rounded (2^-16 of
+// exp_pack in two parts: hi the exponentials cut off to bf16, lo what that left, rounded (2^-15 of
 // the exponential); the sum is over the exponentials in fp32. Neither part is negative, and lo has
 // 2^-40 of the exponential added, so that it is zero only where that is: an infinity in V times
 // either part is that infinity, and no NaN (0 inf, inf - inf) comes of their sum.

@@ -145,6 +145,36 @@ def test_attention_tree(B, T, H, Hkv, d, page, lens, dtype, tree):
     N.check_device(torch.cuda.current_stream().cuda_stream)
 
 
+def cancelling(B, T, H, Hkv, d, page, lens):
+    """Peaked weights over values of one size and alternating sign: |out| is far below sum p |v|."""
+    x = list(setup_attention(B, T, H, Hkv, d, page, lens, BF, seed=sum(lens)))
+    x[0] = x[0] * 3
+    x[2] = (1 - 2 * (torch.arange(T, device=DEV) % 2))[None, :, None, None].expand_as(x[2]).to(BF)
+    for b, n in enumerate(lens):
+        for p in range(-(-n // page)):
+            used = min(page, n - p * page)
+            x[4][int(x[5][b, p]), :, :used] = (1 - 2 * ((torch.arange(used, device=DEV) + p * page) % 2))[:, None].to(BF)
+    return x
+
+
+@pytest.mark.parametrize("T,H,d,page,lens", [(1, 8, 128, 16, [5, 60, 300, 1024]), (9, 8, 64, 16, [0, 33, 129, 1024]),
+                                             (64, 16, 128, 64, [20, 900, 1024]), (100, 4, 64, 24, [77, 1000])])
+def test_attention_keeps_the_exponentials_second_part(T, H, d, page, lens):
+    """bf16, up to 1024 cached positions: the first part of an exponential is cut off (less than
+    2^-7 of it is left), the second is that, rounded (2^-8 of it). So the error is the output's
+    rounding (2^-8 of it), at most 2^-15 sum p |v|, and fp32's part."""
+    x = cancelling(len(lens), T, H, 2, d, page, lens)
+    want, mag = attention_64(*x, None, 1 / math.sqrt(d))
+    err = (ops.attention_tree(*x).double().cpu() - want).abs()
+    bound = 2e-5 * (1 + mag) + (1 + 2.0 ** -6) * 2.0 ** -8 * want.abs() + 2.0 ** -15 * mag
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+def test_attention_past_the_exponentials_second_part():
+    x = cancelling(2, 3, 8, 2, 128, 16, [1025, 1024])
+    check_attention(ops.attention_tree(*x), *attention_64(*x, None, 128 ** -0.5))
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_odd_parents(dtype):
     """Parents that are no earlier token, children of absent tokens, a whole slot absent, a
