@@ -394,7 +394,8 @@ __global__ void __launch_bounds__(kThreads) tree_attention_kernel(const __grid_c
       x.w = fmaf(f, y.w, x.w);
     }
     if (a.splits == 1) {
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;  // 0: an absent token
+      const bool present = !parents || parents[row / a.group] >= -1;
+      const float inv = present ? 1.f / sum : 0.f;
       const int64_t at = (((int64_t)b * a.tokens + row / a.group) * a.heads + kvh * a.group + row % a.group) * a.d + c;
       store4(static_cast<T*>(a.out) + at, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
     } else {
@@ -478,7 +479,8 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   }
   if ((int64_t)blockIdx.x * kRowsHere + mine >= all || c >= a.d || (halves && lane >= 16)) return;
   const int r = (int)(row % rows), kvh = (int)(row / rows % a.kv_heads), b = (int)(row / rows / a.kv_heads);
-  const float inv = l > 0.f ? 1.f / l : 0.f;  // 0: an absent token
+  const bool present = !a.parents || a.parents[(int64_t)b * a.tokens + r / a.group] >= -1;
+  const float inv = present ? 1.f / l : 0.f;
   const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + kvh * a.group + r % a.group) * a.d + c;
   store4(static_cast<T*>(a.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }

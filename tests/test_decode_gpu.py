@@ -330,6 +330,20 @@ def test_attention_nan_scores_alone(dtype, d, page, T):
     check_with_infinities(ops.attention_tree(*x, None), *attention_64(*x, None, 1 / math.sqrt(d)))
 
 
+@pytest.mark.parametrize("dtype,d,page", INFINITIES)
+def test_attention_scores_of_minus_infinity_alone(dtype, d, page):
+    """A token that sees nothing but keys scored minus infinity is 0 / 0, whichever kernel takes it
+    and however its row is cut; an absent one is 0."""
+    q, k, v, kc, vc, tables, lens = setup_attention(3, 3, 4, 2, d, page, [0, 40, 3000], dtype, junk=0.0)
+    q[..., 0] = 1
+    for c in (k, kc):
+        c[..., 0] = float("-inf")
+    x = (q, k, v, kc, vc, tables, lens)
+    parents = i32([[-1, 0, -2]] * 3)
+    got = ops.attention_tree(*x, parents)
+    assert got[:, :2].isnan().all() and (got[:, 2] == 0).all()
+
+
 @pytest.mark.parametrize("dtype,T", [(BF, 1), (BF, 70), (F32, 3)])
 def test_attention_growing_maxima(dtype, T):
     """Every later key scores higher: the running maximum grows in every tile."""
