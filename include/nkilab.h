@@ -358,7 +358,8 @@ size_t nkl_attention_tree_workspace_size(int64_t batch, int64_t tokens, int64_t 
  * and the bf16 tensor-core kernel (head_dim 64 or 128, page_size a multiple of 8, at most
  * 128 query heads per kv head) takes the exponentials in bf16 for their product with v: as a
  * sum of two for sequences of up to 1024 cached positions, rounded to one, with the sum of
- * the rounded ones below it, for longer ones. */
+ * the rounded ones below it, for longer ones. Infinities and NaN that a token sees show as in the
+ * formula, those that it does not see not at all. */
 int nkl_attention_tree(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
                        const int64_t* new_strides, const void* k_cache, const void* v_cache,
                        const int64_t* cache_strides, const int32_t* tables, const int32_t* lens,
@@ -421,7 +422,8 @@ int nkl_cache_compact(void* k_cache, void* v_cache, const int64_t* cache_strides
  * they are a tree (parents as in nkl_attention_tree; NULL: a chain): a node's children are
  * tried in order of index, accepted if u * (1 - mass of the rejected ones) < p(x), and what the
  * rejected ones leave is drawn from. Either way the result is distributed as the target.
- * A token outside the vocabulary is never accepted (in a chain it ends it). Probabilities and
+ * A token outside the vocabulary is never accepted (in a chain it ends it), nor is an absent one
+ * or, unlike in the attention, a child of an absent one. Probabilities and
  * uniform numbers are taken as whole multiples of 2^-31 and summed as whole numbers, so the
  * result does not depend on an order of summation. path [batch, drafted]: the accepted tokens'
  * indices, then -1; count [batch]; token [batch]: the first x whose cumulative weight is

@@ -340,6 +340,8 @@ struct ReserveArgs {
   int batch, max_pages, pages, page;
 };
 
+// One block. Measured, calls in a row: 64 slots of 64 entries, 4096 pages 7.8 us; 256 of 64, 16384 pages
+// 14.8; 1024 of 128, 65536 pages 48: it reads and writes all tables and counts.
 __global__ void __launch_bounds__(kPlanThreads) cache_reserve_kernel(const __grid_constant__ ReserveArgs a) {
   __shared__ u64 scratch[33];
   __shared__ int over;

@@ -32,7 +32,8 @@
 // Measured, GPU time with the join (bf16; 6.5 TB/s is what a copy of memory reaches):
 //   1 token, 203 positions, 32 heads over 8 of 128              9.6 us
 //   16 tokens, 4 sequences of up to 4096, 32 heads of 128      42 us (158 MB: 24 us by bytes)
-//   1 token, 65536 positions, 32 heads over 8 of 128           60.5 us (268 MB: 41 us by bytes)
+//   1 token, 65536 positions, 32 heads over 8 of 128           58.5 us (268 MB: 41 us by bytes)
+//   1 token, 64 sequences of about 700, 32 heads over 8       64.6 us (183 MB: 28 us by bytes)
 //   64 tokens, 2 sequences of up to 65536, 32 heads over 8    126 us (427 MB, 109 GFLOP: 67 us either way)
 // What bounds them: the first is one chain of dependent steps, lengths -> table -> tile ->
 // softmax -> product -> store. In the second a block has some 15 tiles; starting (6 us), the

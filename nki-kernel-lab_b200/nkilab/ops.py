@@ -189,7 +189,8 @@ def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=
     last cached position, -2 for an absent token (its output is zero, none sees it). None:
     each token follows the one before it, so T = 1 is plain decoding and T > 1 a chunk of a
     prompt. At most 128 tokens; scale defaults to 1/sqrt(d). d: a multiple of 8 up to 128
-    (64 and 128 in bf16, with pages of a multiple of 8 positions, run on the tensor cores).
+    (64 and 128 in bf16, with pages of a multiple of 8 positions, run on tcgen05). There is
+    no backward pass: one through it raises.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
@@ -200,7 +201,7 @@ def cache_append(k, v, k_cache, v_cache, tables, lens, path=None, count=None):
     """Writes rows of k and v [(layers,) B, T, Hkv, d] to the pages at positions lens[b]
     onward and returns the new lengths: row path[b, j] for j < count[b] (the accepted path
     of drafted tokens), or all T rows in order. The pages come from cache_reserve; rows
-    without a page are dropped."""
+    without a page are dropped, but counted in the lengths (PagedCache.append bounds them)."""
     if k_cache.dim() == 4:  # one layer
         k, v, k_cache, v_cache = (t.unsqueeze(0) for t in (k, v, k_cache, v_cache))
     return _cache_append(k, v, k_cache, v_cache, tables, lens, path, count)
@@ -239,7 +240,8 @@ def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):
     that the tokens are distributed as the target's. probs [B, T + 1, V]: row 0 after the last
     cached token, row i + 1 after drafted token i; tokens [B, T] int32; uniforms [B, T + 1]
     float32 in [0, 1). A chain with draft_probs [B, T, V] (what each token was drawn from), or
-    a tree with parents [B, T] (None: a chain) and no draft_probs.
+    a tree with parents [B, T] (None: a chain) and no draft_probs. Absent tokens and their
+    children are never accepted.
 
     Returns (path [B, T], the accepted tokens' indices and then -1; count [B]; token [B]).
     Sums are whole numbers of 2^-31, so equal inputs give equal tokens on every launch.
