@@ -379,6 +379,48 @@ int nkl_cache_append(const void* k, const void* v, const int64_t* kv_strides, vo
                      int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages,
                      int dtype, void* stream);
 
+/* Rotary positions of x [batch, tokens, heads, head_dim] (strides [batch, token, head] as for the
+ * attention above, NULL: dense) into out (dense): the first rotary_dim entries of a head are pairs
+ * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if `interleaved`, that turn by the angle position *
+ * freqs[i], times `magnitude`; the others are copied. `inverse` turns back, which is the gradient.
+ * freqs: rotary_dim / 2 doubles on the device, radians to a position; the angle is reduced to one
+ * turn in 64 bits. positions (int32, device): [batch, tokens] if `per_token`, else [batch], where
+ * token j has its sequence's position + j, or with `parents` [batch, tokens] + its depth in the tree
+ * (as in nkl_attention_tree; an absent token: 0; at most NKL_MAX_DRAFTED tokens). head_dim up to 256 and
+ * rotary_dim multiples of 8.
+ * No reference counterpart: rotary embeddings are its listed next step (README.md:89). */
+int nkl_rotary(const void* x, const int64_t* x_strides, const int32_t* positions, const int32_t* parents,
+               const double* freqs, void* out, int64_t batch, int64_t tokens, int64_t heads, int64_t head_dim,
+               int64_t rotary_dim, int per_token, int interleaved, int inverse, float magnitude, int dtype,
+               void* stream);
+
+/* A cache in 8 bits: k_cache and v_cache hold e4m3 numbers, k_scales and v_scales (dense bytes,
+ * e8m0: 2^(byte - 127), 255 is NaN) one power of two for each block of `block` positions of a page
+ * and head: [layers, pages, kv_heads, page_size / block]; a value is number * power. The appends
+ * below choose the smallest 2^e, e >= -100, with which a block's largest magnitude is at most 448 *
+ * 2^e; where a block grows past it, its rows are rounded again. A block that gets an infinity or NaN has the
+ * power NaN. Cache strides are multiples of 16 (elements of one byte), head_dim a multiple of 16 up to 128. */
+
+/* nkl_rotary of q [batch, tokens, heads, head_dim] and k [batch, tokens, kv_heads, head_dim] at the
+ * positions lens[b] + j, into q_out and k_out (dense), and in the same pass the turned k and v to those
+ * positions of one layer's cache: in dtype, or, with k_scales and v_scales, in 8 bits (rounded once,
+ * from fp32). Rows from count[b] on (NULL: none) are turned, but do not go to the cache; nor do rows
+ * without a page. Lengths stay: a step's layers share them. Strides: q and kv [batch, token,
+ * head], cache [page, head, row]. */
+int nkl_rotary_append(const void* q, const int64_t* q_strides, const void* k, const void* v, const int64_t* kv_strides,
+                      void* k_cache, void* v_cache, const int64_t* cache_strides, void* k_scales, void* v_scales,
+                      const int32_t* tables, const int32_t* lens, const int32_t* count, const double* freqs, void* q_out,
+                      void* k_out, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      int64_t rotary_dim, int64_t pages, int64_t page_size, int64_t max_pages, int64_t block,
+                      int interleaved, float magnitude, int dtype, void* stream);
+
+/* nkl_cache_append to a cache in 8 bits; dtype is that of the rows. */
+int nkl_cache_append_8bit(const void* k, const void* v, const int64_t* kv_strides, void* k_cache, void* v_cache,
+                          const int64_t* cache_strides, void* k_scales, void* v_scales, const int32_t* tables,
+                          const int32_t* lens, const int32_t* path, const int32_t* count, int32_t* lens_out,
+                          int64_t layers, int64_t batch, int64_t tokens, int64_t kv_heads, int64_t head_dim,
+                          int64_t pages, int64_t page_size, int64_t max_pages, int64_t block, int dtype, void* stream);
+
 /* Free pages, lowest index first, for extra[b] more positions of each slot b, in order of
  * b. All or nothing: with too few free pages, or rows too long for the tables, missing[0] > 0
  * says how many lack and tables and refs come out as they went in. */

@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
@@ -87,6 +88,46 @@ int check_caches(const Tensor& k, const Tensor& v, int64_t dims) {
                    "k and v caches differ in dtype or device");
   TORCH_CHECK(k.strides() == v.strides() && k.stride(-1) == 1, "caches need equal strides and contiguous rows");
   return dtype_code(k);
+}
+
+// The caches' type and their powers of two, for a cache in 8 bits: [.., pages, kv heads, blocks of a page].
+struct Scales {
+  void *k, *v;
+  int64_t block;
+};
+Scales check_scales(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k, const Tensor& v, int64_t dims) {
+  TORCH_CHECK_VALUE(k_cache.dim() == dims && k_cache.sizes() == v_cache.sizes(), "caches ", k_cache.sizes(), " and ",
+                    v_cache.sizes(), ": need equal shapes of ", dims, " dimensions");
+  const c10::Device dev = k_cache.device();
+  for (const Tensor* c : {&k_cache, &v_cache}) {
+    TORCH_CHECK_TYPE(c->scalar_type() == at::kFloat8_e4m3fn, "a cache with scales is float8_e4m3fn, got ", c->scalar_type());
+    TORCH_CHECK(c->device() == dev, "k and v caches on different devices");
+  }
+  TORCH_CHECK(k_cache.strides() == v_cache.strides() && k_cache.stride(-1) == 1, "caches need equal strides and contiguous rows");
+  for (const Tensor* s : {&k, &v}) {
+    TORCH_CHECK_TYPE(s->scalar_type() == at::kFloat8_e8m0fnu, "scales must be float8_e8m0fnu, got ", s->scalar_type());
+    TORCH_CHECK(s->device() == dev, "scales are on ", s->device(), ", not on ", dev);
+    TORCH_CHECK_VALUE(s->dim() == dims - 1 && s->sizes().slice(0, dims - 2) == k_cache.sizes().slice(0, dims - 2) &&
+                          s->size(-1) >= 1 && s->sizes() == k.sizes() && k_cache.size(-2) % s->size(-1) == 0,
+                      "scales ", k.sizes(), " and ", v.sizes(), ", caches ", k_cache.sizes(),
+                      ": need one for each block of a page and head, and whole blocks");
+    TORCH_CHECK(s->is_contiguous(), "scales must be contiguous");
+  }
+  return {k.data_ptr(), v.data_ptr(), k_cache.size(-2) / k.size(-1)};
+}
+
+void same_device(const Tensor& t, c10::Device dev) {
+  TORCH_CHECK(t.device() == dev, "tensors on different devices: ", t.device(), " vs ", dev);
+}
+
+// The frequencies of a rotation: as many pairs as entries of a head.
+const double* check_freqs(const Tensor& freqs, c10::Device dev, int64_t d) {
+  TORCH_CHECK_TYPE(freqs.scalar_type() == at::kDouble, "freqs must be float64, got ", freqs.scalar_type());
+  same_device(freqs, dev);
+  TORCH_CHECK_VALUE(freqs.dim() == 1 && freqs.size(0) >= 1 && 2 * freqs.size(0) <= d, "freqs ", freqs.sizes(),
+                    ": need one dimension of up to ", d / 2);
+  TORCH_CHECK(freqs.is_contiguous(), "freqs must be contiguous");
+  return static_cast<const double*>(freqs.data_ptr());
 }
 
 // Rows k and v as the kernels read them: equal strides, aligned rows.
@@ -210,6 +251,98 @@ Tensor cache_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cach
                          k_cache.strides().data(), tb, ln, pt, ct, out_ints(lens_out), L, B, T, Hkv, d, P, page, M, dt,
                          c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
   return lens_out;
+}
+
+Tensor cache_append_8bit(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
+                         const Tensor& k_scales, const Tensor& v_scales, const Tensor& tables, const Tensor& lens,
+                         OptTensor path, OptTensor count) {
+  const Scales sc = check_scales(k_cache, v_cache, k_scales, v_scales, 5);
+  const int64_t L = k_cache.size(0), P = k_cache.size(1), Hkv = k_cache.size(2), page = k_cache.size(3),
+                d = k_cache.size(4);
+  TORCH_CHECK_VALUE(k_in.dim() == 5 && k_in.sizes() == v_in.sizes() && k_in.size(0) == L && k_in.size(3) == Hkv &&
+                        k_in.size(4) == d,
+                    "k ", k_in.sizes(), ", v ", v_in.sizes(), ", cache ", k_cache.sizes(),
+                    ": need rows [layers, B, T, kv heads, head_dim]");
+  const int dt = dtype_code(k_in);
+  const int64_t B = k_in.size(1), T = k_in.size(2);
+  same(v_in, k_in);
+  same_device(k_in, k_cache.device());
+  TORCH_CHECK_VALUE(tables.dim() == 2 && tables.size(1) >= 1, "tables ", tables.sizes(), ": need [B, pages of a slot]");
+  const c10::Device dev = k_cache.device();
+  const int64_t M = tables.size(1);
+  const int32_t* tb = ints("tables", tables, dev, {B, M});
+  const int32_t* ln = ints("lens", lens, dev, {B});
+  const int32_t* pt = ints("path", path, dev, {B, T});
+  const int32_t* ct = ints("count", count, dev, {B});
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto [k, v] = rows_of(k_in, v_in);
+  Tensor lens_out = new_ints({B}, dev);
+  check("nkl_cache_append_8bit",
+        nkl_cache_append_8bit(k.data_ptr(), v.data_ptr(), k.strides().data(), k_cache.data_ptr(), v_cache.data_ptr(),
+                              k_cache.strides().data(), sc.k, sc.v, tb, ln, pt, ct, out_ints(lens_out), L, B, T, Hkv, d, P,
+                              page, M, sc.block, dt, c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return lens_out;
+}
+
+Tensor rotary(const Tensor& x_in, const Tensor& positions, const Tensor& freqs, OptTensor parents, bool interleaved,
+              double magnitude, bool inverse) {
+  const int dt = dtype_code(x_in);
+  TORCH_CHECK_VALUE(x_in.dim() == 4, "x ", x_in.sizes(), ": need [B, T, heads, head_dim]");
+  const int64_t B = x_in.size(0), T = x_in.size(1), H = x_in.size(2), d = x_in.size(3);
+  const c10::Device dev = x_in.device();
+  const bool per_token = positions.dim() == 2;
+  const int32_t* at = per_token ? ints("positions", positions, dev, {B, T}) : ints("positions", positions, dev, {B});
+  const int32_t* up = ints("parents", parents, dev, {B, T});
+  const double* f = check_freqs(freqs, dev, d);
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor x = readable(x_in);
+  Tensor out = new_tensor({B, T, H, d}, x.scalar_type(), dev);
+  check("nkl_rotary", nkl_rotary(x.data_ptr(), x.strides().data(), at, up, f, out.data_ptr(), B, T, H, d, 2 * freqs.size(0),
+                                 per_token, interleaved, inverse, (float)magnitude, dt,
+                                 c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> rotary_append(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                                         const Tensor& k_cache, const Tensor& v_cache, OptTensor k_scales,
+                                         OptTensor v_scales, const Tensor& tables, const Tensor& lens, const Tensor& freqs,
+                                         OptTensor count, bool interleaved, double magnitude) {
+  TORCH_CHECK_VALUE(k_scales.has_value() == v_scales.has_value(), "scales: need both or none");
+  Scales sc = {nullptr, nullptr, 0};
+  if (k_scales.has_value()) {
+    sc = check_scales(k_cache, v_cache, *k_scales, *v_scales, 4);
+  } else {
+    check_caches(k_cache, v_cache, 4);
+    same(k_in, k_cache);
+  }
+  const int dt = dtype_code(q_in);
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && k_in.sizes() == v_in.sizes(), "q ", q_in.sizes(), ", k ",
+                    k_in.sizes(), ", v ", v_in.sizes(), ": need [B, T, heads, head_dim]");
+  const int64_t B = q_in.size(0), T = q_in.size(1), H = q_in.size(2), d = q_in.size(3);
+  const int64_t P = k_cache.size(0), Hkv = k_cache.size(1), page = k_cache.size(2);
+  TORCH_CHECK_VALUE(k_in.size(0) == B && k_in.size(1) == T && k_in.size(2) == Hkv && k_in.size(3) == d &&
+                        k_cache.size(3) == d,
+                    "q ", q_in.sizes(), ", k ", k_in.sizes(), ", cache ", k_cache.sizes(), ": sizes do not match");
+  same(k_in, q_in);
+  same(v_in, q_in);
+  const c10::Device dev = k_cache.device();
+  same_device(q_in, dev);
+  TORCH_CHECK_VALUE(tables.dim() == 2 && tables.size(1) >= 1, "tables ", tables.sizes(), ": need [B, pages of a slot]");
+  const int64_t M = tables.size(1);
+  const int32_t* tb = ints("tables", tables, dev, {B, M});
+  const int32_t* ln = ints("lens", lens, dev, {B});
+  const int32_t* ct = ints("count", count, dev, {B});
+  const double* f = check_freqs(freqs, dev, d);
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor q = readable(q_in);
+  const auto [k, v] = rows_of(k_in, v_in);
+  Tensor q_out = new_tensor({B, T, H, d}, q.scalar_type(), dev), k_out = new_tensor({B, T, Hkv, d}, q.scalar_type(), dev);
+  check("nkl_rotary_append",
+        nkl_rotary_append(q.data_ptr(), q.strides().data(), k.data_ptr(), v.data_ptr(), k.strides().data(),
+                          k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), sc.k, sc.v, tb, ln, ct, f,
+                          q_out.data_ptr(), k_out.data_ptr(), B, T, H, Hkv, d, 2 * freqs.size(0), P, page, M, sc.block,
+                          interleaved, (float)magnitude, dt, c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return {q_out, k_out};
 }
 
 std::tuple<Tensor, Tensor, Tensor> cache_reserve(const Tensor& tables, const Tensor& lens, const Tensor& refs,
@@ -337,6 +470,72 @@ Tensor attention_tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v
   return out;
 }
 
+// The gradient of a turn by an angle is the turn by the opposite one, so a pass back through it
+// is the operator itself, and can be passed back through in turn.
+Tensor rotary_op(const Tensor& x, const Tensor& positions, const Tensor& freqs, OptTensor parents, bool interleaved,
+                 double magnitude, bool inverse) {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("nkilab::rotary", "").typed<decltype(rotary)>();
+  return op.call(x, positions, freqs, parents, interleaved, magnitude, inverse);
+}
+
+struct Rotary : public torch::autograd::Function<Rotary> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& positions,
+                        const Tensor& freqs, const std::optional<Tensor>& parents, bool interleaved, double magnitude,
+                        bool inverse) {
+    ctx->save_for_backward({positions, freqs, parents.value_or(Tensor())});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["inverse"] = inverse;
+    at::AutoDispatchBelowADInplaceOrView below;
+    return rotary_op(x, positions, freqs, parents, interleaved, magnitude, inverse);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 const torch::autograd::variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    std::optional<Tensor> parents;
+    if (saved[2].defined()) parents = saved[2];
+    const Tensor grad = rotary_op(grads[0], saved[0], saved[1], parents, ctx->saved_data["interleaved"].toBool(),
+                                  ctx->saved_data["magnitude"].toDouble(), !ctx->saved_data["inverse"].toBool());
+    return {grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& freqs, OptTensor parents,
+                       bool interleaved, double magnitude, bool inverse) {
+  TORCH_CHECK(!torch::autograd::compute_requires_grad(freqs), "nkilab::rotary: freqs have no gradient");
+  if (!torch::autograd::compute_requires_grad(x)) {  // past the graph's bookkeeping: the smallest calls are bound by it
+    at::AutoDispatchBelowADInplaceOrView below;
+    return rotary_op(x, positions, freqs, parents, interleaved, magnitude, inverse);
+  }
+  return Rotary::apply(x, positions, freqs, parents, interleaved, magnitude, inverse);
+}
+
+// The appends are for decoding: what comes out of one that inputs with gradients went into raises
+// when a backward pass gets there.
+std::tuple<Tensor, Tensor> rotary_append_autograd(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                  const Tensor& k_cache, const Tensor& v_cache, OptTensor k_scales,
+                                                  OptTensor v_scales, const Tensor& tables, const Tensor& lens,
+                                                  const Tensor& freqs, OptTensor count, bool interleaved,
+                                                  double magnitude) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("nkilab::rotary_append", "")
+                             .typed<decltype(rotary_append)>();
+  std::tuple<Tensor, Tensor> out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(q, k, v, k_cache, v_cache, k_scales, v_scales, tables, lens, freqs, count, interleaved, magnitude);
+  }
+  if (torch::autograd::compute_requires_grad(q, k, v)) {
+    const std::shared_ptr<torch::autograd::Node> node(
+        new torch::autograd::NotImplemented("nkilab::rotary_append", torch::autograd::collect_next_edges(q, k, v)),
+        torch::autograd::deleteNode);
+    std::vector<Tensor> both = {std::get<0>(out), std::get<1>(out)};
+    torch::autograd::set_history(both, node);
+  }
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nkilab, m) {
@@ -344,6 +543,13 @@ TORCH_LIBRARY_FRAGMENT(nkilab, m) {
         "Tensor? parents, float scale) -> Tensor");
   m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor lens, "
         "Tensor? path, Tensor? count) -> Tensor");
+  m.def("cache_append_8bit(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, "
+        "Tensor(d!) v_scales, Tensor tables, Tensor lens, Tensor? path, Tensor? count) -> Tensor");
+  m.def("rotary(Tensor x, Tensor positions, Tensor freqs, Tensor? parents, bool interleaved, float magnitude, "
+        "bool inverse) -> Tensor");
+  m.def("rotary_append(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!)? k_scales, "
+        "Tensor(d!)? v_scales, Tensor tables, Tensor lens, Tensor freqs, Tensor? count, bool interleaved, "
+        "float magnitude) -> (Tensor, Tensor)");
   m.def("cache_reserve(Tensor tables, Tensor lens, Tensor refs, Tensor extra, int page_size) -> (Tensor, Tensor, Tensor)");
   m.def("cache_fork(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor lens, Tensor refs, Tensor src, "
         "Tensor dst) -> (Tensor, Tensor, Tensor, Tensor)");
@@ -356,6 +562,9 @@ TORCH_LIBRARY_FRAGMENT(nkilab, m) {
 TORCH_LIBRARY_IMPL(nkilab, CUDA, m) {
   m.impl("attention_tree", &attention_tree);
   m.impl("cache_append", &cache_append);
+  m.impl("cache_append_8bit", &cache_append_8bit);
+  m.impl("rotary", &rotary);
+  m.impl("rotary_append", &rotary_append);
   m.impl("cache_reserve", &cache_reserve);
   m.impl("cache_fork", &cache_fork);
   m.impl("cache_free", &cache_free);
@@ -363,4 +572,8 @@ TORCH_LIBRARY_IMPL(nkilab, CUDA, m) {
   m.impl("verify_drafts", &verify_drafts);
 }
 
-TORCH_LIBRARY_IMPL(nkilab, Autograd, m) { m.impl("attention_tree", &attention_tree_autograd); }
+TORCH_LIBRARY_IMPL(nkilab, Autograd, m) {
+  m.impl("attention_tree", &attention_tree_autograd);
+  m.impl("rotary", &rotary_autograd);
+  m.impl("rotary_append", &rotary_append_autograd);
+}

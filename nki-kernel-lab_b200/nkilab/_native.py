@@ -77,6 +77,11 @@ SIGNATURES = {
                                   _i64, _i64, _i64, _f, _int, _p]),
     "nkl_cache_append": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                 _i64, _int, _p]),
+    "nkl_rotary": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _f, _int, _p]),
+    "nkl_rotary_append": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                                 _i64, _i64, _i64, _i64, _i64, _int, _f, _int, _p]),
+    "nkl_cache_append_8bit": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+                                     _i64, _i64, _i64, _int, _p]),
     "nkl_cache_reserve_workspace_size": (_sz, [_i64]),
     "nkl_cache_reserve": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _p]),
     "nkl_cache_fork_workspace_size": (_sz, [_i64, _i64]),

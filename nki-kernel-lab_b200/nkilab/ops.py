@@ -27,7 +27,7 @@ from .kernels import attention as _attn
 
 __all__ = ["choose_blocks", "matmul", "softmax", "rmsnorm", "swiglu", "attention", "ATTENTION_VARIANTS",
            "rope", "attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
-           "verify_drafts"]
+           "verify_drafts", "rotary_frequencies", "rotary", "rotary_append"]
 
 
 # --------------------------------------------------------------------------- matmul
@@ -178,6 +178,7 @@ def _decode(name: str):
 _attention_tree, _cache_append, _cache_reserve, _cache_fork, _cache_free, _cache_compact, _verify_drafts = map(
     _decode, ("attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
               "verify_drafts"))
+_cache_append_8bit, _rotary, _rotary_append = map(_decode, ("cache_append_8bit", "rotary", "rotary_append"))
 
 
 def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=None):
@@ -197,14 +198,87 @@ def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=
     return _attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents, float(scale))
 
 
-def cache_append(k, v, k_cache, v_cache, tables, lens, path=None, count=None):
+def cache_append(k, v, k_cache, v_cache, tables, lens, path=None, count=None, k_scales=None, v_scales=None):
     """Writes rows of k and v [(layers,) B, T, Hkv, d] to the pages at positions lens[b]
     onward and returns the new lengths: row path[b, j] for j < count[b] (the accepted path
     of drafted tokens), or all T rows in order. The pages come from cache_reserve; rows
-    without a page are dropped, but counted in the lengths (PagedCache.append bounds them)."""
+    without a page are dropped, but counted in the lengths (PagedCache.append bounds them).
+
+    With k_scales and v_scales [(layers,) pages, Hkv, blocks of a page] float8_e8m0fnu the caches are
+    float8_e4m3fn (d a multiple of 16 up to 128) and a value is number * scale. Each block of
+    page / blocks positions has the smallest power of two, from 2^-100 on, with which its largest
+    magnitude is at most 448 of it; rows of a block that grows past its power are rounded again. An
+    infinity or NaN makes its block NaN."""
     if k_cache.dim() == 4:  # one layer
         k, v, k_cache, v_cache = (t.unsqueeze(0) for t in (k, v, k_cache, v_cache))
-    return _cache_append(k, v, k_cache, v_cache, tables, lens, path, count)
+        k_scales, v_scales = (t if t is None else t.unsqueeze(0) for t in (k_scales, v_scales))
+    if k_scales is None and v_scales is None:
+        return _cache_append(k, v, k_cache, v_cache, tables, lens, path, count)
+    if k_scales is None or v_scales is None:
+        raise ValueError("scales: need both or none")
+    return _cache_append_8bit(k, v, k_cache, v_cache, k_scales, v_scales, tables, lens, path, count)
+
+
+ROTARY_SCALINGS = (None, "linear", "ntk", "yarn")
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, trained=None, device=None):
+    """(freqs, magnitude) for `rotary`: freqs [rotary_dim / 2] float64, radians to a position, base^(-2i /
+    rotary_dim), stretched by `factor` for contexts longer than the `trained` one:
+
+    "linear"  every frequency / factor (positions interpolated)
+    "ntk"     base * factor^(r / (r - 2)), which divides the lowest frequency by factor
+    "yarn"    frequencies that turn less than once in `trained` positions / factor, those that turn
+              over 32 times as they are, mixed linearly between; magnitude 0.1 ln(factor) + 1
+              (Peng et al., YaRN, 2023)
+    """
+    r = int(rotary_dim)
+    if r < 2 or r % 2:
+        raise ValueError(f"rotary_dim {rotary_dim}: must be even and positive")
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"scaling {scaling!r}: one of {ROTARY_SCALINGS}")
+    if not (base > 1 and factor >= 1):
+        raise ValueError(f"base {base}, factor {factor}: need base > 1 and factor >= 1")
+    if scaling == "yarn" and not trained:
+        raise ValueError("yarn: needs the number of trained positions")
+    if scaling == "ntk":
+        if r < 4:
+            raise ValueError("ntk: needs a rotary_dim of 4 or more")
+        base = base * factor ** (r / (r - 2))
+    f = float(base) ** (-2 * torch.arange(r // 2, dtype=torch.float64) / r)
+    magnitude = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        stay = ((trained * f / (2 * math.pi) - 1) / 31).clamp(0, 1)
+        f = f * (stay + (1 - stay) / factor)
+        magnitude = 0.1 * math.log(factor) + 1
+    return f.to(torch.device("cuda", torch.cuda.current_device()) if device is None else device), magnitude
+
+
+def rotary(x, positions, freqs, parents=None, interleaved=False, magnitude=1.0):
+    """Rotary positions of x [B, T, heads, d] (queries and keys of a fused projection together, as
+    they lie): the first 2 len(freqs) entries of a head are pairs (i, i + len(freqs)), or (2i, 2i + 1) if
+    `interleaved`, turned by position * freqs[i] and times magnitude; the rest stays. Both sizes are
+    multiples of 8, d up to 256.
+
+    positions int32: [B, T], or [B], where token j is at positions[b] + j, or, in a tree (parents
+    [B, T] as in attention_tree), as far behind as it is deep. Angles are reduced in 64 bits. x may
+    need a gradient, which turns the other way.
+    """
+    return _rotary(x, positions, freqs, parents, bool(interleaved), float(magnitude), False)
+
+
+def rotary_append(q, k, v, k_cache, v_cache, tables, lens, freqs, count=None, interleaved=False, magnitude=1.0,
+                  k_scales=None, v_scales=None):
+    """q [B, T, H, d] and k [B, T, Hkv, d] turned as by `rotary` at positions lens[b] + j, and the
+    turned k and v written to those positions of one layer's cache (in 8 bits with scales, see
+    cache_append; rounded once there). Returns (q, k). Rows from count[b] on stay out of
+    the cache, as do rows without a page; lens stays as it is, for a step's layers share it. There
+    is no backward pass: one through it raises.
+    """
+    return _rotary_append(q, k, v, k_cache, v_cache, k_scales, v_scales, tables, lens, freqs, count, bool(interleaved),
+                          float(magnitude))
 
 
 def cache_reserve(tables, lens, refs, extra, page_size):

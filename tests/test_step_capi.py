@@ -1,0 +1,145 @@
+"""Argument checks of the operators around a decoding step, their shape functions and their host
+arithmetic (CPU only: no call here reaches a kernel launch)."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+
+FAKE = ctypes.c_void_p(4096)  # never dereferenced: every call below fails validation first
+ODD = ctypes.c_void_p(4104)   # 8-byte but not 16-byte aligned
+
+
+@pytest.fixture(scope="module")
+def N():
+    from nkilab import _native
+
+    return _native
+
+
+def strides(*s):
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def rotary(N, **kw):
+    a = dict(x=FAKE, xs=None, positions=FAKE, parents=None, freqs=FAKE, out=FAKE, B=2, T=3, H=4, d=64, r=32, per=0, inter=0,
+             inv=0, mag=1.0, dt=N.BFLOAT16)
+    assert not set(kw) - set(a)
+    a.update(kw)
+    return N.lib.nkl_rotary(*a.values(), None)
+
+
+def test_rotary_refusals(N):
+    assert rotary(N, dt=4) == N.ERR_DTYPE
+    for kw in (dict(d=60), dict(d=264), dict(r=0), dict(r=12), dict(r=72), dict(H=0), dict(B=-1), dict(T=-1)):
+        assert rotary(N, **kw) == N.ERR_SHAPE
+    for name in ("x", "positions", "freqs", "out"):
+        assert rotary(N, **{name: None}) == N.ERR_ARG
+    assert rotary(N, parents=FAKE, per=1) == N.ERR_ARG
+    assert rotary(N, parents=FAKE, T=129) == N.ERR_ARG and b"128" in N.lib.nkl_last_error()
+    for name in ("x", "out"):
+        assert rotary(N, **{name: ODD}) == N.ERR_ALIGN
+    assert rotary(N, xs=strides(768, 260, 64)) == N.ERR_ALIGN
+    assert rotary(N, xs=strides(768, 256, -64)) == N.ERR_ALIGN
+    assert rotary(N, B=0, x=None) == N.OK
+    assert rotary(N, T=0, x=None) == N.OK
+
+
+def append(N, **kw):
+    a = dict(q=FAKE, qs=None, k=FAKE, v=FAKE, ns=None, kc=FAKE, vc=FAKE, cs=None, ks=FAKE, vs=FAKE, tables=FAKE, lens=FAKE,
+             count=None, freqs=FAKE, qo=FAKE, ko=FAKE, B=2, T=3, H=8, Hkv=2, d=64, r=64, P=10, page=16, M=4, block=16, inter=0,
+             mag=1.0, dt=N.BFLOAT16)
+    assert not set(kw) - set(a)
+    a.update(kw)
+    return N.lib.nkl_rotary_append(*a.values(), None)
+
+
+def test_rotary_append_refusals(N):
+    assert append(N, dt=4) == N.ERR_DTYPE
+    for kw in (dict(d=72), dict(d=144, r=144), dict(r=0), dict(r=72), dict(block=0), dict(block=5), dict(block=32), dict(page=0),
+               dict(M=0), dict(P=0), dict(Hkv=0), dict(H=0), dict(page=65536, M=1 << 20)):
+        assert append(N, **kw) == N.ERR_SHAPE
+    for name in ("q", "k", "v", "kc", "vc", "tables", "lens", "freqs", "qo", "ko", "ks", "vs"):
+        assert append(N, **{name: None}) == N.ERR_ARG
+    for name in ("q", "k", "v", "kc", "vc", "qo", "ko"):
+        assert append(N, **{name: ODD}) == N.ERR_ALIGN
+    assert append(N, cs=strides(2048, 1024, 72)) == N.ERR_ALIGN
+    assert append(N, ns=strides(384, 128, 63)) == N.ERR_ALIGN
+    assert append(N, B=0, q=None) == N.OK
+    assert append(N, T=0, q=None) == N.OK
+
+
+def test_append_8bit_refusals(N):
+    def call(**kw):
+        a = dict(k=FAKE, v=FAKE, ns=None, kc=FAKE, vc=FAKE, cs=None, ks=FAKE, vs=FAKE, tables=FAKE, lens=FAKE, path=None,
+                 count=None, out=FAKE, L=2, B=2, T=3, Hkv=2, d=64, P=10, page=16, M=4, block=8, dt=N.BFLOAT16)
+        assert not set(kw) - set(a)
+        a.update(kw)
+        return N.lib.nkl_cache_append_8bit(*a.values(), None)
+
+    assert call(dt=9) == N.ERR_DTYPE
+    for kw in (dict(d=72), dict(d=256), dict(L=0), dict(Hkv=0), dict(P=0), dict(page=0), dict(M=0), dict(block=3), dict(B=-1), dict(T=-1)):
+        assert call(**kw) == N.ERR_SHAPE
+    for name in ("k", "v", "kc", "vc", "ks", "vs", "tables", "lens", "out"):
+        assert call(**{name: None}) == N.ERR_ARG
+    for name in ("k", "v", "kc", "vc"):
+        assert call(**{name: ODD}) == N.ERR_ALIGN
+    assert call(B=0) == N.OK
+
+
+def test_shapes_without_a_gpu():
+    import torch
+
+    from nkilab import ops
+
+    def m(*shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    bf = torch.bfloat16
+    B, T, H, Hkv, d = 2, 5, 8, 2, 64
+    x, k = m(B, T, H, d, dtype=bf), m(B, T, Hkv, d, dtype=bf)
+    assert ops.rotary(x, m(B), m(16, dtype=torch.float64)).shape == x.shape
+    c, s = m(20, Hkv, 16, d, dtype=torch.float8_e4m3fn), m(20, Hkv, 2, dtype=torch.float8_e8m0fnu)
+    q2, k2 = ops.rotary_append(x, k, k, c, c, m(B, 3), m(B), m(32, dtype=torch.float64), k_scales=s, v_scales=s)
+    assert q2.shape == x.shape and k2.shape == k.shape and q2.dtype == bf
+    assert ops.cache_append(k, k, c, c, m(B, 3), m(B), None, None, s, s).shape == (B,)
+    with pytest.raises(ValueError):
+        ops.cache_append(k, k, c, c, m(B, 3), m(B), None, None, s)
+
+
+def test_rotary_frequencies():
+    import torch
+
+    from nkilab import ops
+
+    f, m = ops.rotary_frequencies(64, 10000.0, device="cpu")
+    assert f.dtype == torch.float64 and f.shape == (32,) and m == 1.0
+    assert f[0] == 1.0 and f[16].item() == pytest.approx(0.01, rel=1e-12)
+    g, m = ops.rotary_frequencies(64, 10000.0, "linear", 4.0, device="cpu")
+    assert torch.equal(g, f / 4) and m == 1.0
+    g, m = ops.rotary_frequencies(64, 10000.0, "ntk", 8.0, device="cpu")
+    assert g[0] == 1.0 and g[-1].item() == pytest.approx(f[-1].item() / 8, rel=1e-12)
+    g, m = ops.rotary_frequencies(64, 10000.0, "yarn", 8.0, 4096, device="cpu")
+    assert m == pytest.approx(0.1 * math.log(8) + 1)
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.equal(g[turns >= 32], f[turns >= 32]) and torch.allclose(g[turns <= 1], f[turns <= 1] / 8, rtol=1e-14)
+    mid = (turns > 1) & (turns < 32)
+    assert mid.any() and (g[mid] < f[mid]).all() and (g[mid] > f[mid] / 8).all()
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, scaling="cubic"), dict(rotary_dim=8, factor=0.5),
+                dict(rotary_dim=8, base=1.0), dict(rotary_dim=8, scaling="yarn"), dict(rotary_dim=2, scaling="ntk")):
+        with pytest.raises(ValueError):
+            ops.rotary_frequencies(**bad, device="cpu")
+
+
+def test_wrappers_take_no_cpu_tensors():
+    import torch
+
+    from nkilab import ops
+
+    x, i = torch.zeros(1, 1, 2, 64), torch.zeros(1, dtype=torch.int32)
+    f = torch.ones(32, dtype=torch.float64)
+    with pytest.raises(NotImplementedError):
+        ops.rotary(x, i, f)
+    with pytest.raises(NotImplementedError):
+        ops.rotary_append(x, x, x, x, x, i[None], i, f)
