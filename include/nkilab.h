@@ -414,6 +414,20 @@ int nkl_rotary_append(const void* q, const int64_t* q_strides, const void* k, co
                       int64_t rotary_dim, int64_t pages, int64_t page_size, int64_t max_pages, int64_t block,
                       int interleaved, float magnitude, int dtype, void* stream);
 
+/* nkl_attention_tree over one layer's cache in 8 bits; dtype is that of q, the drafted tokens' k_new and
+ * v_new, and out. fp32 accumulation and softmax statistics, weights rounded to f16 (fp32: to 22
+ * bits) for their product with v; the cache's values enter the products as they are. Of its
+ * numbers, the appends never write e4m3's code for NaN, and it is not looked for. head_dim a multiple of 16 up to 128. */
+size_t nkl_attention_tree_8bit_workspace_size(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                              int64_t head_dim, int64_t page_size, int64_t max_pages, int dtype);
+int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
+                            const int64_t* new_strides, const void* k_cache, const void* v_cache,
+                            const int64_t* cache_strides, const void* k_scales, const void* v_scales,
+                            const int32_t* tables, const int32_t* lens, const int32_t* parents, void* out,
+                            void* workspace, size_t workspace_bytes, int64_t batch, int64_t tokens, int64_t heads,
+                            int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages,
+                            int64_t block, float scale, int dtype, void* stream);
+
 /* nkl_cache_append to a cache in 8 bits; dtype is that of the rows. */
 int nkl_cache_append_8bit(const void* k, const void* v, const int64_t* kv_strides, void* k_cache, void* v_cache,
                           const int64_t* cache_strides, void* k_scales, void* v_scales, const int32_t* tables,

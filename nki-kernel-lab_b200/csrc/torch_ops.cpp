@@ -224,6 +224,44 @@ Tensor attention_tree(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in
   return out;
 }
 
+Tensor attention_tree_8bit(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache,
+                           const Tensor& v_cache, const Tensor& k_scales, const Tensor& v_scales, const Tensor& tables,
+                           const Tensor& lens, OptTensor parents, double scale) {
+  const Scales sc = check_scales(k_cache, v_cache, k_scales, v_scales, 4);
+  const int dt = dtype_code(q_in);
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && k_in.sizes() == v_in.sizes(), "q ", q_in.sizes(), ", k ",
+                    k_in.sizes(), ", v ", v_in.sizes(), ": need [B, T, heads, head_dim]");
+  const int64_t B = q_in.size(0), T = q_in.size(1), H = q_in.size(2), d = q_in.size(3);
+  const int64_t P = k_cache.size(0), Hkv = k_cache.size(1), page = k_cache.size(2);
+  TORCH_CHECK_VALUE(k_in.size(0) == B && k_in.size(1) == T && k_in.size(2) == Hkv && k_in.size(3) == d &&
+                        k_cache.size(3) == d && Hkv > 0 && H % Hkv == 0,
+                    "q ", q_in.sizes(), ", k ", k_in.sizes(), ", cache ", k_cache.sizes(),
+                    ": sizes do not match, or the cache's heads do not divide q's");
+  same(k_in, q_in);
+  same(v_in, q_in);
+  const c10::Device dev = k_cache.device();
+  same_device(q_in, dev);
+  TORCH_CHECK_VALUE(T <= NKL_MAX_DRAFTED, T, " drafted tokens, at most ", NKL_MAX_DRAFTED, " are taken");
+  TORCH_CHECK_VALUE(tables.dim() == 2 && tables.size(1) >= 1, "tables ", tables.sizes(), ": need [B, pages of a slot]");
+  const int64_t M = tables.size(1);
+  const int32_t* tb = ints("tables", tables, dev, {B, M});
+  const int32_t* ln = ints("lens", lens, dev, {B});
+  const int32_t* up = ints("parents", parents, dev, {B, T});
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor q = readable(q_in);
+  const auto [k, v] = rows_of(k_in, v_in);
+  const cudaStream_t st = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  Tensor out = new_tensor({B, T, H, d}, q.scalar_type(), dev);
+  const size_t bytes = nkl_attention_tree_8bit_workspace_size(B, T, H, Hkv, d, page, M, dt);
+  const Workspace ws = workspace(dev, st, bytes);
+  check("nkl_attention_tree_8bit",
+        nkl_attention_tree_8bit(q.data_ptr(), q.strides().data(), k.data_ptr(), v.data_ptr(), k.strides().data(),
+                                k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), sc.k, sc.v, tb, ln, up,
+                                out.data_ptr(), ws.data, bytes, B, T, H, Hkv, d, P, page, M, sc.block, (float)scale, dt,
+                                st));
+  return out;
+}
+
 Tensor cache_append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
                     const Tensor& tables, const Tensor& lens, OptTensor path, OptTensor count) {
   const int dt = check_caches(k_cache, v_cache, 5);
@@ -449,6 +487,18 @@ std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& probs_in, const T
 }
 
 // The attention has no backward pass: with inputs that require a gradient, one through it raises.
+Tensor no_backward(Tensor out, const char* name, std::initializer_list<Tensor> inputs) {
+  const std::vector<Tensor> in(inputs);
+  bool any = false;
+  for (const Tensor& t : in) any |= torch::autograd::compute_requires_grad(t);
+  if (any) {
+    const std::shared_ptr<torch::autograd::Node> node(
+        new torch::autograd::NotImplemented(name, torch::autograd::collect_next_edges(in)), torch::autograd::deleteNode);
+    torch::autograd::set_history(out, node);
+  }
+  return out;
+}
+
 Tensor attention_tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_cache,
                                const Tensor& v_cache, const Tensor& tables, const Tensor& lens, OptTensor parents,
                                double scale) {
@@ -460,14 +510,23 @@ Tensor attention_tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v
     at::AutoDispatchBelowADInplaceOrView below;
     out = op.call(q, k, v, k_cache, v_cache, tables, lens, parents, scale);
   }
-  if (torch::autograd::compute_requires_grad(q, k, v, k_cache, v_cache)) {
-    const std::shared_ptr<torch::autograd::Node> node(
-        new torch::autograd::NotImplemented("nkilab::attention_tree",
-                                            torch::autograd::collect_next_edges(q, k, v, k_cache, v_cache)),
-        torch::autograd::deleteNode);
-    torch::autograd::set_history(out, node);
+  if (!torch::autograd::compute_requires_grad(q, k, v, k_cache, v_cache)) return out;
+  return no_backward(out, "nkilab::attention_tree", {q, k, v, k_cache, v_cache});
+}
+
+Tensor attention_tree_8bit_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_cache,
+                                    const Tensor& v_cache, const Tensor& k_scales, const Tensor& v_scales,
+                                    const Tensor& tables, const Tensor& lens, OptTensor parents, double scale) {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("nkilab::attention_tree_8bit", "")
+                             .typed<decltype(attention_tree_8bit_autograd)>();
+  Tensor out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(q, k, v, k_cache, v_cache, k_scales, v_scales, tables, lens, parents, scale);
   }
-  return out;
+  if (!torch::autograd::compute_requires_grad(q, k, v)) return out;
+  return no_backward(out, "nkilab::attention_tree_8bit", {q, k, v});
 }
 
 // The gradient of a turn by an angle is the turn by the opposite one, so a pass back through it
@@ -541,6 +600,8 @@ std::tuple<Tensor, Tensor> rotary_append_autograd(const Tensor& q, const Tensor&
 TORCH_LIBRARY_FRAGMENT(nkilab, m) {
   m.def("attention_tree(Tensor q, Tensor k, Tensor v, Tensor k_cache, Tensor v_cache, Tensor tables, Tensor lens, "
         "Tensor? parents, float scale) -> Tensor");
+  m.def("attention_tree_8bit(Tensor q, Tensor k, Tensor v, Tensor k_cache, Tensor v_cache, Tensor k_scales, Tensor v_scales, "
+        "Tensor tables, Tensor lens, Tensor? parents, float scale) -> Tensor");
   m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor lens, "
         "Tensor? path, Tensor? count) -> Tensor");
   m.def("cache_append_8bit(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, "
@@ -561,6 +622,7 @@ TORCH_LIBRARY_FRAGMENT(nkilab, m) {
 
 TORCH_LIBRARY_IMPL(nkilab, CUDA, m) {
   m.impl("attention_tree", &attention_tree);
+  m.impl("attention_tree_8bit", &attention_tree_8bit);
   m.impl("cache_append", &cache_append);
   m.impl("cache_append_8bit", &cache_append_8bit);
   m.impl("rotary", &rotary);
@@ -574,6 +636,7 @@ TORCH_LIBRARY_IMPL(nkilab, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(nkilab, Autograd, m) {
   m.impl("attention_tree", &attention_tree_autograd);
+  m.impl("attention_tree_8bit", &attention_tree_8bit_autograd);
   m.impl("rotary", &rotary_autograd);
   m.impl("rotary_append", &rotary_append_autograd);
 }

@@ -26,6 +26,8 @@
 #include <cstddef>
 #include <atomic>
 
+#include <cuda_fp16.h>
+
 #include "attn_math.cuh"
 #include "common.cuh"
 #include "sm100.cuh"
@@ -415,7 +417,8 @@ constexpr int kMaxSplits = 256;
 // Joins the splits of each row: WARPS warps take them in turn (and half warps, with head_dim
 // up to 64, every second one of these), so that a row of many splits is one round of loads; the
 // partial sums are added in a fixed order.
-template <typename T, int WARPS>
+// BASE2: the maxima are logarithms to base 2.
+template <typename T, int WARPS, bool BASE2>
 __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
   constexpr int kRowsHere = 4 / WARPS;
   __shared__ float weight[kRowsHere][kMaxSplits];
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   m = warp_max(m);
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    const float w = x[k].x == -INFINITY ? 0.f : expf(x[k].x - m);
+    const float w = x[k].x == -INFINITY ? 0.f : BASE2 ? exp2f(x[k].x - m) : expf(x[k].x - m);
     if (wi == 0) weight[mine][k * 32 + lane] = w;
     l = fmaf(w, x[k].y, l);
   }
@@ -482,6 +485,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   const int r = (int)(row % rows), kvh = (int)(row / rows % a.kv_heads), b = (int)(row / rows / a.kv_heads);
   const bool present = !a.parents || a.parents[(int64_t)b * a.tokens + r / a.group] >= -1;
   const float inv = present ? 1.f / l : 0.f;
+  if (!present) o = make_float4(0.f, 0.f, 0.f, 0.f);  // whatever the cache holds
   const int64_t at = (((int64_t)b * a.tokens + r / a.group) * a.heads + kvh * a.group + r % a.group) * a.d + c;
   store4(static_cast<T*>(a.out) + at, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
@@ -489,6 +493,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
 }  // namespace
 
 #include "tree_attention_tc.cuh"
+#include "tree_attention_8bit.cuh"
 
 namespace {
 
@@ -524,6 +529,19 @@ int launch_split(const TreeArgs& a, dim3 grid, cudaStream_t st) {
   return launch_pdl(tree_attention_kernel<T, ND>, grid, dim3(kThreads), TreeShared<T>(a.d).bytes, st, op, a);
 }
 
+// Joins the splits. Four warps to a row where many splits meet: 5 sequences of up to 1999 positions 18.2 against
+// 19.3 us, one of 8000 28.5 against 33.4; one where few do: 16 of 700, 33 tokens, 118 against 121 us.
+template <bool BASE2>
+int launch_combine(const TreeArgs& a, int dtype, cudaStream_t st, const char* op) {
+  const int64_t rows = (int64_t)a.batch * a.heads * a.tokens;
+  auto join = [&](auto* kernel, int per_block) {
+    return launch_pdl(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(128), 0, st, op, a);
+  };
+  if (a.splits > 8)
+    return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 4, BASE2>, 1) : join(tree_combine_kernel<bf16, 4, BASE2>, 1);
+  return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 1, BASE2>, 4) : join(tree_combine_kernel<bf16, 1, BASE2>, 4);
+}
+
 size_t split_bytes(int64_t splits, int64_t batch, int64_t heads, int64_t tokens, int64_t d) {
   return splits > 1 ? ((size_t)splits * batch * heads * tokens * (d + 2) * 4 + 255) & ~size_t(255) : 0;
 }
@@ -533,6 +551,53 @@ bool tree_sizes_ok(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_head
   return batch >= 0 && batch <= 65535 && tokens >= 0 && tokens <= kMaxDrafted && heads >= 1 && heads <= 65535 &&
          kv_heads >= 1 && heads % kv_heads == 0 && head_dim >= 8 && head_dim <= kMaxDim && head_dim % 8 == 0 &&
          page_size >= 1 && page_size <= 65536 && max_pages >= 1 && max_pages * page_size <= (1LL << 30);
+}
+
+// What the two entry points check and take over; s and n: strides of q [batch, token, head], the drafted tokens' rows
+// [batch, token, head] and the cache [page, head, row], and the sizes stepped over. `done`: nothing to do.
+int tree_args(const char* op, TreeArgs& a, int64_t (&s)[9], int64_t (&n)[9], bool& done, const void* q,
+              const int64_t* q_strides, const void* k_new, const void* v_new, const int64_t* new_strides,
+              const void* k_cache, const void* v_cache, const int64_t* cache_strides, const int32_t* tables,
+              const int32_t* lens, const int32_t* parents, void* out, int64_t batch, int64_t tokens, int64_t heads,
+              int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages, float scale,
+              int dtype, int64_t cache_per, int64_t unit) {
+  if (!valid_dtype(dtype)) return fail(NKL_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
+  if (tokens > kMaxDrafted)
+    return fail(NKL_ERR_SHAPE, "%s: %lld drafted tokens, at most %d are taken", op, (long long)tokens, kMaxDrafted);
+  if (!tree_sizes_ok(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages) || head_dim % unit || pages < 1 ||
+      pages > 0x7fffffffLL)
+    return fail(NKL_ERR_SHAPE,
+                "%s: batch %lld, tokens %lld, heads %lld / %lld, head_dim %lld, page size %lld or table width %lld not "
+                "supported (kv heads divide heads; head_dim a multiple of %lld up to %d; up to 2^30 positions)",
+                op, (long long)batch, (long long)tokens, (long long)heads, (long long)kv_heads, (long long)head_dim,
+                (long long)page_size, (long long)max_pages, (long long)unit, kMaxDim);
+  done = batch == 0 || tokens == 0;
+  if (done) return NKL_OK;
+  if (!q || !k_new || !v_new || !k_cache || !v_cache || !tables || !lens || !out)
+    return fail(NKL_ERR_ARG, "%s: NULL pointer", op);
+  for (const void* p : {q, k_new, v_new, k_cache, v_cache, static_cast<const void*>(out)})
+    if (!is_aligned(p, 16)) return fail(NKL_ERR_ALIGN, "%s: tensors need 16-byte alignment", op);
+  const int64_t dense[9] = {tokens * heads * head_dim,    heads * head_dim,                 head_dim,
+                            tokens * kv_heads * head_dim, kv_heads * head_dim,              head_dim,
+                            kv_heads * page_size * head_dim, page_size * head_dim, head_dim};
+  const int64_t sizes[9] = {batch, tokens, heads, batch, tokens, kv_heads, pages, kv_heads, page_size};
+  const int64_t* given[3] = {q_strides, new_strides, cache_strides};
+  const int64_t per = 16 / (int64_t)dtype_size(dtype);
+  for (int i = 0; i < 9; ++i) {
+    s[i] = given[i / 3] ? given[i / 3][i % 3] : dense[i];
+    n[i] = sizes[i];
+    if (n[i] > 1 && (s[i] < 0 || s[i] % (i < 6 ? per : cache_per)))
+      return fail(NKL_ERR_ALIGN, "%s: stride %lld is not a multiple of 16 bytes", op, (long long)s[i]);
+  }
+  a.q = q; a.k_new = k_new; a.v_new = v_new; a.k_cache = k_cache; a.v_cache = v_cache;
+  a.tables = tables; a.lens = lens; a.parents = parents; a.out = out;
+  a.q_b = s[0]; a.q_t = s[1]; a.q_h = s[2];
+  a.n_b = s[3]; a.n_t = s[4]; a.n_h = s[5];
+  a.c_p = s[6]; a.c_h = s[7]; a.c_s = s[8];
+  a.batch = (int)batch; a.tokens = (int)tokens; a.heads = (int)heads; a.kv_heads = (int)kv_heads;
+  a.group = (int)(heads / kv_heads); a.d = (int)head_dim; a.pages = (int)pages; a.page = (int)page_size;
+  a.max_pages = (int)max_pages; a.scale = scale;
+  return NKL_OK;
 }
 
 }  // namespace
@@ -569,41 +634,14 @@ extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const
                                   int64_t pages, int64_t page_size, int64_t max_pages, float scale, int dtype,
                                   void* stream) {
   const char* op = "nkl_attention_tree";
-  if (!valid_dtype(dtype)) return fail(NKL_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
-  if (tokens > kMaxDrafted)
-    return fail(NKL_ERR_SHAPE, "%s: %lld drafted tokens, at most %d are taken", op, (long long)tokens, kMaxDrafted);
-  if (!tree_sizes_ok(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages) || pages < 1 ||
-      pages > 0x7fffffffLL)
-    return fail(NKL_ERR_SHAPE,
-                "%s: batch %lld, tokens %lld, heads %lld / %lld, head_dim %lld, page size %lld or table width %lld not "
-                "supported (kv heads divide heads; head_dim a multiple of 8 up to %d; up to 2^30 positions)",
-                op, (long long)batch, (long long)tokens, (long long)heads, (long long)kv_heads, (long long)head_dim,
-                (long long)page_size, (long long)max_pages, kMaxDim);
-  if (batch == 0 || tokens == 0) return NKL_OK;
-  if (!q || !k_new || !v_new || !k_cache || !v_cache || !tables || !lens || !out)
-    return fail(NKL_ERR_ARG, "%s: NULL pointer", op);
-  for (const void* p : {q, k_new, v_new, k_cache, v_cache, static_cast<const void*>(out)})
-    if (!is_aligned(p, 16)) return fail(NKL_ERR_ALIGN, "%s: tensors need 16-byte alignment", op);
   TreeArgs a = {};
-  int64_t s[9] = {tokens * heads * head_dim,    heads * head_dim,                 head_dim,
-                  tokens * kv_heads * head_dim, kv_heads * head_dim,              head_dim,
-                  kv_heads * page_size * head_dim, page_size * head_dim, head_dim};
-  const int64_t n[9] = {batch, tokens, heads, batch, tokens, kv_heads, pages, kv_heads, page_size};
-  const int64_t* given[3] = {q_strides, new_strides, cache_strides};
-  const int64_t per = 16 / (int64_t)dtype_size(dtype);
-  for (int i = 0; i < 9; ++i) {
-    if (given[i / 3]) s[i] = given[i / 3][i % 3];
-    if (n[i] > 1 && (s[i] < 0 || s[i] % per))
-      return fail(NKL_ERR_ALIGN, "%s: stride %lld is not a multiple of 16 bytes", op, (long long)s[i]);
-  }
-  a.q = q; a.k_new = k_new; a.v_new = v_new; a.k_cache = k_cache; a.v_cache = v_cache;
-  a.tables = tables; a.lens = lens; a.parents = parents; a.out = out;
-  a.q_b = s[0]; a.q_t = s[1]; a.q_h = s[2];
-  a.n_b = s[3]; a.n_t = s[4]; a.n_h = s[5];
-  a.c_p = s[6]; a.c_h = s[7]; a.c_s = s[8];
-  a.batch = (int)batch; a.tokens = (int)tokens; a.heads = (int)heads; a.kv_heads = (int)kv_heads;
-  a.group = (int)(heads / kv_heads); a.d = (int)head_dim; a.pages = (int)pages; a.page = (int)page_size;
-  a.max_pages = (int)max_pages; a.scale = scale;
+  int64_t s[9], n[9];
+  bool done = false;
+  if (int rc = tree_args(op, a, s, n, done, q, q_strides, k_new, v_new, new_strides, k_cache, v_cache, cache_strides, tables,
+                         lens, parents, out, batch, tokens, heads, kv_heads, head_dim, pages, page_size, max_pages, scale,
+                         dtype, 16 / (int64_t)dtype_size(dtype), 8))
+    return rc;
+  if (done) return NKL_OK;
   const TcPlan p = tc_plan(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages, dtype);
   bool tc = p.on && scale > 0.f && scale < INFINITY;  // the running maximum is one of scaled scores
   for (int i = 0; i < 9; ++i) tc = tc && (n[i] == 1 || (s[i] > 0 && s[i] < (1LL << 38)));  // tensor map strides
@@ -638,13 +676,61 @@ extern "C" int nkl_attention_tree(const void* q, const int64_t* q_strides, const
   else
     rc = head_dim <= 64 ? launch_split<bf16, 8>(a, grid, st) : launch_split<bf16, 16>(a, grid, st);
   if (rc || a.splits == 1) return rc;
-  const int64_t rows = batch * heads * tokens;
-  auto join = [&](auto* kernel, int per_block) {
-    return launch_pdl(kernel, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(128), 0, st, op, a);
-  };
-  // Four warps to a row where many splits meet: 5 sequences of up to 1999 positions 18.2 against 19.3 us,
-  // one of 8000 28.5 against 33.4; one where few do: 16 of 700, 33 tokens, 118 against 121 us.
-  if (a.splits > 8)
-    return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 4>, 1) : join(tree_combine_kernel<bf16, 4>, 1);
-  return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 1>, 4) : join(tree_combine_kernel<bf16, 1>, 4);
+  return launch_combine<false>(a, dtype, st, op);
+}
+
+extern "C" size_t nkl_attention_tree_8bit_workspace_size(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                         int64_t head_dim, int64_t page_size, int64_t max_pages,
+                                                         int dtype) {
+  if (!valid_dtype(dtype) || !tree_sizes_ok(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages) ||
+      batch == 0 || tokens == 0)
+    return 0;
+  return split_bytes(splits_8bit(batch, kv_heads, tokens * (heads / kv_heads), page_size * max_pages), batch, heads, tokens,
+                     head_dim);
+}
+
+extern "C" int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
+                                       const int64_t* new_strides, const void* k_cache, const void* v_cache,
+                                       const int64_t* cache_strides, const void* k_scales, const void* v_scales,
+                                       const int32_t* tables, const int32_t* lens, const int32_t* parents, void* out,
+                                       void* workspace, size_t workspace_bytes, int64_t batch, int64_t tokens,
+                                       int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                                       int64_t page_size, int64_t max_pages, int64_t block, float scale, int dtype,
+                                       void* stream) {
+  const char* op = "nkl_attention_tree_8bit";
+  Bits8Args a = {};
+  int64_t s[9], n[9];
+  bool done = false;
+  if (int rc = tree_args(op, a.t, s, n, done, q, q_strides, k_new, v_new, new_strides, k_cache, v_cache, cache_strides, tables,
+                         lens, parents, out, batch, tokens, heads, kv_heads, head_dim, pages, page_size, max_pages, scale,
+                         dtype, 16, 16))
+    return rc;
+  if (done) return NKL_OK;
+  if (block < 1 || page_size % block)
+    return fail(NKL_ERR_SHAPE, "%s: blocks of %lld positions do not divide pages of %lld", op, (long long)block, (long long)page_size);
+  if (!k_scales || !v_scales) return fail(NKL_ERR_ARG, "%s: NULL pointer", op);
+  a.k_scales = static_cast<const uint8_t*>(k_scales);
+  a.v_scales = static_cast<const uint8_t*>(v_scales);
+  a.block = (int)block;
+  a.per_page = (int)(page_size / block);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t rows = tokens * a.t.group;
+  a.tiles = tiles_8bit(rows);
+  a.t.row_blocks = (int)((rows + 16 * a.tiles - 1) / (16 * a.tiles));
+  a.t.splits = (int)splits_8bit(batch, kv_heads, rows, page_size * max_pages);
+  if (const size_t need = split_bytes(a.t.splits, batch, heads, tokens, head_dim)) {
+    if (!workspace || workspace_bytes < need) return fail(NKL_ERR_ARG, "%s: workspace too small", op);
+    if (!is_aligned(workspace, 256)) return fail(NKL_ERR_ALIGN, "%s: workspace not 256-byte aligned", op);
+    a.t.ws_o = static_cast<float*>(workspace);
+    a.t.ws_ml = a.t.ws_o + (size_t)a.t.splits * batch * heads * tokens * head_dim;
+  }
+  const dim3 grid((unsigned)(a.t.splits * a.t.row_blocks), (unsigned)kv_heads, (unsigned)batch);
+  const bool fast = page_size % 16 == 0 && block % 16 == 0;
+  int rc;
+  if (dtype == NKL_FLOAT32)
+    rc = head_dim <= 64 ? launch_8bit<float, 1>(a, grid, fast, st) : launch_8bit<float, 2>(a, grid, fast, st);
+  else
+    rc = head_dim <= 64 ? launch_8bit<bf16, 1>(a, grid, fast, st) : launch_8bit<bf16, 2>(a, grid, fast, st);
+  if (rc || a.t.splits == 1) return rc;
+  return launch_combine<true>(a.t, dtype, st, op);
 }

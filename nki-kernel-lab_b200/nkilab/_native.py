@@ -80,6 +80,9 @@ SIGNATURES = {
     "nkl_rotary": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _f, _int, _p]),
     "nkl_rotary_append": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
                                  _i64, _i64, _i64, _i64, _i64, _int, _f, _int, _p]),
+    "nkl_attention_tree_8bit_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "nkl_attention_tree_8bit": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64,
+                                       _i64, _i64, _i64, _i64, _i64, _f, _int, _p]),
     "nkl_cache_append_8bit": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
                                      _i64, _i64, _i64, _int, _p]),
     "nkl_cache_reserve_workspace_size": (_sz, [_i64]),

@@ -11,6 +11,7 @@ compose with streams and CUDA-graph capture like any torch op:
     torch.ops.nkilab.matmul_f32out(a, b)            -> nkl_matmul_f32out (bf16 in, fp32 out)
     torch.ops.nkilab.attention(q, k, v, scale, naive) -> nkl_attention_ws / nkl_attention_naive
     torch.ops.nkilab.attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents, scale) -> nkl_attention_tree
+    torch.ops.nkilab.attention_tree_8bit(q, k, v, k_cache, v_cache, k_scales, v_scales, ...) -> nkl_attention_tree_8bit
     torch.ops.nkilab.rotary(x, positions, freqs, parents, interleaved, magnitude, inverse) -> nkl_rotary
     torch.ops.nkilab.rotary_append(q, k, v, k_cache, v_cache, ...) -> nkl_rotary_append
     torch.ops.nkilab.cache_append_8bit(k, v, k_cache, v_cache, ...) -> nkl_cache_append_8bit
@@ -366,6 +367,8 @@ def _like(*ts):
 
 torch.library.register_fake("nkilab::attention_tree",
                             lambda q, k, v, k_cache, v_cache, tables, lens, parents, scale: q.new_empty(q.shape))
+torch.library.register_fake("nkilab::attention_tree_8bit", lambda q, k, v, k_cache, v_cache, k_scales, v_scales, tables, lens,
+                            parents, scale: q.new_empty(q.shape))
 torch.library.register_fake("nkilab::cache_append",
                             lambda k, v, k_cache, v_cache, tables, lens, path, count: _like(lens))
 torch.library.register_fake("nkilab::cache_append_8bit", lambda k, v, k_cache, v_cache, k_scales, v_scales, tables, lens,

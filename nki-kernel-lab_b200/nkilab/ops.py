@@ -178,10 +178,11 @@ def _decode(name: str):
 _attention_tree, _cache_append, _cache_reserve, _cache_fork, _cache_free, _cache_compact, _verify_drafts = map(
     _decode, ("attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
               "verify_drafts"))
-_cache_append_8bit, _rotary, _rotary_append = map(_decode, ("cache_append_8bit", "rotary", "rotary_append"))
+_attention_tree_8bit, _cache_append_8bit, _rotary, _rotary_append = map(
+    _decode, ("attention_tree_8bit", "cache_append_8bit", "rotary", "rotary_append"))
 
 
-def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=None):
+def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=None, k_scales=None, v_scales=None):
     """Attention of T drafted tokens per sequence over its cached positions and, as a tree,
     over each other. q: [B, T, H, d]; k, v: [B, T, Hkv, d], the drafted tokens' own, not yet
     in the cache (views of a fused projection are read as they lie); returns [B, T, H, d].
@@ -192,9 +193,16 @@ def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=
     prompt. At most 128 tokens; scale defaults to 1/sqrt(d). d: a multiple of 8 up to 128
     (64 and 128 in bf16, with pages of a multiple of 8 positions, run on tcgen05). There is
     no backward pass: one through it raises.
+
+    With k_scales and v_scales the caches are in 8 bits, as cache_append writes them (d a multiple
+    of 16); q, k and v are bf16 or fp32 all the same.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
+    if k_scales is not None or v_scales is not None:
+        if k_scales is None or v_scales is None:
+            raise ValueError("scales: need both or none")
+        return _attention_tree_8bit(q, k, v, k_cache, v_cache, k_scales, v_scales, tables, lens, parents, float(scale))
     return _attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents, float(scale))
 
 

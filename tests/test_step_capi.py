@@ -143,3 +143,31 @@ def test_wrappers_take_no_cpu_tensors():
         ops.rotary(x, i, f)
     with pytest.raises(NotImplementedError):
         ops.rotary_append(x, x, x, x, x, i[None], i, f)
+
+
+def test_attention_8bit_refusals(N):
+    def call(**kw):
+        a = dict(q=FAKE, qs=None, k=FAKE, v=FAKE, ns=None, kc=FAKE, vc=FAKE, cs=None, ks=FAKE, vs=FAKE, tables=FAKE, lens=FAKE,
+                 parents=None, out=FAKE, ws=None, wsb=0, B=2, T=4, H=8, Hkv=2, d=64, P=10, page=16, M=4, block=8, scale=0.1,
+                 dt=N.BFLOAT16)
+        assert not set(kw) - set(a)
+        a.update(kw)
+        return N.lib.nkl_attention_tree_8bit(*a.values(), None)
+
+    assert call(dt=5) == N.ERR_DTYPE
+    for kw in (dict(T=129), dict(Hkv=3), dict(Hkv=0), dict(d=72), dict(d=144), dict(page=0), dict(M=0), dict(P=0), dict(B=-1),
+               dict(block=0), dict(block=3), dict(block=32), dict(page=65536, M=1 << 20)):
+        assert call(**kw) == N.ERR_SHAPE
+    for name in ("q", "k", "v", "kc", "vc", "ks", "vs", "tables", "lens", "out"):
+        assert call(**{name: None}) == N.ERR_ARG
+    for name in ("q", "k", "v", "kc", "vc", "out"):
+        assert call(**{name: ODD}) == N.ERR_ALIGN
+    assert call(qs=strides(512, 130, 64)) == N.ERR_ALIGN
+    assert call(cs=strides(2048, 1024, 72)) == N.ERR_ALIGN
+    need = N.lib.nkl_attention_tree_8bit_workspace_size(2, 4, 8, 2, 64, 16, 4000, N.FLOAT32)
+    assert need > 0
+    assert call(M=4000, dt=N.FLOAT32) == N.ERR_ARG and b"workspace" in N.lib.nkl_last_error()
+    assert call(M=4000, dt=N.FLOAT32, ws=FAKE, wsb=need - 1) == N.ERR_ARG
+    assert call(M=4000, dt=N.FLOAT32, ws=ctypes.c_void_p(4096 + 16), wsb=need) == N.ERR_ALIGN
+    assert call(B=0, q=None) == N.OK
+    assert call(T=0, q=None) == N.OK
