@@ -489,6 +489,22 @@ int nkl_verify_drafts(const void* probs, const void* draft_probs, const int32_t*
                       const int32_t* parents, int32_t* path, int32_t* count, int32_t* token, int64_t batch,
                       int64_t drafted, int64_t vocab, int dtype, void* stream);
 
+/* The next token of each row of logits [batch, vocab] (rows row_stride elements apart), from the uniform
+ * numbers [batch] in [0, 1). With weights w = floor(2^31 exp((x - max) / T)), in order of the logits
+ * (of equal ones the lowest index first), what is drawn from is the longest beginning of that order that
+ * has no more than top_k tokens, no more than it takes for the share top_p of the first top_k's
+ * weights, and only weights of at least min_p 2^31; its first token is always in it. token [batch]: the
+ * first, by index, with which the cumulative weight is over the uniform number's share of the sum; prob
+ * [batch]: its weight over the sum. T of 0, below or NaN: the order's first token. top_k of 0 or below, top_p
+ * of 1 and over, min_p of 0 and below: off, as is NaN. Minus infinity and NaN are never drawn; a row of nothing else
+ * gives token -1, prob 0. temperatures, top_ks, top_ps, min_ps: one value for each row (device), or NULL:
+ * the number given. Shares and uniform numbers are whole multiples of 2^-31, sums whole numbers. */
+#define NKL_MAX_VOCAB 393216
+int nkl_sample(const void* logits, int64_t row_stride, const float* uniforms, const float* temperatures,
+               const int32_t* top_ks, const float* top_ps, const float* min_ps, float temperature, int top_k,
+               float top_p, float min_p, int32_t* token, float* prob, int64_t batch, int64_t vocab, int dtype,
+               void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -486,6 +486,35 @@ std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& probs_in, const T
   return {path, count, token};
 }
 
+std::tuple<Tensor, Tensor> sample(const Tensor& logits_in, const Tensor& uniforms, OptTensor temperatures,
+                                  OptTensor top_ks, OptTensor top_ps, OptTensor min_ps, double temperature,
+                                  int64_t top_k, double top_p, double min_p) {
+  const int dt = dtype_code(logits_in);
+  TORCH_CHECK_VALUE(logits_in.dim() == 2 && logits_in.size(1) >= 1, "logits ", logits_in.sizes(), ": need [B, vocabulary]");
+  const c10::Device dev = logits_in.device();
+  const int64_t B = logits_in.size(0), V = logits_in.size(1);
+  auto floats = [&](const char* name, const Tensor& t) {
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, name, " must be float32, got ", t.scalar_type());
+    TORCH_CHECK(t.device() == dev, name, " is on ", t.device(), ", not on ", dev);
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == B, name, " has shape ", t.sizes(), ", expected [", B, "]");
+    TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+    return static_cast<const float*>(t.data_ptr());
+  };
+  auto each = [&](const char* name, OptTensor t) { return t.has_value() ? floats(name, *t) : nullptr; };
+  const float* u = floats("uniforms", uniforms);
+  const float *ts = each("temperature", temperatures), *ps = each("top_p", top_ps), *ms = each("min_p", min_ps);
+  const int32_t* ks = ints("top_k", top_ks, dev, {B});
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor logits = logits_in.stride(1) == 1 || V == 1 ? logits_in : logits_in.contiguous();
+  Tensor token = new_ints({B}, dev), prob = new_tensor({B}, at::kFloat, dev);
+  check("nkl_sample",
+        nkl_sample(logits.data_ptr(), logits.stride(0), u, ts, ks, ps, ms, (float)temperature,
+                   (int)std::max<int64_t>(std::min<int64_t>(top_k, INT32_MAX), 0), (float)top_p, (float)min_p,
+                   out_ints(token), static_cast<float*>(prob.data_ptr()), B, V, dt,
+                   c10::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return {token, prob};
+}
+
 // The attention has no backward pass: with inputs that require a gradient, one through it raises.
 Tensor no_backward(Tensor out, const char* name, std::initializer_list<Tensor> inputs) {
   const std::vector<Tensor> in(inputs);
@@ -527,6 +556,20 @@ Tensor attention_tree_8bit_autograd(const Tensor& q, const Tensor& k, const Tens
   }
   if (!torch::autograd::compute_requires_grad(q, k, v)) return out;
   return no_backward(out, "nkilab::attention_tree_8bit", {q, k, v});
+}
+
+std::tuple<Tensor, Tensor> sample_autograd(const Tensor& logits, const Tensor& uniforms, OptTensor temperatures,
+                                           OptTensor top_ks, OptTensor top_ps, OptTensor min_ps, double temperature,
+                                           int64_t top_k, double top_p, double min_p) {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("nkilab::sample", "").typed<decltype(sample)>();
+  std::tuple<Tensor, Tensor> out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(logits, uniforms, temperatures, top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p);
+  }
+  if (torch::autograd::compute_requires_grad(logits)) no_backward(std::get<1>(out), "nkilab::sample", {logits});
+  return out;
 }
 
 // The gradient of a turn by an angle is the turn by the opposite one, so a pass back through it
@@ -616,6 +659,8 @@ TORCH_LIBRARY_FRAGMENT(nkilab, m) {
         "Tensor dst) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("cache_free(Tensor tables, Tensor lens, Tensor refs, Tensor slots) -> (Tensor, Tensor, Tensor)");
   m.def("cache_compact(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor refs) -> (Tensor, Tensor)");
+  m.def("sample(Tensor logits, Tensor uniforms, Tensor? temperatures, Tensor? top_ks, Tensor? top_ps, Tensor? min_ps, "
+        "float temperature, int top_k, float top_p, float min_p) -> (Tensor, Tensor)");
   m.def("verify_drafts(Tensor probs, Tensor tokens, Tensor uniforms, Tensor? parents, Tensor? draft_probs) "
         "-> (Tensor, Tensor, Tensor)");
 }
@@ -632,6 +677,7 @@ TORCH_LIBRARY_IMPL(nkilab, CUDA, m) {
   m.impl("cache_free", &cache_free);
   m.impl("cache_compact", &cache_compact);
   m.impl("verify_drafts", &verify_drafts);
+  m.impl("sample", &sample);
 }
 
 TORCH_LIBRARY_IMPL(nkilab, Autograd, m) {
@@ -639,4 +685,5 @@ TORCH_LIBRARY_IMPL(nkilab, Autograd, m) {
   m.impl("attention_tree_8bit", &attention_tree_8bit_autograd);
   m.impl("rotary", &rotary_autograd);
   m.impl("rotary_append", &rotary_append_autograd);
+  m.impl("sample", &sample_autograd);
 }

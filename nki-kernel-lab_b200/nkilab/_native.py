@@ -94,12 +94,14 @@ SIGNATURES = {
     "nkl_cache_compact_workspace_size": (_sz, [_i64]),
     "nkl_cache_compact": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p]),
     "nkl_verify_drafts": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
+    "nkl_sample": (_int, [_p, _i64, _p, _p, _p, _p, _p, _f, _int, _f, _f, _p, _p, _i64, _i64, _int, _p]),
     "nkl_attention_naive_workspace_size": (_sz, [_i64, _i64, _int]),
     "nkl_attention_naive": (_int, [_p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _f, _int, _p]),
 }
 
 ABI_VERSION = 1
 MAX_DRAFTED = 128  # NKL_MAX_DRAFTED
+MAX_VOCAB = 393216  # NKL_MAX_VOCAB
 SOFTMAX_UNFUSED_STATIC_BYTES = 16 * 1024 * 1024  # NKL_SOFTMAX_UNFUSED_STATIC_BYTES
 
 

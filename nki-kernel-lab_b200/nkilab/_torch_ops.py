@@ -17,6 +17,7 @@ compose with streams and CUDA-graph capture like any torch op:
     torch.ops.nkilab.cache_append_8bit(k, v, k_cache, v_cache, ...) -> nkl_cache_append_8bit
     torch.ops.nkilab.cache_{append,reserve,fork,free,compact}  -> nkl_cache_*
     torch.ops.nkilab.verify_drafts(probs, tokens, uniforms, parents, draft_probs) -> nkl_verify_drafts
+    torch.ops.nkilab.sample(logits, uniforms, temperatures, top_ks, top_ps, min_ps, ...) -> nkl_sample
 
 There is no CPU implementation: a CPU tensor is an error, never a fallback.
 """
@@ -385,3 +386,5 @@ torch.library.register_fake("nkilab::cache_free", lambda tables, lens, refs, slo
 torch.library.register_fake("nkilab::cache_compact", lambda k_cache, v_cache, tables, refs: _like(tables, refs))
 torch.library.register_fake("nkilab::verify_drafts", lambda probs, tokens, uniforms, parents, draft_probs:
                             (_like(tokens), tokens.new_empty(tokens.shape[0]), tokens.new_empty(tokens.shape[0])))
+torch.library.register_fake("nkilab::sample", lambda logits, uniforms, *_:
+                            (uniforms.new_empty(uniforms.shape, dtype=torch.int32), uniforms.new_empty(uniforms.shape)))

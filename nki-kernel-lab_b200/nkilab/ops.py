@@ -27,7 +27,7 @@ from .kernels import attention as _attn
 
 __all__ = ["choose_blocks", "matmul", "softmax", "rmsnorm", "swiglu", "attention", "ATTENTION_VARIANTS",
            "rope", "attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
-           "verify_drafts", "rotary_frequencies", "rotary", "rotary_append"]
+           "verify_drafts", "rotary_frequencies", "rotary", "rotary_append", "sample"]
 
 
 # --------------------------------------------------------------------------- matmul
@@ -178,8 +178,8 @@ def _decode(name: str):
 _attention_tree, _cache_append, _cache_reserve, _cache_fork, _cache_free, _cache_compact, _verify_drafts = map(
     _decode, ("attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
               "verify_drafts"))
-_attention_tree_8bit, _cache_append_8bit, _rotary, _rotary_append = map(
-    _decode, ("attention_tree_8bit", "cache_append_8bit", "rotary", "rotary_append"))
+_attention_tree_8bit, _cache_append_8bit, _rotary, _rotary_append, _sample = map(
+    _decode, ("attention_tree_8bit", "cache_append_8bit", "rotary", "rotary_append", "sample"))
 
 
 def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=None, k_scales=None, v_scales=None):
@@ -329,3 +329,25 @@ def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):
     Sums are whole numbers of 2^-31, so equal inputs give equal tokens on every launch.
     """
     return _verify_drafts(probs, tokens, uniforms, parents, draft_probs)
+
+
+def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The next token of each row of logits [B, V] from the uniform numbers [B] (float32 in [0, 1)).
+
+    Weights are exp((x - max) / temperature); tokens in order of their logits, of equal ones the
+    lowest index first, are kept while they are among the first top_k, needed for the share top_p of
+    the top_k's weights, and weigh at least min_p of the first one; the first one always is. temperature
+    0 takes the first one; top_k 0, top_p 1 and min_p 0 keep all. Each is a number, or one for each row: a
+    tensor [B] on the GPU (top_k int32, the others float32), where NaN is off. Minus infinity and NaN are never
+    drawn. Returns (token [B] int32, -1 if there is none; prob [B] float32, its share of what was kept).
+    Weights are whole multiples of 2^-31, so equal inputs give equal tokens on every launch. V up to 393216.
+    """
+    numbers, rows = [], []
+    for name, x, low, high in (("temperature", temperature, 0, math.inf), ("top_k", top_k, 0, 2 ** 31), ("top_p", top_p, 0, 1),
+                               ("min_p", min_p, 0, 1)):
+        each = isinstance(x, torch.Tensor)
+        if not each and not low <= x <= high:
+            raise ValueError(f"{name} {x}: must be between {low} and {high}")
+        rows.append(x if each else None)
+        numbers.append(0 if each else x)
+    return _sample(logits, uniforms, *rows, float(numbers[0]), int(numbers[1]), float(numbers[2]), float(numbers[3]))

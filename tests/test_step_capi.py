@@ -171,3 +171,34 @@ def test_attention_8bit_refusals(N):
     assert call(M=4000, dt=N.FLOAT32, ws=ctypes.c_void_p(4096 + 16), wsb=need) == N.ERR_ALIGN
     assert call(B=0, q=None) == N.OK
     assert call(T=0, q=None) == N.OK
+
+
+def test_sample_refusals(N):
+    def call(**kw):
+        a = dict(x=FAKE, stride=100, u=FAKE, ts=None, ks=None, ps=None, ms=None, t=1.0, k=0, p=1.0, m=0.0, token=FAKE, prob=FAKE,
+                 B=2, V=100, dt=N.FLOAT32)
+        assert not set(kw) - set(a)
+        a.update(kw)
+        return N.lib.nkl_sample(*a.values(), None)
+
+    assert call(dt=3) == N.ERR_DTYPE
+    for kw in (dict(V=0), dict(V=N.MAX_VOCAB + 1), dict(B=-1), dict(stride=-1)):
+        assert call(**kw) == N.ERR_SHAPE
+    for name in ("x", "u", "token", "prob"):
+        assert call(**{name: None}) == N.ERR_ARG
+    assert call(x=ctypes.c_void_p(4098)) == N.ERR_ALIGN
+    assert call(B=0, x=None) == N.OK
+
+
+def test_sample_numbers_out_of_range():
+    import torch
+
+    from nkilab import ops
+
+    x, u = torch.empty(2, 10, device="meta"), torch.empty(2, device="meta")
+    assert [tuple(t.shape) for t in ops.sample(x, u, 0.5, 3, 0.9, 0.1)] == [(2,), (2,)]
+    for kw in (dict(temperature=-1.0), dict(temperature=math.nan), dict(top_k=-1), dict(top_p=1.1), dict(top_p=-0.1), dict(min_p=2.0)):
+        with pytest.raises(ValueError):
+            ops.sample(x, u, **kw)
+    with pytest.raises(NotImplementedError):
+        ops.sample(torch.zeros(2, 10), torch.zeros(2))
