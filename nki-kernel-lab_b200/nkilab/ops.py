@@ -296,13 +296,38 @@ def cache_reserve(tables, lens, refs, extra, page_size):
     return _cache_reserve(tables, lens, refs, extra, int(page_size))
 
 
-def cache_fork(k_cache, v_cache, tables, lens, refs, src, dst):
+def _as_bf16(*caches):
+    """Caches in 8 bits as pairs of bytes: what moves whole rows does not look into them."""
+    return tuple(c.view(torch.bfloat16) if c.dtype == torch.float8_e4m3fn else c for c in caches)
+
+
+def cache_fork(k_cache, v_cache, tables, lens, refs, src, dst, k_scales=None, v_scales=None):
     """Slot dst[f] becomes a copy of slot src[f]: full pages are shared, the last, partly
     filled one is copied to a free page. Returns (tables, lens, refs, missing); with
-    missing [1] > 0 (too few free pages) nothing is forked."""
+    missing [1] > 0 (too few free pages) nothing is forked. The scales of a cache in 8 bits go along."""
     if k_cache.dim() == 4:  # one layer
         k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-    return _cache_fork(k_cache, v_cache, tables, lens, refs, src, dst)
+        k_scales, v_scales = (t if t is None else t.unsqueeze(0) for t in (k_scales, v_scales))
+    out = _cache_fork(*_as_bf16(k_cache, v_cache), tables, lens, refs, src, dst)
+    if k_scales is not None:
+        # the copied page of each fork that was made, by the operator's rules; the others' turn is a live
+        # page that is written onto itself (a copied one was free)
+        B, M = tables.shape
+        s, t, each = src.long(), dst.long(), torch.arange(src.numel(), device=src.device)
+        good = (s >= 0) & (s < B) & (t >= 0) & (t < B) & (s != t)
+        again = ((t[:, None] == t) & good & (each < each[:, None])).any(1)
+        s, t = s.clamp(0, B - 1), t.clamp(0, B - 1)
+        page = k_cache.shape[3]
+        n = lens[s].clamp(0, M * page)
+        col = (n // page).clamp(max=M - 1).long()
+        come, go = tables[s, col].long(), out[0][t, col].long()
+        made = good & ~again & (n % page > 0) & (out[3] == 0) & (come >= 0) & (come < refs.numel()) & (go >= 0)
+        live = (refs > 0).int().argmax()
+        come, go = torch.where(made, come, live), torch.where(made, go, live)
+        for x in (k_scales, v_scales):
+            b = x.view(torch.uint8)
+            b[:, go] = b[:, come]
+    return out
 
 
 def cache_free(tables, lens, refs, slots):
@@ -310,11 +335,22 @@ def cache_free(tables, lens, refs, slots):
     return _cache_free(tables, lens, refs, slots)
 
 
-def cache_compact(k_cache, v_cache, tables, refs):
-    """Moves the pages in use to the lowest indices. Returns (tables, refs)."""
+def cache_compact(k_cache, v_cache, tables, refs, k_scales=None, v_scales=None):
+    """Moves the pages in use to the lowest indices. Returns (tables, refs). The scales of a cache in 8
+    bits go along."""
     if k_cache.dim() == 4:  # one layer
         k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-    return _cache_compact(k_cache, v_cache, tables, refs)
+        k_scales, v_scales = (t if t is None else t.unsqueeze(0) for t in (k_scales, v_scales))
+    out = _cache_compact(*_as_bf16(k_cache, v_cache), tables, refs)
+    if k_scales is not None:
+        P = refs.numel()
+        there = (tables >= 0) & (tables < P) & (out[0] >= 0)
+        come = torch.arange(P + 1, device=refs.device)  # where each page's contents were
+        come.scatter_(0, torch.where(there, out[0], P).flatten().long(), torch.where(there, tables, P).flatten().long())
+        for x in (k_scales, v_scales):
+            b = x.view(torch.uint8)
+            b.copy_(b[:, come[:P].clamp(max=P - 1)])
+    return out
 
 
 def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):
