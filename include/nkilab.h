@@ -499,7 +499,7 @@ int nkl_verify_drafts(const void* probs, const void* draft_probs, const int32_t*
  * of 1 and over, min_p of 0 and below: off, as is NaN. Minus infinity and NaN are never drawn; a row of nothing else
  * gives token -1, prob 0. temperatures, top_ks, top_ps, min_ps: one value for each row (device), or NULL:
  * the number given. Shares and uniform numbers are whole multiples of 2^-31, sums whole numbers. */
-#define NKL_MAX_VOCAB 393216
+#define NKL_MAX_VOCAB 360448
 int nkl_sample(const void* logits, int64_t row_stride, const float* uniforms, const float* temperatures,
                const int32_t* top_ks, const float* top_ps, const float* min_ps, float temperature, int top_k,
                float top_p, float min_p, int32_t* token, float* prob, int64_t batch, int64_t vocab, int dtype,

@@ -11,12 +11,13 @@
 // inputs give equal tokens on every launch. NaN counts as minus infinity, and minus infinity is never
 // drawn; T of 0 (or below, or NaN) takes the first token.
 //
-// A cluster of up to eight blocks takes a row; each holds its part in shared memory as keys whose order
-// is the logits'. The order's end is found without sorting: a histogram of weights and counts
-// over 1024 ranges of the logit (by distance from the maximum, which spreads them out), in it the
-// range where the first filter ends the order; then, among that range's keys, over 1024 ranges of the
-// key, until a range is one key; of equal ones the lowest indices stay. Blocks add their
-// histograms up through distributed shared memory, an eighth of the ranges each.
+// A cluster of up to eight blocks takes a row; each holds its part in shared memory, first as logits,
+// then as weights, which are computed once, in 64 bits (in 32 they would shift a border between two
+// tokens of a long row now and then). The order's end is found without sorting: a histogram of
+// weights and counts over 1024 ranges of the weight, a thirty-second of it wide, tells the range where it
+// is; the weights of that range over 512 parts of it, and so on, until a part is one weight or one
+// token. Of tokens with the weight at the end as many stay as it takes, by logit and then by index.
+// Blocks add their histograms up through distributed shared memory.
 #include <algorithm>
 #include <atomic>
 
@@ -30,10 +31,12 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kBins = 1024;
-constexpr int kPerBlock = 49152;  // keys that a block holds: 192 KB
+constexpr int kBins = 1024;       // of the first round: 992 are used
+constexpr int kParts = 512;       // of a range, in the rounds after it
+constexpr int kStep = 128;        // tokens that a warp looks at at once, four to a lane
+constexpr int kPerBlock = 45056;  // tokens that a block holds: 176 KB
 constexpr u64 kOne = 1ull << 31;
-constexpr uint32_t kNever = 0u;   // the key of minus infinity and NaN: below all others
+constexpr u64 kNone = ~0ull;
 
 struct SampleArgs {
   const void* logits;
@@ -44,30 +47,13 @@ struct SampleArgs {
   int top_k;
   int* token;
   float* prob;
-  int batch, vocab, part;  // part: keys of a block
+  int batch, vocab, part;  // part: tokens of a block, whole steps of its warps
 };
 
-// Keys in the order of the numbers; -0 counts as 0.
+// Keys in the order of the numbers; -0 counts as 0. NaN and minus infinity do not come here.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (!(x > -INFINITY)) return kNever;
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
-
-// exp(z) for z <= 0, to some 2^-52 of it, times 2^31 and rounded down: exp(z) = 2^n 2^(j / 64) e^r, n and j
-// whole, |r| <= ln 2 / 128, with e^r by its series.
-__device__ __forceinline__ uint32_t weight_of(double z, const double* table) {
-  if (!(z > -22.0)) return 0u;  // below 2^-31
-  const double t = z * 92.332482616893656877;  // 64 / ln 2
-  const double k = rint(t);
-  const int i = (int)k;
-  const double r = fma(k, -0.010830424696249145, z);  // ln 2 / 64
-  const double e = fma(fma(fma(fma(fma(r, 1.0 / 120, 1.0 / 24), r, 1.0 / 6), r, 0.5), r, 1.0), r, 1.0);
-  const double power = __hiloint2double(((i >> 6) + 31 + 1023) << 20, 0);  // 2^(n + 31)
-  return __double2uint_rd(e * table[i & 63] * power);
 }
 
 __device__ __forceinline__ uint32_t whole_share(float x) {  // of [0, 1], in multiples of 2^-31
@@ -77,6 +63,19 @@ __device__ __forceinline__ u64 share_of(u64 total, u64 share) {
   return (total >> 31) * share + (((total & (kOne - 1)) * share) >> 31);
 }
 
+// The first round's range of a weight w > 0: by the upper 5 bits behind the leading one; 0 is the highest.
+constexpr uint32_t kTopBits = 158u << 23;  // 2^31 as a float
+__device__ __forceinline__ int range_of(uint32_t w) { return (int)((kTopBits - __float_as_uint(__uint2float_rz(w))) >> 18); }
+// Its least and largest weight.
+__device__ __forceinline__ uint32_t least_of(int range) {
+  const float f = __uint_as_float(max(kTopBits - ((uint32_t)(range + 1) << 18) + 1u, 1u));
+  return max((uint32_t)ceilf(f), 1u);
+}
+__device__ __forceinline__ uint32_t most_of(int range) {
+  const float f = __uint_as_float(kTopBits - ((uint32_t)range << 18) + 1u);  // the next float
+  return min((uint32_t)ceilf(f) - 1u, (uint32_t)kOne);
+}
+
 __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
   uint32_t at;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
@@ -84,6 +83,15 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
 }
 __device__ __forceinline__ void put(u64* p, uint32_t rank, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void put(uint32_t* p, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void add_remote(u64* p, uint32_t rank, u64 v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
+}
+__device__ __forceinline__ void add_remote(uint32_t* p, uint32_t rank, uint32_t v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(remote(p, rank)), "r"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t get(const uint32_t* p, uint32_t rank) {
   uint32_t v;
@@ -97,23 +105,25 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
   return v;
 }
 
-struct Histogram {  // a range's weights as two halves of 16 and 15 bits, which do not overflow for 2^16 keys
-  uint32_t lo[kBins], hi[kBins], count[kBins];
+template <int N>
+struct Sums {  // over the cluster: weights and counts of the ranges
+  u64 w[N];
+  uint32_t c[N];
 };
 struct Shared {
-  Histogram h;
-  double table[64];
-  u64 all[2][kMaxCluster][2];                // what each block has to tell the others, in turn
-  u64 bins[kMaxCluster][kBins / kMaxCluster][2];  // sums over the blocks: weights and counts of each range
-  u64 scan[kWarps][2];
-  uint32_t reduce[kWarps];
-  int bin, token;
-  u64 before[2];
+  uint32_t lo[kBins], hi[kBins], count[kBins];  // the block's: weights in halves of 16 bits, which 2^16 tokens do not overflow
+  Sums<kBins> first;
+  Sums<kParts> next[2];  // in turn; all zero when they are added to
+  double table[64];      // 2^(j / 64)
+  u64 all[2][kMaxCluster][3];  // what each block has to tell the others, in turn
+  u64 scan[kWarps][3];
+  int bin;
+  u64 before[2], in[2];
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
-  extern __shared__ __align__(16) uint32_t keys[];
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
+  extern __shared__ __align__(16) uint32_t weights[];  // the part's: logits at first
   __shared__ Shared s;
   cluster_started();
   pdl_enter();
@@ -125,309 +135,416 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   const T* const row = static_cast<const T*>(a.logits) + b * a.stride + x0;
   const float temperature = a.temperatures ? a.temperatures[b] : a.temperature;
   const float top_p = a.top_ps ? a.top_ps[b] : a.top_p, min_p = a.min_ps ? a.min_ps[b] : a.min_p;
-  const int asked = a.top_ks ? a.top_ks[b] : a.top_k;
+  const int top_k = a.top_ks ? a.top_ks[b] : a.top_k;
+  // this warp's tokens: [lo, hi) of the block's, whole steps; behind n there is nothing to draw
+  const int per = a.part / kWarps, lo = warp * per, hi = min(lo + per, (n + kStep - 1) / kStep * kStep);
   if (tid < 64) s.table[tid] = exp2((double)tid / 64);
+  for (int i = tid; i < kBins; i += kThreads) s.lo[i] = s.hi[i] = s.count[i] = 0u;
+  for (int i = tid; i < 2 * kParts; i += kThreads) {
+    s.next[i / kParts].w[i % kParts] = 0ull;
+    s.next[i / kParts].c[i % kParts] = 0u;
+  }
 
-  // Every block's (x, y) to every block. The places take turns: what a call wrote is read before the next
-  // call's barrier, and written again after it.
+  // A block's numbers, the same in all its threads, to every block. The places take turns: what a call wrote is
+  // read before the next call's barrier, and written again after it.
   int turn = 0;
-  auto tell = [&](u64 x, u64 y) -> const u64(&)[kMaxCluster][2] {
-    u64(&to)[kMaxCluster][2] = s.all[turn];
+  auto tell = [&](u64 x, u64 y, u64 z) -> const u64(&)[kMaxCluster][3] {
+    u64(&to)[kMaxCluster][3] = s.all[turn];
     turn ^= 1;
     if (tid < (int)blocks) {
       put(&to[rank][0], tid, x);
       put(&to[rank][1], tid, y);
+      put(&to[rank][2], tid, z);
     }
     cluster_sync();
     return to;
   };
+  // Sums of the warps' numbers over the block, in every thread.
+  auto block_sums = [&](u64 x, u64 y, u64 (&sum)[2]) {
+    x = warp_sum64(x);
+    y = warp_sum64(y);
+    __syncthreads();
+    if (lane == 0) {
+      s.scan[warp][0] = x;
+      s.scan[warp][1] = y;
+    }
+    __syncthreads();
+    sum[0] = sum[1] = 0;
+    for (int k = 0; k < kWarps; ++k) {
+      sum[0] += s.scan[k][0];
+      sum[1] += s.scan[k][1];
+    }
+  };
 
-  // ---------------------------------------------------------------- keys and their maximum
-  uint32_t top = kNever;
-  int first = 0x7fffffff;
+  // ---------------------------------------------------------------- logits and their maximum
+  float top = -INFINITY;
   {
     constexpr int VE = Vec16<T>::N;
     const bool vec = reinterpret_cast<uintptr_t>(row) % 16 == 0;
-    const int whole = vec ? n / VE * VE : 0;
+    const int whole = vec ? min(hi, n) : lo;
 #pragma unroll 4
-    for (int i = tid * VE; i < whole; i += kThreads * VE) {
-      Vec16<T> v;
-      v.raw = *reinterpret_cast<const uint4*>(row + i);
+    for (int i = lo + lane * VE; i < whole; i += 32 * VE) {
+      float x[VE];
+      if (i + VE <= n) {
+        Vec16<T> v;
+        v.raw = *reinterpret_cast<const uint4*>(row + i);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] = v.get(e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] = i + e < n ? to_f32(row[i + e]) : -INFINITY;
+      }
 #pragma unroll
       for (int e = 0; e < VE; e += 4) {
-        const uint4 k = make_uint4(key_of(v.get(e)), key_of(v.get(e + 1)), key_of(v.get(e + 2)), key_of(v.get(e + 3)));
-        *reinterpret_cast<uint4*>(keys + i + e) = k;
-        top = max(top, max(max(k.x, k.y), max(k.z, k.w)));
+#pragma unroll
+        for (int z = 0; z < 4; ++z) top = fmaxf(top, x[e + z]);
+        *reinterpret_cast<float4*>(weights + i + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
       }
     }
-    for (int i = whole + tid; i < n; i += kThreads) {
-      const uint32_t k = key_of(to_f32(row[i]));
-      keys[i] = k;
-      top = max(top, k);
+    if (vec) {  // what is left of the last step
+      const int end = (n + VE - 1) / VE * VE;
+      for (int i = max(lo, end) + lane; i < hi; i += 32) weights[i] = __float_as_uint(-INFINITY);
+    } else {
+#pragma unroll 4
+      for (int i = lo + lane; i < hi; i += 32) {
+        const float x = i < n ? to_f32(row[i]) : -INFINITY;
+        weights[i] = __float_as_uint(x);
+        top = fmaxf(top, x);
+      }
     }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) s.reduce[warp] = top;
-  __syncthreads();
-  top = __reduce_max_sync(0xffffffffu, s.reduce[lane & (kWarps - 1)]);
-  // the first index of the block's maximum: the first token of the order, if it is the row's
-  for (int i = tid; i < n && first == 0x7fffffff; i += kThreads)
-    if (keys[i] == top) first = x0 + i;
-  first = (int)__reduce_min_sync(0xffffffffu, (uint32_t)first);
-  __syncthreads();
-  if (lane == 0) s.reduce[warp] = (uint32_t)first;
-  __syncthreads();
-  first = (int)__reduce_min_sync(0xffffffffu, s.reduce[lane & (kWarps - 1)]);
+  auto block_max = [&](uint32_t x) {
+    x = __reduce_max_sync(0xffffffffu, x);
+    __syncthreads();
+    if (lane == 0) s.scan[warp][0] = x;
+    __syncthreads();
+    return __reduce_max_sync(0xffffffffu, (uint32_t)s.scan[lane & (kWarps - 1)][0]);
+  };
+  // (fmaxf passes NaN over; a key of 0 stands for minus infinity)
+  uint32_t top_key = block_max(top > -INFINITY ? key_of(top) : 0u);
   cluster_wait_started();
   {
-    const auto& all = tell(top, (u64)first);
-    for (uint32_t r = 0; r < blocks; ++r) {
-      const uint32_t its = (uint32_t)all[r][0];
-      if (its > top || (its == top && (int)all[r][1] < first)) first = (int)all[r][1];
-      top = max(top, its);
-    }
+    const auto& all = tell(top_key, 0, 0);
+    for (uint32_t r = 0; r < blocks; ++r) top_key = max(top_key, (uint32_t)all[r][0]);
   }
-  if (top == kNever || !(temperature > 0.f) || asked == 1) {
+  if (top_key == 0u || !(temperature > 0.f) || top_k == 1) {
+    uint32_t first = 0xffffffffu;  // the lowest index of the maximum
+    if (top_key != 0u)
+      for (int i = tid; i < n; i += kThreads) {
+        const float x = __uint_as_float(weights[i]);
+        if (x > -INFINITY && key_of(x) == top_key) first = min(first, (uint32_t)(x0 + i));
+      }
+    first = ~block_max(~first);
+    const auto& all = tell(first, 0, 0);
+    for (uint32_t r = 0; r < blocks; ++r) first = min(first, (uint32_t)all[r][0]);
     if (rank == 0 && tid == 0) {
-      a.token[b] = top == kNever ? -1 : first;
-      a.prob[b] = top == kNever ? 0.f : 1.f;
+      a.token[b] = top_key == 0u ? -1 : (int)first;
+      a.prob[b] = top_key == 0u ? 0.f : 1.f;
     }
     return;
   }
 
-  const double highest = (double)value_of(top), rate = 1.0 / (double)temperature;
-  auto weigh = [&](uint32_t key) -> uint32_t {
-    if (key == kNever) return 0u;
-    return key == top ? (uint32_t)kOne : weight_of(((double)value_of(key) - highest) * rate, s.table);
-  };
-  const bool by_count = asked > 0 && asked < a.vocab, by_share = top_p < 1.f;
-  // min-p's least weight: a token stays if its weight is at least that
-  const uint32_t least = min_p > 0.f ? (uint32_t)__double2ull_ru((double)fminf(min_p, 1.f) * 2147483648.0) : 0u;
+  // ---------------------------------------------------------------- weights
+  const bool by_count = top_k > 0 && top_k < a.vocab, by_share = top_p < 1.f;
+  const bool ranges = by_count || by_share;
+  const uint32_t least = min_p > 0.f ? max((uint32_t)__double2ull_ru((double)fminf(min_p, 1.f) * 2147483648.0), 1u) : 1u;
+  u64 total, fit;  // of all weights; how many tokens weigh at least `least`
+  {
+    const float top_x = __uint_as_float(top_key & 0x80000000u ? top_key & 0x7fffffffu : ~top_key);
+    const double highest = (double)top_x, rate = 92.332482616893656877 / (double)temperature;  // 64 / ln 2
+    // exp(z) = 2^n 2^(j / 64) e^y, n and j whole, |y| <= ln 2 / 128, with e^y by its series, to 2^-44 of it
+    auto weigh = [&](float x) -> uint32_t {
+      if (x == top_x) return (uint32_t)kOne;
+      const double t = ((double)x - highest) * rate;
+      if (!(t > -2016.0)) return 0u;  // below 2^-31
+      const double big = t + 6755399441055744.0, r = t - (big - 6755399441055744.0);  // 1.5 2^52
+      const int i = __double2loint(big);
+      constexpr double c = 0.010830424696249145;  // ln 2 / 64
+      const double e = fma(fma(fma(fma(r, c * c * c * c / 24, c * c * c / 6), r, c * c / 2), r, c), r, 1.0);
+      const double p = s.table[i & 63];
+      const double w = e * __hiloint2double(__double2hiint(p) + (((i >> 6) + 31) << 20), __double2loint(p));
+      return (uint32_t)__double2loint(__dadd_rd(w, 4503599627370496.0));  // 2^52
+    };
+    u64 sum = 0, some = 0;
+    for (int i = lo + lane * 4; i < hi; i += kStep) {
+      uint4& at = *reinterpret_cast<uint4*>(weights + i);
+      const uint4 x = at;
+      const uint4 w = make_uint4(weigh(__uint_as_float(x.x)), weigh(__uint_as_float(x.y)), weigh(__uint_as_float(x.z)), weigh(__uint_as_float(x.w)));
+      at = w;
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const uint32_t y = z == 0 ? w.x : z == 1 ? w.y : z == 2 ? w.z : w.w;
+        sum += y;
+        some += y >= least;
+        if (!ranges) continue;
+        const int bin = y ? range_of(y) : -1;
+        // a warp with one range adds up first: rows of few different logits would queue up
+        if (__all_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, 0))) {
+          const u64 its = warp_sum64(y);
+          if (lane == 0 && bin >= 0) {
+            atomicAdd(&s.count[bin], 32u);
+            atomicAdd(&s.lo[bin], (uint32_t)(its & 0xffffu));
+            atomicAdd(&s.hi[bin], (uint32_t)(its >> 16));
+          }
+        } else if (bin >= 0) {
+          atomicAdd(&s.count[bin], 1u);
+          atomicAdd(&s.lo[bin], y & 0xffffu);
+          atomicAdd(&s.hi[bin], y >> 16);
+        }
+      }
+    }
+    u64 mine[2];
+    block_sums(sum, some, mine);
+    const auto& all = tell(mine[0], mine[1], 0);
+    total = fit = 0;
+    for (uint32_t r = 0; r < blocks; ++r) {
+      total += all[r][0];
+      fit += all[r][1];
+    }
+  }
 
   // ---------------------------------------------------------------- where the order ends
-  // Tokens above `border` stay, of those at it the `ties` first ones.
-  uint32_t border = kNever;
-  u64 ties = ~0ull;
-  // One descent: the place in the order where the count reaches `count` or the weights reach `need`
-  // (whichever is first), among the keys of [lo, hi].
-  auto descend = [&](u64 count, u64 need) {
-    uint32_t lo = 1u, hi = top;
-    u64 c0 = 0, w0 = 0;  // of the keys above hi
-    for (int round = 0;; ++round) {
-      // ranges of the first round: distance from the maximum, in steps of T / 32, the last one open
-      // (32 T below it weights are 0); then equal parts of [lo, hi]
-      const float step = 32.f / temperature;
-      const uint32_t span = hi - lo;
-      const int shift = max(0, 32 - __clz(span) - 10);
-      auto bin_of = [&](uint32_t key) {  // 0: the highest
-        if (round == 0) {
-          const float d = (value_of(top) - value_of(key)) * step;
-          return key == top ? 0 : d < (float)(kBins - 1) ? (int)d : kBins - 1;  // NaN and infinity: the last
-        }
-        return (int)((hi - key) >> shift);
-      };
-      for (int i = tid; i < kBins; i += kThreads) s.h.lo[i] = s.h.hi[i] = s.h.count[i] = 0u;
-      __syncthreads();
-      for (int base = 0; base < n; base += kThreads) {
-        const int i = base + tid;
-        const uint32_t key = i < n ? keys[i] : kNever;
-        const bool in = key >= lo && key <= hi;
-        const int bin = in ? bin_of(key) : -1;
-        const uint32_t w = in && by_share ? weigh(key) : 0u;
-        // equal ranges of a warp are added up first: rows of few different logits would queue up
-        const unsigned same = __match_any_sync(0xffffffffu, bin);
-        if (same == 0xffffffffu) {
-          const u64 sum = warp_sum64(w);
-          if (lane == 0 && bin >= 0) {
-            atomicAdd(&s.h.count[bin], 32u);
-            atomicAdd(&s.h.lo[bin], (uint32_t)(sum & 0xffffu));
-            atomicAdd(&s.h.hi[bin], (uint32_t)(sum >> 16));
-          }
-        } else if (in) {
-          atomicAdd(&s.h.count[bin], 1u);
-          if (by_share) {
-            atomicAdd(&s.h.lo[bin], w & 0xffffu);
-            atomicAdd(&s.h.hi[bin], w >> 16);
-          }
-        }
-      }
-      cluster_sync();
-      // this block's ranges, over all blocks; to all blocks
-      const int per = kBins / (int)blocks;
-      for (int i = tid; i < per; i += kThreads) {
-        const int bin = (int)rank * per + i;
-        u64 w = 0, c = 0;
-        for (uint32_t r = 0; r < blocks; ++r) {
-          w += get(&s.h.lo[bin], r) + ((u64)get(&s.h.hi[bin], r) << 16);
-          c += get(&s.h.count[bin], r);
-        }
-        for (uint32_t r = 0; r < blocks; ++r) {
-          u64* const to = &s.bins[0][0][0] + 2 * bin;
-          put(to, r, w);
-          put(to + 1, r, c);
-        }
-      }
-      cluster_sync();
-      // the range where the order ends: two ranges to a thread
-      const u64* const sums = &s.bins[0][0][0];
-      u64 w[2], c[2];
+  // The scan of two ranges to a thread: what is before them, and what is in them.
+  u64 w[2] = {0, 0}, c[2] = {0, 0}, w_to = 0, c_to = 0;
+  auto scan = [&](auto& sums) {
+    constexpr int kEach = sizeof(sums.c) / 4 / kThreads;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        w[k] = sums[2 * (2 * tid + k)];
-        c[k] = sums[2 * (2 * tid + k) + 1];
-      }
-      u64 wi = w[0] + w[1], ci = c[0] + c[1];
+    for (int k = 0; k < 2; ++k) {
+      w[k] = k < kEach ? sums.w[kEach * tid + k] : 0;
+      c[k] = k < kEach ? sums.c[kEach * tid + k] : 0;
+    }
+    w_to = w[0] + w[1];
+    c_to = c[0] + c[1];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 p = __shfl_up_sync(0xffffffffu, wi, o), q = __shfl_up_sync(0xffffffffu, ci, o);
-        if (lane >= o) {
-          wi += p;
-          ci += q;
-        }
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 p = __shfl_up_sync(0xffffffffu, w_to, o), q = __shfl_up_sync(0xffffffffu, c_to, o);
+      if (lane >= o) {
+        w_to += p;
+        c_to += q;
       }
-      if (lane == 31) {
-        s.scan[warp][0] = wi;
-        s.scan[warp][1] = ci;
-      }
-      if (tid == 0) s.bin = -1;
-      __syncthreads();
-      wi += w0;
-      ci += c0;
-      for (int k = 0; k < warp; ++k) {
-        wi += s.scan[k][0];
-        ci += s.scan[k][1];
-      }
-      // inclusive up to the thread's second range; the range that crosses first
-      const u64 w_before = wi - w[0] - w[1], c_before = ci - c[0] - c[1];
-      if (w_before < need && c_before < count && (wi >= need || ci >= count)) {
-        const bool one = w_before + w[0] >= need || c_before + c[0] >= count;
-        s.bin = 2 * tid + (one ? 0 : 1);
-        s.before[0] = w_before + (one ? 0 : w[0]);
-        s.before[1] = c_before + (one ? 0 : c[0]);
-      }
-      __syncthreads();
-      const int bin = s.bin;
-      if (bin < 0) {  // no end: the whole order
-        border = kNever;
-        ties = ~0ull;
-        return;
-      }
+    }
+    __syncthreads();
+    if (lane == 31) {
+      s.scan[warp][0] = w_to;
+      s.scan[warp][1] = c_to;
+    }
+    __syncthreads();
+    for (int k = 0; k < warp; ++k) {
+      w_to += s.scan[k][0];
+      c_to += s.scan[k][1];
+    }
+    return kEach;
+  };
+  // The range, in scanned sums, where the count comes to `count` or the weights to `need`; -1: none. w0 and c0:
+  // what is before all of them, and then before the range; wb and cb: what is in it.
+  auto cross = [&](int each, u64 count, u64 need, u64& w0, u64& c0, u64& wb, u64& cb) {
+    if (tid == 0) s.bin = -1;
+    __syncthreads();
+    const u64 we = w0 + w_to, ce = c0 + c_to, ws = we - w[0] - w[1], cs = ce - c[0] - c[1];
+    if (ws < need && cs < count && (we >= need || ce >= count)) {
+      const bool one = ws + w[0] >= need || cs + c[0] >= count;
+      s.bin = each * tid + (one ? 0 : 1);
+      s.before[0] = ws + (one ? 0 : w[0]);
+      s.before[1] = cs + (one ? 0 : c[0]);
+      s.in[0] = one ? w[0] : w[1];
+      s.in[1] = one ? c[0] : c[1];
+    }
+    __syncthreads();
+    const int bin = s.bin;
+    if (bin >= 0) {
       w0 = s.before[0];
       c0 = s.before[1];
-      if (round == 0) {
-        // the range's keys: from its lowest to its highest, found among the keys
-        uint32_t low = 0xffffffffu, high = 0u;
-        for (int i = tid; i < n; i += kThreads) {
-          const uint32_t key = keys[i];
-          if (key == kNever || bin_of(key) != bin) continue;
-          low = min(low, key);
-          high = max(high, key);
-        }
-        low = __reduce_min_sync(0xffffffffu, low);
-        high = __reduce_max_sync(0xffffffffu, high);
-        __syncthreads();
-        if (lane == 0) s.scan[warp][0] = (u64)low << 32 | high;
-        __syncthreads();
-        for (int k = 0; k < kWarps; ++k) {
-          low = min(low, (uint32_t)(s.scan[k][0] >> 32));
-          high = max(high, (uint32_t)s.scan[k][0]);
-        }
-        const auto& all = tell(low, high);
+      wb = s.in[0];
+      cb = s.in[1];
+    }
+    __syncthreads();
+    return bin;
+  };
+  int buffer = 0;
+  // From the values [v0, v1] on, of which there are cb, to the one where the order ends: each(f) calls f(value,
+  // weight) for the warp's tokens there.
+  auto narrow = [&](uint32_t v0, uint32_t v1, u64 count, u64 need, u64& w0, u64& c0, u64& wb, u64& cb, auto each) {
+    while (v0 < v1) {
+      const int shift = max(0, 32 - __clz(v1 - v0) - 9);
+      for (int i = tid; i < kParts; i += kThreads) s.lo[i] = s.hi[i] = s.count[i] = 0u;
+      __syncthreads();
+      each([&](uint32_t v, uint32_t y) {
+        if (v < v0 || v > v1) return;
+        const int part = (int)((v1 - v) >> shift);
+        atomicAdd(&s.count[part], 1u);
+        atomicAdd(&s.lo[part], y & 0xffffu);
+        atomicAdd(&s.hi[part], y >> 16);
+      });
+      __syncthreads();
+      auto& sums = s.next[buffer];
+      for (int i = tid; i < kParts; i += kThreads) {
+        if (s.count[i] == 0u) continue;
+        const u64 y = s.lo[i] + ((u64)s.hi[i] << 16);
         for (uint32_t r = 0; r < blocks; ++r) {
-          low = min(low, (uint32_t)all[r][0]);
-          high = max(high, (uint32_t)all[r][1]);
+          add_remote(&sums.w[i], r, y);
+          add_remote(&sums.c[i], r, s.count[i]);
         }
-        lo = low;
-        hi = high;
-      } else {
-        const uint32_t to = hi - ((uint32_t)bin << shift);
-        lo = max(lo, shift ? to - min(to - lo, (1u << shift) - 1u) : to);
-        hi = to;
       }
-      __syncthreads();  // the histogram and the sums are used again
-      if (lo == hi) {   // one key: of its tokens as many stay as it takes
-        const uint32_t w = weigh(lo);
-        u64 t = count - c0;
-        if (by_share && need != ~0ull && w > 0) t = min(t, (need - w0 + w - 1) / w);
-        border = lo;
-        ties = t;
-        return;
+      cluster_sync();
+      const int k = scan(sums);
+      for (int i = tid; i < kParts; i += kThreads) {  // for the round after the next one, whose barrier is behind the next one's
+        sums.w[i] = 0ull;
+        sums.c[i] = 0u;
       }
+      buffer ^= 1;
+      const int part = cross(k, count, need, w0, c0, wb, cb);
+      v1 -= (uint32_t)part << shift;
+      v0 = shift ? max(v0, v1 - min(v1 - v0, (1u << shift) - 1u)) : v1;
+    }
+    return v0;
+  };
+  // Tokens that weigh more than `border` stay, and of those that weigh as much the `ties` first ones of `tied`.
+  uint32_t border = least - 1u;
+  u64 ties = 0, tied = 0;
+  auto all_weights = [&](auto f) {
+    for (int i = lo + lane * 4; i < hi; i += kStep) {
+      const uint4 x = *reinterpret_cast<const uint4*>(weights + i);
+      f(x.x, x.x);
+      f(x.y, x.y);
+      f(x.z, x.z);
+      f(x.w, x.w);
     }
   };
-  auto stays = [&](uint32_t key) { return key > border; };
-
-  // the sum over the cluster of a block's value, thread by thread
-  auto total_of = [&](u64 mine, u64& before) {
-    mine = warp_sum64(mine);
-    __syncthreads();
-    if (lane == 0) s.scan[warp][0] = mine;
-    __syncthreads();
-    u64 block = 0;
-    for (int k = 0; k < kWarps; ++k) block += s.scan[k][0];
-    const auto& each = tell(block, 0);
-    u64 all = 0;
-    before = 0;
-    for (uint32_t r = 0; r < blocks; ++r) {
-      if (r == rank) before = all;
-      all += each[r][0];
+  int first_each = 0;
+  u64 scanned[6] = {};
+  // Ends the order where its count comes to `count` or its weights to `need`; returns the weights in it.
+  auto end_order = [&](u64 count, u64 need) {
+    w[0] = scanned[0], w[1] = scanned[1], c[0] = scanned[2], c[1] = scanned[3], w_to = scanned[4], c_to = scanned[5];
+    u64 w0 = 0, c0 = 0, wb = 0, cb = 0;
+    const int range = cross(first_each, count, need, w0, c0, wb, cb);
+    if (range < 0) {
+      border = 0u;
+      ties = tied = 0;
+      return total;
     }
-    return all;
+    // one token: its weight is the range's sum
+    const uint32_t at = cb == 1 ? (uint32_t)wb : narrow(least_of(range), most_of(range), count, need, w0, c0, wb, cb, all_weights);
+    border = at;
+    tied = cb;
+    ties = min(cb, count == kNone ? kNone : count - c0);
+    if (need != kNone) ties = min(ties, (need - w0 + at - 1) / at);
+    return w0 + ties * at;
   };
-  u64 need = ~0ull, before;
-  if (by_count) {
-    descend((u64)asked, ~0ull);
-    if (by_share) {  // the top-k's weights
-      u64 sum = 0;
-      for (int i = tid; i < n; i += kThreads) sum += stays(keys[i]) ? weigh(keys[i]) : 0u;
-      sum = total_of(sum, before) + (ties == ~0ull ? 0 : ties * weigh(border));
-      need = max(share_of(sum, whole_share(top_p)), (u64)1);
-      descend((u64)asked, need);
+  if (ranges && (by_share || fit > (u64)top_k)) {
+    // each block's share of the ranges over all blocks, to all blocks
+    const int share = kBins / (int)blocks;
+    for (int i = tid; i < share; i += kThreads) {
+      const int bin = (int)rank * share + i;
+      u64 y = 0;
+      uint32_t m = 0;
+      for (uint32_t r = 0; r < blocks; ++r) {
+        y += get(&s.lo[bin], r) + ((u64)get(&s.hi[bin], r) << 16);
+        m += get(&s.count[bin], r);
+      }
+      for (uint32_t r = 0; r < blocks; ++r) {
+        put(&s.first.w[bin], r, y);
+        put(&s.first.c[bin], r, m);
+      }
     }
-  } else if (by_share) {
-    u64 sum = 0;
-    for (int i = tid; i < n; i += kThreads) sum += weigh(keys[i]);
-    sum = total_of(sum, before);
-    need = max(share_of(sum, whole_share(top_p)), (u64)1);
-    descend(~0ull, need);
+    cluster_sync();
+    first_each = scan(s.first);
+    scanned[0] = w[0], scanned[1] = w[1], scanned[2] = c[0], scanned[3] = c[1], scanned[4] = w_to, scanned[5] = c_to;
+    const u64 k = by_count ? (u64)top_k : kNone;
+    u64 need = kNone;
+    if (by_share) need = max(share_of(by_count ? end_order(k, kNone) : total, whole_share(top_p)), (u64)1);
+    const uint32_t floor_ = least - 1u;
+    const u64 limit = least > 1u ? min(k, fit) : k;
+    end_order(limit, need);
+    if (border == 0u) border = floor_;  // nothing ended it but what weighs nothing
   }
 
   // ---------------------------------------------------------------- the draw
-  // Of the tokens at the border those of the lowest indices stay: how many a block has of them, and the
-  // blocks before it.
-  u64 left = 0;
-  if (ties != ~0ull) {
-    u64 mine = 0;
-    for (int i = tid; i < n; i += kThreads) mine += keys[i] == border;
-    total_of(mine, before);
-    left = ties > before ? ties - before : 0;  // that this block's keep
-  }
-  // Warps take contiguous parts: the kept weights in index order.
-  const int per = (n + kWarps * 32 - 1) / (kWarps * 32) * 32, lo = min(warp * per, n), hi = min(lo + per, n);
-  u64 tied = 0;  // at the border, in this warp's part
-  if (ties != ~0ull) {
-    for (int i = lo + lane; i < hi; i += 32) tied += keys[i] == border;
-    tied = warp_sum64(tied);
-    __syncthreads();
-    if (lane == 0) s.scan[warp][1] = tied;
-    __syncthreads();
-    u64 at = 0;
-    for (int k = 0; k < warp; ++k) at += s.scan[k][1];
-    left = left > at ? left - at : 0;  // that this warp's part keeps
-  }
-  auto kept = [&](int i, u64& room) -> uint32_t {  // the warp's, 32 in a row from i; room: border tokens that may stay
-    const uint32_t key = i + lane < hi ? keys[i + lane] : kNever;
-    bool stay = key > border && key != kNever;
-    if (ties != ~0ull) {
-      const unsigned at = __ballot_sync(0xffffffffu, key == border && i + lane < hi);
-      if (key == border) stay = (u64)__popc(at & ((1u << lane) - 1u)) < room;
-      room -= min(room, (u64)__popc(at));
+  // Not all that weigh as much as the last one stay: those of the highest logits, and of equal ones of
+  // the lowest indices. `last`: the key at the end; `room`: how many with it stay of this warp's tokens.
+  const bool split = ties < tied;
+  uint32_t last = 0u;
+  u64 room = 0;
+  auto key_at = [&](int i) { return key_of(to_f32(row[i])); };
+  if (split) {
+    auto tied_keys = [&](auto f) {
+      for (int i = lo + lane; i < min(hi, n); i += 32)
+        if (weights[i] == border) f(key_at(i), 1u);
+    };
+    uint32_t low = 0xffffffffu, high = 0u;
+    tied_keys([&](uint32_t v, uint32_t) {
+      low = min(low, v);
+      high = max(high, v);
+    });
+    low = ~block_max(~low);
+    high = block_max(high);
+    {
+      const auto& all = tell(low, high, 0);
+      for (uint32_t r = 0; r < blocks; ++r) {
+        low = min(low, (uint32_t)all[r][0]);
+        high = max(high, (uint32_t)all[r][1]);
+      }
     }
-    const uint32_t w = stay ? weigh(key) : 0u;
-    return w >= least ? w : 0u;
+    u64 w0 = 0, c0 = 0, wb = 0, cb = 0;
+    last = narrow(low, high, ties, kNone, w0, c0, wb, cb, tied_keys);
+    u64 mine = 0;
+    tied_keys([&](uint32_t v, uint32_t) { mine += v == last; });
+    mine = warp_sum64(mine);
+    __syncthreads();
+    if (lane == 0) s.scan[warp][2] = mine;
+    __syncthreads();
+    u64 before = 0, block = 0;
+    for (int k = 0; k < kWarps; ++k) {
+      if (k < warp) before += s.scan[k][2];
+      block += s.scan[k][2];
+    }
+    const auto& all = tell(block, 0, 0);
+    for (uint32_t r = 0; r < rank; ++r) before += all[r][0];
+    room = ties - c0 > before ? ties - c0 - before : 0;
+  }
+  // The weights that stay of the warp's step from i on, four to a lane; `left`: of `room`.
+  auto kept = [&](int i, u64& left) {
+    uint4 x = *reinterpret_cast<const uint4*>(weights + i + lane * 4);
+    if (!split) {
+      const uint32_t from = tied ? border : border + 1u;
+      return make_uint4(x.x >= from ? x.x : 0u, x.y >= from ? x.y : 0u, x.z >= from ? x.z : 0u, x.w >= from ? x.w : 0u);
+    }
+    uint32_t y[4] = {x.x, x.y, x.z, x.w}, at = 0u;  // at: which of the four are at the end
+    u64 mine = 0;
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+      if (y[z] > border) continue;
+      if (y[z] == border) {
+        const uint32_t key = key_at(i + lane * 4 + z);
+        if (key > last) continue;
+        if (key == last) {
+          at |= 1u << z;
+          ++mine;
+          continue;
+        }
+      }
+      y[z] = 0u;
+    }
+    u64 to = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 p = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += p;
+    }
+    u64 rank_of = to - mine;
+#pragma unroll
+    for (int z = 0; z < 4; ++z)
+      if ((at >> z) & 1u) {
+        if (rank_of >= left) y[z] = 0u;
+        ++rank_of;
+      }
+    left -= min(left, (u64)__shfl_sync(0xffffffffu, to, 31));
+    return make_uint4(y[0], y[1], y[2], y[3]);
   };
-  u64 sum = 0, room = left;
-  for (int i = lo; i < hi; i += 32) sum += kept(i, room);
+  u64 sum = 0, left = room;
+  for (int i = lo; i < hi; i += kStep) {
+    const uint4 x = kept(i, left);
+    sum += (u64)x.x + x.y + x.z + x.w;
+  }
   sum = warp_sum64(sum);
   __syncthreads();
   if (lane == 0) s.scan[warp][0] = sum;
@@ -437,26 +554,35 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     if (k < warp) at += s.scan[k][0];
     block += s.scan[k][0];
   }
-  const auto& each = tell(block, 0);  // no block's shared memory is looked at by another from here on
-  u64 total = 0;
+  const auto& each = tell(block, 0, 0);  // no block's shared memory is looked at by another from here on
+  u64 all = 0;
   for (uint32_t r = 0; r < blocks; ++r) {
     if (r < rank) at += each[r][0];
-    total += each[r][0];
+    all += each[r][0];
   }
-  const u64 u = min((u64)whole_share(a.uniforms[b]), kOne - 1), t = share_of(total, u);
-  if (t < at || t >= at + sum) return;
-  room = left;
-  for (int i = lo; i < hi; i += 32) {
-    const uint32_t w = kept(i, room);
-    u64 to = w;
+  const u64 u = min((u64)whole_share(a.uniforms[b]), kOne - 1), t = share_of(all, u);
+  if (t < at || t >= at + sum) return;  // another warp has it
+  left = room;
+  for (int i = lo; i < hi; i += kStep) {
+    const uint4 x = kept(i, left);
+    const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+    const u64 mine = (u64)x.x + x.y + x.z + x.w;
+    u64 to = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, to, o);
-      if (lane >= o) to += y;
+      const u64 p = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += p;
     }
-    if (t >= at + to - w && t < at + to) {
-      a.token[b] = x0 + i + lane;
-      a.prob[b] = (float)((double)w / (double)total);
+    u64 from = at + to - mine;
+    if (t >= from && t < from + mine) {
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        if (t >= from && t < from + y[z]) {
+          a.token[b] = x0 + i + lane * 4 + z;
+          a.prob[b] = (float)((double)y[z] / (double)all);
+        }
+        from += y[z];
+      }
     }
     at += __shfl_sync(0xffffffffu, to, 31);
     if (t < at) return;
@@ -472,7 +598,7 @@ int launch_sample(SampleArgs& a, cudaStream_t st) {
   while (blocks < kMaxCluster && ((a.vocab + blocks - 1) / blocks > kPerBlock ||
                                   ((int64_t)a.batch * blocks * 2 <= 2LL * sm_count() && a.vocab >= 2 * blocks * 1024)))
     blocks *= 2;
-  a.part = ((a.vocab + blocks - 1) / blocks + 15) / 16 * 16;
+  a.part = ((a.vocab + blocks - 1) / blocks + kWarps * kStep - 1) / (kWarps * kStep) * (kWarps * kStep);
   const size_t smem = (size_t)a.part * 4;
   static std::atomic<bool> set[64] = {};  // per device: the shared memory attribute is set (idempotent)
   int dev = 0;

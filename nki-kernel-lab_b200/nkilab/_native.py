@@ -101,7 +101,7 @@ SIGNATURES = {
 
 ABI_VERSION = 1
 MAX_DRAFTED = 128  # NKL_MAX_DRAFTED
-MAX_VOCAB = 393216  # NKL_MAX_VOCAB
+MAX_VOCAB = 360448  # NKL_MAX_VOCAB
 SOFTMAX_UNFUSED_STATIC_BYTES = 16 * 1024 * 1024  # NKL_SOFTMAX_UNFUSED_STATIC_BYTES
 
 

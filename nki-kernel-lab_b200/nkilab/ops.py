@@ -376,7 +376,7 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     0 takes the first one; top_k 0, top_p 1 and min_p 0 keep all. Each is a number, or one for each row: a
     tensor [B] on the GPU (top_k int32, the others float32), where NaN is off. Minus infinity and NaN are never
     drawn. Returns (token [B] int32, -1 if there is none; prob [B] float32, its share of what was kept).
-    Weights are whole multiples of 2^-31, so equal inputs give equal tokens on every launch. V up to 393216.
+    Weights are whole multiples of 2^-31, so equal inputs give equal tokens on every launch. V up to 360448.
     """
     numbers, rows = [], []
     for name, x, low, high in (("temperature", temperature, 0, math.inf), ("top_k", top_k, 0, 2 ** 31), ("top_p", top_p, 0, 1),
