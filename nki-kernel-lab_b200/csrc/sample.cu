@@ -12,8 +12,8 @@
 // drawn; T of 0 (or below, or NaN) takes the first token.
 //
 // A cluster of up to eight blocks takes a row; each holds its part in shared memory, first as logits,
-// then as weights, which are computed once, in 64 bits (in 32 they would shift a border between two
-// tokens of a long row now and then). The order's end is found without sorting: a histogram of
+// then as weights, which are computed once, to a unit of their last place (a float's 24 bits would shift
+// a border between two tokens of a long row now and then). The order's end is found without sorting: a histogram of
 // weights and counts over 1024 ranges of the weight, a thirty-second of it wide, tells the range where it
 // is; the weights of that range over 512 parts of it, and so on, until a part is one weight or one
 // token. Of tokens with the weight at the end as many stay as it takes, by logit and then by index.
@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "attn_math.cuh"
 #include "common.cuh"
 
 namespace nkl {
@@ -35,6 +36,7 @@ constexpr int kBins = 1024;       // of the first round: 992 are used
 constexpr int kParts = 512;       // of a range, in the rounds after it
 constexpr int kStep = 128;        // tokens that a warp looks at at once, four to a lane
 constexpr int kPerBlock = 45056;  // tokens that a block holds: 176 KB
+constexpr int kTable = 256;
 constexpr u64 kOne = 1ull << 31;
 constexpr u64 kNone = ~0ull;
 
@@ -105,6 +107,23 @@ __device__ __forceinline__ u64 warp_sum64(u64 v) {
   return v;
 }
 
+// 2^31 2^(-j / kTable): the whole part, and the rest as a float. By Taylor's series for e^-x, x below ln 2.
+struct Table {
+  uint32_t whole[kTable];
+  float rest[kTable];
+  constexpr Table() : whole(), rest() {
+    for (int j = 0; j < kTable; ++j) {
+      const double x = 0.69314718055994530942 * j / kTable;
+      double e = 1.0;
+      for (int n = 24; n > 0; --n) e = 1.0 - x / n * e;
+      e *= 2147483648.0;
+      whole[j] = (uint32_t)e;
+      rest[j] = (float)(e - whole[j]);
+    }
+  }
+};
+__device__ constexpr Table kPowers;
+
 template <int N>
 struct Sums {  // over the cluster: weights and counts of the ranges
   u64 w[N];
@@ -114,7 +133,7 @@ struct Shared {
   uint32_t lo[kBins], hi[kBins], count[kBins];  // the block's: weights in halves of 16 bits, which 2^16 tokens do not overflow
   Sums<kBins> first;
   Sums<kParts> next[2];  // in turn; all zero when they are added to
-  double table[64];      // 2^(j / 64)
+  uint2 table[kTable];   // 2^31 2^(-j / kTable): whole part, and the rest as a float
   u64 all[2][kMaxCluster][3];  // what each block has to tell the others, in turn
   u64 scan[kWarps][3];
   int bin;
@@ -138,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int top_k = a.top_ks ? a.top_ks[b] : a.top_k;
   // this warp's tokens: [lo, hi) of the block's, whole steps; behind n there is nothing to draw
   const int per = a.part / kWarps, lo = warp * per, hi = min(lo + per, (n + kStep - 1) / kStep * kStep);
-  if (tid < 64) s.table[tid] = exp2((double)tid / 64);
+  if (tid < kTable) s.table[tid] = make_uint2(kPowers.whole[tid], __float_as_uint(kPowers.rest[tid]));
   for (int i = tid; i < kBins; i += kThreads) s.lo[i] = s.hi[i] = s.count[i] = 0u;
   for (int i = tid; i < 2 * kParts; i += kThreads) {
     s.next[i / kParts].w[i % kParts] = 0ull;
@@ -251,46 +270,61 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   u64 total, fit;  // of all weights; how many tokens weigh at least `least`
   {
     const float top_x = __uint_as_float(top_key & 0x80000000u ? top_key & 0x7fffffffu : ~top_key);
-    const double highest = (double)top_x, rate = 92.332482616893656877 / (double)temperature;  // 64 / ln 2
-    // exp(z) = 2^n 2^(j / 64) e^y, n and j whole, |y| <= ln 2 / 128, with e^y by its series, to 2^-44 of it
-    auto weigh = [&](float x) -> uint32_t {
-      if (x == top_x) return (uint32_t)kOne;
-      const double t = ((double)x - highest) * rate;
-      if (!(t > -2016.0)) return 0u;  // below 2^-31
-      const double big = t + 6755399441055744.0, r = t - (big - 6755399441055744.0);  // 1.5 2^52
-      const int i = __double2loint(big);
-      constexpr double c = 0.010830424696249145;  // ln 2 / 64
-      const double e = fma(fma(fma(fma(r, c * c * c * c / 24, c * c * c / 6), r, c * c / 2), r, c), r, 1.0);
-      const double p = s.table[i & 63];
-      const double w = e * __hiloint2double(__double2hiint(p) + (((i >> 6) + 31) << 20), __double2loint(p));
-      return (uint32_t)__double2loint(__dadd_rd(w, 4503599627370496.0));  // 2^52
+    // exp(z) = 2^(-k / kTable) 2^(y / kTable), k whole, |y| <= 1/2 + a little. z comes to 2^-33 of a whole in pairs of
+    // floats: x - max and what rounding left of it, times a constant in two parts. Two tokens at a time.
+    const double rate = min(kTable / 0.69314718055994530942 / (double)temperature, 3e38);
+    const float ch = (float)rate, cl = (float)(rate - (double)ch);
+    const f32x2 up = f2_pack(ch, ch), down = f2_pack(-ch, -ch), rest = f2_pack(cl, cl), minus = f2_pack(-1.f, -1.f);
+    const f32x2 ntop = f2_pack(-top_x, -top_x), magic = f2_pack(12582912.f, 12582912.f), back = f2_pack(-12582912.f, -12582912.f);
+    constexpr double l = 0.69314718055994530942 / kTable;
+    const f32x2 a1 = f2_pack((float)l, (float)l), a2 = f2_pack((float)(l * l / 2), (float)(l * l / 2)),
+                a3 = f2_pack((float)(l * l * l / 6), (float)(l * l * l / 6));
+    auto weigh = [&](float x0, float x1, uint32_t& w0, uint32_t& w1) {
+      const f32x2 x = f2_pack(x0, x1), d = f2_add(x, ntop), g = f2_fma(x, minus, d);
+      const f32x2 e = f2_add(f2_fma(f2_fma(g, minus, d), minus, x), f2_fma(g, minus, ntop));  // d + e = x - max
+      const f32x2 u = f2_mul(d, down);  // how far below, in steps of the table
+      const f32x2 t = f2_fma(e, up, f2_fma(d, rest, f2_fma(d, up, u)));
+      const f32x2 k = f2_add(u, magic), y = f2_add(f2_fma(u, minus, f2_add(k, back)), t);
+      const f32x2 q = f2_mul(y, f2_fma(y, f2_fma(y, a3, a2), a1));  // 2^(y / kTable) - 1
+      auto one = [&](float far, float at, float more) -> uint32_t {
+        if (!(far < 31.5f * kTable)) return 0u;  // below 2^-31; NaN
+        const int i = __float_as_int(at) - 0x4b400000;
+        const uint2 p = s.table[i & (kTable - 1)];
+        const uint32_t w = p.x + (uint32_t)__float2int_rd(fmaf(__uint2float_rn(p.x), more, __uint_as_float(p.y)));
+        return w >> (i / kTable);
+      };
+      w0 = one(f2_lo(u), f2_lo(k), f2_lo(q));
+      w1 = one(f2_hi(u), f2_hi(k), f2_hi(q));
     };
-    u64 sum = 0, some = 0;
+    const bool infinite = !(top_x < INFINITY);
+    auto add = [&](uint32_t y) {
+      if (y == 0u) return;
+      const int range = range_of(y);
+      atomicAdd(&s.lo[range], y & 0xffffu);
+      atomicAdd(&s.hi[range], y >> 16);
+      atomicAdd(&s.count[range], 1u);
+    };
+    u64 sum = 0;
+    uint32_t some = 0;
     for (int i = lo + lane * 4; i < hi; i += kStep) {
       uint4& at = *reinterpret_cast<uint4*>(weights + i);
       const uint4 x = at;
-      const uint4 w = make_uint4(weigh(__uint_as_float(x.x)), weigh(__uint_as_float(x.y)), weigh(__uint_as_float(x.z)), weigh(__uint_as_float(x.w)));
-      at = w;
-#pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        const uint32_t y = z == 0 ? w.x : z == 1 ? w.y : z == 2 ? w.z : w.w;
-        sum += y;
-        some += y >= least;
-        if (!ranges) continue;
-        const int bin = y ? range_of(y) : -1;
-        // a warp with one range adds up first: rows of few different logits would queue up
-        if (__all_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, 0))) {
-          const u64 its = warp_sum64(y);
-          if (lane == 0 && bin >= 0) {
-            atomicAdd(&s.count[bin], 32u);
-            atomicAdd(&s.lo[bin], (uint32_t)(its & 0xffffu));
-            atomicAdd(&s.hi[bin], (uint32_t)(its >> 16));
-          }
-        } else if (bin >= 0) {
-          atomicAdd(&s.count[bin], 1u);
-          atomicAdd(&s.lo[bin], y & 0xffffu);
-          atomicAdd(&s.hi[bin], y >> 16);
-        }
+      uint4 y;
+      weigh(__uint_as_float(x.x), __uint_as_float(x.y), y.x, y.y);
+      weigh(__uint_as_float(x.z), __uint_as_float(x.w), y.z, y.w);
+      if (infinite) {
+        const uint32_t one = (uint32_t)kOne, in = __float_as_uint(INFINITY);
+        y = make_uint4(x.x == in ? one : 0u, x.y == in ? one : 0u, x.z == in ? one : 0u, x.w == in ? one : 0u);
+      }
+      at = y;
+      sum += ((u64)y.x + y.y) + ((u64)y.z + y.w);
+      if (least > 1u) some += (uint32_t)(y.x >= least) + (uint32_t)(y.y >= least) + (uint32_t)(y.z >= least) + (uint32_t)(y.w >= least);
+      else if (by_count) some += (uint32_t)(y.x > 0u) + (uint32_t)(y.y > 0u) + (uint32_t)(y.z > 0u) + (uint32_t)(y.w > 0u);
+      if (ranges) {
+        add(y.x);
+        add(y.y);
+        add(y.z);
+        add(y.w);
       }
     }
     u64 mine[2];
@@ -371,9 +405,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       each([&](uint32_t v, uint32_t y) {
         if (v < v0 || v > v1) return;
         const int part = (int)((v1 - v) >> shift);
-        atomicAdd(&s.count[part], 1u);
         atomicAdd(&s.lo[part], y & 0xffffu);
         atomicAdd(&s.hi[part], y >> 16);
+        atomicAdd(&s.count[part], 1u);
       });
       __syncthreads();
       auto& sums = s.next[buffer];
