@@ -15,9 +15,9 @@
 // then as weights, which are computed once, to a unit of their last place (a float's 24 bits would shift
 // a border between two tokens of a long row now and then). The order's end is found without sorting: a histogram of
 // weights and counts over 1024 ranges of the weight, a thirty-second of it wide, tells the range where it
-// is; the weights of that range over 512 parts of it, and so on, until a part is one weight or one
-// token. Of tokens with the weight at the end as many stay as it takes, by logit and then by index.
-// Blocks add their histograms up through distributed shared memory.
+// is. Up to 768 tokens of that range go to every block, by distributed shared memory, and each finds
+// the end among them for itself; more are taken apart by histograms over 512 parts of the range, added up over
+// the blocks, and so on, until a part is one weight. Of equal ones as many stay as it takes, by logit and then by index.
 #include <algorithm>
 #include <atomic>
 
@@ -34,8 +34,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 1024;       // of the first round: 992 are used
 constexpr int kParts = 512;       // of a range, in the rounds after it
+constexpr int kList = 768;        // tokens of a range that are gathered
 constexpr int kStep = 128;        // tokens that a warp looks at at once, four to a lane
-constexpr int kPerBlock = 45056;  // tokens that a block holds: 176 KB
+constexpr int kPerBlock = 45056;  // tokens that a block holds: 176 KB; blocks of up to 16384 go two to an SM
 constexpr int kTable = 256;
 constexpr u64 kOne = 1ull << 31;
 constexpr u64 kNone = ~0ull;
@@ -89,6 +90,9 @@ __device__ __forceinline__ void put(u64* p, uint32_t rank, u64 v) {
 __device__ __forceinline__ void put(uint32_t* p, uint32_t rank, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote(p, rank)), "r"(v) : "memory");
 }
+__device__ __forceinline__ void put(uint4* p, uint32_t rank, uint4 v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(remote(p, rank)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ void add_remote(u64* p, uint32_t rank, u64 v) {
   asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
 }
@@ -132,11 +136,16 @@ struct Sums {  // over the cluster: weights and counts of the ranges
 struct Shared {
   uint32_t lo[kBins], hi[kBins], count[kBins];  // the block's: weights in halves of 16 bits, which 2^16 tokens do not overflow
   Sums<kBins> first;
-  Sums<kParts> next[2];  // in turn; all zero when they are added to
+  union {
+    Sums<kParts> next[2];  // in turn; all zero when they are added to
+    uint4 list[kList];     // a range's tokens: key, weight, index
+  };
+  uint32_t part_lo[kParts], part_hi[kParts], part_count[kParts];
   uint2 table[kTable];   // 2^31 2^(-j / kTable): whole part, and the rest as a float
   u64 all[2][kMaxCluster][3];  // what each block has to tell the others, in turn
   u64 scan[kWarps][3];
-  int bin;
+  int bin, slots;
+  uint32_t ahead;
   u64 before[2], in[2];
 };
 
@@ -338,42 +347,41 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   }
 
   // ---------------------------------------------------------------- where the order ends
-  // The scan of two ranges to a thread: what is before them, and what is in them.
+  // The scan of N ranges, two or one to a thread: what is in them, and up to and with them.
   u64 w[2] = {0, 0}, c[2] = {0, 0}, w_to = 0, c_to = 0;
-  auto scan = [&](auto& sums) {
-    constexpr int kEach = sizeof(sums.c) / 4 / kThreads;
+  auto scan = [&](int each, auto weight, auto number) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      w[k] = k < kEach ? sums.w[kEach * tid + k] : 0;
-      c[k] = k < kEach ? sums.c[kEach * tid + k] : 0;
+      w[k] = k < each ? weight(each * tid + k) : 0;
+      c[k] = k < each ? number(each * tid + k) : 0;
     }
     w_to = w[0] + w[1];
-    c_to = c[0] + c[1];
+    uint32_t n_to = (uint32_t)(c[0] + c[1]);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const u64 p = __shfl_up_sync(0xffffffffu, w_to, o), q = __shfl_up_sync(0xffffffffu, c_to, o);
+      const u64 p = __shfl_up_sync(0xffffffffu, w_to, o);
+      const uint32_t q = __shfl_up_sync(0xffffffffu, n_to, o);
       if (lane >= o) {
         w_to += p;
-        c_to += q;
+        n_to += q;
       }
     }
     __syncthreads();
     if (lane == 31) {
       s.scan[warp][0] = w_to;
-      s.scan[warp][1] = c_to;
+      s.scan[warp][1] = n_to;
     }
+    if (tid == 0) s.bin = -1;
     __syncthreads();
+    c_to = n_to;
     for (int k = 0; k < warp; ++k) {
       w_to += s.scan[k][0];
       c_to += s.scan[k][1];
     }
-    return kEach;
   };
   // The range, in scanned sums, where the count comes to `count` or the weights to `need`; -1: none. w0 and c0:
   // what is before all of them, and then before the range; wb and cb: what is in it.
   auto cross = [&](int each, u64 count, u64 need, u64& w0, u64& c0, u64& wb, u64& cb) {
-    if (tid == 0) s.bin = -1;
-    __syncthreads();
     const u64 we = w0 + w_to, ce = c0 + c_to, ws = we - w[0] - w[1], cs = ce - c[0] - c[1];
     if (ws < need && cs < count && (we >= need || ce >= count)) {
       const bool one = ws + w[0] >= need || cs + c[0] >= count;
@@ -391,8 +399,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       wb = s.in[0];
       cb = s.in[1];
     }
-    __syncthreads();
-    return bin;
+    return bin;  // a scan's first barrier comes before the next crossing
   };
   int buffer = 0;
   // From the values [v0, v1] on, of which there are cb, to the one where the order ends: each(f) calls f(value,
@@ -400,33 +407,33 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   auto narrow = [&](uint32_t v0, uint32_t v1, u64 count, u64 need, u64& w0, u64& c0, u64& wb, u64& cb, auto each) {
     while (v0 < v1) {
       const int shift = max(0, 32 - __clz(v1 - v0) - 9);
-      for (int i = tid; i < kParts; i += kThreads) s.lo[i] = s.hi[i] = s.count[i] = 0u;
+      for (int i = tid; i < kParts; i += kThreads) s.part_lo[i] = s.part_hi[i] = s.part_count[i] = 0u;
       __syncthreads();
       each([&](uint32_t v, uint32_t y) {
         if (v < v0 || v > v1) return;
         const int part = (int)((v1 - v) >> shift);
-        atomicAdd(&s.lo[part], y & 0xffffu);
-        atomicAdd(&s.hi[part], y >> 16);
-        atomicAdd(&s.count[part], 1u);
+        atomicAdd(&s.part_lo[part], y & 0xffffu);
+        atomicAdd(&s.part_hi[part], y >> 16);
+        atomicAdd(&s.part_count[part], 1u);
       });
       __syncthreads();
       auto& sums = s.next[buffer];
       for (int i = tid; i < kParts; i += kThreads) {
-        if (s.count[i] == 0u) continue;
-        const u64 y = s.lo[i] + ((u64)s.hi[i] << 16);
+        if (s.part_count[i] == 0u) continue;
+        const u64 y = s.part_lo[i] + ((u64)s.part_hi[i] << 16);
         for (uint32_t r = 0; r < blocks; ++r) {
           add_remote(&sums.w[i], r, y);
-          add_remote(&sums.c[i], r, s.count[i]);
+          add_remote(&sums.c[i], r, s.part_count[i]);
         }
       }
       cluster_sync();
-      const int k = scan(sums);
+      scan(kParts / kThreads, [&](int i) { return sums.w[i]; }, [&](int i) { return sums.c[i]; });
       for (int i = tid; i < kParts; i += kThreads) {  // for the round after the next one, whose barrier is behind the next one's
         sums.w[i] = 0ull;
         sums.c[i] = 0u;
       }
       buffer ^= 1;
-      const int part = cross(k, count, need, w0, c0, wb, cb);
+      const int part = cross(kParts / kThreads, count, need, w0, c0, wb, cb);
       v1 -= (uint32_t)part << shift;
       v0 = shift ? max(v0, v1 - min(v1 - v0, (1u << shift) - 1u)) : v1;
     }
@@ -444,18 +451,125 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       f(x.w, x.w);
     }
   };
-  int first_each = 0;
+  auto key_at = [&](int i) { return key_of(to_f32(row[i])); };
+  // A range of few tokens: they go to every block, which then finds the end for itself. With `apply` the weights of
+  // this block's tokens behind the end become 0. Returns the weights up to the end.
+  bool listed = false, narrowed = false;  // what the shared place was used for last
+  auto end_in_list = [&](int range, u64 count, u64 need, u64 w0, u64 c0, int number, bool apply) {
+    // where this block's begin in the list: behind those of the blocks before it
+    uint32_t mine = lane < (int)blocks ? get(&s.count[range], lane) : 0u, to = mine;
+#pragma unroll
+    for (int o = 1; o < kMaxCluster; o <<= 1) {
+      const uint32_t p = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += p;
+    }
+    const int end = (int)__shfl_sync(0xffffffffu, to, rank), begin = end - (int)__shfl_sync(0xffffffffu, mine, rank);
+    if (tid == 0) {
+      s.slots = begin;
+      s.ahead = 0u;
+    }
+    if (listed || narrowed) cluster_sync();  // others may still read theirs
+    __syncthreads();
+    listed = true;
+    constexpr int kKeyShift = sizeof(T) == 2 ? 16 : 0;  // a bf16's key is its upper half
+    const uint32_t y0 = least_of(range), y1 = most_of(range);
+    for (int i = lo + lane * 4; i < hi; i += kStep) {
+      const uint4 x = *reinterpret_cast<const uint4*>(weights + i);
+      const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        if (y[z] < y0 || y[z] > y1) continue;
+        const uint4 e = make_uint4(key_at(i + z) >> kKeyShift, y[z], (uint32_t)(i + z), 0u);
+        const int slot = atomicAdd(&s.slots, 1);
+        for (uint32_t r = 0; r < blocks; ++r) put(&s.list[slot], r, e);
+      }
+    }
+    cluster_sync();
+    const bool one = tid < number, two = tid + kThreads < number;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u), e0 = one ? s.list[tid] : none, e1 = two ? s.list[tid + kThreads] : none;
+    auto pair_max = [&](uint32_t p, uint32_t q) {  // of two numbers of a thread, over the block
+      p = __reduce_max_sync(0xffffffffu, p);
+      q = __reduce_max_sync(0xffffffffu, q);
+      __syncthreads();
+      if (lane == 0) s.scan[warp][2] = (u64)p << 32 | q;
+      __syncthreads();
+      const u64 x = s.scan[lane & (kWarps - 1)][2];
+      return make_uint2(__reduce_max_sync(0xffffffffu, (uint32_t)(x >> 32)), __reduce_max_sync(0xffffffffu, (uint32_t)x));
+    };
+    const uint2 most = pair_max(max(e0.x, e1.x), max(one ? ~e0.x : 0u, two ? ~e1.x : 0u));
+    uint32_t v1 = most.x, v0 = ~most.y;
+    u64 wb = 0, cb = 0;
+    do {  // as in narrow, among the block's own copy
+      const int shift = max(0, 32 - __clz(v1 - v0) - 9);
+      for (int i = tid; i < kParts; i += kThreads) s.part_lo[i] = s.part_hi[i] = s.part_count[i] = 0u;
+      __syncthreads();
+      auto add = [&](const uint4& e, bool there) {
+        if (!there || e.x < v0 || e.x > v1) return;
+        const int part = (int)((v1 - e.x) >> shift);
+        atomicAdd(&s.part_lo[part], e.y & 0xffffu);
+        atomicAdd(&s.part_hi[part], e.y >> 16);
+        atomicAdd(&s.part_count[part], 1u);
+      };
+      add(e0, one);
+      add(e1, two);
+      __syncthreads();
+      scan(kParts / kThreads, [&](int i) { return s.part_lo[i] + ((u64)s.part_hi[i] << 16); }, [&](int i) { return s.part_count[i]; });
+      const int part = cross(kParts / kThreads, count, need, w0, c0, wb, cb);
+      v1 -= (uint32_t)part << shift;
+      v0 = shift ? max(v0, v1 - min(v1 - v0, (1u << shift) - 1u)) : v1;
+    } while (v0 < v1);
+    // tokens of one logit, so of one weight: as many stay as it takes, the lowest indices
+    const uint32_t y = (uint32_t)(wb / cb);
+    u64 stay = min(cb, count == kNone ? kNone : count - c0);
+    if (need != kNone) stay = min(stay, (need - w0 + y - 1) / y);
+    if (apply) {
+      const uint32_t before = (uint32_t)(one && tid < begin && e0.x == v1) + (uint32_t)(two && tid + kThreads < begin && e1.x == v1);
+      if (before) atomicAdd(&s.ahead, before);
+      __syncthreads();
+      const u64 ahead = s.ahead;
+      auto settle = [&](const uint4& e, int at) {
+        if (at < begin || at >= end || e.x > v1) return;
+        bool out = e.x < v1;
+        if (!out && stay < cb) {
+          u64 place = ahead;
+          for (int j = begin; j < end; ++j) place += s.list[j].x == v1 && s.list[j].z < e.z;
+          out = place >= stay;
+        }
+        if (out) weights[e.z] = 0u;
+      };
+      if (one) settle(e0, tid);
+      if (two) settle(e1, tid + kThreads);
+      __syncthreads();
+    }
+    return w0 + stay * y;
+  };
   u64 scanned[6] = {};
   // Ends the order where its count comes to `count` or its weights to `need`; returns the weights in it.
-  auto end_order = [&](u64 count, u64 need) {
+  auto end_order = [&](u64 count, u64 need, bool apply) {
+    __syncthreads();
+    if (tid == 0) s.bin = -1;
+    __syncthreads();
     w[0] = scanned[0], w[1] = scanned[1], c[0] = scanned[2], c[1] = scanned[3], w_to = scanned[4], c_to = scanned[5];
     u64 w0 = 0, c0 = 0, wb = 0, cb = 0;
-    const int range = cross(first_each, count, need, w0, c0, wb, cb);
+    const int range = cross(kBins / kThreads, count, need, w0, c0, wb, cb);
+    ties = tied = 0;
     if (range < 0) {
-      border = 0u;
-      ties = tied = 0;
+      border = least - 1u;  // nothing ends it but what weighs nothing
       return total;
     }
+    if (cb > 1 && cb <= (u64)kList) {
+      border = least_of(range) - 1u;
+      return end_in_list(range, count, need, w0, c0, (int)cb, apply);
+    }
+    if (cb > 1 && listed) {  // the list's place is that of the sums
+      for (int i = tid; i < 2 * kParts; i += kThreads) {
+        s.next[i / kParts].w[i % kParts] = 0ull;
+        s.next[i / kParts].c[i % kParts] = 0u;
+      }
+      cluster_sync();
+      listed = false;
+    }
+    narrowed = cb > 1;
     // one token: its weight is the range's sum
     const uint32_t at = cb == 1 ? (uint32_t)wb : narrow(least_of(range), most_of(range), count, need, w0, c0, wb, cb, all_weights);
     border = at;
@@ -481,15 +595,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
     }
     cluster_sync();
-    first_each = scan(s.first);
+    scan(kBins / kThreads, [&](int i) { return s.first.w[i]; }, [&](int i) { return s.first.c[i]; });
     scanned[0] = w[0], scanned[1] = w[1], scanned[2] = c[0], scanned[3] = c[1], scanned[4] = w_to, scanned[5] = c_to;
     const u64 k = by_count ? (u64)top_k : kNone;
     u64 need = kNone;
-    if (by_share) need = max(share_of(by_count ? end_order(k, kNone) : total, whole_share(top_p)), (u64)1);
-    const uint32_t floor_ = least - 1u;
-    const u64 limit = least > 1u ? min(k, fit) : k;
-    end_order(limit, need);
-    if (border == 0u) border = floor_;  // nothing ended it but what weighs nothing
+    if (by_share) need = max(share_of(by_count ? end_order(k, kNone, false) : total, whole_share(top_p)), (u64)1);
+    end_order(least > 1u ? min(k, fit) : k, need, true);
   }
 
   // ---------------------------------------------------------------- the draw
@@ -498,7 +609,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const bool split = ties < tied;
   uint32_t last = 0u;
   u64 room = 0;
-  auto key_at = [&](int i) { return key_of(to_f32(row[i])); };
   if (split) {
     auto tied_keys = [&](auto f) {
       for (int i = lo + lane; i < min(hi, n); i += 32)
@@ -519,6 +629,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       }
     }
     u64 w0 = 0, c0 = 0, wb = 0, cb = 0;
+    // (an end found in a list splits nothing: the sums' place is theirs)
     last = narrow(low, high, ties, kNone, w0, c0, wb, cb, tied_keys);
     u64 mine = 0;
     tied_keys([&](uint32_t v, uint32_t) { mine += v == last; });
