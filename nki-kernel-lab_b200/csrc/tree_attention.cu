@@ -715,8 +715,9 @@ extern "C" int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, 
   a.per_page = (int)(page_size / block);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t rows = tokens * a.t.group;
-  a.tiles = tiles_8bit(rows);
-  a.t.row_blocks = (int)((rows + 16 * a.tiles - 1) / (16 * a.tiles));
+  const Shape8 shape = shape_8bit(rows);
+  a.tiles = shape.tiles;
+  a.t.row_blocks = shape.row_blocks;
   a.t.splits = (int)splits_8bit(batch, kv_heads, rows, page_size * max_pages);
   if (const size_t need = split_bytes(a.t.splits, batch, heads, tokens, head_dim)) {
     if (!workspace || workspace_bytes < need) return fail(NKL_ERR_ARG, "%s: workspace too small", op);
@@ -728,9 +729,9 @@ extern "C" int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, 
   const bool fast = page_size % 16 == 0 && block % 16 == 0;
   int rc;
   if (dtype == NKL_FLOAT32)
-    rc = head_dim <= 64 ? launch_8bit<float, 1>(a, grid, fast, st) : launch_8bit<float, 2>(a, grid, fast, st);
+    rc = head_dim <= 64 ? launch_8bit<float, 1>(a, shape.nt, grid, fast, st) : launch_8bit<float, 2>(a, shape.nt, grid, fast, st);
   else
-    rc = head_dim <= 64 ? launch_8bit<bf16, 1>(a, grid, fast, st) : launch_8bit<bf16, 2>(a, grid, fast, st);
+    rc = head_dim <= 64 ? launch_8bit<bf16, 1>(a, shape.nt, grid, fast, st) : launch_8bit<bf16, 2>(a, shape.nt, grid, fast, st);
   if (rc || a.t.splits == 1) return rc;
   return launch_combine<true>(a.t, dtype, st, op);
 }

@@ -3,12 +3,14 @@
 //
 // Cached k and v are e4m3 numbers with a power of two for each block of positions and head. They go
 // from global memory into registers, 16 bytes to a lane, and from there, as f16 (which has every
-// e4m3 number), into the products, without shared memory and without barriers:
-//   S = Q K^T  the lanes of a row hold other entries of a head than the fragment's layout says, in
-//              Q and K alike, so that a lane's 16 bytes of K are the fragments of four products
-//   O += P V   two keys' bytes are interleaved to pairs; a lane's 16 bytes are its column of 16
-//              products, and it ends up with 16 entries in a row of O
-// A warp meets one tile of 16 query rows with one window of 32 keys after the other, the windows
+// e4m3 number), into the products, without shared memory and without barriers. Both products have the
+// cache's values as their first operand, 16 rows high, and 8 query rows as their second, so that a decoding
+// step's few rows waste little:
+//   S^T = K Q^T      the lanes of a row hold other entries of a head than the fragment's layout says, in
+//                    Q and K alike, so that a lane's 16 bytes of K are the fragments of four products
+//   O^T += V^T P^T   two keys' bytes are interleaved to pairs; a lane's 16 bytes of a key are its rows of eight
+//                    products, and it ends up with 16 entries in a row of O. P is transposed by movmatrix
+// A warp meets its 8 or 16 query rows with one window of 32 keys after the other, the windows
 // dealt out over a block's warps; their (max, sum, O) meet in shared memory, those of several blocks
 // in the workspace (tree_combine_kernel).
 //
@@ -21,6 +23,9 @@
 
 namespace {
 
+#ifndef KMIN8
+#define KMIN8 4
+#endif
 constexpr int kThreads8 = 128;
 constexpr int kWarps8 = kThreads8 / 32;
 constexpr int kWindow = 32;     // keys that a warp looks up at a time
@@ -31,12 +36,19 @@ struct Bits8Args {
   TreeArgs t;  // c_p, c_h, c_s: in bytes
   const uint8_t *k_scales, *v_scales;
   int block, per_page;  // positions of a block, blocks of a page
-  int tiles;            // tiles of 16 query rows that a block's warps share
+  int tiles;            // of 8 NT query rows, which a block's warps share
 };
 
-__device__ __forceinline__ uint32_t e4m3_pair(uint32_t two) {  // the lower 16 bits
+// Four e4m3 numbers as two pairs of f16.
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 x, y;\n mov.b32 {x, y}, %2;\n cvt.rn.f16x2.e4m3x2 %0, x;\n cvt.rn.f16x2.e4m3x2 %1, y;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+// An 8 x 8 matrix, row g at the lanes 4 g .. 4 g + 3, transposed.
+__device__ __forceinline__ uint32_t transpose(uint32_t x) {
   uint32_t r;
-  asm("{\n .reg .b16 x;\n mov.b32 {x, _}, %1;\n cvt.rn.f16x2.e4m3x2 %0, x;\n}" : "=r"(r) : "r"(two));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -83,13 +95,16 @@ __device__ __forceinline__ void bf16_parts(float lo, float hi, uint32_t (&p)[N])
 }
 
 // DC: head_dim up to 64 DC. FAST: pages and blocks are multiples of 16 positions, so that the 16 keys of a
-// product lie in a row and share their powers of two.
-template <typename T, int DC, bool FAST>
-__global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
+// product lie in a row and share their powers of two. NT: tiles of 8 query rows to a warp.
+template <typename T, int DC, bool FAST, int NT>
+__global__ void __launch_bounds__(kThreads8, NT == 1 && sizeof(T) == 2 ? KMIN8 : 2)
+attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int kParts = kF32 ? 3 : 1;   // of drafted k and v, in bf16
+  constexpr int kPParts = kF32 ? 3 : 2;  // of the weights for them
   constexpr int kSteps = 4 * DC;         // products over the entries of a head
-  constexpr int kCols = 8 * DC;          // entries of V that a lane has of a key, and products P V
+  constexpr int kCols = 8 * DC;          // entries of V that a lane has of a key
+  constexpr int kRowsW = 8 * NT;         // a warp's query rows
   extern __shared__ __align__(16) float joined[];
   __shared__ int s_bad;                  // a drafted v that is not finite
   const TreeArgs& a = args.t;
@@ -98,7 +113,7 @@ __global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __gr
   const int split = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
   const int kvh = blockIdx.y, b = blockIdx.z;
   const int tile = warp % args.tiles, stream = warp / args.tiles, streams = kWarps8 / args.tiles;
-  const int rows = a.tokens * a.group, r0 = (rb * args.tiles + tile) * 16;
+  const int rows = a.tokens * a.group, r0 = (rb * args.tiles + tile) * kRowsW;
   const int n = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
   const int windows = (n + kWindow - 1) / kWindow, per = (windows + a.splits - 1) / a.splits;
   const int w0 = min(split * per, windows), w1 = min(w0 + per, windows);
@@ -106,15 +121,12 @@ __global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __gr
   if (tid == 0) s_bad = 0;
   __syncthreads();
 
-  // the lane's rows, g and g + 8: where their q lies
-  const T* qp[2];
-  bool real[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = r0 + g + 8 * i, token = row / a.group;
-    real[i] = row < rows && (!parents || parents[token] >= -1);  // an absent token's q is not looked at
-    qp[i] = static_cast<const T*>(a.q) + b * a.q_b + (real[i] ? token * a.q_t + (kvh * a.group + row - token * a.group) * a.q_h : 0);
-  }
+  // Query row r of the warp's: where it lies, and whether it is one (an absent token's is not looked at).
+  auto query = [&](int r, bool& real) {
+    const int row = r0 + r, token = row / a.group;
+    real = row < rows && (!parents || parents[token] >= -1);
+    return static_cast<const T*>(a.q) + b * a.q_b + (real ? token * a.q_t + (kvh * a.group + row - token * a.group) * a.q_h : 0);
+  };
   // Four consecutive entries of the lane's: step s takes those at entry(s).
   auto entry = [&](int s) { return (t4 + 4 * (s >> 2)) * 16 + (s & 3) * 4; };
   auto four = [&](const T* p) {
@@ -127,177 +139,187 @@ __global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __gr
     }
     return x;
   };
-  uint32_t qh[kSteps][4], ql[kF32 ? kSteps : 1][4];
-  float factor[2];  // of a row's scores
-  {
-    float top[2] = {0.f, 0.f};
+  // Row g of each tile, for the products; the factors of the scores of the rows 2 t4 and 2 t4 + 1, which the
+  // lane has then.
+  uint32_t qh[NT][kSteps][2], ql[NT][kF32 ? kSteps : 1][2];
+  float factor[NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+  for (int t = 0; t < NT; ++t) {
+    bool real;
+    const T* const qp = query(8 * t + g, real);
+    float top = 0.f;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        if (!real[i] || entry(s) >= a.d) continue;
-        const float4 x = four(qp[i] + entry(s));
-        for (float y : {x.x, x.y, x.z, x.w}) top[i] = fmaxf(top[i], fabsf(y) < INFINITY ? fabsf(y) : 0.f);
-      }
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      const int e = max((int)(__float_as_uint(top[i]) >> 23) - 127, -112);  // 2^e <= top
-      const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-      factor[i] = a.scale * kLog2e * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+    for (int s = 0; s < kSteps; ++s) {
+      if (!real || entry(s) >= a.d) continue;
+      const float4 x = four(qp + entry(s));
+      for (float y : {x.x, x.y, x.z, x.w}) top = fmaxf(top, fabsf(y) < INFINITY ? fabsf(y) : 0.f);
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);  // 2^e <= top
+    const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+    const float f = a.scale * kLog2e * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+    factor[t][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
+    factor[t][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (real[i] && entry(s) < a.d) x = four(qp[i] + entry(s));
-        x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
-        qh[s][i] = half_pair(x.x, x.y);
-        qh[s][2 + i] = half_pair(x.z, x.w);
-        if constexpr (kF32) {
-          const float2 u = rest_half(qh[s][i], x.x, x.y), v = rest_half(qh[s][2 + i], x.z, x.w);
-          ql[s][i] = half_pair(u.x, u.y);
-          ql[s][2 + i] = half_pair(v.x, v.y);
-        }
+    for (int s = 0; s < kSteps; ++s) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (real && entry(s) < a.d) x = four(qp + entry(s));
+      x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
+      qh[t][s][0] = half_pair(x.x, x.y);
+      qh[t][s][1] = half_pair(x.z, x.w);
+      if constexpr (kF32) {
+        const float2 u = rest_half(qh[t][s][0], x.x, x.y), v = rest_half(qh[t][s][1], x.z, x.w);
+        ql[t][s][0] = half_pair(u.x, u.y);
+        ql[t][s][1] = half_pair(v.x, v.y);
       }
     }
   }
 
-  // m: the rows' reference for sums l of 2^(s - m); v: that for O, sums of 2^(s + e - v + kRaise) v
-  float m[2] = {-INFINITY, -INFINITY}, mv[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[kCols][4];
+  // m: the rows' reference for sums l of 2^(s - m); mv: that for O, sums of 2^(s + e - mv + kRaise) v
+  float m[NT][2], mv[NT][2], l[NT][2], o[NT][kCols / 2][4];
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  for (int t = 0; t < NT; ++t) {
+    m[t][0] = m[t][1] = mv[t][0] = mv[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kCols / 2; ++j) o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.f;
+  }
 
-  // Weights of 16 keys: x[2 k + ..] the scores of rows g (0, 1) and g + 8 (2, 3) with keys 8 k + 2 t4 and
-  // the one after it, e[..] their powers of two for O. Comes back with x the weights for O.
-  auto weigh = [&](float (&x)[2][4], const float (&e)[2][2]) {
+  // Weights of 16 keys: x[t][2 k + i] the score of key 8 k + g with row 2 t4 + i of tile t, e[k] the key's power of
+  // two for O. Comes back with x the weights for O.
+  auto weigh = [&](float (&x)[NT][4], const float (&e)[2]) {
     bool grows = false;
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) grows |= x[k][i] > m[i >> 1] + kLag8 || x[k][i] + e[k][i & 1] > mv[i >> 1] + kLag8;
-    if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float top = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
-        float tv = fmaxf(fmaxf(x[0][2 * i] + e[0][0], x[0][2 * i + 1] + e[0][1]), fmaxf(x[1][2 * i] + e[1][0], x[1][2 * i + 1] + e[1][1]));
-#pragma unroll
-        for (int z = 1; z < 4; z *= 2) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
-          tv = fmaxf(tv, __shfl_xor_sync(0xffffffffu, tv, z));
-        }
-        if (top > m[i] + kLag8) {  // a row goes by its own scores alone
-          l[i] *= fast_exp2(m[i] - top);
-          m[i] = top;
-        }
-        float f = 1.f;
-        if (tv > mv[i] + kLag8) {
-          f = fast_exp2(mv[i] - tv);
-          mv[i] = tv;
-        }
-#pragma unroll
-        for (int j = 0; j < kCols; ++j) {
-          o[j][2 * i] *= f;
-          o[j][2 * i + 1] *= f;
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float rm = m[i] == -INFINITY ? 0.f : m[i], rv = mv[i] == -INFINITY ? 0.f : mv[i] - kRaise;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          float& s = x[k][2 * i + z];
-          l[i] += fast_exp2(s - rm);
-          s = fast_exp2(s + e[k][z] - rv);
+        for (int i = 0; i < 2; ++i) grows |= x[t][2 * k + i] > m[t][i] + kLag8 || x[t][2 * k + i] + e[k] > mv[t][i] + kLag8;
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = fmaxf(x[t][i], x[t][2 + i]), tv = fmaxf(x[t][i] + e[0], x[t][2 + i] + e[1]);
+#pragma unroll
+          for (int z = 4; z < 32; z *= 2) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
+            tv = fmaxf(tv, __shfl_xor_sync(0xffffffffu, tv, z));
+          }
+          if (top > m[t][i] + kLag8) {  // a row goes by its own scores alone
+            l[t][i] *= fast_exp2(m[t][i] - top);
+            m[t][i] = top;
+          }
+          float f = 1.f;
+          if (tv > mv[t][i] + kLag8) {
+            f = fast_exp2(mv[t][i] - tv);
+            mv[t][i] = tv;
+          }
+#pragma unroll
+          for (int j = 0; j < kCols / 2; ++j) {
+            o[t][j][i] *= f;
+            o[t][j][2 + i] *= f;
+          }
         }
     }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float rm = m[t][i] == -INFINITY ? 0.f : m[t][i], rv = mv[t][i] == -INFINITY ? 0.f : mv[t][i] - kRaise;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float& s = x[t][2 * k + i];
+          l[t][i] += fast_exp2(s - rm);
+          s = fast_exp2(s + e[k] - rv);
+        }
+      }
   };
 
   // ------------------------------------------------ the drafted tokens
   if (split == a.splits - 1) {
-    uint32_t seen[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int token = (r0 + g + 8 * i) / a.group;
-      seen[i][0] = seen[i][1] = seen[i][2] = seen[i][3] = 0u;
-      if (real[i]) ancestor_bits(parents, token, seen[i]);
-    }
     const T* const kn = static_cast<const T*>(a.k_new) + b * a.n_b + kvh * a.n_h;
     const T* const vn = static_cast<const T*>(a.v_new) + b * a.n_b + kvh * a.n_h;
     bool bad = false;
 #pragma unroll 1
     for (int k0 = stream * 16; k0 < a.tokens; k0 += streams * 16) {
-      float x[2][4] = {};
+      float x[NT][4] = {};
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        uint32_t q[kParts][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (real[i] && entry(s) < a.d) y = four(qp[i] + entry(s));
-          uint32_t p[kParts];
-          bf16_parts(y.x, y.y, p);
-#pragma unroll
-          for (int z = 0; z < kParts; ++z) q[z][i] = p[z];
-          bf16_parts(y.z, y.w, p);
-#pragma unroll
-          for (int z = 0; z < kParts; ++z) q[z][2 + i] = p[z];
-        }
+        uint32_t ka[kParts][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int key = k0 + 8 * k + g;
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
           if (key < a.tokens && entry(s) < a.d) y = four(kn + key * a.n_t + entry(s));
-          uint32_t p0[kParts], p1[kParts];
-          bf16_parts(y.x, y.y, p0);
-          bf16_parts(y.z, y.w, p1);
+          uint32_t p[kParts];
+          bf16_parts(y.x, y.y, p);
+#pragma unroll
+          for (int z = 0; z < kParts; ++z) ka[z][k] = p[z];
+          bf16_parts(y.z, y.w, p);
+#pragma unroll
+          for (int z = 0; z < kParts; ++z) ka[z][2 + k] = p[z];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          bool real;
+          const T* const qp = query(8 * t + g, real);
+          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (real && entry(s) < a.d) y = four(qp + entry(s));
+          uint32_t q0[kParts], q1[kParts];
+          bf16_parts(y.x, y.y, q0);
+          bf16_parts(y.z, y.w, q1);
 #pragma unroll
           for (int sum = kParts - 1; sum >= 0; --sum)  // the smallest products first
 #pragma unroll
-            for (int z = 0; z <= sum; ++z) mma_b16(x[k], q[z], p0[sum - z], p1[sum - z]);
+            for (int z = 0; z <= sum; ++z) mma_b16(x[t], ka[z], q0[sum - z], q1[sum - z]);
         }
       }
-      if constexpr (kF32) {
-        // an infinity's product with a part that is zero is no part of its product
+      const float none[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = k0 + 8 * k + 2 * t4 + (i & 1);
-            if (fabsf(x[k][i]) < INFINITY || !real[i >> 1] || key >= a.tokens) continue;
-            float y = 0.f;
-            for (int c = 0; c < a.d; ++c) y = fmaf(qp[i >> 1][c], kn[key * a.n_t + c], y);
-            x[k][i] = y;
-          }
-      }
-      const float none[2][2] = {};
-      const int word = k0 >> 5, first = k0 & 31;
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t (&w)[4] = seen[i >> 1];
+        for (int i = 0; i < 2; ++i) {
+          const int r = 8 * t + 2 * t4 + i;
+          bool real;
+          const T* const qp = query(r, real);
+          uint32_t w[4] = {0u, 0u, 0u, 0u};
+          if (real) ancestor_bits(parents, (r0 + r) / a.group, w);
+          const int word = k0 >> 5;
           const uint32_t bits = word == 0 ? w[0] : word == 1 ? w[1] : word == 2 ? w[2] : w[3];
-          x[k][i] = (bits >> (first + 8 * k + 2 * t4 + (i & 1))) & 1u ? x[k][i] * (a.scale * kLog2e) : -INFINITY;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int key = k0 + 8 * k + g;
+            float& y = x[t][2 * k + i];
+            // an infinity's product with a part that is zero is no part of its product
+            if (kF32 && !(fabsf(y) < INFINITY) && real && key < a.tokens) {
+              y = 0.f;
+              for (int c = 0; c < a.d; ++c) y = fmaf(to_f32(qp[c]), to_f32(kn[key * a.n_t + c]), y);
+            }
+            y = (bits >> (key & 31)) & 1u ? y * (a.scale * kLog2e) : -INFINITY;
+          }
         }
       weigh(x, none);
-      uint32_t p[kF32 ? 3 : 2][4];
+      uint32_t p[NT][kPParts][2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t y[kF32 ? 3 : 2];
-        bf16_parts(x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1], y);
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int z = 0; z < (kF32 ? 3 : 2); ++z) p[z][i] = y[z];
-      }
+        for (int k = 0; k < 2; ++k) {
+          uint32_t y[kPParts];
+          bf16_parts(x[t][2 * k], x[t][2 * k + 1], y);
 #pragma unroll
-      for (int j = 0; j < kCols; j += 4) {
+          for (int z = 0; z < kPParts; ++z) p[t][z][k] = transpose(y[z]);
+        }
+#pragma unroll
+      for (int c = 0; c < kCols; c += 4) {
         float v[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = k0 + 2 * t4 + (i & 1) + 8 * (i >> 1), c = g * kCols + j;
+          const int key = k0 + 2 * t4 + (i & 1) + 8 * (i >> 1);
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
           // an absent token's v is left out; weights of 0 must meet no infinity, which is put in at the end
-          if (key < a.tokens && c < a.d && (!parents || parents[key] >= -1)) y = four(vn + key * a.n_t + c);
+          if (key < a.tokens && g * kCols + c < a.d && (!parents || parents[key] >= -1)) y = four(vn + key * a.n_t + g * kCols + c);
           v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
 #pragma unroll
           for (int z = 0; z < 4; ++z)
@@ -307,19 +329,21 @@ __global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __gr
             }
         }
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          uint32_t v0[kParts], v1[kParts];
-          bf16_parts(v[0][z], v[1][z], v0);
-          bf16_parts(v[2][z], v[3][z], v1);
-          if constexpr (kF32) {
+        for (int z = 0; z < 4; z += 2) {
+          uint32_t va[kParts][4];
 #pragma unroll
-            for (int sum = 2; sum >= 0; --sum)
+          for (int i = 0; i < 4; ++i) {  // keys 2 t4, 2 t4 + 1 (i < 2) or 8 more, entries z, z + 1
+            uint32_t y[kParts];
+            bf16_parts(v[2 * (i >> 1)][z + (i & 1)], v[2 * (i >> 1) + 1][z + (i & 1)], y);
 #pragma unroll
-              for (int y = 0; y <= sum; ++y) mma_b16(o[j + z], p[y], v0[sum - y], v1[sum - y]);
-          } else {
-            mma_b16(o[j + z], p[1], v0[0], v1[0]);
-            mma_b16(o[j + z], p[0], v0[0], v1[0]);
+            for (int q = 0; q < kParts; ++q) va[q][i] = y[q];
           }
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int sum = (kF32 ? 2 : 1); sum >= 0; --sum)
+#pragma unroll
+              for (int q = 0; q < kParts && q <= sum; ++q) mma_b16(o[t][(c + z) / 2], va[q], p[t][sum - q][0], p[t][sum - q][1]);
         }
       }
     }
@@ -391,62 +415,60 @@ __global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __gr
   auto meet = [&](const Found& f, int w, int h, const Keys& x) {
     const int left = n - w * kWindow - 16 * h;
     if (left <= 0) return;
-    float s[2][4] = {};
+    float s[NT][4] = {};
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int c = 0; c < DC; ++c) {
+      const uint32_t k0[4] = {x.k[0][c].x, x.k[0][c].y, x.k[0][c].z, x.k[0][c].w};
+      const uint32_t k1[4] = {x.k[1][c].x, x.k[1][c].y, x.k[1][c].z, x.k[1][c].w};
 #pragma unroll
-      for (int c = 0; c < DC; ++c) {
-        const uint32_t words[4] = {x.k[k][c].x, x.k[k][c].y, x.k[k][c].z, x.k[k][c].w};
+      for (int z = 0; z < 4; ++z) {
+        uint32_t ka[4];
+        e4m3_pairs(k0[z], ka[0], ka[2]);
+        e4m3_pairs(k1[z], ka[1], ka[3]);
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const uint32_t b0 = e4m3_pair(words[z]), b1 = e4m3_pair(words[z] >> 16);
-          if constexpr (kF32) mma_f16(s[k], ql[4 * c + z], b0, b1);
-          mma_f16(s[k], qh[4 * c + z], b0, b1);
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (kF32) mma_f16(s[t], ka, ql[t][4 * c + z][0], ql[t][4 * c + z][1]);
+          mma_f16(s[t], ka, qh[t][4 * c + z][0], qh[t][4 * c + z][1]);
         }
       }
-    float e[2][2];
-    float ks = 0.f, ve = 0.f;
-    if (FAST) {
-      ks = __shfl_sync(0xffffffffu, f.ks, 16 * h);
-      ve = __shfl_sync(0xffffffffu, f.ve, 16 * h);
     }
+    float e[2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 2; ++k) {
+      const int key = 8 * k + g, from = 16 * h + (FAST ? 0 : key);
+      const float ks = __shfl_sync(0xffffffffu, f.ks, from), ve = __shfl_sync(0xffffffffu, f.ve, from);
+      e[k] = key < left ? ve : 0.f;
 #pragma unroll
-      for (int z = 0; z < 2; ++z) {
-        const int key = 8 * k + 2 * t4 + z;
-        if (!FAST) {
-          ks = __shfl_sync(0xffffffffu, f.ks, 16 * h + key);
-          ve = __shfl_sync(0xffffffffu, f.ve, 16 * h + key);
-        }
-        e[k][z] = key < left ? ve : 0.f;
-        s[k][z] = key < left ? s[k][z] * factor[0] * ks : -INFINITY;
-        s[k][2 + z] = key < left ? s[k][2 + z] * factor[1] * ks : -INFINITY;
-      }
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[t][2 * k + i] = key < left ? s[t][2 * k + i] * factor[t][i] * ks : -INFINITY;
+    }
     weigh(s, e);
-    uint32_t p[4], pl[4];
+    uint32_t p[NT][2], pl[NT][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float lo = s[i >> 1][2 * (i & 1)], hi = s[i >> 1][2 * (i & 1) + 1];
-      p[i] = half_pair(lo, hi);
-      if constexpr (kF32) {
-        const float2 r = rest_half(p[i], lo, hi);
-        pl[i] = half_pair(r.x, r.y);
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t y = half_pair(s[t][2 * k], s[t][2 * k + 1]);
+        p[t][k] = transpose(y);
+        if constexpr (kF32) {
+          const float2 r = rest_half(y, s[t][2 * k], s[t][2 * k + 1]);
+          pl[t][k] = transpose(half_pair(r.x, r.y));
+        }
       }
-    }
     const uint32_t vw[4][4] = {{x.v[0].x, x.v[0].y, x.v[0].z, x.v[0].w}, {x.v[1].x, x.v[1].y, x.v[1].z, x.v[1].w},
                                {x.v[2].x, x.v[2].y, x.v[2].z, x.v[2].w}, {x.v[3].x, x.v[3].y, x.v[3].z, x.v[3].w}};
 #pragma unroll
     for (int z = 0; z < kCols / 4; ++z)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const uint32_t u0 = __byte_perm(vw[0][z], vw[1][z], y ? 0x7362 : 0x5140), u1 = __byte_perm(vw[2][z], vw[3][z], y ? 0x7362 : 0x5140);
+        uint32_t va[4];
+        e4m3_pairs(__byte_perm(vw[0][z], vw[1][z], y ? 0x7362 : 0x5140), va[0], va[1]);
+        e4m3_pairs(__byte_perm(vw[2][z], vw[3][z], y ? 0x7362 : 0x5140), va[2], va[3]);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t b0 = e4m3_pair(q ? u0 >> 16 : u0), b1 = e4m3_pair(q ? u1 >> 16 : u1);
-          float (&to)[4] = o[4 * z + 2 * y + q];
-          if constexpr (kF32) mma_f16(to, pl, b0, b1);
-          mma_f16(to, p, b0, b1);
+        for (int t = 0; t < NT; ++t) {
+          if constexpr (kF32) mma_f16(o[t][2 * z + y], va, pl[t][0], pl[t][1]);
+          mma_f16(o[t][2 * z + y], va, p[t][0], p[t][1]);
         }
       }
   };
@@ -471,29 +493,27 @@ __global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __gr
   }
 
   // ------------------------------------------------ the warps' (max, sum, O), in their order
-  const int d = a.d, all = args.tiles * 16;  // the block's rows
+  const int d = a.d, all = args.tiles * kRowsW;          // the block's rows
   float* const ro = joined;                              // [stream][row][d]
   float* const rml = ro + (size_t)streams * all * d;     // [stream][row][2]
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    const int r = stream * all + tile * 16 + g + 8 * i;
-    if (t4 == 0) {
-      rml[2 * r] = m[i];
-      rml[2 * r + 1] = l[i];
-    }
-    const float f = mv[i] == -INFINITY ? 1.f : fast_exp2(mv[i] - kRaise - m[i]);  // O's reference becomes the sums'
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int z = 0; z < 2; ++z) {  // entries c .. c + kCols - 1
-      const int c = (2 * t4 + z) * kCols;
-      if (c >= d) continue;
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int j = 0; j < kCols; j += 4)
-        *reinterpret_cast<float4*>(ro + (size_t)r * d + c + j) =
-            make_float4(o[j][2 * i + z] * f, o[j + 1][2 * i + z] * f, o[j + 2][2 * i + z] * f, o[j + 3][2 * i + z] * f);
+      for (int z = 4; z < 32; z *= 2) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], z);
+      const int r = stream * all + tile * kRowsW + 8 * t + 2 * t4 + i;
+      if (g == 0) {
+        rml[2 * r] = m[t][i];
+        rml[2 * r + 1] = l[t][i];
+      }
+      const float f = mv[t][i] == -INFINITY ? 1.f : fast_exp2(mv[t][i] - kRaise - m[t][i]);  // O's reference becomes the sums'
+      if (g * kCols < d)
+#pragma unroll
+        for (int j = 0; j < kCols / 2; j += 2)
+          *reinterpret_cast<float4*>(ro + (size_t)r * d + g * kCols + 2 * j) =
+              make_float4(o[t][j][i] * f, o[t][j][2 + i] * f, o[t][j + 1][i] * f, o[t][j + 1][2 + i] * f);
     }
-  }
   __syncthreads();
   const int quads = d / 4;
   for (int i = tid; i < all * quads; i += kThreads8) {
@@ -545,25 +565,44 @@ __global__ void __launch_bounds__(kThreads8, 2) attention_8bit_kernel(const __gr
 
 // ------------------------------------------------------------------ host
 
-// Tiles of 16 query rows that a block's warps share: as many as there are, up to its warps.
-int tiles_8bit(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : kWarps8; }
+// How a block's warps share query rows and keys: tiles of 8 rows (16 from 9 rows on), as many as there are, up to
+// the warps, which share the keys if there are fewer.
+struct Shape8 {
+  int nt, tiles, row_blocks, streams;
+};
+Shape8 shape_8bit(int64_t rows) {
+  Shape8 s;
+  s.nt = rows <= 8 ? 1 : 2;
+  s.tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : kWarps8;
+  s.row_blocks = (int)((rows + 8 * s.nt * s.tiles - 1) / (8 * s.nt * s.tiles));
+  s.streams = kWarps8 / s.tiles;
+  return s;
+}
 
 // Blocks that share a sequence's keys, of at least two windows to a warp, as long as there are no
-// more than four for each SM where all sequences are as long as the tables allow.
+// more than kRoom8 for each SM where all sequences are as long as the tables allow.
+#ifndef KROOM8
+#define KROOM8 4
+#endif
+#ifndef KLEAST8
+#define KLEAST8 2
+#endif
+constexpr int kRoom8 = KROOM8, kLeast8 = KLEAST8;
 int64_t splits_8bit(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity) {
-  const int64_t tiles = tiles_8bit(rows), row_blocks = (rows + 16 * tiles - 1) / (16 * tiles), streams = kWarps8 / tiles;
+  const Shape8 s = shape_8bit(rows);
   const int64_t windows = std::max<int64_t>((capacity + kWindow - 1) / kWindow, 1);
-  const int64_t room = std::max<int64_t>(4 * (int64_t)sm_count() / (batch * kv_heads * row_blocks), 1);
-  return std::max<int64_t>(1, std::min({room, (windows + 2 * streams - 1) / (2 * streams), (int64_t)kMaxSplits}));
+  const int64_t room = std::max<int64_t>(kRoom8 * (int64_t)sm_count() / (batch * kv_heads * s.row_blocks), 1);
+  return std::max<int64_t>(1, std::min({room, (windows + kLeast8 * s.streams - 1) / (kLeast8 * s.streams), (int64_t)kMaxSplits}));
 }
 
 template <typename T, int DC>
-int launch_8bit(const Bits8Args& a, dim3 grid, bool fast, cudaStream_t st) {
+int launch_8bit(const Bits8Args& a, int nt, dim3 grid, bool fast, cudaStream_t st) {
   const char* op = "nkl_attention_tree_8bit";
-  const size_t smem = (size_t)kWarps8 * 16 * (a.t.d + 2) * 4;
+  const size_t smem = (size_t)kWarps8 * 8 * nt * (a.t.d + 2) * 4;
   static_assert((size_t)kWarps8 * 16 * (128 + 2) * 4 <= 48 * 1024, "no attribute needed");
-  return fast ? launch_pdl(attention_8bit_kernel<T, DC, true>, grid, dim3(kThreads8), smem, st, op, a)
-              : launch_pdl(attention_8bit_kernel<T, DC, false>, grid, dim3(kThreads8), smem, st, op, a);
+  auto go = [&](auto* kernel) { return launch_pdl(kernel, grid, dim3(kThreads8), smem, st, op, a); };
+  if (nt == 1) return fast ? go(attention_8bit_kernel<T, DC, true, 1>) : go(attention_8bit_kernel<T, DC, false, 1>);
+  return fast ? go(attention_8bit_kernel<T, DC, true, 2>) : go(attention_8bit_kernel<T, DC, false, 2>);
 }
 
 }  // namespace
