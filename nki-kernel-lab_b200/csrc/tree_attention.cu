@@ -542,6 +542,11 @@ int launch_combine(const TreeArgs& a, int dtype, cudaStream_t st, const char* op
   return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 1, BASE2>, 4) : join(tree_combine_kernel<bf16, 1, BASE2>, 4);
 }
 
+#ifndef KTCROWS
+#define KTCROWS 16
+#endif
+constexpr int kTcRows = KTCROWS;
+
 size_t split_bytes(int64_t splits, int64_t batch, int64_t heads, int64_t tokens, int64_t d) {
   return splits > 1 ? ((size_t)splits * batch * heads * tokens * (d + 2) * 4 + 255) & ~size_t(255) : 0;
 }
@@ -685,8 +690,9 @@ extern "C" size_t nkl_attention_tree_8bit_workspace_size(int64_t batch, int64_t 
   if (!valid_dtype(dtype) || !tree_sizes_ok(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages) ||
       batch == 0 || tokens == 0)
     return 0;
-  return split_bytes(splits_8bit(batch, kv_heads, tokens * (heads / kv_heads), page_size * max_pages), batch, heads, tokens,
-                     head_dim);
+  const TcPlan p = tc_plan(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages, dtype);
+  return std::max(p.on ? p.bytes : 0, split_bytes(splits_8bit(batch, kv_heads, tokens * (heads / kv_heads), page_size * max_pages),
+                                                  batch, heads, tokens, head_dim));
 }
 
 extern "C" int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
@@ -715,6 +721,22 @@ extern "C" int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, 
   a.per_page = (int)(page_size / block);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t rows = tokens * a.t.group;
+  const TcPlan p = tc_plan(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages, dtype);
+  bool tc = p.on && rows > kTcRows && scale > 0.f && scale < INFINITY;
+  for (int i = 0; i < 9; ++i) tc = tc && (n[i] == 1 || (s[i] > 0 && s[i] < (1LL << 38)));
+  if (tc) {
+    if (p.bytes) {
+      if (!workspace || workspace_bytes < p.bytes) return fail(NKL_ERR_ARG, "%s: workspace too small", op);
+      if (!is_aligned(workspace, 256)) return fail(NKL_ERR_ALIGN, "%s: workspace not 256-byte aligned", op);
+    }
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    int64_t* const steps[9] = {&a.t.q_b, &a.t.q_t, &a.t.q_h, &a.t.n_b, &a.t.n_t, &a.t.n_h, &a.t.c_p, &a.t.c_h, &a.t.c_s};
+    for (int i = 0; i < 9; ++i)
+      if (n[i] == 1) *steps[i] = head_dim;
+    const TcScales sc = {k_scales, v_scales, (int)block};
+    if (head_dim == 128) return p.nq == 1 ? tc_launch<128, 1, true>(a.t, p, ws, st, sc) : tc_launch<128, 2, true>(a.t, p, ws, st, sc);
+    return p.nq == 1 ? tc_launch<64, 1, true>(a.t, p, ws, st, sc) : tc_launch<64, 2, true>(a.t, p, ws, st, sc);
+  }
   const Shape8 shape = shape_8bit(rows);
   a.tiles = shape.tiles;
   a.t.row_blocks = shape.row_blocks;

@@ -56,7 +56,8 @@ using namespace sm100;
 __device__ unsigned int g_tree_dev_error = 0;
 
 constexpr int kTile = 128;
-constexpr int kTcThreads = 384;
+constexpr int kTcThreads = 384, kTcThreads8 = 512;
+constexpr int kConvertWarp = 12, kConverters = 4;  // of a cache in 8 bits
 constexpr int kKeyWarp = 8, kMmaWarp = 9, kValueWarp = 10, kMendWarp = 11;
 constexpr int kFewDrafts = 16;   // so many drafted tokens can share the last cached tile
 constexpr int kWhole = 4;        // segments of up to so many tiles are not cut: a cut costs kExtra
@@ -89,6 +90,8 @@ struct TcArgs {
   int boxes_per_page, log_bpp;  // log_bpp < 0: no power of two
   unsigned long long bpp_magic;  // ceil(2^36 / boxes_per_page)
   float scale_log2;
+  const uint8_t *k_scales, *v_scales;  // of a cache in 8 bits
+  int block, per_page;                 // positions of a block of theirs, blocks of a page
 };
 
 __device__ __forceinline__ int tree_len(const TcArgs& a, int b) {
@@ -124,14 +127,19 @@ struct Piece {
   bool shares;  // the drafted tokens are in the last cached tile
 };
 
-template <int D, int NQ>
+template <int D, int NQ, bool C8>
 struct TreeSmem {
   static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kRingK = D == 128 ? 3 : 5;
-  static constexpr int kRingV = (D == 128 ? 4 : 6) - NQ;
+  static constexpr int kRawBytes = C8 ? kTile * D : 0;
+  static constexpr int kRingK = C8 ? 2 : D == 128 ? 3 : 5;
+  static constexpr int kRingV = C8 ? 2 : (D == 128 ? 4 : 6) - NQ;
+  static constexpr int kRaw = C8 ? (D == 128 ? 3 - NQ : 4) : 1;  // tiles of 8-bit keys and values
   uint8_t q[NQ][kTileBytes];
   uint8_t k[kRingK][kTileBytes];
   uint8_t v[kRingV][kTileBytes];
+  uint8_t raw[kRaw][C8 ? 2 : 1][C8 ? kRawBytes : 16];
+  uint8_t powers[kRaw][2][C8 ? kTile : 4];  // of the rows, as they are in the cache
+  uint64_t raw_full[kRaw], raw_empty[kRaw];
   uint64_t q_full, q_empty;
   uint64_t k_full[kRingK], k_empty[kRingK], k_land[kRingK];  // land: the copies of a tile that is mended before it is full
   uint64_t v_full[kRingV], v_empty[kRingV], v_land[kRingV];
@@ -139,20 +147,38 @@ struct TreeSmem {
   uint64_t o_free[2];
   uint64_t x_full;
   uint64_t mma_done;
-  float xm[2][kTile], xl[2][kTile];  // NQ = 1: the groups' maxima and sums
+  float xm[2][NQ == 1 ? kTile : 1], xl[2][NQ == 1 ? kTile : 1];  // NQ = 1: the groups' maxima and sums
   // Drafted tokens whose v holds infinities or NaN, of the last pieces: products wait for the
   // end of the piece before, so the mending warp is at most kRingV pieces ahead of a reader.
   uint32_t bad[8][4];
   uint32_t tmem_base;
   int abort;
 };
-template <int D, int NQ>
+template <int D, int NQ, bool C8>
 constexpr bool tiles_aligned() {
-  using S = TreeSmem<D, NQ>;
-  return offsetof(S, k) % 1024 == 0 && offsetof(S, v) % 1024 == 0;
+  using S = TreeSmem<D, NQ, C8>;
+  return offsetof(S, k) % 1024 == 0 && offsetof(S, v) % 1024 == 0 && (!C8 || offsetof(S, raw) % 1024 == 0);
 }
-static_assert(tiles_aligned<128, 1>() && tiles_aligned<128, 2>() && tiles_aligned<64, 1>() && tiles_aligned<64, 2>(),
+static_assert(tiles_aligned<128, 1, false>() && tiles_aligned<128, 2, false>() && tiles_aligned<64, 1, false>() &&
+                  tiles_aligned<64, 2, false>() && tiles_aligned<128, 1, true>() && tiles_aligned<128, 2, true>() &&
+                  tiles_aligned<64, 1, true>() && tiles_aligned<64, 2, true>(),
               "swizzled tiles are 1024-byte aligned");
+
+// Two e4m3 numbers of w (the bytes that `select` picks into the upper halves) as bf16, exactly: exponent and
+// mantissa moved into place make 2^-120 of the number, and the row's factor holds 2^120 besides its power of two.
+__device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, uint32_t select, uint32_t factor) {
+  const uint32_t x = __byte_perm(w, 0u, select);
+  const uint32_t y = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&factor));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// A row's factors for the power of two with this code, in bf16: 2^120 2^e, or 2^127 and the rest above that.
+__device__ __forceinline__ uint32_t factors_of(int code) {
+  if (code == 255) return 0x3f807fc0u;  // NaN
+  const int e = code - 127 + 120;       // -7 .. 247
+  const uint32_t first = (uint32_t)min(e, 127), second = (uint32_t)max(e - 127, 0);
+  return ((second + 127u) << 23) | ((first + 127u) << 7);
+}
 
 __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
@@ -235,8 +261,11 @@ __device__ __forceinline__ Walk tree_plan(const TcArgs& a) {
   return w;
 }
 
-template <int D, int NQ>
-__global__ void __launch_bounds__(kTcThreads, 1)
+// C8: the cache holds e4m3 numbers with powers of two for blocks of rows. The TMA warps then fetch its tiles as
+// they are, warp 11 looks up their rows' powers of two, and warps 12-15 (32 rows each) turn them into the bf16
+// tiles that the products read, which is exact, and put the drafted tokens in place.
+template <int D, int NQ, bool C8>
+__global__ void __launch_bounds__(C8 ? kTcThreads8 : kTcThreads, 1)
 tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kn,
                          const __grid_constant__ CUtensorMap map_vn, const __grid_constant__ CUtensorMap map_kc,
                          const __grid_constant__ CUtensorMap map_vc, const __grid_constant__ TcArgs a) {
@@ -246,7 +275,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     return;
   }
   pdl_launch_dependents();
-  using Smem = TreeSmem<D, NQ>;
+  using Smem = TreeSmem<D, NQ, C8>;
   Smem& s = *reinterpret_cast<Smem*>(smem_raw);
   constexpr int kRingK = Smem::kRingK, kRingV = Smem::kRingV;
   constexpr uint32_t kTileBytes = Smem::kTileBytes;
@@ -260,13 +289,19 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, 1);
     mbar_init(&s.q_empty, 1);
+    if constexpr (C8) {
+      for (int i = 0; i < Smem::kRaw; ++i) {
+        mbar_init(&s.raw_full[i], 3);  // both TMA warps and the one of the powers
+        mbar_init(&s.raw_empty[i], kConverters);
+      }
+    }
     for (int i = 0; i < kRingK; ++i) {
-      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.k_full[i], C8 ? kConverters : 1);
       mbar_init(&s.k_empty[i], 1);
       mbar_init(&s.k_land[i], 1);
     }
     for (int i = 0; i < kRingV; ++i) {
-      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_full[i], C8 ? kConverters : 1);
       mbar_init(&s.v_empty[i], 1);
       mbar_init(&s.v_land[i], 1);
     }
@@ -301,7 +336,230 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   Walk w = tree_plan(a);
   if (a.ws_start && threadIdx.x == 0) a.ws_start[blockIdx.x] = make_int4(w.b, w.hm, w.t, 0);
 
-  if (warp == kKeyWarp || warp == kValueWarp) {
+  // C8: 2 x 168 + 2 x 80 registers a thread, of 4 x 128
+  auto fewer_registers = [] { if constexpr (C8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::: "memory"); };
+  if (C8 && (warp == kKeyWarp || warp == kValueWarp)) {
+    // ------------------------------------------------ TMA, 8 bits
+    fewer_registers();
+    const bool keys = warp == kKeyWarp;
+    const CUtensorMap* const cached = keys ? &map_kc : &map_vc;
+    const int per_tile = 1 << a.log_bpt;
+    uint32_t st = 0, par = 0, uc = 0, used = 0u;
+    bool ok = true;
+    Piece p = {};
+    auto look_up = [&](int box, int& page, int& slot) {
+      page = slot = 0;
+      if (box * a.box < p.len) {
+        const int pi = a.log_bpp >= 0 ? box >> a.log_bpp : (int)(((uint32_t)box * a.bpp_magic) >> 36);
+        slot = (box - pi * a.boxes_per_page) * a.box;
+        page = a.tables[(int64_t)p.b * a.max_pages + pi];
+        if ((uint32_t)page >= (uint32_t)a.pages) page = a.pages;  // outside: read as zeros
+      }
+    };
+    while (ok && next_piece(a, w, p)) {
+      int first = p.t0 * per_tile, page, slot, next_page, next_slot;
+      look_up(first + lane, page, slot);
+      if (keys) {
+        if (!tree_wait(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&s.q_full, (uint32_t)(NQ * D * 2 * a.tt * a.group));
+#pragma unroll
+          for (int i = 0; i < NQ * kSub; ++i)
+            tma_load_4d(s.q[i / kSub] + (i % kSub) * (kTile * 128), &map_q, &s.q_full, (i % kSub) * 64,
+                        p.kvh * a.group, (p.mb * NQ + i / kSub) * a.tt, p.b);
+        }
+        __syncwarp();
+      }
+      ++uc;
+      look_up(first + 32 + lane, next_page, next_slot);
+      for (int t = p.t0; t < p.t0 + p.n && t * kTile < p.len; ++t) {
+        const int boxes = (min(kTile, p.len - t * kTile) + a.box - 1) / a.box;
+        const int at = t * per_tile - first;
+        if (!tree_wait(&s.raw_empty[st], par ^ 1u, &s.abort, 11)) { ok = false; break; }
+        used |= 1u << st;
+        if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[st], (uint32_t)(boxes * a.box * D));
+        uint8_t* const to = s.raw[st][keys ? 0 : C8 ? 1 : 0];
+        for (int i = 0; i < boxes; ++i) {
+          const int pg = __shfl_sync(0xffffffffu, page, at + i), sl = __shfl_sync(0xffffffffu, slot, at + i);
+          if (lane == 0) tma_load_4d(to + i * a.box * D, cached, &s.raw_full[st], 0, sl, p.kvh, pg);
+        }
+        __syncwarp();
+        if (at + per_tile == 32) {
+          first += 32;
+          page = next_page;
+          slot = next_slot;
+          look_up(first + 32 + lane, next_page, next_slot);
+        }
+        if (++st == Smem::kRaw) { st = 0; par ^= 1u; }
+      }
+    }
+    if (!ok && lane == 0) {  // let issued copies land before shared memory is released (or the time run out)
+      const uint64_t begin = globaltimer();
+      if (keys && uc > 0)
+        while (!mbar_try_wait(&s.q_full, (uc - 1) & 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
+      for (uint32_t i = 0; i < (uint32_t)Smem::kRaw; ++i)
+        if ((used >> i) & 1u)
+          while (!mbar_try_wait(&s.raw_full[i], i < st ? par : par ^ 1u) && globaltimer() - begin < kWaitTimeoutNs) {}
+    }
+    __syncwarp();
+  } else if (C8 && warp == kMendWarp) {
+    // ------------------------------------------------ the rows' powers of two, 8 bits
+    fewer_registers();
+    uint32_t st = 0, par = 0;
+    bool ok = true;
+    Piece p;
+    while (ok && next_piece(a, w, p)) {
+      const int end = min(p.t0 + p.n, (p.len + kTile - 1) / kTile);
+      auto find = [&](int t, int (&at)[4]) {  // where the powers of this lane's four rows of tile t are; -1: nowhere
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = t * kTile + 32 * i + lane;
+          at[i] = -1;
+          if (t >= end || key >= p.len) continue;
+          const int pi = key / a.page, pg = a.tables[(int64_t)p.b * a.max_pages + pi];
+          if ((uint32_t)pg < (uint32_t)a.pages) at[i] = pg;
+        }
+      };
+      int page[4], next[4];
+      find(p.t0, page);
+      for (int t = p.t0; t < end; ++t) {
+        find(t + 1, next);
+        uint32_t ks[4], vs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = t * kTile + 32 * i + lane;
+          ks[i] = vs[i] = 127u;
+          if (page[i] >= 0) {
+            const int64_t at = ((int64_t)page[i] * a.kv_heads + p.kvh) * a.per_page + (key % a.page) / a.block;
+            ks[i] = a.k_scales[at];
+            vs[i] = a.v_scales[at];
+          }
+          page[i] = next[i];
+        }
+        if (!tree_wait(&s.raw_empty[st], par ^ 1u, &s.abort, 12)) { ok = false; break; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s.powers[st][0][C8 ? 32 * i + lane : 0] = (uint8_t)ks[i];
+          s.powers[st][1][C8 ? 32 * i + lane : 0] = (uint8_t)vs[i];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.raw_full[st]);
+        if (++st == Smem::kRaw) { st = 0; par ^= 1u; }
+      }
+    }
+  } else if (C8 && warp >= kConvertWarp) {
+    // ------------------------------------------------ 8 bits to bf16, 32 rows of each tile
+    fewer_registers();
+    const int cw = warp - kConvertWarp;
+    uint32_t st = 0, par = 0, ki = 0, k_par = 0, vi = 0, v_par = 0, uc = 0;
+    bool ok = true;
+    Piece p;
+    auto chunk = [&](uint8_t* tile, int row, int c) {  // 16 bytes of a bf16 row, where the swizzle puts them
+      return reinterpret_cast<uint4*>(tile + (c / 8) * (kTile * 128) + row * 128 + ((c ^ row) & 7) * 16);
+    };
+    // Rows [32 cw, 32 cw + 32) below `rest` of a raw tile: 8 rows at a time, D / 16 steps of 4 lanes a row.
+    auto convert = [&](const uint8_t* raw, const uint8_t* powers, uint8_t* tile, int rest) {
+      constexpr int kChunks = D / 16;  // of a raw row
+#pragma unroll 2
+      for (int r8 = 0; r8 < 32; r8 += 8) {
+        const int row = 32 * cw + r8 + (lane & 7);
+        const uint32_t f = factors_of(powers[row]);
+        const uint32_t f1 = __byte_perm(f, 0u, 0x1010), f2 = __byte_perm(f, 0u, 0x3232);
+        if (row < rest) {
+#pragma unroll
+          for (int j0 = 0; j0 < kChunks; j0 += 4) {
+            const int j = j0 + (lane >> 3);
+            // the box's swizzle: of 128 bytes, or of 64
+            const int at = D == 128 ? row * 128 + ((j ^ row) & 7) * 16 : row * 64 + ((j ^ (row >> 1)) & 3) * 16;
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + at);
+            uint32_t y[8];
+            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              y[2 * z] = bf16_of_e4m3(words[z], 0x1404, f1);
+              y[2 * z + 1] = bf16_of_e4m3(words[z], 0x3424, f1);
+            }
+            if (f2 != 0x3f803f80u) {
+#pragma unroll
+              for (int z = 0; z < 8; ++z) {
+                const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y[z]), *reinterpret_cast<const __nv_bfloat162*>(&f2));
+                y[z] = *reinterpret_cast<const uint32_t*>(&r);
+              }
+            }
+            *chunk(tile, row, 2 * j) = make_uint4(y[0], y[1], y[2], y[3]);
+            *chunk(tile, row, 2 * j + 1) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
+        }
+      }
+    };
+    while (ok && next_piece(a, w, p)) {
+      const int* const parents = a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr;
+      for (int tile = p.t0; tile < p.t0 + p.n; ++tile) {
+        const int rest = p.len - tile * kTile;  // cached rows; none: the drafted tokens' own tile
+        const bool drafts = tile == p.tiles - 1;
+        // drafted tokens are rows [d0, d0 + tokens), of which this warp has [r0, r1): all of them where they share
+        const int d0 = rest > 0 ? rest : 0;
+        const int r0 = !drafts ? 0 : rest > 0 ? (cw == 0 ? d0 : 0) : min(32 * cw, a.tokens);
+        const int r1 = !drafts ? 0 : rest > 0 ? (cw == 0 ? d0 + a.tokens : 0) : min(32 * cw + 32, a.tokens);
+        if (rest > 0 && !tree_wait(&s.raw_full[st], par, &s.abort, 43)) { ok = false; break; }
+        if (!tree_wait(&s.k_empty[ki], k_par ^ 1u, &s.abort, 44)) { ok = false; break; }
+        uint8_t* const kt = s.k[ki];
+        if (rest > 0) convert(s.raw[st][0], s.powers[st][0], kt, rest);
+        for (int x = r0 * (D / 8) + lane; x < r1 * (D / 8); x += 32) {
+          const int row = x / (D / 8), c = x % (D / 8);
+          *chunk(kt, row, c) = *reinterpret_cast<const uint4*>(a.k_new + p.b * a.n_b + (row - d0) * a.n_t + p.kvh * a.n_h + c * 8);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.k_full[ki]);
+        if (++ki == kRingK) { ki = 0; k_par ^= 1u; }
+
+        if (!tree_wait(&s.v_empty[vi], v_par ^ 1u, &s.abort, 45)) { ok = false; break; }
+        uint8_t* const vt = s.v[vi];
+        if (rest > 0) convert(s.raw[st][C8 ? 1 : 0], s.powers[st][1], vt, rest);
+        if (rest < kTile) {
+          // Rows past the end, and absent tokens, are zeros; infinities and NaN of the others are left out here and
+          // put back at the end for the rows that see them: products with P = 0 have to leave no trace of them.
+          const int filled = max(rest, 0) + (drafts ? a.tokens : 0);
+          for (int x = 32 * cw * (D / 8) + lane; x < (32 * cw + 32) * (D / 8); x += 32) {
+            const int row = x / (D / 8);
+            if (row >= filled) *chunk(vt, row, x % (D / 8)) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          uint32_t odd = 0u;  // this warp's tokens with such a value, from 32 cw on (or 0, where they share)
+          for (int x = r0 * (D / 8) + lane; x < r1 * (D / 8); x += 32) {
+            const int row = x / (D / 8), c = x % (D / 8), token = row - d0;
+            uint4 y = make_uint4(0u, 0u, 0u, 0u);
+            if (!parents || parents[token] >= -1)
+              y = *reinterpret_cast<const uint4*>(a.v_new + p.b * a.n_b + token * a.n_t + p.kvh * a.n_h + c * 8);
+            uint32_t* const z = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t hit = ((z[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;  // exponents of all ones
+              if (hit) odd |= 1u << (token & 31);
+              if (hit & 0x8000u) z[i] &= 0xffff0000u;
+              if (hit & 0x80000000u) z[i] &= 0x0000ffffu;
+            }
+            *chunk(vt, row, c) = y;
+          }
+          odd = __reduce_or_sync(0xffffffffu, odd);
+          if (drafts && lane == 0) {
+            if (rest <= 0) s.bad[uc & 7][cw] = odd;
+            else if (cw == 0) s.bad[uc & 7][0] = odd;
+            else s.bad[uc & 7][cw] = 0u;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s.v_full[vi]);
+          if (rest > 0) mbar_arrive(&s.raw_empty[st]);
+        }
+        if (++vi == kRingV) { vi = 0; v_par ^= 1u; }
+        if (rest > 0 && ++st == Smem::kRaw) { st = 0; par ^= 1u; }
+      }
+      ++uc;
+    }
+  } else if (warp == kKeyWarp || warp == kValueWarp) {
     // ------------------------------------------------ TMA
     const bool keys = warp == kKeyWarp;
     const CUtensorMap* const cached = keys ? &map_kc : &map_vc;
@@ -393,6 +651,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------ MMA
+    fewer_registers();
     if (elect_one()) {
       uint32_t uc = 0, gt = 0;
       uint32_t kt = 0, k_par = 0, vt = 0, v_par = 0;  // the rings' next places
@@ -626,6 +885,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
   } else {
     // ------------------------------------------------ softmax groups
+    if constexpr (C8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n" ::: "memory");
     const int g = warp >> 2, qd = warp & 3;
     const int r = qd * 32 + lane;  // row of the query tile == TMEM lane
     const uint32_t lane_off = (uint32_t)(qd * 32) << 16;
@@ -748,8 +1008,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       if constexpr (NQ == 1) {
         // both groups' results: this one writes half of the columns
         if (uc > 0 && !tree_wait(&s.o_free[0], (uc - 1) & 1u, &s.abort, 34)) { ok = false; break; }
-        s.xm[g][r] = m;
-        s.xl[g][r] = l;
+        s.xm[g][NQ == 1 ? r : 0] = m;
+        s.xl[g][NQ == 1 ? r : 0] = l;
         mbar_arrive(&s.x_full);
         // This group's last product first: with it all products before it are complete, so the
         // other group's barrier is at most one phase short of the one waited for (a parity says
@@ -963,9 +1223,15 @@ TcPlan tc_plan(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, i
   return p;
 }
 
-template <int D, int NQ>
-int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_t st) {
-  const char* op = "nkl_attention_tree";
+// For a cache in 8 bits: its powers of two.
+struct TcScales {
+  const void *k, *v;
+  int block;
+};
+
+template <int D, int NQ, bool C8 = false>
+int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_t st, TcScales scales = {}) {
+  const char* op = C8 ? "nkl_attention_tree_8bit" : "nkl_attention_tree";
   CUtensorMap mq, mkn, mvn, mkc, mvc;
   {
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)g.heads, (uint64_t)g.tokens, (uint64_t)g.batch};
@@ -980,7 +1246,13 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
     if (int rc = make_tensor_map_bf16(&mkn, g.k_new, 4, dims, strides, box, op)) return rc;
     if (int rc = make_tensor_map_bf16(&mvn, g.v_new, 4, dims, strides, box, op)) return rc;
   }
-  {
+  if constexpr (C8) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)g.page, (uint64_t)g.kv_heads, (uint64_t)g.pages};
+    const uint64_t strides[3] = {(uint64_t)g.c_s, (uint64_t)g.c_h, (uint64_t)g.c_p};
+    const uint32_t box[4] = {D, (uint32_t)p.box, 1, 1};
+    if (int rc = make_tensor_map_u8(&mkc, g.k_cache, 4, dims, strides, box, op)) return rc;
+    if (int rc = make_tensor_map_u8(&mvc, g.v_cache, 4, dims, strides, box, op)) return rc;
+  } else {
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)g.page, (uint64_t)g.kv_heads, (uint64_t)g.pages};
     const uint64_t strides[3] = {(uint64_t)g.c_s * 2, (uint64_t)g.c_h * 2, (uint64_t)g.c_p * 2};
     const uint32_t box[4] = {64, (uint32_t)p.box, 1, 1};
@@ -1013,19 +1285,25 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
     if (a.boxes_per_page == 1 << i) a.log_bpp = i;
   a.bpp_magic = ((1ull << 36) + a.boxes_per_page - 1) / a.boxes_per_page;
   a.scale_log2 = g.scale * kLog2e;
-  constexpr size_t smem = sizeof(TreeSmem<D, NQ>);
+  if (C8) {
+    a.k_scales = static_cast<const uint8_t*>(scales.k);
+    a.v_scales = static_cast<const uint8_t*>(scales.v);
+    a.block = scales.block;
+    a.per_page = g.page / scales.block;
+  }
+  constexpr size_t smem = sizeof(TreeSmem<D, NQ, C8>);
   static_assert(smem <= 232448, "shared memory of a block");
   static std::atomic<bool> set[64] = {};  // per device: the smem attribute is set (idempotent)
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(tree_attention_tc_kernel<D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(tree_attention_tc_kernel<D, NQ, C8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
   }
-  int rc = launch_pdl(tree_attention_tc_kernel<D, NQ>, dim3((unsigned)p.grid), dim3(kTcThreads), smem, st, op, mq, mkn,
-                      mvn, mkc, mvc, a);
+  int rc = launch_pdl(tree_attention_tc_kernel<D, NQ, C8>, dim3((unsigned)p.grid), dim3(C8 ? kTcThreads8 : kTcThreads), smem, st,
+                      op, mq, mkn, mvn, mkc, mvc, a);
   if (rc || !p.join || p.grid < 2) return rc;
   const int rows = std::min<int>(NQ == 1 ? p.tt * g.group : NQ * kTile, NQ == 1 ? g.tokens * g.group : NQ * kTile);
   return launch_pdl(tree_join_kernel<D, NQ>, dim3((unsigned)((rows + 7) / 8), (unsigned)(p.grid - 1)), dim3(2 * D), 0, st,
