@@ -111,6 +111,23 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// mbar_wait whose tries may suspend the thread (up to 2 us each) instead of returning at once, for kernels
+// with warps that need the issue slots meanwhile.
+__device__ __forceinline__ bool mbar_wait_asleep(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                                 unsigned int* dev_err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+    if (mbar_try_wait_sleep(bar, parity, 2000)) return true;
+    if (*abort) return false;
+    if (globaltimer() - t0 > kWaitTimeoutNs) {
+      *abort = 1;
+      atomicCAS(dev_err, 0u, (unsigned int)code);
+      return false;
+    }
+  }
+}
+
 // ------------------------------------------------------------------ TMA
 
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {

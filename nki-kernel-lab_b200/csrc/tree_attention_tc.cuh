@@ -164,26 +164,32 @@ static_assert(tiles_aligned<128, 1, false>() && tiles_aligned<128, 2, false>() &
                   tiles_aligned<64, 1, true>() && tiles_aligned<64, 2, true>(),
               "swizzled tiles are 1024-byte aligned");
 
-// Two e4m3 numbers of w (the bytes that `select` picks into the upper halves) as bf16, exactly: exponent and
-// mantissa moved into place make 2^-120 of the number, and the row's factor holds 2^120 besides its power of two.
+// Two e4m3 numbers of w (the bytes that `select` picks) as bf16, exactly: sign, exponent and mantissa moved into
+// place make 2^-120 of the number, and the row's factor holds 2^120 besides its power of two. The moves are
+// multiplications, so that half of the work is the multipliers' and not all the integer units'.
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, uint32_t select, uint32_t factor) {
-  const uint32_t x = __byte_perm(w, 0u, select);
-  const uint32_t y = ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
+  const uint32_t x = __byte_perm(w, 0u, select);  // 0 s eeee mmm 0 s eeee mmm
+  const uint32_t y = x * 16u + (x & 0x00800080u) * 240u;
   const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y), *reinterpret_cast<const __nv_bfloat162*>(&factor));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// A row's factors for the power of two with this code, in bf16: 2^120 2^e, or 2^127 and the rest above that.
-__device__ __forceinline__ uint32_t factors_of(int code) {
-  if (code == 255) return 0x3f807fc0u;  // NaN
-  const int e = code - 127 + 120;       // -7 .. 247
-  const uint32_t first = (uint32_t)min(e, 127), second = (uint32_t)max(e - 127, 0);
-  return ((second + 127u) << 23) | ((first + 127u) << 7);
+__device__ __forceinline__ uint32_t times(uint32_t x, uint32_t y) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// C8: the converting warps need the issue slots that polling would take (one in four of a scheduler's warps
+// converts: a tile took them 3400 to 15000 cycles beside polling warps).
+template <bool C8>
+__device__ __forceinline__ bool one_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
+  return C8 ? mbar_wait_asleep(bar, parity, abort, &g_tree_dev_error, code)
+            : mbar_wait(bar, parity, abort, &g_tree_dev_error, code);
+}
+template <bool C8>
 __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   int ok = 1;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort, &g_tree_dev_error, code) ? 1 : 0;
+  if ((threadIdx.x & 31) == 0) ok = one_wait<C8>(bar, parity, abort, code) ? 1 : 0;
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
@@ -262,8 +268,8 @@ __device__ __forceinline__ Walk tree_plan(const TcArgs& a) {
 }
 
 // C8: the cache holds e4m3 numbers with powers of two for blocks of rows. The TMA warps then fetch its tiles as
-// they are, warp 11 looks up their rows' powers of two, and warps 12-15 (32 rows each) turn them into the bf16
-// tiles that the products read, which is exact, and put the drafted tokens in place.
+// they are, warp 11 looks up their rows' powers of two, and warps 12-15 (two for the keys, two for the values) turn
+// them into the bf16 tiles that the products read, which is exact, and put the drafted tokens in place.
 template <int D, int NQ, bool C8>
 __global__ void __launch_bounds__(C8 ? kTcThreads8 : kTcThreads, 1)
 tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kn,
@@ -296,12 +302,12 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
     }
     for (int i = 0; i < kRingK; ++i) {
-      mbar_init(&s.k_full[i], C8 ? kConverters : 1);
+      mbar_init(&s.k_full[i], C8 ? kConverters / 2 : 1);
       mbar_init(&s.k_empty[i], 1);
       mbar_init(&s.k_land[i], 1);
     }
     for (int i = 0; i < kRingV; ++i) {
-      mbar_init(&s.v_full[i], C8 ? kConverters : 1);
+      mbar_init(&s.v_full[i], C8 ? kConverters / 2 : 1);
       mbar_init(&s.v_empty[i], 1);
       mbar_init(&s.v_land[i], 1);
     }
@@ -360,7 +366,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       int first = p.t0 * per_tile, page, slot, next_page, next_slot;
       look_up(first + lane, page, slot);
       if (keys) {
-        if (!tree_wait(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
+        if (!tree_wait<C8>(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
         if (lane == 0) {
           mbar_arrive_expect_tx(&s.q_full, (uint32_t)(NQ * D * 2 * a.tt * a.group));
 #pragma unroll
@@ -375,7 +381,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       for (int t = p.t0; t < p.t0 + p.n && t * kTile < p.len; ++t) {
         const int boxes = (min(kTile, p.len - t * kTile) + a.box - 1) / a.box;
         const int at = t * per_tile - first;
-        if (!tree_wait(&s.raw_empty[st], par ^ 1u, &s.abort, 11)) { ok = false; break; }
+        if (!tree_wait<C8>(&s.raw_empty[st], par ^ 1u, &s.abort, 11)) { ok = false; break; }
         used |= 1u << st;
         if (lane == 0) mbar_arrive_expect_tx(&s.raw_full[st], (uint32_t)(boxes * a.box * D));
         uint8_t* const to = s.raw[st][keys ? 0 : C8 ? 1 : 0];
@@ -436,7 +442,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
           page[i] = next[i];
         }
-        if (!tree_wait(&s.raw_empty[st], par ^ 1u, &s.abort, 12)) { ok = false; break; }
+        if (!tree_wait<C8>(&s.raw_empty[st], par ^ 1u, &s.abort, 12)) { ok = false; break; }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s.powers[st][0][C8 ? 32 * i + lane : 0] = (uint8_t)ks[i];
@@ -448,44 +454,56 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
     }
   } else if (C8 && warp >= kConvertWarp) {
-    // ------------------------------------------------ 8 bits to bf16, 32 rows of each tile
+    // ------------------------------------------------ 8 bits to bf16: two warps for the keys, two for the
+    // values, 64 rows of a tile each
     fewer_registers();
-    const int cw = warp - kConvertWarp;
-    uint32_t st = 0, par = 0, ki = 0, k_par = 0, vi = 0, v_par = 0, uc = 0;
+    const bool values = warp >= kConvertWarp + kConverters / 2;
+    const int half = (warp - kConvertWarp) & 1, first = 64 * half;
+    uint8_t* const ring = values ? s.v[0] : s.k[0];
+    uint64_t* const full = values ? s.v_full : s.k_full;
+    uint64_t* const empty = values ? s.v_empty : s.k_empty;
+    static_assert(!C8 || kRingK == kRingV, "one place for both");
+    uint32_t st = 0, par = 0, ri = 0, r_par = 0, uc = 0;
     bool ok = true;
     Piece p;
     auto chunk = [&](uint8_t* tile, int row, int c) {  // 16 bytes of a bf16 row, where the swizzle puts them
       return reinterpret_cast<uint4*>(tile + (c / 8) * (kTile * 128) + row * 128 + ((c ^ row) & 7) * 16);
     };
-    // Rows [32 cw, 32 cw + 32) below `rest` of a raw tile: 8 rows at a time, D / 16 steps of 4 lanes a row.
+    // This warp's rows below `rest` of a raw tile: 8 rows and 4 chunks of 16 numbers at a time. A short loop: its
+    // code has to stay with the one warp of its scheduler that runs it.
     auto convert = [&](const uint8_t* raw, const uint8_t* powers, uint8_t* tile, int rest) {
-      constexpr int kChunks = D / 16;  // of a raw row
-#pragma unroll 2
-      for (int r8 = 0; r8 < 32; r8 += 8) {
-        const int row = 32 * cw + r8 + (lane & 7);
-        const uint32_t f = factors_of(powers[row]);
-        const uint32_t f1 = __byte_perm(f, 0u, 0x1010), f2 = __byte_perm(f, 0u, 0x3232);
-        if (row < rest) {
+      constexpr int kTimes = D / 64;
+      int row = first + (lane & 7);
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i, row += 8) {
+        const uint32_t code = powers[row];
+        uint4 x[kTimes];
 #pragma unroll
-          for (int j0 = 0; j0 < kChunks; j0 += 4) {
-            const int j = j0 + (lane >> 3);
-            // the box's swizzle: of 128 bytes, or of 64
-            const int at = D == 128 ? row * 128 + ((j ^ row) & 7) * 16 : row * 64 + ((j ^ (row >> 1)) & 3) * 16;
-            const uint4 x = *reinterpret_cast<const uint4*>(raw + at);
-            uint32_t y[8];
-            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+        for (int z = 0; z < kTimes; ++z) {
+          const int j = 4 * z + (lane >> 3);
+          // the box's swizzle: of 128 bytes, or of 64
+          const int at = D == 128 ? row * 128 + ((j ^ row) & 7) * 16 : row * 64 + ((j ^ (row >> 1)) & 3) * 16;
+          x[z] = *reinterpret_cast<const uint4*>(raw + at);
+        }
+        uint32_t f = (code + 120u) * 0x00800080u;  // 2^120 2^(code - 127) twice, as long as that is one number
+        const bool high = code > 134u;
+        if (high) f = 0x7f007f00u;  // 2^127, and the rest later
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              y[2 * z] = bf16_of_e4m3(words[z], 0x1404, f1);
-              y[2 * z + 1] = bf16_of_e4m3(words[z], 0x3424, f1);
-            }
-            if (f2 != 0x3f803f80u) {
+        for (int z = 0; z < kTimes; ++z) {
+          const int j = 4 * z + (lane >> 3);
+          uint32_t y[8];
+          const uint32_t words[4] = {x[z].x, x[z].y, x[z].z, x[z].w};
 #pragma unroll
-              for (int z = 0; z < 8; ++z) {
-                const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&y[z]), *reinterpret_cast<const __nv_bfloat162*>(&f2));
-                y[z] = *reinterpret_cast<const uint32_t*>(&r);
-              }
-            }
+          for (int k = 0; k < 4; ++k) {
+            y[2 * k] = bf16_of_e4m3(words[k], 0x4140, f);
+            y[2 * k + 1] = bf16_of_e4m3(words[k], 0x4342, f);
+          }
+          if (high) {
+            const uint32_t more = code == 255u ? 0x7fc07fc0u : (code - 7u) * 0x00800080u;  // 2^(code - 134)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = times(y[k], more);
+          }
+          if (row < rest) {
             *chunk(tile, row, 2 * j) = make_uint4(y[0], y[1], y[2], y[3]);
             *chunk(tile, row, 2 * j + 1) = make_uint4(y[4], y[5], y[6], y[7]);
           }
@@ -494,67 +512,58 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     };
     while (ok && next_piece(a, w, p)) {
       const int* const parents = a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr;
+      const bf16* const rows_new = (values ? a.v_new : a.k_new) + p.b * a.n_b + p.kvh * a.n_h;
       for (int tile = p.t0; tile < p.t0 + p.n; ++tile) {
         const int rest = p.len - tile * kTile;  // cached rows; none: the drafted tokens' own tile
         const bool drafts = tile == p.tiles - 1;
-        // drafted tokens are rows [d0, d0 + tokens), of which this warp has [r0, r1): all of them where they share
-        const int d0 = rest > 0 ? rest : 0;
-        const int r0 = !drafts ? 0 : rest > 0 ? (cw == 0 ? d0 : 0) : min(32 * cw, a.tokens);
-        const int r1 = !drafts ? 0 : rest > 0 ? (cw == 0 ? d0 + a.tokens : 0) : min(32 * cw + 32, a.tokens);
-        if (rest > 0 && !tree_wait(&s.raw_full[st], par, &s.abort, 43)) { ok = false; break; }
-        if (!tree_wait(&s.k_empty[ki], k_par ^ 1u, &s.abort, 44)) { ok = false; break; }
-        uint8_t* const kt = s.k[ki];
-        if (rest > 0) convert(s.raw[st][0], s.powers[st][0], kt, rest);
-        for (int x = r0 * (D / 8) + lane; x < r1 * (D / 8); x += 32) {
-          const int row = x / (D / 8), c = x % (D / 8);
-          *chunk(kt, row, c) = *reinterpret_cast<const uint4*>(a.k_new + p.b * a.n_b + (row - d0) * a.n_t + p.kvh * a.n_h + c * 8);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.k_full[ki]);
-        if (++ki == kRingK) { ki = 0; k_par ^= 1u; }
-
-        if (!tree_wait(&s.v_empty[vi], v_par ^ 1u, &s.abort, 45)) { ok = false; break; }
-        uint8_t* const vt = s.v[vi];
-        if (rest > 0) convert(s.raw[st][C8 ? 1 : 0], s.powers[st][1], vt, rest);
-        if (rest < kTile) {
+        // drafted tokens are rows [d0, d0 + tokens), of which this warp has [r0, r1): the first one all where they share
+        const int d0 = max(rest, 0);
+        const int r0 = !drafts ? 0 : rest > 0 ? d0 : min(first, a.tokens);
+        const int r1 = !drafts || (rest > 0 && half) ? r0 : rest > 0 ? d0 + a.tokens : min(first + 64, a.tokens);
+        if (rest > 0 && !tree_wait<C8>(&s.raw_full[st], par, &s.abort, 43)) { ok = false; break; }
+        if (!tree_wait<C8>(&empty[ri], r_par ^ 1u, &s.abort, 44)) { ok = false; break; }
+        uint8_t* const to = ring + ri * kTileBytes;
+        if (rest > 0) convert(s.raw[st][values && C8 ? 1 : 0], s.powers[st][values ? 1 : 0], to, rest);
+        if (!values) {
+          for (int x = r0 * (D / 8) + lane; x < r1 * (D / 8); x += 32) {
+            const int row = x / (D / 8), c = x % (D / 8);
+            *chunk(to, row, c) = *reinterpret_cast<const uint4*>(rows_new + (row - d0) * a.n_t + c * 8);
+          }
+        } else if (rest < kTile) {
           // Rows past the end, and absent tokens, are zeros; infinities and NaN of the others are left out here and
           // put back at the end for the rows that see them: products with P = 0 have to leave no trace of them.
-          const int filled = max(rest, 0) + (drafts ? a.tokens : 0);
-          for (int x = 32 * cw * (D / 8) + lane; x < (32 * cw + 32) * (D / 8); x += 32) {
-            const int row = x / (D / 8);
-            if (row >= filled) *chunk(vt, row, x % (D / 8)) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          uint32_t odd = 0u;  // this warp's tokens with such a value, from 32 cw on (or 0, where they share)
+          const int filled = d0 + (drafts ? a.tokens : 0);
+          for (int x = max(first, filled) * (D / 8) + lane; x < (first + 64) * (D / 8); x += 32)
+            *chunk(to, x / (D / 8), x % (D / 8)) = make_uint4(0u, 0u, 0u, 0u);
+          uint32_t odd[2] = {0u, 0u};  // this warp's tokens with such a value, from 64 half on
           for (int x = r0 * (D / 8) + lane; x < r1 * (D / 8); x += 32) {
             const int row = x / (D / 8), c = x % (D / 8), token = row - d0;
             uint4 y = make_uint4(0u, 0u, 0u, 0u);
-            if (!parents || parents[token] >= -1)
-              y = *reinterpret_cast<const uint4*>(a.v_new + p.b * a.n_b + token * a.n_t + p.kvh * a.n_h + c * 8);
+            if (!parents || parents[token] >= -1) y = *reinterpret_cast<const uint4*>(rows_new + token * a.n_t + c * 8);
             uint32_t* const z = reinterpret_cast<uint32_t*>(&y);
+            bool mine = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t hit = ((z[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;  // exponents of all ones
-              if (hit) odd |= 1u << (token & 31);
+              mine |= hit != 0u;
               if (hit & 0x8000u) z[i] &= 0xffff0000u;
               if (hit & 0x80000000u) z[i] &= 0x0000ffffu;
             }
-            *chunk(vt, row, c) = y;
+            if (mine && !(token & 32)) odd[0] |= 1u << (token & 31);
+            if (mine && (token & 32)) odd[1] |= 1u << (token & 31);
+            *chunk(to, row, c) = y;
           }
-          odd = __reduce_or_sync(0xffffffffu, odd);
-          if (drafts && lane == 0) {
-            if (rest <= 0) s.bad[uc & 7][cw] = odd;
-            else if (cw == 0) s.bad[uc & 7][0] = odd;
-            else s.bad[uc & 7][cw] = 0u;
-          }
+          odd[0] = __reduce_or_sync(0xffffffffu, odd[0]);
+          odd[1] = __reduce_or_sync(0xffffffffu, odd[1]);
+          if (drafts && lane < 2) s.bad[uc & 7][2 * half + lane] = lane ? odd[1] : odd[0];
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&s.v_full[vi]);
+          mbar_arrive(&full[ri]);
           if (rest > 0) mbar_arrive(&s.raw_empty[st]);
         }
-        if (++vi == kRingV) { vi = 0; v_par ^= 1u; }
+        if (++ri == (uint32_t)kRingK) { ri = 0; r_par ^= 1u; }
         if (rest > 0 && ++st == Smem::kRaw) { st = 0; par ^= 1u; }
       }
       ++uc;
@@ -589,7 +598,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       int first = p.t0 * per_tile, page, slot, next_page, next_slot;
       look_up(first + lane, page, slot);
       if (keys) {
-        if (!tree_wait(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
+        if (!tree_wait<C8>(&s.q_empty, (uc & 1u) ^ 1u, &s.abort, 10)) { ok = false; break; }
         if (lane == 0) {
           mbar_arrive_expect_tx(&s.q_full, (uint32_t)(NQ * D * 2 * a.tt * a.group));
 #pragma unroll
@@ -605,7 +614,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const bool old = t * kTile < p.len;
         const int boxes = old ? (min(kTile, p.len - t * kTile) + a.box - 1) / a.box : 0;
         const int at = t * per_tile - first;
-        if (!tree_wait(&empty[st], par ^ 1u, &s.abort, 11)) { ok = false; break; }
+        if (!tree_wait<C8>(&empty[st], par ^ 1u, &s.abort, 11)) { ok = false; break; }
         const bool mend = keys ? p.shares && t == p.tiles - 1 : (t + 1) * kTile > p.len;
         uint64_t* const bar = mend ? &land[st] : &full[st];
         used |= 1u << st;
@@ -662,7 +671,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const uint64_t k_desc = smem_desc_sw128(smem_u32(s.k[0]), 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(smem_u32(s.v[0]), kTile * 128, 1024);
       auto wait_k = [&]() {
-        const bool y = mbar_wait(&s.k_full[kt], k_par, &s.abort, &g_tree_dev_error, 21);
+        const bool y = one_wait<C8>(&s.k_full[kt], k_par, &s.abort, 21);
         tc_fence_after();
         return y;
       };
@@ -704,7 +713,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       while (ok && next_piece(a, w, p)) {
         const int n = p.n;
         const bool two = p.len <= kFine;
-        if (!mbar_wait(&s.q_full, uc & 1u, &s.abort, &g_tree_dev_error, 20)) { ok = false; break; }
+        if (!one_wait<C8>(&s.q_full, uc & 1u, &s.abort, 20)) { ok = false; break; }
         tc_fence_after();
         // t = -2 .. n - 1 (NQ = 1), -1 .. n - 1 (NQ = 2): P V of tile t, and the scores of the tile
         // whose place that frees
@@ -712,17 +721,17 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll 1
         for (int t = -kAhead; ok && t < n; ++t) {
           const bool more = t + kAhead < n;
-          if (t >= 0 && !(ok = mbar_wait(&s.v_full[vt], v_par, &s.abort, &g_tree_dev_error, 22))) break;
+          if (t >= 0 && !(ok = one_wait<C8>(&s.v_full[vt], v_par, &s.abort, 22))) break;
 #pragma unroll 1
           for (int i = 0; i < NQ; ++i) {
             const uint32_t G = gt + (uint32_t)t;
             const int g = NQ == 1 ? (int)(G & 1u) : i;
             const uint32_t use = NQ == 1 ? G >> 1 : G;
             if (t == 0 &&
-                !(ok = mbar_wait(&s.o_free[i], (uc & 1u) ^ 1u, &s.abort, &g_tree_dev_error, 23)))
+                !(ok = one_wait<C8>(&s.o_free[i], (uc & 1u) ^ 1u, &s.abort, 23)))
               break;
             for (int h = 0; t >= 0 && h < 2; ++h) {
-              if (!(ok = mbar_wait(&s.p_full[g][h], use & 1u, &s.abort, &g_tree_dev_error, 24))) break;
+              if (!(ok = one_wait<C8>(&s.p_full[g][h], use & 1u, &s.abort, 24))) break;
               tc_fence_after();
               issue_pv(g, h, t >= kAhead || h > 0, two);
               if (NQ == 2 && t == 0 && i == 0 && h == 0) {
@@ -807,7 +816,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
               vx[i] = *reinterpret_cast<const uint4*>(a.v_new + at);
             }
           }
-          if (!tree_wait(&s.k_land[ki], (k_par >> ki) & 1u, &s.abort, 41)) { ok = false; break; }
+          if (!tree_wait<C8>(&s.k_land[ki], (k_par >> ki) & 1u, &s.abort, 41)) { ok = false; break; }
           k_par ^= 1u << ki;
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
@@ -817,7 +826,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.k_full[ki]);
-          if (!tree_wait(&s.v_land[vi], v_phase, &s.abort, 42)) { ok = false; break; }
+          if (!tree_wait<C8>(&s.v_land[vi], v_phase, &s.abort, 42)) { ok = false; break; }
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
             const int x = i * 32 + lane, row = x / (D / 8);
@@ -835,7 +844,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           }
           bad[0] = __reduce_or_sync(0xffffffffu, bad[0]);
         } else {
-          if (!tree_wait(&s.v_land[vi], v_phase, &s.abort, 43)) { ok = false; break; }
+          if (!tree_wait<C8>(&s.v_land[vi], v_phase, &s.abort, 43)) { ok = false; break; }
           if (drafts) {
             uint32_t any_bad = 0u;
 #pragma unroll 4
@@ -911,7 +920,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int rest = p.len - tile * kTile;  // cached keys of the tile
         const bool drafts = tile == p.tiles - 1;
         if (drafts && r < rows) ancestor_bits(a.parents ? a.parents + (int64_t)p.b * a.tokens : nullptr, token, seen);
-        if (!tree_wait(&s.s_full[g], use & 1u, &s.abort, 31)) { ok = false; break; }
+        if (!tree_wait<C8>(&s.s_full[g], use & 1u, &s.abort, 31)) { ok = false; break; }
         tc_fence_after();
         // A loop and not straight code for the halves: the code's first pass is fetched from L2,
         // and that is what a short call waits for.
@@ -970,7 +979,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             l = l * factor + ((f2_lo(rs[0]) + f2_hi(rs[0])) + (f2_lo(rs[1]) + f2_hi(rs[1])));
             if ((any || h > 0) && __any_sync(0xffffffffu, factor != 1.f)) {
               // O *= factor; it must hold every product before this one
-              if (!tree_wait(&s.o_done[g][h ^ 1], (h ? use : use - 1) & 1u, &s.abort, 32)) { ok = false; break; }
+              if (!tree_wait<C8>(&s.o_done[g][h ^ 1], (h ? use : use - 1) & 1u, &s.abort, 32)) { ok = false; break; }
               tc_fence_after();
               tmem_wait_st();
 #pragma unroll 1
@@ -1007,7 +1016,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       int c0 = 0, c1 = D;
       if constexpr (NQ == 1) {
         // both groups' results: this one writes half of the columns
-        if (uc > 0 && !tree_wait(&s.o_free[0], (uc - 1) & 1u, &s.abort, 34)) { ok = false; break; }
+        if (uc > 0 && !tree_wait<C8>(&s.o_free[0], (uc - 1) & 1u, &s.abort, 34)) { ok = false; break; }
         s.xm[g][NQ == 1 ? r : 0] = m;
         s.xl[g][NQ == 1 ? r : 0] = l;
         mbar_arrive(&s.x_full);
@@ -1016,9 +1025,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         // nothing about a phase two ahead).
         const uint32_t own = (last & 1u) == (uint32_t)g ? last : last - 1;
         const uint32_t other = own == last ? last - 1 : last;
-        if ((n > 1 || own == last) && !tree_wait(&s.o_done[g][1], (own >> 1) & 1u, &s.abort, 35)) { ok = false; break; }
-        if ((n > 1 || other == last) && !tree_wait(&s.o_done[g ^ 1][1], (other >> 1) & 1u, &s.abort, 36)) { ok = false; break; }
-        if (!tree_wait(&s.x_full, uc & 1u, &s.abort, 37)) { ok = false; break; }
+        if ((n > 1 || own == last) && !tree_wait<C8>(&s.o_done[g][1], (own >> 1) & 1u, &s.abort, 35)) { ok = false; break; }
+        if ((n > 1 || other == last) && !tree_wait<C8>(&s.o_done[g ^ 1][1], (other >> 1) & 1u, &s.abort, 36)) { ok = false; break; }
+        if (!tree_wait<C8>(&s.x_full, uc & 1u, &s.abort, 37)) { ok = false; break; }
         use0 = n > 1 || (last & 1u) == 0u;
         use1 = n > 1 || (last & 1u) == 1u;
         const float m0 = use0 ? s.xm[0][r] : -INFINITY, m1 = use1 ? s.xm[1][r] : -INFINITY;
@@ -1029,7 +1038,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         c0 = g * (D / 2);
         c1 = c0 + D / 2;
       } else {
-        if (!tree_wait(&s.o_done[g][1], last & 1u, &s.abort, 35)) { ok = false; break; }
+        if (!tree_wait<C8>(&s.o_done[g][1], last & 1u, &s.abort, 35)) { ok = false; break; }
       }
       tc_fence_after();
       const float inv = cut ? 1.f : here ? 1.f / l : 0.f;
