@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
 
 #include "tree_attention_tc.cuh"
 #include "tree_attention_8bit.cuh"
+#include "tree_attention_8bit_ring.cuh"
 
 namespace {
 
@@ -541,11 +542,6 @@ int launch_combine(const TreeArgs& a, int dtype, cudaStream_t st, const char* op
     return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 4, BASE2>, 1) : join(tree_combine_kernel<bf16, 4, BASE2>, 1);
   return dtype == NKL_FLOAT32 ? join(tree_combine_kernel<float, 1, BASE2>, 4) : join(tree_combine_kernel<bf16, 1, BASE2>, 4);
 }
-
-#ifndef KTCROWS
-#define KTCROWS 16
-#endif
-constexpr int kTcRows = KTCROWS;
 
 size_t split_bytes(int64_t splits, int64_t batch, int64_t heads, int64_t tokens, int64_t d) {
   return splits > 1 ? ((size_t)splits * batch * heads * tokens * (d + 2) * 4 + 255) & ~size_t(255) : 0;
@@ -722,7 +718,7 @@ extern "C" int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t rows = tokens * a.t.group;
   const TcPlan p = tc_plan(batch, tokens, heads, kv_heads, head_dim, page_size, max_pages, dtype);
-  bool tc = p.on && rows > kTcRows && scale > 0.f && scale < INFINITY;
+  bool tc = p.on && scale > 0.f && scale < INFINITY;
   for (int i = 0; i < 9; ++i) tc = tc && (n[i] == 1 || (s[i] > 0 && s[i] < (1LL << 38)));
   if (tc) {
     if (p.bytes) {
@@ -734,6 +730,10 @@ extern "C" int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, 
     for (int i = 0; i < 9; ++i)
       if (n[i] == 1) *steps[i] = head_dim;
     const TcScales sc = {k_scales, v_scales, (int)block};
+    if (rows <= 8)
+      return head_dim == 128 ? ring_launch<128, 1>(a.t, p, ws, st, sc) : ring_launch<64, 1>(a.t, p, ws, st, sc);
+    if (rows <= kRingRows)
+      return head_dim == 128 ? ring_launch<128, 2>(a.t, p, ws, st, sc) : ring_launch<64, 2>(a.t, p, ws, st, sc);
     if (head_dim == 128) return p.nq == 1 ? tc_launch<128, 1, true>(a.t, p, ws, st, sc) : tc_launch<128, 2, true>(a.t, p, ws, st, sc);
     return p.nq == 1 ? tc_launch<64, 1, true>(a.t, p, ws, st, sc) : tc_launch<64, 2, true>(a.t, p, ws, st, sc);
   }

@@ -94,101 +94,24 @@ __device__ __forceinline__ void bf16_parts(float lo, float hi, uint32_t (&p)[N])
   }
 }
 
-// DC: head_dim up to 64 DC. FAST: pages and blocks are multiples of 16 positions, so that the 16 keys of a
-// product lie in a row and share their powers of two. NT: tiles of 8 query rows to a warp.
-template <typename T, int DC, bool FAST, int NT>
-__global__ void __launch_bounds__(kThreads8, NT == 1 && sizeof(T) == 2 ? KMIN8 : 2)
-attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
-  constexpr bool kF32 = sizeof(T) == 4;
-  constexpr int kParts = kF32 ? 3 : 1;   // of drafted k and v, in bf16
-  constexpr int kPParts = kF32 ? 3 : 2;  // of the weights for them
-  constexpr int kSteps = 4 * DC;         // products over the entries of a head
-  constexpr int kCols = 8 * DC;          // entries of V that a lane has of a key
-  constexpr int kRowsW = 8 * NT;         // a warp's query rows
-  extern __shared__ __align__(16) float joined[];
-  __shared__ int s_bad;                  // a drafted v that is not finite
-  const TreeArgs& a = args.t;
-  pdl_enter();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const int split = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
-  const int kvh = blockIdx.y, b = blockIdx.z;
-  const int tile = warp % args.tiles, stream = warp / args.tiles, streams = kWarps8 / args.tiles;
-  const int rows = a.tokens * a.group, r0 = (rb * args.tiles + tile) * kRowsW;
-  const int n = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
-  const int windows = (n + kWindow - 1) / kWindow, per = (windows + a.splits - 1) / a.splits;
-  const int w0 = min(split * per, windows), w1 = min(w0 + per, windows);
-  const int* const parents = a.parents ? a.parents + (int64_t)b * a.tokens : nullptr;
-  if (tid == 0) s_bad = 0;
-  __syncthreads();
-
-  // Query row r of the warp's: where it lies, and whether it is one (an absent token's is not looked at).
-  auto query = [&](int r, bool& real) {
-    const int row = r0 + r, token = row / a.group;
-    real = row < rows && (!parents || parents[token] >= -1);
-    return static_cast<const T*>(a.q) + b * a.q_b + (real ? token * a.q_t + (kvh * a.group + row - token * a.group) * a.q_h : 0);
-  };
-  // Four consecutive entries of the lane's: step s takes those at entry(s).
-  auto entry = [&](int s) { return (t4 + 4 * (s >> 2)) * 16 + (s & 3) * 4; };
-  auto four = [&](const T* p) {
-    float4 x;
-    if constexpr (kF32) {
-      x = *reinterpret_cast<const float4*>(p);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-      x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-    }
-    return x;
-  };
-  // Row g of each tile, for the products; the factors of the scores of the rows 2 t4 and 2 t4 + 1, which the
-  // lane has then.
-  uint32_t qh[NT][kSteps][2], ql[NT][kF32 ? kSteps : 1][2];
-  float factor[NT][2];
+// The sums of a lane: rows 2 t4 and 2 t4 + 1 (the last index of m, mv, l) of NT tiles of 8 query rows. m: the
+// rows' reference for sums l of 2^(s - m), over the lane's keys; mv: that for O, sums of 2^(s + e - mv + kRaise) v.
+// O's products j hold two entries of a head: o[t][j][i] and o[t][j][2 + i].
+template <int NT, int DC>
+struct Sums8 {
+  float m[NT][2], mv[NT][2], l[NT][2], o[NT][4 * DC][4];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    bool real;
-    const T* const qp = query(8 * t + g, real);
-    float top = 0.f;
+    for (int t = 0; t < NT; ++t) {
+      m[t][0] = m[t][1] = mv[t][0] = mv[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      if (!real || entry(s) >= a.d) continue;
-      const float4 x = four(qp + entry(s));
-      for (float y : {x.x, x.y, x.z, x.w}) top = fmaxf(top, fabsf(y) < INFINITY ? fabsf(y) : 0.f);
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);  // 2^e <= top
-    const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
-    const float f = a.scale * kLog2e * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
-    factor[t][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
-    factor[t][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (real && entry(s) < a.d) x = four(qp + entry(s));
-      x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
-      qh[t][s][0] = half_pair(x.x, x.y);
-      qh[t][s][1] = half_pair(x.z, x.w);
-      if constexpr (kF32) {
-        const float2 u = rest_half(qh[t][s][0], x.x, x.y), v = rest_half(qh[t][s][1], x.z, x.w);
-        ql[t][s][0] = half_pair(u.x, u.y);
-        ql[t][s][1] = half_pair(v.x, v.y);
-      }
+      for (int j = 0; j < 4 * DC; ++j) o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.f;
     }
   }
-
-  // m: the rows' reference for sums l of 2^(s - m); mv: that for O, sums of 2^(s + e - mv + kRaise) v
-  float m[NT][2], mv[NT][2], l[NT][2], o[NT][kCols / 2][4];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m[t][0] = m[t][1] = mv[t][0] = mv[t][1] = -INFINITY;
-    l[t][0] = l[t][1] = 0.f;
-#pragma unroll
-    for (int j = 0; j < kCols / 2; ++j) o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.f;
-  }
-
   // Weights of 16 keys: x[t][2 k + i] the score of key 8 k + g with row 2 t4 + i of tile t, e[k] the key's power of
   // two for O. Comes back with x the weights for O.
-  auto weigh = [&](float (&x)[NT][4], const float (&e)[2]) {
+  __device__ __forceinline__ void weigh(float (&x)[NT][4], const float (&e)[2]) {
     bool grows = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -217,7 +140,7 @@ attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
             mv[t][i] = tv;
           }
 #pragma unroll
-          for (int j = 0; j < kCols / 2; ++j) {
+          for (int j = 0; j < 4 * DC; ++j) {
             o[t][j][i] *= f;
             o[t][j][2 + i] *= f;
           }
@@ -235,120 +158,229 @@ attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
           s = fast_exp2(s + e[k] - rv);
         }
       }
-  };
+  }
+};
 
-  // ------------------------------------------------ the drafted tokens
-  if (split == a.splits - 1) {
-    const T* const kn = static_cast<const T*>(a.k_new) + b * a.n_b + kvh * a.n_h;
-    const T* const vn = static_cast<const T*>(a.v_new) + b * a.n_b + kvh * a.n_h;
-    bool bad = false;
+// Four consecutive numbers in fp32.
+__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four_of(const bf16* p) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                     __uint_as_float(w.y & 0xffff0000u));
+}
+
+// The drafted tokens first, first + 1, .. (16 at a time, then the ones `step` further on) against a warp's rows r0
+// .. r0 + 8 NT - 1 of a key/value head: query(r, real) says where row r's q lies and whether it is one, entry(s) where
+// the lane's four entries of product s are, col(j) its two of O's product j. Returns whether a v was not finite.
+template <typename T, int NT, int DC, typename Query, typename Entry, typename Col>
+__device__ __forceinline__ bool drafted_8bit(const TreeArgs& a, int b, int kvh, int r0, int first, int step, Query query,
+                                             Entry entry, Col col, Sums8<NT, DC>& sums) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int kParts = kF32 ? 3 : 1;   // of k and v, in bf16
+  constexpr int kPParts = kF32 ? 3 : 2;  // of the weights
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int* const parents = a.parents ? a.parents + (int64_t)b * a.tokens : nullptr;
+  const T* const kn = static_cast<const T*>(a.k_new) + b * a.n_b + kvh * a.n_h;
+  const T* const vn = static_cast<const T*>(a.v_new) + b * a.n_b + kvh * a.n_h;
+  bool bad = false;
 #pragma unroll 1
-    for (int k0 = stream * 16; k0 < a.tokens; k0 += streams * 16) {
-      float x[NT][4] = {};
+  for (int k0 = first; k0 < a.tokens; k0 += step) {
+    float x[NT][4] = {};
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        uint32_t ka[kParts][4];
+    for (int s = 0; s < 4 * DC; ++s) {
+      uint32_t ka[kParts][4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int key = k0 + 8 * k + g;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (key < a.tokens && entry(s) < a.d) y = four_of(kn + key * a.n_t + entry(s));
+        uint32_t p[kParts];
+        bf16_parts(y.x, y.y, p);
+#pragma unroll
+        for (int z = 0; z < kParts; ++z) ka[z][k] = p[z];
+        bf16_parts(y.z, y.w, p);
+#pragma unroll
+        for (int z = 0; z < kParts; ++z) ka[z][2 + k] = p[z];
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        bool real;
+        const T* const qp = query(8 * t + g, real);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (real && entry(s) < a.d) y = four_of(qp + entry(s));
+        uint32_t q0[kParts], q1[kParts];
+        bf16_parts(y.x, y.y, q0);
+        bf16_parts(y.z, y.w, q1);
+#pragma unroll
+        for (int sum = kParts - 1; sum >= 0; --sum)  // the smallest products first
+#pragma unroll
+          for (int z = 0; z <= sum; ++z) mma_b16(x[t], ka[z], q0[sum - z], q1[sum - z]);
+      }
+    }
+    const float none[2] = {0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = 8 * t + 2 * t4 + i;
+        bool real;
+        const T* const qp = query(r, real);
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (real) ancestor_bits(parents, (r0 + r) / a.group, w);
+        const int word = k0 >> 5;
+        const uint32_t bits = word == 0 ? w[0] : word == 1 ? w[1] : word == 2 ? w[2] : w[3];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int key = k0 + 8 * k + g;
-          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (key < a.tokens && entry(s) < a.d) y = four(kn + key * a.n_t + entry(s));
-          uint32_t p[kParts];
-          bf16_parts(y.x, y.y, p);
-#pragma unroll
-          for (int z = 0; z < kParts; ++z) ka[z][k] = p[z];
-          bf16_parts(y.z, y.w, p);
-#pragma unroll
-          for (int z = 0; z < kParts; ++z) ka[z][2 + k] = p[z];
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          bool real;
-          const T* const qp = query(8 * t + g, real);
-          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (real && entry(s) < a.d) y = four(qp + entry(s));
-          uint32_t q0[kParts], q1[kParts];
-          bf16_parts(y.x, y.y, q0);
-          bf16_parts(y.z, y.w, q1);
-#pragma unroll
-          for (int sum = kParts - 1; sum >= 0; --sum)  // the smallest products first
-#pragma unroll
-            for (int z = 0; z <= sum; ++z) mma_b16(x[t], ka[z], q0[sum - z], q1[sum - z]);
+          float& y = x[t][2 * k + i];
+          // an infinity's product with a part that is zero is no part of its product
+          if (kF32 && !(fabsf(y) < INFINITY) && real && key < a.tokens) {
+            y = 0.f;
+            for (int c = 0; c < a.d; ++c) y = fmaf(to_f32(qp[c]), to_f32(kn[key * a.n_t + c]), y);
+          }
+          y = (bits >> (key & 31)) & 1u ? y * (a.scale * kLog2e) : -INFINITY;
         }
       }
-      const float none[2] = {0.f, 0.f};
+    sums.weigh(x, none);
+    uint32_t p[NT][kPParts][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t y[kPParts];
+        bf16_parts(x[t][2 * k], x[t][2 * k + 1], y);
+#pragma unroll
+        for (int z = 0; z < kPParts; ++z) p[t][z][k] = transpose(y[z]);
+      }
+#pragma unroll
+    for (int j = 0; j < 4 * DC; ++j) {
+      float v[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = k0 + 2 * t4 + (i & 1) + 8 * (i >> 1);
+        v[i][0] = v[i][1] = 0.f;
+        // an absent token's v is left out; weights of 0 must meet no infinity, which is put in at the end
+        if (key < a.tokens && col(j) < a.d && (!parents || parents[key] >= -1)) {
+          const T* const y = vn + key * a.n_t + col(j);
+          v[i][0] = to_f32(y[0]);
+          v[i][1] = to_f32(y[1]);
+        }
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+          if (!(fabsf(v[i][z]) < INFINITY)) {
+            bad = true;
+            v[i][z] = 0.f;
+          }
+      }
+      uint32_t va[kParts][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // keys 2 t4, 2 t4 + 1 (i < 2) or 8 more, the first entry or the second
+        uint32_t y[kParts];
+        bf16_parts(v[2 * (i >> 1)][i & 1], v[2 * (i >> 1) + 1][i & 1], y);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) va[q][i] = y[q];
+      }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = 8 * t + 2 * t4 + i;
-          bool real;
-          const T* const qp = query(r, real);
-          uint32_t w[4] = {0u, 0u, 0u, 0u};
-          if (real) ancestor_bits(parents, (r0 + r) / a.group, w);
-          const int word = k0 >> 5;
-          const uint32_t bits = word == 0 ? w[0] : word == 1 ? w[1] : word == 2 ? w[2] : w[3];
+        for (int sum = (kF32 ? 2 : 1); sum >= 0; --sum)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int key = k0 + 8 * k + g;
-            float& y = x[t][2 * k + i];
-            // an infinity's product with a part that is zero is no part of its product
-            if (kF32 && !(fabsf(y) < INFINITY) && real && key < a.tokens) {
-              y = 0.f;
-              for (int c = 0; c < a.d; ++c) y = fmaf(to_f32(qp[c]), to_f32(kn[key * a.n_t + c]), y);
-            }
-            y = (bits >> (key & 31)) & 1u ? y * (a.scale * kLog2e) : -INFINITY;
-          }
-        }
-      weigh(x, none);
-      uint32_t p[NT][kPParts][2];
+          for (int q = 0; q < kParts && q <= sum; ++q) mma_b16(sums.o[t][j], va[q], p[t][sum - q][0], p[t][sum - q][1]);
+    }
+  }
+  return bad;
+}
+
+// A warp's query rows as the second operand of the products: row g of each tile, scaled by a power of two so that
+// f16 holds it, and (fp32) what that leaves of it; factor: of the scores of the rows 2 t4 and 2 t4 + 1.
+template <typename T, int NT, int DC>
+struct Queries8 {
+  static constexpr bool kF32 = sizeof(T) == 4;
+  uint32_t hi[NT][4 * DC][2], lo[NT][kF32 ? 4 * DC : 1][2];
+  float factor[NT][2];
+  template <typename Query, typename Entry>
+  __device__ __forceinline__ void load(const TreeArgs& a, Query query, Entry entry) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) {
+      bool real;
+      const T* const qp = query(8 * t + g, real);
+      float top = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t y[kPParts];
-          bf16_parts(x[t][2 * k], x[t][2 * k + 1], y);
+      for (int s = 0; s < 4 * DC; ++s) {
+        if (!real || entry(s) >= a.d) continue;
+        const float4 x = four_of(qp + entry(s));
+        for (float y : {x.x, x.y, x.z, x.w}) top = fmaxf(top, fabsf(y) < INFINITY ? fabsf(y) : 0.f);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = max((int)(__float_as_uint(top) >> 23) - 127, -112);  // 2^e <= top
+      const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+      const float f = a.scale * kLog2e * __uint_as_float((uint32_t)(e - 14 + 127) << 23);
+      factor[t][0] = __shfl_sync(0xffffffffu, f, 8 * t4);
+      factor[t][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
-          for (int z = 0; z < kPParts; ++z) p[t][z][k] = transpose(y[z]);
-        }
-#pragma unroll
-      for (int c = 0; c < kCols; c += 4) {
-        float v[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = k0 + 2 * t4 + (i & 1) + 8 * (i >> 1);
-          float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-          // an absent token's v is left out; weights of 0 must meet no infinity, which is put in at the end
-          if (key < a.tokens && g * kCols + c < a.d && (!parents || parents[key] >= -1)) y = four(vn + key * a.n_t + g * kCols + c);
-          v[i][0] = y.x; v[i][1] = y.y; v[i][2] = y.z; v[i][3] = y.w;
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            if (!(fabsf(v[i][z]) < INFINITY)) {
-              bad = true;
-              v[i][z] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int z = 0; z < 4; z += 2) {
-          uint32_t va[kParts][4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {  // keys 2 t4, 2 t4 + 1 (i < 2) or 8 more, entries z, z + 1
-            uint32_t y[kParts];
-            bf16_parts(v[2 * (i >> 1)][z + (i & 1)], v[2 * (i >> 1) + 1][z + (i & 1)], y);
-#pragma unroll
-            for (int q = 0; q < kParts; ++q) va[q][i] = y[q];
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int sum = (kF32 ? 2 : 1); sum >= 0; --sum)
-#pragma unroll
-              for (int q = 0; q < kParts && q <= sum; ++q) mma_b16(o[t][(c + z) / 2], va[q], p[t][sum - q][0], p[t][sum - q][1]);
+      for (int s = 0; s < 4 * DC; ++s) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (real && entry(s) < a.d) x = four_of(qp + entry(s));
+        x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
+        hi[t][s][0] = half_pair(x.x, x.y);
+        hi[t][s][1] = half_pair(x.z, x.w);
+        if constexpr (kF32) {
+          const float2 u = rest_half(hi[t][s][0], x.x, x.y), v = rest_half(hi[t][s][1], x.z, x.w);
+          lo[t][s][0] = half_pair(u.x, u.y);
+          lo[t][s][1] = half_pair(v.x, v.y);
         }
       }
     }
-    if (bad) s_bad = 1;
   }
+};
+
+// DC: head_dim up to 64 DC. FAST: pages and blocks are multiples of 16 positions, so that the 16 keys of a
+// product lie in a row and share their powers of two. NT: tiles of 8 query rows to a warp.
+template <typename T, int DC, bool FAST, int NT>
+__global__ void __launch_bounds__(kThreads8, NT == 1 && sizeof(T) == 2 ? KMIN8 : 2)
+attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  constexpr int kCols = 8 * DC;          // entries of V that a lane has of a key
+  constexpr int kRowsW = 8 * NT;         // a warp's query rows
+  extern __shared__ __align__(16) float joined[];
+  __shared__ int s_bad;                  // a drafted v that is not finite
+  const TreeArgs& a = args.t;
+  pdl_enter();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const int split = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int tile = warp % args.tiles, stream = warp / args.tiles, streams = kWarps8 / args.tiles;
+  const int rows = a.tokens * a.group, r0 = (rb * args.tiles + tile) * kRowsW;
+  const int n = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page);
+  const int windows = (n + kWindow - 1) / kWindow, per = (windows + a.splits - 1) / a.splits;
+  const int w0 = min(split * per, windows), w1 = min(w0 + per, windows);
+  const int* const parents = a.parents ? a.parents + (int64_t)b * a.tokens : nullptr;
+  if (tid == 0) s_bad = 0;
+  __syncthreads();
+
+  // Query row r of the warp's: where it lies, and whether it is one (an absent token's is not looked at).
+  auto query = [&](int r, bool& real) {
+    const int row = r0 + r, token = row / a.group;
+    real = row < rows && (!parents || parents[token] >= -1);
+    return static_cast<const T*>(a.q) + b * a.q_b + (real ? token * a.q_t + (kvh * a.group + row - token * a.group) * a.q_h : 0);
+  };
+  // Four consecutive entries of the lane's: step s takes those at entry(s).
+  auto entry = [&](int s) { return (t4 + 4 * (s >> 2)) * 16 + (s & 3) * 4; };
+  Queries8<T, NT, DC> q;
+  q.load(a, query, entry);
+
+  Sums8<NT, DC> rows_of_sums;
+  rows_of_sums.clear();
+  auto& m = rows_of_sums.m;
+  auto& mv = rows_of_sums.mv;
+  auto& l = rows_of_sums.l;
+  auto& o = rows_of_sums.o;
+
+  auto col = [&](int j) { return g * kCols + 2 * j; };
+  if (split == a.splits - 1 && drafted_8bit<T, NT, DC>(a, b, kvh, r0, stream * 16, streams * 16, query, entry, col, rows_of_sums))
+    s_bad = 1;
 
   // ------------------------------------------------ the cached keys
   const uint8_t* const kc = static_cast<const uint8_t*>(a.k_cache);
@@ -427,8 +459,8 @@ attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
         e4m3_pairs(k1[z], ka[1], ka[3]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          if constexpr (kF32) mma_f16(s[t], ka, ql[t][4 * c + z][0], ql[t][4 * c + z][1]);
-          mma_f16(s[t], ka, qh[t][4 * c + z][0], qh[t][4 * c + z][1]);
+          if constexpr (kF32) mma_f16(s[t], ka, q.lo[t][4 * c + z][0], q.lo[t][4 * c + z][1]);
+          mma_f16(s[t], ka, q.hi[t][4 * c + z][0], q.hi[t][4 * c + z][1]);
         }
       }
     }
@@ -441,9 +473,9 @@ attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[t][2 * k + i] = key < left ? s[t][2 * k + i] * factor[t][i] * ks : -INFINITY;
+        for (int i = 0; i < 2; ++i) s[t][2 * k + i] = key < left ? s[t][2 * k + i] * q.factor[t][i] * ks : -INFINITY;
     }
-    weigh(s, e);
+    rows_of_sums.weigh(s, e);
     uint32_t p[NT][2], pl[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -541,7 +573,7 @@ attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
       for (int j = 0; j < a.tokens; ++j) {
         const uint32_t bits = j < 32 ? seen[0] : j < 64 ? seen[1] : j < 96 ? seen[2] : seen[3];
         if (!((bits >> (j & 31)) & 1u)) continue;
-        const float4 v = four(static_cast<const T*>(a.v_new) + b * a.n_b + j * a.n_t + kvh * a.n_h + c);
+        const float4 v = four_of(static_cast<const T*>(a.v_new) + b * a.n_b + j * a.n_t + kvh * a.n_h + c);
         x.x += fabsf(v.x) < INFINITY ? 0.f : v.x;
         x.y += fabsf(v.y) < INFINITY ? 0.f : v.y;
         x.z += fabsf(v.z) < INFINITY ? 0.f : v.z;

@@ -1238,6 +1238,50 @@ struct TcScales {
   int block;
 };
 
+TcArgs tc_args(const TreeArgs& g, const TcPlan& p, unsigned char* ws) {
+  TcArgs a = {};
+  a.tables = g.tables;
+  a.lens = g.lens;
+  a.parents = g.parents;
+  a.k_new = static_cast<const bf16*>(g.k_new);
+  a.v_new = static_cast<const bf16*>(g.v_new);
+  a.n_b = g.n_b;
+  a.n_t = g.n_t;
+  a.n_h = g.n_h;
+  a.out = static_cast<bf16*>(g.out);
+  if (p.join) {
+    a.ws_start = reinterpret_cast<int4*>(ws);
+    a.ws_ml = reinterpret_cast<float*>(ws + p.ml_off);
+    a.ws_o = reinterpret_cast<float4*>(ws + p.o_off);
+  }
+  a.batch = g.batch; a.tokens = g.tokens; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.group;
+  a.pages = g.pages; a.page = g.page; a.max_pages = g.max_pages; a.capacity = g.max_pages * g.page;
+  a.tt = p.tt; a.row_blocks = p.row_blocks; a.box = p.box;
+  a.boxes_per_page = g.page / p.box;
+  a.log_bpt = 0;
+  while (p.box << a.log_bpt < kTile) ++a.log_bpt;
+  a.log_bpp = -1;
+  for (int i = 0; i < 9; ++i)
+    if (a.boxes_per_page == 1 << i) a.log_bpp = i;
+  a.bpp_magic = ((1ull << 36) + a.boxes_per_page - 1) / a.boxes_per_page;
+  a.scale_log2 = g.scale * kLog2e;
+  return a;
+}
+
+// Allows a kernel its shared memory, once for each device (idempotent).
+template <auto* Kernel>
+int allow_smem(size_t smem, const char* op) {
+  static std::atomic<bool> set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+  }
+  return NKL_OK;
+}
+
 template <int D, int NQ, bool C8 = false>
 int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_t st, TcScales scales = {}) {
   const char* op = C8 ? "nkl_attention_tree_8bit" : "nkl_attention_tree";
@@ -1268,32 +1312,7 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
     if (int rc = make_tensor_map_bf16(&mkc, g.k_cache, 4, dims, strides, box, op)) return rc;
     if (int rc = make_tensor_map_bf16(&mvc, g.v_cache, 4, dims, strides, box, op)) return rc;
   }
-  TcArgs a = {};
-  a.tables = g.tables;
-  a.lens = g.lens;
-  a.parents = g.parents;
-  a.k_new = static_cast<const bf16*>(g.k_new);
-  a.v_new = static_cast<const bf16*>(g.v_new);
-  a.n_b = g.n_b;
-  a.n_t = g.n_t;
-  a.n_h = g.n_h;
-  a.out = static_cast<bf16*>(g.out);
-  if (p.join) {
-    a.ws_start = reinterpret_cast<int4*>(ws);
-    a.ws_ml = reinterpret_cast<float*>(ws + p.ml_off);
-    a.ws_o = reinterpret_cast<float4*>(ws + p.o_off);
-  }
-  a.batch = g.batch; a.tokens = g.tokens; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.group;
-  a.pages = g.pages; a.page = g.page; a.max_pages = g.max_pages; a.capacity = g.max_pages * g.page;
-  a.tt = p.tt; a.row_blocks = p.row_blocks; a.box = p.box;
-  a.boxes_per_page = g.page / p.box;
-  a.log_bpt = 0;
-  while (p.box << a.log_bpt < kTile) ++a.log_bpt;
-  a.log_bpp = -1;
-  for (int i = 0; i < 9; ++i)
-    if (a.boxes_per_page == 1 << i) a.log_bpp = i;
-  a.bpp_magic = ((1ull << 36) + a.boxes_per_page - 1) / a.boxes_per_page;
-  a.scale_log2 = g.scale * kLog2e;
+  TcArgs a = tc_args(g, p, ws);
   if (C8) {
     a.k_scales = static_cast<const uint8_t*>(scales.k);
     a.v_scales = static_cast<const uint8_t*>(scales.v);
@@ -1302,15 +1321,7 @@ int tc_launch(const TreeArgs& g, const TcPlan& p, unsigned char* ws, cudaStream_
   }
   constexpr size_t smem = sizeof(TreeSmem<D, NQ, C8>);
   static_assert(smem <= 232448, "shared memory of a block");
-  static std::atomic<bool> set[64] = {};  // per device: the smem attribute is set (idempotent)
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(tree_attention_tc_kernel<D, NQ, C8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
-    if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
-    if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
-  }
+  if (int rc = allow_smem<tree_attention_tc_kernel<D, NQ, C8>>(smem, op)) return rc;
   int rc = launch_pdl(tree_attention_tc_kernel<D, NQ, C8>, dim3((unsigned)p.grid), dim3(C8 ? kTcThreads8 : kTcThreads), smem, st,
                       op, mq, mkn, mvn, mkc, mvc, a);
   if (rc || !p.join || p.grid < 2) return rc;
