@@ -161,13 +161,32 @@ struct Sums8 {
   }
 };
 
-// Four consecutive numbers in fp32.
-__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float4 four_of(const bf16* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
+// Four consecutive numbers as they lie, and in fp32.
+template <typename T> struct Four;
+template <> struct Four<float> { typedef float4 type; };
+template <> struct Four<bf16> { typedef uint2 type; };
+__device__ __forceinline__ float4 in_f32(float4 x) { return x; }
+__device__ __forceinline__ float4 in_f32(uint2 w) {
   return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                      __uint_as_float(w.y & 0xffff0000u));
 }
+// Loads without branches, so that they go out together: where `there` does not hold, `any` is read and zeros come back.
+template <typename T>
+__device__ __forceinline__ typename Four<T>::type load_four(const T* p, bool there, const T* any) {
+  typename Four<T>::type x = *reinterpret_cast<const typename Four<T>::type*>(there ? p : any);
+  if (!there) x = typename Four<T>::type{};
+  return x;
+}
+__device__ __forceinline__ float2 load_two(const float* p, bool there, const float* any) {
+  const float2 x = *reinterpret_cast<const float2*>(there ? p : any);
+  return there ? x : make_float2(0.f, 0.f);
+}
+__device__ __forceinline__ float2 load_two(const bf16* p, bool there, const bf16* any) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(there ? p : any);
+  return there ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : make_float2(0.f, 0.f);
+}
+__device__ __forceinline__ float4 four_of(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 four_of(const bf16* p) { return in_f32(*reinterpret_cast<const uint2*>(p)); }
 
 // The drafted tokens first, first + 1, .. (16 at a time, then the ones `step` further on) against a warp's rows r0
 // .. r0 + 8 NT - 1 of a key/value head: query(r, real) says where row r's q lies and whether it is one, entry(s) where
@@ -186,35 +205,49 @@ __device__ __forceinline__ bool drafted_8bit(const TreeArgs& a, int b, int kvh, 
 #pragma unroll 1
   for (int k0 = first; k0 < a.tokens; k0 += step) {
     float x[NT][4] = {};
+    const T* qp[NT];
+    bool real[NT];
 #pragma unroll
-    for (int s = 0; s < 4 * DC; ++s) {
-      uint32_t ka[kParts][4];
+    for (int t = 0; t < NT; ++t) qp[t] = query(8 * t + g, real[t]);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int key = k0 + 8 * k + g;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (key < a.tokens && entry(s) < a.d) y = four_of(kn + key * a.n_t + entry(s));
-        uint32_t p[kParts];
-        bf16_parts(y.x, y.y, p);
+    for (int s0 = 0; s0 < 4 * DC; s0 += 4) {  // four products' loads at a time
+      typename Four<T>::type kr[4][2], qr[4][NT];
 #pragma unroll
-        for (int z = 0; z < kParts; ++z) ka[z][k] = p[z];
-        bf16_parts(y.z, y.w, p);
+      for (int s = 0; s < 4; ++s) {
+        const int e = entry(s0 + s);
 #pragma unroll
-        for (int z = 0; z < kParts; ++z) ka[z][2 + k] = p[z];
+        for (int k = 0; k < 2; ++k) {
+          const int key = k0 + 8 * k + g;
+          kr[s][k] = load_four(kn + key * a.n_t + e, key < a.tokens && e < a.d, kn);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) qr[s][t] = load_four(qp[t] + e, real[t] && e < a.d, qp[t]);
       }
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        bool real;
-        const T* const qp = query(8 * t + g, real);
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (real && entry(s) < a.d) y = four_of(qp + entry(s));
-        uint32_t q0[kParts], q1[kParts];
-        bf16_parts(y.x, y.y, q0);
-        bf16_parts(y.z, y.w, q1);
+      for (int s = 0; s < 4; ++s) {
+        uint32_t ka[kParts][4];
 #pragma unroll
-        for (int sum = kParts - 1; sum >= 0; --sum)  // the smallest products first
+        for (int k = 0; k < 2; ++k) {
+          const float4 y = in_f32(kr[s][k]);
+          uint32_t p[kParts];
+          bf16_parts(y.x, y.y, p);
 #pragma unroll
-          for (int z = 0; z <= sum; ++z) mma_b16(x[t], ka[z], q0[sum - z], q1[sum - z]);
+          for (int z = 0; z < kParts; ++z) ka[z][k] = p[z];
+          bf16_parts(y.z, y.w, p);
+#pragma unroll
+          for (int z = 0; z < kParts; ++z) ka[z][2 + k] = p[z];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float4 y = in_f32(qr[s][t]);
+          uint32_t q0[kParts], q1[kParts];
+          bf16_parts(y.x, y.y, q0);
+          bf16_parts(y.z, y.w, q1);
+#pragma unroll
+          for (int sum = kParts - 1; sum >= 0; --sum)  // the smallest products first
+#pragma unroll
+            for (int z = 0; z <= sum; ++z) mma_b16(x[t], ka[z], q0[sum - z], q1[sum - z]);
+        }
       }
     }
     const float none[2] = {0.f, 0.f};
@@ -223,10 +256,10 @@ __device__ __forceinline__ bool drafted_8bit(const TreeArgs& a, int b, int kvh, 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int r = 8 * t + 2 * t4 + i;
-        bool real;
-        const T* const qp = query(r, real);
+        bool there;
+        const T* const row = query(r, there);
         uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (real) ancestor_bits(parents, (r0 + r) / a.group, w);
+        if (there) ancestor_bits(parents, (r0 + r) / a.group, w);
         const int word = k0 >> 5;
         const uint32_t bits = word == 0 ? w[0] : word == 1 ? w[1] : word == 2 ? w[2] : w[3];
 #pragma unroll
@@ -234,9 +267,9 @@ __device__ __forceinline__ bool drafted_8bit(const TreeArgs& a, int b, int kvh, 
           const int key = k0 + 8 * k + g;
           float& y = x[t][2 * k + i];
           // an infinity's product with a part that is zero is no part of its product
-          if (kF32 && !(fabsf(y) < INFINITY) && real && key < a.tokens) {
+          if (kF32 && !(fabsf(y) < INFINITY) && there && key < a.tokens) {
             y = 0.f;
-            for (int c = 0; c < a.d; ++c) y = fmaf(to_f32(qp[c]), to_f32(kn[key * a.n_t + c]), y);
+            for (int c = 0; c < a.d; ++c) y = fmaf(to_f32(row[c]), to_f32(kn[key * a.n_t + c]), y);
           }
           y = (bits >> (key & 31)) & 1u ? y * (a.scale * kLog2e) : -INFINITY;
         }
@@ -252,40 +285,52 @@ __device__ __forceinline__ bool drafted_8bit(const TreeArgs& a, int b, int kvh, 
 #pragma unroll
         for (int z = 0; z < kPParts; ++z) p[t][z][k] = transpose(y[z]);
       }
+    bool here[4];  // an absent token's v is left out
 #pragma unroll
-    for (int j = 0; j < 4 * DC; ++j) {
-      float v[4][2];
+    for (int i = 0; i < 4; ++i) {
+      const int key = k0 + 2 * t4 + (i & 1) + 8 * (i >> 1);
+      here[i] = key < a.tokens && (!parents || parents[key] >= -1);
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = k0 + 2 * t4 + (i & 1) + 8 * (i >> 1);
-        v[i][0] = v[i][1] = 0.f;
-        // an absent token's v is left out; weights of 0 must meet no infinity, which is put in at the end
-        if (key < a.tokens && col(j) < a.d && (!parents || parents[key] >= -1)) {
-          const T* const y = vn + key * a.n_t + col(j);
-          v[i][0] = to_f32(y[0]);
-          v[i][1] = to_f32(y[1]);
+    for (int j0 = 0; j0 < 4 * DC; j0 += 4) {
+      float2 v[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 2 * t4 + (i & 1) + 8 * (i >> 1), c = col(j0 + j);
+          v[j][i] = load_two(vn + key * a.n_t + c, here[i] && c < a.d, vn);
         }
 #pragma unroll
-        for (int z = 0; z < 2; ++z)
-          if (!(fabsf(v[i][z]) < INFINITY)) {
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // weights of 0 must meet no infinity, which is put in at the end
+          if (!(fabsf(v[j][i].x) < INFINITY)) {
             bad = true;
-            v[i][z] = 0.f;
+            v[j][i].x = 0.f;
           }
+          if (!(fabsf(v[j][i].y) < INFINITY)) {
+            bad = true;
+            v[j][i].y = 0.f;
+          }
+        }
+        uint32_t va[kParts][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // keys 2 t4, 2 t4 + 1 (i < 2) or 8 more, the first entry or the second
+          uint32_t y[kParts];
+          const float2 p = v[j][2 * (i >> 1)], q = v[j][2 * (i >> 1) + 1];
+          bf16_parts((i & 1) ? p.y : p.x, (i & 1) ? q.y : q.x, y);
+#pragma unroll
+          for (int q2 = 0; q2 < kParts; ++q2) va[q2][i] = y[q2];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int sum = (kF32 ? 2 : 1); sum >= 0; --sum)
+#pragma unroll
+            for (int q = 0; q < kParts && q <= sum; ++q)
+              mma_b16(sums.o[t][j0 + j], va[q], p[t][sum - q][0], p[t][sum - q][1]);
       }
-      uint32_t va[kParts][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // keys 2 t4, 2 t4 + 1 (i < 2) or 8 more, the first entry or the second
-        uint32_t y[kParts];
-        bf16_parts(v[2 * (i >> 1)][i & 1], v[2 * (i >> 1) + 1][i & 1], y);
-#pragma unroll
-        for (int q = 0; q < kParts; ++q) va[q][i] = y[q];
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int sum = (kF32 ? 2 : 1); sum >= 0; --sum)
-#pragma unroll
-          for (int q = 0; q < kParts && q <= sum; ++q) mma_b16(sums.o[t][j], va[q], p[t][sum - q][0], p[t][sum - q][1]);
     }
   }
   return bad;
@@ -305,11 +350,13 @@ struct Queries8 {
     for (int t = 0; t < NT; ++t) {
       bool real;
       const T* const qp = query(8 * t + g, real);
+      typename Four<T>::type raw[4 * DC];
       float top = 0.f;
 #pragma unroll
+      for (int s = 0; s < 4 * DC; ++s) raw[s] = load_four(qp + entry(s), real && entry(s) < a.d, qp);
+#pragma unroll
       for (int s = 0; s < 4 * DC; ++s) {
-        if (!real || entry(s) >= a.d) continue;
-        const float4 x = four_of(qp + entry(s));
+        const float4 x = in_f32(raw[s]);
         for (float y : {x.x, x.y, x.z, x.w}) top = fmaxf(top, fabsf(y) < INFINITY ? fabsf(y) : 0.f);
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -321,8 +368,7 @@ struct Queries8 {
       factor[t][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
       for (int s = 0; s < 4 * DC; ++s) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (real && entry(s) < a.d) x = four_of(qp + entry(s));
+        float4 x = in_f32(raw[s]);
         x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
         hi[t][s][0] = half_pair(x.x, x.y);
         hi[t][s][1] = half_pair(x.z, x.w);

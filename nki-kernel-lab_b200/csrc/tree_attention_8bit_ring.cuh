@@ -3,8 +3,9 @@
 //
 // The work is shared out as by the tcgen05 kernel (tree_plan: all segments' tiles of 128 positions in a row,
 // cut into equal shares on the GPU; the drafted tokens count as a tile of their own), one block to an SM.
-//   warp 8    TMA: tiles of keys and values, as bytes, through a ring of five or six
+//   warp 8    TMA: tiles of keys and values, as bytes, through a ring of four, five or eight
 //   warp 9    the powers of two of their rows
+//   warp 10   the drafted tokens, while the others are at the cached ones
 //   warps 0-7 16 keys of each tile: the products of tree_attention_8bit.cuh with fragments by ldmatrix (transposed
 //             for the values, two entries of a key at a time, which __byte_perm pairs with the next key's), sums of
 //             their own; at a piece's end the sums meet in shared memory, while the ring goes on
@@ -13,15 +14,15 @@
 
 namespace {
 
-constexpr int kRingWarps = 8, kRingThreads = 32 * (kRingWarps + 2);
+constexpr int kRingWarps = 8, kRingThreads = 32 * (kRingWarps + 3);
 
 template <int D, int NT>
 struct RingSmem {
-  static constexpr int kStages = D == 128 ? 7 - NT : 8;
+  static constexpr int kStages = D == 128 ? 6 - NT : 8;
   uint8_t tile[kStages][2][kTile * D];
-  float o[kRingWarps][8 * NT][D];
-  float ml[kRingWarps][8 * NT][2];
-  uint8_t powers[kStages][2][kTile];
+  float o[kRingWarps + 1][8 * NT][D];
+  float ml[kRingWarps + 1][8 * NT][2];
+  alignas(4) uint8_t powers[kStages][2][kTile];
   uint64_t full[kStages], empty[kStages], joined, read;
   int bad, abort;
 };
@@ -57,7 +58,7 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
       mbar_init(&s.full[i], 2);
       mbar_init(&s.empty[i], kRingWarps);
     }
-    mbar_init(&s.joined, kRingWarps);
+    mbar_init(&s.joined, kRingWarps + 1);
     mbar_init(&s.read, kRingWarps);
     s.abort = 0;
     s.bad = 0;
@@ -75,6 +76,44 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
   bool ok = true;
   Piece p = {};
   auto cached_end = [&] { return min(p.t0 + p.n, (p.len + kTile - 1) / kTile); };  // of the piece's tiles of cached keys
+
+  // the piece's query rows, where a row of 16 entries' products lies, and the sums' columns
+  const int rows = t.tokens * t.group, g = lane >> 2, t4 = lane & 3;
+  auto parents_of = [&] { return t.parents ? t.parents + (int64_t)p.b * t.tokens : nullptr; };
+  auto query = [&](int r, bool& real) {
+    const int token = r / t.group;
+    const int* const parents = parents_of();
+    real = r < rows && (!parents || parents[token] >= -1);
+    return static_cast<const bf16*>(t.q) + p.b * t.q_b + (real ? token * t.q_t + (p.kvh * t.group + r - token * t.group) * t.q_h : 0);
+  };
+  auto entry = [&](int x) { return 16 * x + 4 * t4; };
+  auto col = [&](int j) { return 16 * j + 2 * g; };
+  // a warp's sums of its piece, into shared memory once the piece before is read out of it
+  uint32_t uc = 0;
+  auto leave = [&](Sums8<NT, DC>& sums, int at, bool bad) {
+    if (uc > 0 && !tree_wait<true>(&s.read, (uc - 1) & 1u, &s.abort, 54)) return false;
+    if (at == kRingWarps && lane == 0) s.bad = bad;
+#pragma unroll
+    for (int y = 0; y < NT; ++y)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int z = 4; z < 32; z *= 2) sums.l[y][i] += __shfl_xor_sync(0xffffffffu, sums.l[y][i], z);
+        const int r = 8 * y + 2 * t4 + i;
+        if (g == 0) {
+          s.ml[at][r][0] = sums.m[y][i];
+          s.ml[at][r][1] = sums.l[y][i];
+        }
+        // O's reference becomes the sums'
+        const float f = sums.mv[y][i] == -INFINITY ? 1.f : fast_exp2(sums.mv[y][i] - kRaise - sums.m[y][i]);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+          *reinterpret_cast<float2*>(&s.o[at][r][col(j)]) = make_float2(sums.o[y][j][i] * f, sums.o[y][j][2 + i] * f);
+      }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.joined);
+    return true;
+  };
 
   if (warp == kRingWarps) {
     // ------------------------------------------------ TMA
@@ -127,62 +166,43 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
     // ------------------------------------------------ the rows' powers of two
     while (ok && next_piece(a, w, p)) {
       const int end = cached_end();
-      auto find = [&](int x, int (&page)[4]) {  // the pages of this lane's four rows of tile x; -1: none
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = x * kTile + 32 * i + lane;
-          page[i] = -1;
-          if (x >= end || key >= p.len) continue;
-          const int pg = a.tables[(int64_t)p.b * a.max_pages + key / a.page];
-          if ((uint32_t)pg < (uint32_t)a.pages) page[i] = pg;
-        }
-      };
-      int page[4], next[4];
-      find(p.t0, page);
+      Powers now, next;  // tables two tiles ahead, powers one
+      now.find(a, p, p.t0, end);
+      next.find(a, p, p.t0 + 1, end);
+      now.load(a, p, p.t0);
       for (int x = p.t0; x < end; ++x) {
-        find(x + 1, next);
-        uint32_t ks[4], vs[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = x * kTile + 32 * i + lane;
-          ks[i] = vs[i] = 127u;
-          if (page[i] >= 0) {
-            const int64_t at = ((int64_t)page[i] * a.kv_heads + p.kvh) * a.per_page + (key % a.page) / a.block;
-            ks[i] = a.k_scales[at];
-            vs[i] = a.v_scales[at];
-          }
-          page[i] = next[i];
-        }
+        Powers after;
+        after.find(a, p, x + 2, end);
+        next.load(a, p, x + 1);
         if (!tree_wait<true>(&s.empty[st], par ^ 1u, &s.abort, 52)) { ok = false; break; }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s.powers[st][0][32 * i + lane] = (uint8_t)ks[i];
-          s.powers[st][1][32 * i + lane] = (uint8_t)vs[i];
-        }
+        reinterpret_cast<uint32_t*>(s.powers[st][0])[lane] = now.k;
+        reinterpret_cast<uint32_t*>(s.powers[st][1])[lane] = now.v;
+        now = next;
+        next = after;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.full[st]);
         if (++st == (uint32_t)kStages) { st = 0; par ^= 1u; }
       }
     }
+  } else if (warp == kRingWarps + 2) {
+    // ------------------------------------------------ the drafted tokens, at most 16, of pieces that end a segment
+    while (ok && next_piece(a, w, p)) {
+      Sums8<NT, DC> sums;
+      sums.clear();
+      bool bad = false;
+      if (p.t0 + p.n == p.tiles) bad = drafted_8bit<bf16, NT, DC>(t, p.b, p.kvh, 0, 0, 16, query, entry, col, sums);
+      bad = __any_sync(0xffffffffu, bad);
+      ok = leave(sums, kRingWarps, bad);
+      ++uc;
+    }
   } else {
     // ------------------------------------------------ products
-    const int g = lane >> 2, t4 = lane & 3;
-    uint32_t uc = 0;
     // what ldmatrix reads: lane l gives the address of row l % 8 of matrix l / 8; the matrices are the first and last 8
     // of the warp's 16 keys, of a chunk of 16 entries and the next one
     const int key_row = 16 * warp + (lane & 15), chunk0 = lane >> 4;
     const uint32_t row_at = (uint32_t)(key_row * D);
     const uint32_t swizzle = D == 128 ? key_row & 7 : (key_row >> 1) & 3;
     while (ok && next_piece(a, w, p)) {
-      const int* const parents = t.parents ? t.parents + (int64_t)p.b * t.tokens : nullptr;
-      const int rows = t.tokens * t.group;
-      auto query = [&](int r, bool& real) {
-        const int token = r / t.group;
-        real = r < rows && (!parents || parents[token] >= -1);
-        return static_cast<const bf16*>(t.q) + p.b * t.q_b + (real ? token * t.q_t + (p.kvh * t.group + r - token * t.group) * t.q_h : 0);
-      };
-      auto entry = [&](int x) { return 16 * x + 4 * t4; };
-      auto col = [&](int j) { return 16 * j + 2 * g; };
       Queries8<bf16, NT, DC> q;
       q.load(t, query, entry);
       Sums8<NT, DC> sums;
@@ -251,44 +271,21 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
         if (++st == (uint32_t)kStages) { st = 0; par ^= 1u; }
       }
       if (!ok) break;
-      const bool whole = p.t0 + p.n == p.tiles;  // the drafted tokens are this piece's
-      const bool bad = whole && drafted_8bit<bf16, NT, DC>(t, p.b, p.kvh, 0, 16 * warp, 16 * kRingWarps, query, entry, col, sums);
       // ------------------------------------------------ the piece's end: the warps' sums, in their order
-      if (uc > 0 && !tree_wait<true>(&s.read, (uc - 1) & 1u, &s.abort, 54)) { ok = false; break; }
-      if (warp == 0 && lane == 0) s.bad = 0;  // only the first warp has drafted tokens: there are at most 16
-      __syncwarp();
-      if (bad) s.bad = 1;
-#pragma unroll
-      for (int y = 0; y < NT; ++y)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int z = 4; z < 32; z *= 2) sums.l[y][i] += __shfl_xor_sync(0xffffffffu, sums.l[y][i], z);
-          const int r = 8 * y + 2 * t4 + i;
-          if (g == 0) {
-            s.ml[warp][r][0] = sums.m[y][i];
-            s.ml[warp][r][1] = sums.l[y][i];
-          }
-          // O's reference becomes the sums'
-          const float f = sums.mv[y][i] == -INFINITY ? 1.f : fast_exp2(sums.mv[y][i] - kRaise - sums.m[y][i]);
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j)
-            *reinterpret_cast<float2*>(&s.o[warp][r][col(j)]) = make_float2(sums.o[y][j][i] * f, sums.o[y][j][2 + i] * f);
-        }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.joined);
+      if (!leave(sums, warp, false)) { ok = false; break; }
       if (!tree_wait<true>(&s.joined, uc & 1u, &s.abort, 55)) { ok = false; break; }
-      const bool cut = !(p.t0 == 0 && whole);
+      const int* const parents = parents_of();
+      const bool whole = p.t0 + p.n == p.tiles, cut = !(p.t0 == 0 && whole);
       const int slot = 2 * (int)blockIdx.x + (p.t0 == 0 ? 1 : 0);
       for (int i = threadIdx.x; i < 8 * NT * (D / 4); i += 32 * kRingWarps) {
         const int r = i / (D / 4), c = (i - r * (D / 4)) * 4;
         if (r >= rows) break;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < kRingWarps; ++k) top = fmaxf(top, s.ml[k][r][0]);
+        for (int k = 0; k <= kRingWarps; ++k) top = fmaxf(top, s.ml[k][r][0]);
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < kRingWarps; ++k) {
+        for (int k = 0; k <= kRingWarps; ++k) {
           const float mk = s.ml[k][r][0], lk = s.ml[k][r][1];
           if (mk == -INFINITY && lk == 0.f) continue;  // nothing seen (a sum of NaN: only NaN was)
           const float f = mk == top ? 1.f : fast_exp2(mk - top);

@@ -138,7 +138,7 @@ struct TreeSmem {
   uint8_t k[kRingK][kTileBytes];
   uint8_t v[kRingV][kTileBytes];
   uint8_t raw[kRaw][C8 ? 2 : 1][C8 ? kRawBytes : 16];
-  uint8_t powers[kRaw][2][C8 ? kTile : 4];  // of the rows, as they are in the cache
+  alignas(4) uint8_t powers[kRaw][2][C8 ? kTile : 4];  // of the rows, as they are in the cache
   uint64_t raw_full[kRaw], raw_empty[kRaw];
   uint64_t q_full, q_empty;
   uint64_t k_full[kRingK], k_empty[kRingK], k_land[kRingK];  // land: the copies of a tile that is mended before it is full
@@ -266,6 +266,42 @@ __device__ __forceinline__ Walk tree_plan(const TcArgs& a) {
   w.end_t = __shfl_sync(0xffffffffu, t, 1);
   return w;
 }
+
+// The powers of two of four rows of a tile of a cache in 8 bits, from 4 times the lane on: where they are, then
+// their codes, a byte each.
+struct Powers {
+  int page[4];  // -1: none
+  uint32_t k, v;
+  // Where blocks and pages end on multiples of four rows, the four have one place.
+  static __device__ __forceinline__ bool alike(const TcArgs& a) { return a.block % 4 == 0; }
+  __device__ __forceinline__ void find(const TcArgs& a, const Piece& p, int tile, int end) {
+    const int key = tile * kTile + 4 * (threadIdx.x & 31);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      page[i] = -1;
+      if ((i && alike(a)) || tile >= end || key + i >= p.len) continue;
+      const int pg = a.tables[(int64_t)p.b * a.max_pages + (key + i) / a.page];
+      if ((uint32_t)pg < (uint32_t)a.pages) page[i] = pg;
+    }
+  }
+  __device__ __forceinline__ void load(const TcArgs& a, const Piece& p, int tile) {
+    const int key = tile * kTile + 4 * (threadIdx.x & 31);
+    k = v = 0x7f7f7f7fu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (page[i] < 0) continue;
+      const int64_t at = ((int64_t)page[i] * a.kv_heads + p.kvh) * a.per_page + (key + i) % a.page / a.block;
+      const uint32_t x = a.k_scales[at], y = a.v_scales[at];
+      if (alike(a)) {
+        k = x * 0x01010101u;
+        v = y * 0x01010101u;
+      } else {
+        k = (k & ~(0xffu << (8 * i))) | x << (8 * i);
+        v = (v & ~(0xffu << (8 * i))) | y << (8 * i);
+      }
+    }
+  }
+};
 
 // C8: the cache holds e4m3 numbers with powers of two for blocks of rows. The TMA warps then fetch its tiles as
 // they are, warp 11 looks up their rows' powers of two, and warps 12-15 (two for the keys, two for the values) turn
@@ -416,38 +452,19 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     Piece p;
     while (ok && next_piece(a, w, p)) {
       const int end = min(p.t0 + p.n, (p.len + kTile - 1) / kTile);
-      auto find = [&](int t, int (&at)[4]) {  // where the powers of this lane's four rows of tile t are; -1: nowhere
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = t * kTile + 32 * i + lane;
-          at[i] = -1;
-          if (t >= end || key >= p.len) continue;
-          const int pi = key / a.page, pg = a.tables[(int64_t)p.b * a.max_pages + pi];
-          if ((uint32_t)pg < (uint32_t)a.pages) at[i] = pg;
-        }
-      };
-      int page[4], next[4];
-      find(p.t0, page);
-      for (int t = p.t0; t < end; ++t) {
-        find(t + 1, next);
-        uint32_t ks[4], vs[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = t * kTile + 32 * i + lane;
-          ks[i] = vs[i] = 127u;
-          if (page[i] >= 0) {
-            const int64_t at = ((int64_t)page[i] * a.kv_heads + p.kvh) * a.per_page + (key % a.page) / a.block;
-            ks[i] = a.k_scales[at];
-            vs[i] = a.v_scales[at];
-          }
-          page[i] = next[i];
-        }
-        if (!tree_wait<C8>(&s.raw_empty[st], par ^ 1u, &s.abort, 12)) { ok = false; break; }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s.powers[st][0][C8 ? 32 * i + lane : 0] = (uint8_t)ks[i];
-          s.powers[st][1][C8 ? 32 * i + lane : 0] = (uint8_t)vs[i];
-        }
+      Powers now, next;  // tables two tiles ahead, powers one
+      now.find(a, p, p.t0, end);
+      next.find(a, p, p.t0 + 1, end);
+      now.load(a, p, p.t0);
+      for (int x = p.t0; x < end; ++x) {
+        Powers after;
+        after.find(a, p, x + 2, end);
+        next.load(a, p, x + 1);
+        if (!tree_wait<true>(&s.raw_empty[st], par ^ 1u, &s.abort, 12)) { ok = false; break; }
+        reinterpret_cast<uint32_t*>(s.powers[st][0])[C8 ? lane : 0] = now.k;
+        reinterpret_cast<uint32_t*>(s.powers[st][1])[C8 ? lane : 0] = now.v;
+        now = next;
+        next = after;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.raw_full[st]);
         if (++st == Smem::kRaw) { st = 0; par ^= 1u; }
