@@ -343,20 +343,25 @@ struct Queries8 {
   static constexpr bool kF32 = sizeof(T) == 4;
   uint32_t hi[NT][4 * DC][2], lo[NT][kF32 ? 4 * DC : 1][2];
   float factor[NT][2];
+  typename Four<T>::type raw[NT][4 * DC];  // as they lie
   template <typename Query, typename Entry>
-  __device__ __forceinline__ void load(const TreeArgs& a, Query query, Entry entry) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  __device__ __forceinline__ void fetch(const TreeArgs& a, Query query, Entry entry) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       bool real;
-      const T* const qp = query(8 * t + g, real);
-      typename Four<T>::type raw[4 * DC];
+      const T* const qp = query(8 * t + ((threadIdx.x & 31) >> 2), real);
+#pragma unroll
+      for (int s = 0; s < 4 * DC; ++s) raw[t][s] = load_four(qp + entry(s), real && entry(s) < a.d, qp);
+    }
+  }
+  __device__ __forceinline__ void turn(const TreeArgs& a) {
+    const int t4 = threadIdx.x & 3;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
       float top = 0.f;
 #pragma unroll
-      for (int s = 0; s < 4 * DC; ++s) raw[s] = load_four(qp + entry(s), real && entry(s) < a.d, qp);
-#pragma unroll
       for (int s = 0; s < 4 * DC; ++s) {
-        const float4 x = in_f32(raw[s]);
+        const float4 x = in_f32(raw[t][s]);
         for (float y : {x.x, x.y, x.z, x.w}) top = fmaxf(top, fabsf(y) < INFINITY ? fabsf(y) : 0.f);
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -368,7 +373,7 @@ struct Queries8 {
       factor[t][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
 #pragma unroll
       for (int s = 0; s < 4 * DC; ++s) {
-        float4 x = in_f32(raw[s]);
+        float4 x = in_f32(raw[t][s]);
         x = make_float4(x.x * up, x.y * up, x.z * up, x.w * up);
         hi[t][s][0] = half_pair(x.x, x.y);
         hi[t][s][1] = half_pair(x.z, x.w);
@@ -415,7 +420,8 @@ attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
   // Four consecutive entries of the lane's: step s takes those at entry(s).
   auto entry = [&](int s) { return (t4 + 4 * (s >> 2)) * 16 + (s & 3) * 4; };
   Queries8<T, NT, DC> q;
-  q.load(a, query, entry);
+  q.fetch(a, query, entry);
+  q.turn(a);
 
   Sums8<NT, DC> rows_of_sums;
   rows_of_sums.clear();

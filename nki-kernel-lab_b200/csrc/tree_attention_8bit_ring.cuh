@@ -36,6 +36,115 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t at) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
+// The drafted tokens, at most 16, of a piece that ends a segment, by one warp, as drafted_8bit has it; but the loads go
+// out together, the ancestors are followed from lane to lane, and k and v stay in bf16. It is short because it runs
+// cold, between the others' products: instructions that are not there yet cost it more than memory.
+template <int NT, int DC>
+__device__ __forceinline__ bool drafted_few(const TreeArgs& t, const Piece& p, Sums8<NT, DC>& sums) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int64_t from = p.b * t.n_b + p.kvh * t.n_h;
+  const bf16* const kn = static_cast<const bf16*>(t.k_new) + from;
+  const bf16* const vn = static_cast<const bf16*>(t.v_new) + from;
+  const bf16* const qn = static_cast<const bf16*>(t.q) + p.b * t.q_b;
+  const int up0 = lane >= t.tokens ? -2 : t.parents ? t.parents[(int64_t)p.b * t.tokens + lane] : lane - 1;  // this lane's token
+  uint2 kr[4 * DC][2], qr[4 * DC][NT];
+  uint32_t v[4 * DC][4];
+  int token_of[NT];
+#pragma unroll
+  for (int y = 0; y < NT; ++y) {
+    const int r = 8 * y + g, token = r / t.group;
+    const bool real = r < t.tokens * t.group;
+    token_of[y] = real ? token : 31;  // its `up` is -2
+    const bf16* const row = qn + (real ? token * t.q_t + (p.kvh * t.group + r - token * t.group) * t.q_h : 0);
+#pragma unroll
+    for (int s = 0; s < 4 * DC; ++s) qr[s][y] = *reinterpret_cast<const uint2*>(row + 16 * s + 4 * t4);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const bf16* const row = kn + min(8 * k + g, t.tokens - 1) * t.n_t + 4 * t4;
+#pragma unroll
+    for (int s = 0; s < 4 * DC; ++s) kr[s][k] = *reinterpret_cast<const uint2*>(row + 16 * s);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bf16* const row = vn + min(2 * t4 + (i & 1) + 8 * (i >> 1), t.tokens - 1) * t.n_t + 2 * g;
+#pragma unroll
+    for (int j = 0; j < 4 * DC; ++j) v[j][i] = *reinterpret_cast<const uint32_t*>(row + 16 * j);
+  }
+  uint32_t seen = 0u;  // the tokens that this lane's sees, itself one of them
+  {
+    int at = lane, up = up0;
+    bool on = up >= -1;
+    while (__any_sync(0xffffffffu, on)) {
+      if (on) seen |= 1u << at;
+      on = on && up >= 0 && up < at;  // not the root, nor a parent that comes later, which is none
+      if (on) at = up;
+      up = __shfl_sync(0xffffffffu, up0, at);
+      on = on && up >= -1;  // an absent parent ends the path
+    }
+  }
+  float x[NT][4] = {};
+#pragma unroll
+  for (int y = 0; y < NT; ++y) {
+    const bool real = __shfl_sync(0xffffffffu, up0, token_of[y]) >= -1;  // rows that are none, or absent, stay unread
+#pragma unroll
+    for (int s = 0; s < 4 * DC; ++s) {
+      const uint32_t ka[4] = {kr[s][0].x, kr[s][1].x, kr[s][0].y, kr[s][1].y};
+      mma_b16(x[y], ka, real ? qr[s][y].x : 0u, real ? qr[s][y].y : 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 8 * y + 2 * t4 + i;
+      const uint32_t bits = __shfl_sync(0xffffffffu, seen, r < t.tokens * t.group ? r / t.group : 31);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) x[y][2 * k + i] = (bits >> (8 * k + g)) & 1u ? x[y][2 * k + i] * (t.scale * kLog2e) : -INFINITY;
+    }
+  }
+  const float none[2] = {0.f, 0.f};
+  sums.weigh(x, none);
+  uint32_t w[NT][2][2];  // the weights in two parts
+#pragma unroll
+  for (int y = 0; y < NT; ++y)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float a = x[y][2 * k], b = x[y][2 * k + 1];
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(a, b);
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(a - __low2float(hi), b - __high2float(hi));
+      w[y][0][k] = transpose(*reinterpret_cast<const uint32_t*>(&hi));
+      w[y][1][k] = transpose(*reinterpret_cast<const uint32_t*>(&lo));
+    }
+  // weights of 0 must meet no infinity: v that are not finite, or of absent tokens, are left out here
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool here = __shfl_sync(0xffffffffu, up0, 2 * t4 + (i & 1) + 8 * (i >> 1)) >= -1;
+#pragma unroll
+    for (int j = 0; j < 4 * DC; ++j) {
+      if (!here) v[j][i] = 0u;
+      bad |= (v[j][i] & 0x7f80u) == 0x7f80u || (v[j][i] & 0x7f800000u) == 0x7f800000u;
+    }
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  if (bad)
+#pragma unroll
+    for (int j = 0; j < 4 * DC; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if ((v[j][i] & 0x7f80u) == 0x7f80u) v[j][i] &= 0xffff0000u;
+        if ((v[j][i] & 0x7f800000u) == 0x7f800000u) v[j][i] &= 0xffffu;
+      }
+#pragma unroll
+  for (int j = 0; j < 4 * DC; ++j) {
+    const uint32_t va[4] = {__byte_perm(v[j][0], v[j][1], 0x5410), __byte_perm(v[j][0], v[j][1], 0x7632),
+                            __byte_perm(v[j][2], v[j][3], 0x5410), __byte_perm(v[j][2], v[j][3], 0x7632)};
+#pragma unroll
+    for (int y = 0; y < NT; ++y)
+#pragma unroll
+      for (int z = 1; z >= 0; --z) mma_b16(sums.o[y][j], va, w[y][z][0], w[y][z][1]);
+  }
+  return bad;
+}
+
 // t: the call, for the drafted tokens and the queries; a: the plan's view of it, whose `tokens` says that the
 // drafted tokens have a tile of their own.
 template <int D, int NT>
@@ -79,12 +188,14 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
 
   // the piece's query rows, where a row of 16 entries' products lies, and the sums' columns
   const int rows = t.tokens * t.group, g = lane >> 2, t4 = lane & 3;
-  auto parents_of = [&] { return t.parents ? t.parents + (int64_t)p.b * t.tokens : nullptr; };
-  auto query = [&](int r, bool& real) {
-    const int token = r / t.group;
-    const int* const parents = parents_of();
-    real = r < rows && (!parents || parents[token] >= -1);
-    return static_cast<const bf16*>(t.q) + p.b * t.q_b + (real ? token * t.q_t + (p.kvh * t.group + r - token * t.group) * t.q_h : 0);
+  auto parents_of = [&](const Piece& p) { return t.parents ? t.parents + (int64_t)p.b * t.tokens : nullptr; };
+  auto queries_of = [&](const Piece& p) {
+    return [&](int r, bool& real) {
+      const int token = r / t.group;
+      const int* const parents = parents_of(p);
+      real = r < rows && (!parents || parents[token] >= -1);
+      return static_cast<const bf16*>(t.q) + p.b * t.q_b + (real ? token * t.q_t + (p.kvh * t.group + r - token * t.group) * t.q_h : 0);
+    };
   };
   auto entry = [&](int x) { return 16 * x + 4 * t4; };
   auto col = [&](int j) { return 16 * j + 2 * g; };
@@ -190,8 +301,7 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
       Sums8<NT, DC> sums;
       sums.clear();
       bool bad = false;
-      if (p.t0 + p.n == p.tiles) bad = drafted_8bit<bf16, NT, DC>(t, p.b, p.kvh, 0, 0, 16, query, entry, col, sums);
-      bad = __any_sync(0xffffffffu, bad);
+      if (p.t0 + p.n == p.tiles) bad = drafted_few(t, p, sums);
       ok = leave(sums, kRingWarps, bad);
       ++uc;
     }
@@ -202,9 +312,13 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
     const int key_row = 16 * warp + (lane & 15), chunk0 = lane >> 4;
     const uint32_t row_at = (uint32_t)(key_row * D);
     const uint32_t swizzle = D == 128 ? key_row & 7 : (key_row >> 1) & 3;
-    while (ok && next_piece(a, w, p)) {
-      Queries8<bf16, NT, DC> q;
-      q.load(t, query, entry);
+    Queries8<bf16, NT, DC> q;
+    Piece next = {};
+    bool more = next_piece(a, w, next);
+    if (more) q.fetch(t, queries_of(next), entry);
+    while (ok && more) {
+      p = next;
+      q.turn(t);
       Sums8<NT, DC> sums;
       sums.clear();
       const int end = cached_end();
@@ -272,9 +386,11 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
       }
       if (!ok) break;
       // ------------------------------------------------ the piece's end: the warps' sums, in their order
+      more = next_piece(a, w, next);
+      if (more) q.fetch(t, queries_of(next), entry);  // on their way while the sums meet
       if (!leave(sums, warp, false)) { ok = false; break; }
       if (!tree_wait<true>(&s.joined, uc & 1u, &s.abort, 55)) { ok = false; break; }
-      const int* const parents = parents_of();
+      const int* const parents = parents_of(p);
       const bool whole = p.t0 + p.n == p.tiles, cut = !(p.t0 == 0 && whole);
       const int slot = 2 * (int)blockIdx.x + (p.t0 == 0 ? 1 : 0);
       for (int i = threadIdx.x; i < 8 * NT * (D / 4); i += 32 * kRingWarps) {
