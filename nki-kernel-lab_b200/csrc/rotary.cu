@@ -24,6 +24,7 @@
 // cache is one warp's, which holds its rows as they were read, finds the largest magnitude, and
 // turns and rounds them then.
 #include <algorithm>
+#include <atomic>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -33,12 +34,14 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPasses = 8;       // of a warp's lanes over the rows that it holds
+constexpr int kHeld = 8192;      // bytes of rows that a warp holds, at most
 constexpr int kMaxTokens = 32;   // whose angles are held at a time
 constexpr int kMaxHead = 256;
 constexpr int kMaxHead8 = 128;   // in 8 bits: as the attention
 constexpr int kLowest = -100;    // of the powers of two
 constexpr uint8_t kNanScale = 255;
+
+constexpr int kMostSmem = 2 * kMaxTokens * (kMaxHead / 2) * 4 + kWarps * kHeld;
 
 enum Kind { kPlain, kSame, kBits8 };  // where rows go: no cache, one of their type, one of 8 bits
 
@@ -53,6 +56,7 @@ struct RotaryArgs {
   int batch, tokens, heads, kv_heads, d, half, layers, pages, page, max_pages, block;
   int group, groups;  // tokens of a thread block; thread blocks of a sequence
   int chunk;          // tokens whose angles are held at a time
+  int buffer, two;    // bytes of a warp's rows; whether it has two such buffers
   int per_token;      // whether positions are given for each token
   int splits;         // thread blocks that share the heads of a group
   int inverse;
@@ -87,41 +91,65 @@ struct Part {
     if (!INTER && o1 >= 0) y = *reinterpret_cast<const V*>(row + o1);
   }
   static __device__ __forceinline__ void unpack(const V& x, float (&a)[VE]) {
-    const T* const e = reinterpret_cast<const T*>(&x);
+    const uint32_t* const w = reinterpret_cast<const uint32_t*>(&x);
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) a[i] = to_f32(e[i]);
+      for (int i = 0; i < VE; ++i) a[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE / 2; ++i) {
+        a[2 * i] = __uint_as_float(w[i] << 16);
+        a[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
   }
   static __device__ __forceinline__ V pack(const float (&a)[VE]) {
     V x;
-    T* const e = reinterpret_cast<T*>(&x);
+    uint32_t* const w = reinterpret_cast<uint32_t*>(&x);
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) e[i] = from_f32<T>(a[i]);
+      for (int i = 0; i < VE; ++i) w[i] = __float_as_uint(a[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE / 2; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a[2 * i], a[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
     return x;
   }
-  // The entries at o0 and o1, turned by the token's cosines and sines c and s.
-  __device__ __forceinline__ void turn(const V& x, const V& y, const float* c, const float* s, float (&a)[VE], float (&b)[VE]) const {
-    unpack(x, a);
+  // The cosines and sines of its pairs, of a token's c and s.
+  static constexpr int kPairs = INTER ? VE / 2 : VE;
+  struct Angles {
+    float c[kPairs], s[kPairs];
+  };
+  __device__ __forceinline__ void load(const float* c, const float* s, Angles& to) const {
     if (f < 0) return;
-    if (INTER) {
+    if constexpr (kPairs % 4 == 0) {  // f is a multiple of 4
 #pragma unroll
-      for (int i = 0; i < VE; i += 2) {
-        const float co = c[f + i / 2], si = s[f + i / 2], p = a[i], q = a[i + 1];
-        a[i] = p * co - q * si;
-        a[i + 1] = q * co + p * si;
+      for (int i = 0; i < kPairs; i += 4) {
+        *reinterpret_cast<float4*>(to.c + i) = *reinterpret_cast<const float4*>(c + f + i);
+        *reinterpret_cast<float4*>(to.s + i) = *reinterpret_cast<const float4*>(s + f + i);
       }
     } else {
-      unpack(y, b);
 #pragma unroll
-      for (int i = 0; i < VE; i += 4) {
-        const float4 co = *reinterpret_cast<const float4*>(c + f + i), si = *reinterpret_cast<const float4*>(s + f + i);
-        const float cs[4] = {co.x, co.y, co.z, co.w}, sn[4] = {si.x, si.y, si.z, si.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = a[i + j], q = b[i + j];
-          a[i + j] = p * cs[j] - q * sn[j];
-          b[i + j] = q * cs[j] + p * sn[j];
-        }
+      for (int i = 0; i < kPairs; ++i) {
+        to.c[i] = c[f + i];
+        to.s[i] = s[f + i];
       }
+    }
+  }
+  // The entries at o0 and o1, turned.
+  __device__ __forceinline__ void turn(const V& x, const V& y, const Angles& by, float (&a)[VE], float (&b)[VE]) const {
+    unpack(x, a);
+    if (f < 0) return;
+    if (!INTER) unpack(y, b);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      float &u = INTER ? a[2 * i] : a[i], &w = INTER ? a[2 * i + 1] : b[i];
+      const float p = u, q = w;
+      u = p * by.c[i] - q * by.s[i];
+      w = q * by.c[i] + p * by.s[i];
     }
   }
   __device__ __forceinline__ void store(T* row, const float (&a)[VE], const float (&b)[VE]) const {
@@ -130,6 +158,19 @@ struct Part {
   }
 };
 
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_landed() {  // all but the last N groups
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN (0x7fffffff) if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // e4m3 codes of VE values times 2^-e.
@@ -237,47 +278,59 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
   auto rows = [&](int t0, int n, bool ready) {
     const int all = a.heads + (KIND == kSame ? 2 * a.kv_heads : 0);
     const int h0 = (int)((int64_t)all * blockIdx.y / a.splits), h1 = (int)((int64_t)all * (blockIdx.y + 1) / a.splits);
+    // A thread stays with its entries and with a token, whose cosines and sines it keeps, and goes from head to head.
+    // (Counting rows through, with divisions for token and head and the cosines from shared memory for each: 29
+    // instructions to a pair, and 112 us for 4 x 4096 tokens of 64 heads of 128; so 85.)
     const int per = kThreads / items, row0 = tid / items;
+    const int tokens = min(n, per), step = per / tokens;  // tokens of a pass, and its heads
+    const int my_t = row0 % tokens, my_h = row0 / tokens;
     const P part(tid - row0 * items, a.half);
-    const int end = row0 < per ? (h1 - h0) * n : 0;
     constexpr int kAhead = 4;
-    for (int r0 = row0; r0 < end || !ready; r0 += kAhead * per) {
-      V x[kAhead], y[kAhead];
+    for (int ts = 0; ts < n; ts += tokens) {
+      const int t = t0 + ts + my_t;
+      const bool on = row0 < per && my_h < step && ts + my_t < n;
+      const T* const q_t = q + t * a.q_t;
+      const T* const kv_t = k + t * a.n_t;
+      T* const out = static_cast<T*>(a.q_out) + ((int64_t)b * a.tokens + t) * a.heads * a.d;
+      T* const k_out = static_cast<T*>(a.k_out) + ((int64_t)b * a.tokens + t) * a.kv_heads * a.d;
+      const int at = len + t, page = KIND == kSame && on && t < count ? page_of(at) : -1;
+      const int64_t cached = KIND == kSame ? page * a.c_p + (at % a.page) * a.c_s : 0;
+      typename P::Angles by;
+      for (int hb = h0; hb < h1 || !ready; hb += kAhead * step) {
+        V x[kAhead], y[kAhead];
 #pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        const int r = r0 + s * per;
-        if (r >= end) continue;
-        const int h = h0 + r / n, t = t0 + r % n;
-        const T* from = h < a.heads ? q + t * a.q_t + h * a.q_h
-                        : h < a.heads + a.kv_heads ? k + t * a.n_t + (h - a.heads) * a.n_h
-                                                   : v + t * a.n_t + (h - a.heads - a.kv_heads) * a.n_h;
-        part.load(from, x[s], y[s]);
-      }
-      if (!ready) {  // the first rows are on their way while the angles are computed
-        fill_angles(t0, n);
-        __syncthreads();
-        ready = true;
-      }
-#pragma unroll
-      for (int s = 0; s < kAhead; ++s) {
-        const int r = r0 + s * per;
-        if (r >= end) continue;
-        const int h = h0 + r / n, t = t0 + r % n;
-        float e[VE], o[VE];
-        if (KIND == kSame && h >= a.heads + a.kv_heads) {
-          P::unpack(x[s], e);
-          if (!INTER && part.o1 >= 0) P::unpack(y[s], o);
-        } else {
-          part.turn(x[s], y[s], cosines + (t - t0) * a.half, sines + (t - t0) * a.half, e, o);
+        for (int s = 0; s < kAhead; ++s) {
+          const int h = hb + my_h + s * step;
+          if (!on || h >= h1) continue;
+          const T* from = q_t + h * a.q_h;
+          if (KIND == kSame && h >= a.heads)
+            from = h < a.heads + a.kv_heads ? kv_t + (h - a.heads) * a.n_h : v + t * a.n_t + (h - a.heads - a.kv_heads) * a.n_h;
+          part.load(from, x[s], y[s]);
         }
-        if (h < a.heads) part.store(static_cast<T*>(a.q_out) + (((int64_t)b * a.tokens + t) * a.heads + h) * a.d, e, o);
-        if (KIND == kSame && h >= a.heads) {
-          const bool key = h < a.heads + a.kv_heads;
-          const int g = h - a.heads - (key ? 0 : a.kv_heads);
-          if (key) part.store(static_cast<T*>(a.k_out) + (((int64_t)b * a.tokens + t) * a.kv_heads + g) * a.d, e, o);
-          const int at = len + t, p = t < count ? page_of(at) : -1;
-          if (p >= 0)
-            part.store(static_cast<T*>(key ? a.k_cache : a.v_cache) + p * a.c_p + g * a.c_h + (at % a.page) * a.c_s, e, o);
+        if (!ready) {  // the first rows are on their way while the angles are computed
+          fill_angles(t0, n);
+          __syncthreads();
+          ready = true;
+        }
+        if (hb == h0 && on) part.load(cosines + (t - t0) * a.half, sines + (t - t0) * a.half, by);
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s) {
+          const int h = hb + my_h + s * step;
+          if (!on || h >= h1) continue;
+          float e[VE], o[VE];
+          if (KIND == kSame && h >= a.heads + a.kv_heads) {
+            P::unpack(x[s], e);
+            if (!INTER && part.o1 >= 0) P::unpack(y[s], o);
+          } else {
+            part.turn(x[s], y[s], by, e, o);
+          }
+          if (h < a.heads) part.store(out + h * a.d, e, o);
+          if (KIND == kSame && h >= a.heads) {
+            const bool key = h < a.heads + a.kv_heads;
+            const int g = h - a.heads - (key ? 0 : a.kv_heads);
+            if (key) part.store(k_out + g * a.d, e, o);
+            if (page >= 0) part.store(static_cast<T*>(key ? a.k_cache : a.v_cache) + cached + g * a.c_h, e, o);
+          }
         }
       }
     }
@@ -295,7 +348,9 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
   const int units = 2 * a.kv_heads * subs;
   const int u0 = (int)((int64_t)units * blockIdx.y / a.splits), u1 = (int)((int64_t)units * (blockIdx.y + 1) / a.splits);
   const int nb = a.page / a.block;  // blocks of a page
-  V x[kPasses], y[kPasses];
+  // a warp's two buffers of rows, dense, filled 16 bytes at a time
+  uint8_t* const held = reinterpret_cast<uint8_t*>(sines + a.chunk * a.half) + (a.two + 1) * warp * a.buffer;
+  const int row_bytes = a.d * (int)sizeof(T), chunks = row_bytes / 16, per_c = 32 / chunks, row_c = lane / chunks;
   struct Unit {
     bool key;
     int g, p0;  // head, first position
@@ -310,58 +365,59 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
     const int r = path ? path[j] : j;
     return r >= 0 && r < a.tokens ? r : -1;
   };
-  // The rows of tokens t0 .. t0 + n - 1 (n <= kPasses * per) to x and y.
-  auto fetch = [&](const Unit& u, int t0, int n) {
-#pragma unroll
-    for (int s = 0; s < kPasses; ++s) {
-      const int t = s * per + row0;
-      if (s * per >= n) break;
-      x[s] = V{};
-      y[s] = V{};
-      if (row0 >= per || t >= n) continue;
-      const bool out = u.key && a.k_out;
-      const int r = out ? t0 + t : source(t0 + t);
-      if (r >= 0) part.load((u.key ? k : v) + r * a.n_t + u.g * a.n_h, x[s], y[s]);
+  // The rows of tokens t0 .. t0 + n - 1 into a buffer, as one group of copies.
+  auto fetch = [&](const Unit& u, int t0, int n, int buf) {
+    const T* const from = (u.key ? k : v) + u.g * a.n_h + (lane - row_c * chunks) * (16 / (int)sizeof(T));
+    uint8_t* const to = held + buf * a.buffer + (lane - row_c * chunks) * 16;
+    for (int t = row_c; t < n && row_c < per_c; t += per_c) {
+      const int r = u.key && a.k_out ? t0 + t : source(t0 + t);
+      if (r >= 0) copy16(to + t * row_bytes, from + r * a.n_t);
     }
+    copies_issued();
   };
-  auto values = [&](const Unit& u, int s, int t, float (&e)[VE], float (&o)[VE]) {
+  // Row t of a buffer, token t + t0, whose angles are the chunk's at c, turned.
+  auto values = [&](const Unit& u, const uint8_t* rows, int t, int c, float (&e)[VE], float (&o)[VE]) {
+    V x, y;
+    part.load(reinterpret_cast<const T*>(rows + t * row_bytes), x, y);
     if (u.key && a.freqs) {
-      part.turn(x[s], y[s], cosines + t * a.half, sines + t * a.half, e, o);
+      typename P::Angles by;
+      part.load(cosines + c * a.half, sines + c * a.half, by);
+      part.turn(x, y, by, e, o);
     } else {
-      P::unpack(x[s], e);
-      if (!INTER && part.o1 >= 0) P::unpack(y[s], o);
+      P::unpack(x, e);
+      if (!INTER && part.o1 >= 0) P::unpack(y, o);
     }
   };
-  // Their largest magnitude's bits, of those that go to the cache; turned keys to k_out.
-  auto largest = [&](const Unit& u, int t0, int n, int c0) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int s = 0; s < kPasses; ++s) {
-      const int t = s * per + row0;
-      if (s * per >= n) break;
-      if (row0 >= per || t >= n) continue;
+  // The largest magnitude's bits, of the rows that go to the cache; turned keys to k_out.
+  auto largest = [&](const Unit& u, int t0, int n, int c0, int buf) {
+    float top = 0.f;
+    T* const k_out = static_cast<T*>(a.k_out) + (((int64_t)b * a.tokens + t0) * a.kv_heads + u.g) * a.d;
+    const int64_t k_row = (int64_t)a.kv_heads * a.d;
+#pragma unroll 2
+    for (int t = row0; t < n && row0 < per; t += per) {
+      const bool cached = source(t0 + t) >= 0, out = u.key && a.k_out;
+      if (!cached && !out) continue;  // not read
       float e[VE], o[VE];
-      values(u, s, t0 + t - c0, e, o);
-      if (u.key && a.k_out) part.store(static_cast<T*>(a.k_out) + (((int64_t)b * a.tokens + t0 + t) * a.kv_heads + u.g) * a.d, e, o);
-      if (source(t0 + t) < 0) continue;
+      values(u, held + buf * a.buffer, t, t0 + t - c0, e, o);
+      if (out) part.store(k_out + t * k_row, e, o);
+      if (!cached) continue;
 #pragma unroll
       for (int z = 0; z < VE; ++z) {
-        top = max(top, __float_as_uint(e[z]) & 0x7fffffffu);
-        if (!INTER && part.o1 >= 0) top = max(top, __float_as_uint(o[z]) & 0x7fffffffu);
+        top = max_nan(top, fabsf(e[z]));
+        if (!INTER && part.o1 >= 0) top = max_nan(top, fabsf(o[z]));
       }
     }
-    return __reduce_max_sync(0xffffffffu, top);
+    return __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   };
-  auto write = [&](const Unit& u, int t0, int n, int c0, uint8_t* rows8, int code) {
+  auto write = [&](const Unit& u, int t0, int n, int c0, int buf, uint8_t* rows8, int code) {
     const float inv = code == kNanScale ? 0.f : power_of_two(127 - code);
-#pragma unroll
-    for (int s = 0; s < kPasses; ++s) {
-      const int t = s * per + row0;
-      if (s * per >= n) break;
-      if (row0 >= per || t >= n || source(t0 + t) < 0) continue;
+    uint8_t* const to0 = rows8 + (u.p0 % a.page + len + t0 - u.p0) * a.c_s;
+#pragma unroll 2
+    for (int t = row0; t < n && row0 < per; t += per) {
+      if (source(t0 + t) < 0) continue;
       float e[VE], o[VE];
-      values(u, s, t0 + t - c0, e, o);
-      uint8_t* const to = rows8 + ((len + t0 + t) % a.page) * a.c_s;
+      values(u, held + buf * a.buffer, t, t0 + t - c0, e, o);
+      uint8_t* const to = to0 + t * a.c_s;
       store_codes<VE>(to + part.o0, e, inv);
       if (!INTER && part.o1 >= 0) store_codes<VE>(to + part.o1, o, inv);
     }
@@ -399,28 +455,50 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
   };
   // whether any row of the tokens [t0, t1) goes to the cache (an accepted path may leave rows out)
   auto any_row = [&](int t0, int t1) {
+    if (!path) return t0 < count;
     bool any = false;
     for (int t = t0 + lane; t < t1; t += 32) any |= source(t) >= 0;
     return __any_sync(0xffffffffu, any) != 0;
   };
   if (a.group <= a.chunk) {  // the blocks' rows are held
+    auto span = [&](const Unit& u, int& t0) {  // its tokens
+      t0 = max(u.p0 - len, 0);
+      return min(u.p0 + a.block - len, j1) - t0;
+    };
+    auto fetch_unit = [&](int z, int buf) {
+      int t0;
+      const Unit u = unit_of(min(z, units - 1));
+      const int n = span(u, t0);
+      fetch(u, t0, z < u1 ? n : 0, buf);
+    };
+    fetch_unit(u0 + warp, 0);  // on their way while the queries are turned
     if (a.q) {
       rows(j0, j1 - j0, false);
     } else {
       fill_angles(j0, j1 - j0);
       __syncthreads();
     }
+    int buf = 0;
     for (int z = u0 + warp; z < u1; z += kWarps) {
       const Unit u = unit_of(z);
-      const int t0 = max(u.p0 - len, 0), n = min(u.p0 + a.block - len, j1) - t0;
-      if (n <= 0) continue;
-      fetch(u, t0, n);
-      uint8_t *rows8, *scale;
-      const bool there = place(u, rows8, scale) && any_row(t0, t0 + n);
-      const uint32_t top = largest(u, t0, n, j0);
-      if (!there) continue;
-      const int code = settle(u, top, rows8, scale);
-      write(u, t0, n, j0, rows8, code);
+      int t0;
+      const int n = span(u, t0);
+      if (a.two) {
+        fetch_unit(z + kWarps, buf ^ 1);
+        copies_landed<1>();
+      } else {
+        copies_landed<0>();
+      }
+      __syncwarp();
+      if (n > 0) {
+        uint8_t *rows8, *scale;
+        const bool there = place(u, rows8, scale) && any_row(t0, t0 + n);
+        const uint32_t top = largest(u, t0, n, j0, buf);
+        if (there) write(u, t0, n, j0, buf, rows8, settle(u, top, rows8, scale));
+      }
+      __syncwarp();  // the buffer is read
+      if (a.two) buf ^= 1;
+      else fetch_unit(z + kWarps, 0);
     }
     return;
   }
@@ -443,16 +521,18 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
         uint8_t *rows8, *scale;
         const bool there = place(u, rows8, scale) && any_row(j0, j1);
         if (pass == 1 && !there) continue;
-        fetch(u, c0, n);
+        fetch(u, c0, n, 0);
+        copies_landed<0>();
+        __syncwarp();
         if (pass == 0) {
-          const uint32_t top = max(largest(u, c0, n, c0), s_top[z - u0]);
+          const uint32_t top = max(largest(u, c0, n, c0, 0), s_top[z - u0]);
           __syncwarp();
           if (lane == 0) s_top[z - u0] = top;
         } else {
           int code;
           if (c0 == j0) code = settle(u, s_top[z - u0], rows8, scale);
           else code = *scale;
-          write(u, c0, n, c0, rows8, code);
+          write(u, c0, n, c0, 0, rows8, code);
         }
         __syncwarp();
       }
@@ -461,6 +541,21 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------ host
+
+template <auto Kernel>
+int launch_kernel(const RotaryArgs& a, dim3 grid, size_t smem, cudaStream_t st, const char* op) {
+  if (smem > 48 * 1024) {
+    static std::atomic<bool> set[64] = {};  // per device: the shared memory attribute is set (idempotent)
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
+      const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+      if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+      if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
+    }
+  }
+  return launch_pdl(Kernel, grid, dim3(kThreads), smem, st, op, a);
+}
 
 // Vectors of 16 bytes, or of 8 where the half layout's pairs are not so many bytes apart.
 template <typename T, int KIND>
@@ -472,10 +567,12 @@ int launch_rotary(RotaryArgs& a, bool interleaved, cudaStream_t st, const char* 
   if (KIND == kBits8) {
     // 16 tokens to a thread block where the cache's blocks are short
     const int subs = std::max(1, 16 / a.block);
-    const int held = std::min(kMaxTokens, kPasses * (32 / items));
+    const int row_bytes = a.d * (int)sizeof(T), held = std::min(kMaxTokens, kHeld / row_bytes);
     a.group = a.block <= held ? a.block * subs : a.block;
     a.chunk = a.group <= kMaxTokens ? (a.block <= held ? a.group : held) : held;
     a.groups = (a.tokens + a.group - 2) / a.group + 1;
+    a.buffer = std::min(a.block, held) * row_bytes;
+    a.two = a.buffer <= kHeld / 2;
   } else {
     // Tokens share a thread block's launch and the angles' latency where there are enough of them.
     a.group = 1;
@@ -491,13 +588,12 @@ int launch_rotary(RotaryArgs& a, bool interleaved, cudaStream_t st, const char* 
   while (a.splits < 16 && blocks * a.splits * 2 <= 2LL * sm_count() && heads * a.group * items >= 2LL * a.splits * kThreads) a.splits *= 2;
   if (KIND == kBits8 && a.group > a.chunk)  // s_top
     while ((2 * a.kv_heads + a.splits - 1) / a.splits > 512) ++a.splits;
-  const size_t smem = (size_t)2 * a.chunk * a.half * 4;
+  const size_t smem = (size_t)2 * a.chunk * a.half * 4 + (size_t)(a.two + 1) * kWarps * a.buffer;
   const dim3 grid((unsigned)blocks, (unsigned)a.splits);
-  auto go = [&](auto* kernel) { return launch_pdl(kernel, grid, dim3(kThreads), smem, st, op, a); };
-  if (interleaved) return go(rotary_kernel<T, full, true, KIND>);
+  if (interleaved) return launch_kernel<rotary_kernel<T, full, true, KIND>>(a, grid, smem, st, op);
   if constexpr (full == 8)
-    if (ve == 4) return go(rotary_kernel<T, 4, false, KIND>);
-  return go(rotary_kernel<T, full, false, KIND>);
+    if (ve == 4) return launch_kernel<rotary_kernel<T, 4, false, KIND>>(a, grid, smem, st, op);
+  return launch_kernel<rotary_kernel<T, full, false, KIND>>(a, grid, smem, st, op);
 }
 
 template <int KIND>

@@ -36,7 +36,8 @@ constexpr int kBins = 1024;       // of the first round: 992 are used
 constexpr int kParts = 512;       // of a range, in the rounds after it
 constexpr int kList = 768;        // tokens of a range that are gathered
 constexpr int kStep = 128;        // tokens that a warp looks at at once, four to a lane
-constexpr int kPerBlock = 45056;  // tokens that a block holds: 176 KB; blocks of up to 16384 go two to an SM
+constexpr int kPerBlock = 45056;  // tokens that a block holds: 176 KB; blocks of up to kPerHalf go two to an SM
+constexpr int kPerHalf = 16384;
 constexpr int kTable = 256;
 constexpr u64 kOne = 1ull << 31;
 constexpr u64 kNone = ~0ull;
@@ -737,11 +738,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 template <typename T>
 int launch_sample(SampleArgs& a, cudaStream_t st) {
   const char* op = "nkl_sample";
-  // Blocks to a row: as many as its keys need; more, up to eight, as long as there are no more than two for
-  // each SM and each has 1024 keys.
+  // Blocks to a row: as many as it takes for two blocks to fit on an SM (fp32 128 x 131072 121 us with 8, 124 with 4);
+  // more, up to eight, as long as no SM gets a third block and each has 2048 tokens (64 x 32768 22 us with 4, 28 with 2, 37
+  // with 8; 16 x 8192 13.8 with 4, 15.7 with 8; one row of 32768 14 with 8, 29 with 1).
   int blocks = 1;
-  while (blocks < kMaxCluster && ((a.vocab + blocks - 1) / blocks > kPerBlock ||
-                                  ((int64_t)a.batch * blocks * 2 <= 2LL * sm_count() && a.vocab >= 2 * blocks * 1024)))
+  while (blocks < kMaxCluster && (a.vocab > blocks * kPerHalf ||
+                                  ((int64_t)a.batch * blocks <= sm_count() && a.vocab >= 4096 * blocks)))
     blocks *= 2;
   a.part = ((a.vocab + blocks - 1) / blocks + kWarps * kStep - 1) / (kWarps * kStep) * (kWarps * kStep);
   const size_t smem = (size_t)a.part * 4;

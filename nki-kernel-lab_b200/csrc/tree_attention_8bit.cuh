@@ -23,9 +23,6 @@
 
 namespace {
 
-#ifndef KMIN8
-#define KMIN8 4
-#endif
 constexpr int kThreads8 = 128;
 constexpr int kWarps8 = kThreads8 / 32;
 constexpr int kWindow = 32;     // keys that a warp looks up at a time
@@ -94,8 +91,16 @@ __device__ __forceinline__ void bf16_parts(float lo, float hi, uint32_t (&p)[N])
   }
 }
 
+// 2^x for a whole number, 0 below 2^-126.
+constexpr float kRound = 12582912.f;  // 1.5 2^23: added, it rounds to whole numbers
+__device__ __forceinline__ float power2(float x) {
+  return __uint_as_float(__float_as_uint(fminf(fmaxf(x, -127.f), 127.f) + (kRound + 127.f)) << 23);
+}
+
 // The sums of a lane: rows 2 t4 and 2 t4 + 1 (the last index of m, mv, l) of NT tiles of 8 query rows. m: the
-// rows' reference for sums l of 2^(s - m), over the lane's keys; mv: that for O, sums of 2^(s + e - mv + kRaise) v.
+// rows' reference for sums l of 2^(s - m), over the lane's keys; mv: that for O, sums of 2^(s + e - mv + kRaise) v. Both
+// are whole numbers, and a power of two comes to a weight by its exponent alone: the weights' bits do not depend on how a
+// block's numbers are shared out between e4m3 codes and their power of two, which changes when the block grows.
 // O's products j hold two entries of a head: o[t][j][i] and o[t][j][2 + i].
 template <int NT, int DC>
 struct Sums8 {
@@ -130,6 +135,8 @@ struct Sums8 {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
             tv = fmaxf(tv, __shfl_xor_sync(0xffffffffu, tv, z));
           }
+          top = floorf(top);
+          tv = floorf(tv);
           if (top > m[t][i] + kLag8) {  // a row goes by its own scores alone
             l[t][i] *= fast_exp2(m[t][i] - top);
             m[t][i] = top;
@@ -154,8 +161,14 @@ struct Sums8 {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           float& s = x[t][2 * k + i];
-          l[t][i] += fast_exp2(s - rm);
-          s = fast_exp2(s + e[k] - rv);
+          const float z = s - rm, d = e[k] + (rm - rv), p = fast_exp2(z);
+          l[t][i] += p;
+          if (d <= 100.f) {  // where p is 0, so is p 2^d in f16
+            s = p * power2(d);
+          } else {  // v's block has by far the largest numbers: p may be 0 too early; or d is NaN
+            const float least = z < -2000.f ? -2000.f : z, whole = least + kRound - kRound;
+            s = (fast_exp2(least - whole) + (d - d)) * power2(whole + d);
+          }
         }
       }
   }
@@ -390,7 +403,7 @@ struct Queries8 {
 // DC: head_dim up to 64 DC. FAST: pages and blocks are multiples of 16 positions, so that the 16 keys of a
 // product lie in a row and share their powers of two. NT: tiles of 8 query rows to a warp.
 template <typename T, int DC, bool FAST, int NT>
-__global__ void __launch_bounds__(kThreads8, NT == 1 && sizeof(T) == 2 ? KMIN8 : 2)
+__global__ void __launch_bounds__(kThreads8, NT == 1 && sizeof(T) == 2 ? 4 : 2)
 attention_8bit_kernel(const __grid_constant__ Bits8Args args) {
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr int kCols = 8 * DC;          // entries of V that a lane has of a key
@@ -665,13 +678,7 @@ Shape8 shape_8bit(int64_t rows) {
 
 // Blocks that share a sequence's keys, of at least two windows to a warp, as long as there are no
 // more than kRoom8 for each SM where all sequences are as long as the tables allow.
-#ifndef KROOM8
-#define KROOM8 4
-#endif
-#ifndef KLEAST8
-#define KLEAST8 2
-#endif
-constexpr int kRoom8 = KROOM8, kLeast8 = KLEAST8;
+constexpr int kRoom8 = 4, kLeast8 = 2;
 int64_t splits_8bit(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity) {
   const Shape8 s = shape_8bit(rows);
   const int64_t windows = std::max<int64_t>((capacity + kWindow - 1) / kWindow, 1);

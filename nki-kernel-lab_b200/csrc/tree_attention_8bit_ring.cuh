@@ -277,23 +277,15 @@ attention_8bit_ring_kernel(const __grid_constant__ CUtensorMap map_kc, const __g
     // ------------------------------------------------ the rows' powers of two
     while (ok && next_piece(a, w, p)) {
       const int end = cached_end();
-      Powers now, next;  // tables two tiles ahead, powers one
-      now.find(a, p, p.t0, end);
-      next.find(a, p, p.t0 + 1, end);
-      now.load(a, p, p.t0);
-      for (int x = p.t0; x < end; ++x) {
-        Powers after;
-        after.find(a, p, x + 2, end);
-        next.load(a, p, x + 1);
-        if (!tree_wait<true>(&s.empty[st], par ^ 1u, &s.abort, 52)) { ok = false; break; }
-        reinterpret_cast<uint32_t*>(s.powers[st][0])[lane] = now.k;
-        reinterpret_cast<uint32_t*>(s.powers[st][1])[lane] = now.v;
-        now = next;
-        next = after;
+      ok = put_powers(a, p, end, [&](uint32_t k, uint32_t v) {
+        if (!tree_wait<true>(&s.empty[st], par ^ 1u, &s.abort, 52)) return false;
+        reinterpret_cast<uint32_t*>(s.powers[st][0])[lane] = k;
+        reinterpret_cast<uint32_t*>(s.powers[st][1])[lane] = v;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.full[st]);
         if (++st == (uint32_t)kStages) { st = 0; par ^= 1u; }
-      }
+        return true;
+      });
     }
   } else if (warp == kRingWarps + 2) {
     // ------------------------------------------------ the drafted tokens, at most 16, of pieces that end a segment

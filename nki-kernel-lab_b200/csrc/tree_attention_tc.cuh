@@ -267,41 +267,77 @@ __device__ __forceinline__ Walk tree_plan(const TcArgs& a) {
   return w;
 }
 
-// The powers of two of four rows of a tile of a cache in 8 bits, from 4 times the lane on: where they are, then
-// their codes, a byte each.
-struct Powers {
-  int page[4];  // -1: none
-  uint32_t k, v;
-  // Where blocks and pages end on multiples of four rows, the four have one place.
-  static __device__ __forceinline__ bool alike(const TcArgs& a) { return a.block % 4 == 0; }
-  __device__ __forceinline__ void find(const TcArgs& a, const Piece& p, int tile, int end) {
-    const int key = tile * kTile + 4 * (threadIdx.x & 31);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      page[i] = -1;
-      if ((i && alike(a)) || tile >= end || key + i >= p.len) continue;
-      const int pg = a.tables[(int64_t)p.b * a.max_pages + (key + i) / a.page];
-      if ((uint32_t)pg < (uint32_t)a.pages) page[i] = pg;
+// The powers of two of a piece's cached tiles up to `end`, tile by tile: put(k, v) gets the codes of the four rows from
+// 4 times the lane on, a byte each, and says whether to go on. Where blocks are multiples of four rows, the four have
+// one place: kBatch tiles' codes are read while those before them are put and the tables for the ones after are on
+// their way, as a tile must not wait for a load (one tile ahead: a decoding step over 32 sequences of up to 8192
+// positions took 107 us, so 80; 64 drafted tokens over 2 x 65536 took 190, so 186).
+template <typename Put>
+__device__ __forceinline__ bool put_powers(const TcArgs& a, const Piece& p, int end, Put put) {
+  constexpr int kBatch = 4;
+  const int row = 4 * (threadIdx.x & 31);
+  const int* const table = a.tables + (int64_t)p.b * a.max_pages;
+  auto code_at = [&](int page, int key) { return ((int64_t)page * a.kv_heads + p.kvh) * a.per_page + key % a.page / a.block; };
+  if (a.block % 4) {
+    for (int x = p.t0; x < end; ++x) {
+      uint32_t k = 0x7f7f7f7fu, v = 0x7f7f7f7fu;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const int key = x * kTile + row + i;
+        const int page = key < p.len ? table[key / a.page] : -1;
+        if ((uint32_t)page >= (uint32_t)a.pages) continue;
+        const int64_t at = code_at(page, key);
+        k = (k & ~(0xffu << (8 * i))) | (uint32_t)a.k_scales[at] << (8 * i);
+        v = (v & ~(0xffu << (8 * i))) | (uint32_t)a.v_scales[at] << (8 * i);
+      }
+      if (!put(k, v)) return false;
     }
+    return true;
   }
-  __device__ __forceinline__ void load(const TcArgs& a, const Piece& p, int tile) {
-    const int key = tile * kTile + 4 * (threadIdx.x & 31);
-    k = v = 0x7f7f7f7fu;
+  int page[kBatch];
+  uint32_t k[kBatch], v[kBatch], next_k[kBatch], next_v[kBatch];
+  auto look_up = [&](int x0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (page[i] < 0) continue;
-      const int64_t at = ((int64_t)page[i] * a.kv_heads + p.kvh) * a.per_page + (key + i) % a.page / a.block;
-      const uint32_t x = a.k_scales[at], y = a.v_scales[at];
-      if (alike(a)) {
-        k = x * 0x01010101u;
-        v = y * 0x01010101u;
-      } else {
-        k = (k & ~(0xffu << (8 * i))) | x << (8 * i);
-        v = (v & ~(0xffu << (8 * i))) | y << (8 * i);
+    for (int i = 0; i < kBatch; ++i) {
+      const int key = (x0 + i) * kTile + row;
+      page[i] = x0 + i < end && key < p.len ? table[key / a.page] : -1;
+    }
+  };
+  auto read = [&](int x0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      next_k[i] = next_v[i] = 127u;
+      if ((uint32_t)page[i] < (uint32_t)a.pages) {
+        const int64_t at = code_at(page[i], (x0 + i) * kTile + row);
+        next_k[i] = a.k_scales[at];
+        next_v[i] = a.v_scales[at];
+      }
+    }
+  };
+  look_up(p.t0);
+  read(p.t0);
+  look_up(p.t0 + kBatch);
+#pragma unroll 1
+  for (int x0 = p.t0; x0 < end; x0 += kBatch) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      k[i] = next_k[i];
+      v[i] = next_v[i];
+    }
+    read(x0 + kBatch);
+    look_up(x0 + 2 * kBatch);
+#pragma unroll 1
+    for (int x = x0; x < min(x0 + kBatch, end); ++x) {
+      if (!put(k[0] * 0x01010101u, v[0] * 0x01010101u)) return false;
+#pragma unroll
+      for (int i = 0; i + 1 < kBatch; ++i) {
+        k[i] = k[i + 1];
+        v[i] = v[i + 1];
       }
     }
   }
-};
+  return true;
+}
 
 // C8: the cache holds e4m3 numbers with powers of two for blocks of rows. The TMA warps then fetch its tiles as
 // they are, warp 11 looks up their rows' powers of two, and warps 12-15 (two for the keys, two for the values) turn
@@ -452,23 +488,15 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     Piece p;
     while (ok && next_piece(a, w, p)) {
       const int end = min(p.t0 + p.n, (p.len + kTile - 1) / kTile);
-      Powers now, next;  // tables two tiles ahead, powers one
-      now.find(a, p, p.t0, end);
-      next.find(a, p, p.t0 + 1, end);
-      now.load(a, p, p.t0);
-      for (int x = p.t0; x < end; ++x) {
-        Powers after;
-        after.find(a, p, x + 2, end);
-        next.load(a, p, x + 1);
-        if (!tree_wait<true>(&s.raw_empty[st], par ^ 1u, &s.abort, 12)) { ok = false; break; }
-        reinterpret_cast<uint32_t*>(s.powers[st][0])[C8 ? lane : 0] = now.k;
-        reinterpret_cast<uint32_t*>(s.powers[st][1])[C8 ? lane : 0] = now.v;
-        now = next;
-        next = after;
+      ok = put_powers(a, p, end, [&](uint32_t k, uint32_t v) {
+        if (!tree_wait<true>(&s.raw_empty[st], par ^ 1u, &s.abort, 12)) return false;
+        reinterpret_cast<uint32_t*>(s.powers[st][0])[C8 ? lane : 0] = k;
+        reinterpret_cast<uint32_t*>(s.powers[st][1])[C8 ? lane : 0] = v;
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.raw_full[st]);
         if (++st == Smem::kRaw) { st = 0; par ^= 1u; }
-      }
+        return true;
+      });
     }
   } else if (C8 && warp >= kConvertWarp) {
     // ------------------------------------------------ 8 bits to bf16: two warps for the keys, two for the
