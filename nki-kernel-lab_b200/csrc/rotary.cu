@@ -264,10 +264,13 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
       else at = a.per_token ? a.positions[(int64_t)b * a.tokens + t0 + t] : a.positions[b] + t0 + t;
       double turns = (double)at * a.freqs[f] * 0.15915494309189533577;  // 1 / (2 pi)
       turns -= rint(turns);
+      // what the rounding to 32 bits leaves of the angle, up to 1.9e-7, is put right to first order
+      const float near = (float)turns, rest = (float)(turns - (double)near) * 6.2831853f;
       float s, c;
-      sincospif(2.f * (float)turns, &s, &c);
-      cosines[x] = c * a.magnitude;
-      sines[x] = (a.inverse ? -s : s) * a.magnitude;
+      sincospif(2.f * near, &s, &c);
+      cosines[x] = fmaf(-s, rest, c) * a.magnitude;
+      const float sine = fmaf(c, rest, s) * a.magnitude;
+      sines[x] = a.inverse ? -sine : sine;
     }
   };
   const T* const q = static_cast<const T*>(a.q) + b * a.q_b;

@@ -19,6 +19,12 @@
 // scaled by a power of two per row, so that f16 holds it; fp32 queries and weights are two f16
 // numbers. Both maxima may lag behind by 2^8: sums are rescaled when a row's grow by more.
 // The drafted tokens' own k and v multiply in bf16, fp32 ones in three parts.
+//
+// This kernel takes fp32 and the bf16 layouts that neither tree_attention_8bit_ring.cuh (up to 16 query rows to a
+// key/value head) nor tree_attention_tc.cuh does. Measured, fp32: 1 token, 16 sequences of up to 4000, 32 heads over 8 of
+// 128 67 us (15 by bytes), 7 tokens, 5 of up to 1999, 8 heads over 4 of 64 24 us: queries and weights are two f16 numbers
+// each, so that a product is two, or three with the first's rest; bf16, 3 tokens, 4 of up to 3000, 12 heads over 4 of 80
+// 18 us. What bounds it is issue: converting and interleaving a tile costs more than its products.
 #pragma once
 
 namespace {

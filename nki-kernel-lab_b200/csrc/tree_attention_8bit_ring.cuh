@@ -10,6 +10,20 @@
 //             for the values, two entries of a key at a time, which __byte_perm pairs with the next key's), sums of
 //             their own; at a piece's end the sums meet in shared memory, while the ring goes on
 // Segments that are cut leave (max, sum, O) of a piece in the workspace for tree_join_kernel.
+//
+// Measured against the kernel of tree_attention_8bit.cuh on the same calls, GPU time with the join (32 heads over 8 of
+// 128 but where it says so):
+//   1 token, 203 positions                                7.2 and 11 us
+//   1 token, 32 sequences of up to 8192                    84 and 150 us (60 by bytes)
+//   1 token, 65536 positions                               41 and 49 us (20 by bytes)
+//   1 token, 64 sequences of about 700                     37 and 35 us (10 by bytes)
+//   4 tokens, 8 sequences of up to 4096                    34 and 47 us (6 by bytes)
+//   16 tokens, 4 sequences of up to 4096, 32 heads of 128  50 and 70 us (12 by bytes)
+// so every call that it can take goes here. What bounds it: on long rows the products' warps, 1130 cycles to a tile of 32
+// KB, of which the conversions to f16 and the products with one, two or three eighths of their columns in use are most;
+// on short ones a piece's beginning and end (5000 cycles) and the start: plan, tables and the first tiles take 7000. More
+// than eight such warps do not fit: their sums are 64 or 128 registers each. The drafted tokens by one of the eight warps at
+// a piece's end instead of by warp 10: 32 sequences 117 us for 109, 203 positions 11.8 for 7.8 (at that time).
 #pragma once
 
 namespace {
