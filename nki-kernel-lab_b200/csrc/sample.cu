@@ -18,6 +18,13 @@
 // is. Up to 768 tokens of that range go to every block, by distributed shared memory, and each finds
 // the end among them for itself; more are taken apart by histograms over 512 parts of the range, added up over
 // the blocks, and so on, until a part is one weight. Of equal ones as many stay as it takes, by logit and then by index.
+//
+// Measured (temperature 0.8, top-p 0.95): fp32: one row of 32768 14 us, 64 rows of 131072 63 us (34 MB: 5 us by bytes),
+// with settings of their own, some of which need no filter, 46. What bounds it is the chain of phases: maximum -> weights and histogram -> the end's range ->
+// its tokens -> sums -> draw, each with a barrier of the block, most with one of the cluster (1700 to 2000 cycles), and
+// 69 instructions to 32 tokens in the first two, of which the weights' powers take most. With 64-bit
+// atomics in the histogram (which loop) instead of two of 32 it took 291 us, with further rounds over the cluster instead of the
+// list of a range's tokens 79.
 #include <algorithm>
 #include <atomic>
 

@@ -47,6 +47,13 @@
 // positions 126 and 3250 us. NQ = 2 against NQ = 1 with the keys read by two blocks, 256 rows: up
 // to 65536 positions 126 and 149 us, about 5000 79 and 78 us, 240 rows of 64 over up to 5809
 // positions 19.5 and 18.5 us: it gains where rows are long and costs little where they are not.
+//
+// Over a cache in 8 bits (C8) the tiles come as bytes, and four more warps turn them to bf16 for the tensor core (e4m3 has
+// no place beside bf16 in one product; a value's power of two is an exponent's addition). 64 tokens, 2 sequences of up to
+// 65536, 32 heads over 8 of 128: 186 us alone, 200 in a stream of calls (65 us by operations; the kernel of
+// tree_attention_8bit.cuh 997). The converting warps wait for instructions more than for
+// the pipes: their loop unrolled once instead of in full took 207 -> 189 us, and eight of them instead of four 187.5 for 189.
+// The rest is the chain of a bf16 tile, 126 us alone.
 #pragma once
 
 namespace {
