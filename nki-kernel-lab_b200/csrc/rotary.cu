@@ -78,23 +78,22 @@ template <> struct Raw<bf16, 4> { typedef uint2 type; };
 template <typename T, int VE, bool INTER>
 struct Part {
   typedef typename Raw<T, VE>::type V;
-  int o0, o1, f;  // f: the first pair; -1: entries that stay as they are
+  int o0, o1, f;  // o1: o0 where there are none; f: the first pair, -1: entries that stay as they are
   __device__ __forceinline__ Part(int item, int half) {
-    o1 = -1;
     if (INTER) {
-      o0 = item * VE;
+      o1 = o0 = item * VE;
       f = o0 < 2 * half ? o0 / 2 : -1;
     } else {
       const int pairs = half / VE;
       o0 = item < pairs ? item * VE : 2 * half + (item - pairs) * VE;
       f = item < pairs ? o0 : -1;
-      if (item < pairs) o1 = o0 + half;
+      o1 = item < pairs ? o0 + half : o0;
     }
   }
   static __device__ __forceinline__ int items(int d, int half) { return INTER ? d / VE : half / VE + (d - 2 * half) / VE; }
   __device__ __forceinline__ void load(const T* row, V& x, V& y) const {
     x = *reinterpret_cast<const V*>(row + o0);
-    if (!INTER && o1 >= 0) y = *reinterpret_cast<const V*>(row + o1);
+    if (!INTER) y = *reinterpret_cast<const V*>(row + o1);
   }
   static __device__ __forceinline__ void unpack(const V& x, float (&a)[VE]) {
     const uint32_t* const w = reinterpret_cast<const uint32_t*>(&x);
@@ -148,8 +147,8 @@ struct Part {
   // The entries at o0 and o1, turned.
   __device__ __forceinline__ void turn(const V& x, const V& y, const Angles& by, float (&a)[VE], float (&b)[VE]) const {
     unpack(x, a);
-    if (f < 0) return;
     if (!INTER) unpack(y, b);
+    if (f < 0) return;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       float &u = INTER ? a[2 * i] : a[i], &w = INTER ? a[2 * i + 1] : b[i];
@@ -160,12 +159,12 @@ struct Part {
   }
   __device__ __forceinline__ void store(T* row, const float (&a)[VE], const float (&b)[VE]) const {
     *reinterpret_cast<V*>(row + o0) = pack(a);
-    if (!INTER && o1 >= 0) *reinterpret_cast<V*>(row + o1) = pack(b);
+    if (!INTER) *reinterpret_cast<V*>(row + o1) = pack(b);
   }
 };
 
-__device__ __forceinline__ void copy16(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -329,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
           float e[VE], o[VE];
           if (KIND == kSame && h >= a.heads + a.kv_heads) {
             P::unpack(x[s], e);
-            if (!INTER && part.o1 >= 0) P::unpack(y[s], o);
+            if (!INTER) P::unpack(y[s], o);
           } else {
             part.turn(x[s], y[s], by, e, o);
           }
@@ -365,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
     int g, p0;  // head, first position
   };
   auto unit_of = [&](int u) {
-    const int sub = u / (2 * a.kv_heads), kg = u - sub * 2 * a.kv_heads;
+    const int sub = subs == 1 ? 0 : u / (2 * a.kv_heads), kg = u - sub * 2 * a.kv_heads;
     return Unit{kg < a.kv_heads, kg < a.kv_heads ? kg : kg - a.kv_heads, first + sub * a.block};
   };
   // source row of token j for the cache, -1: none
@@ -374,61 +373,76 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
     const int r = path ? path[j] : j;
     return r >= 0 && r < a.tokens ? r : -1;
   };
-  // The rows of tokens t0 .. t0 + n - 1 into a buffer, as one group of copies.
+  // Of the tokens t0 .. t0 + n - 1, how many a unit looks at: without a path those that go to the cache are the first.
+  auto kept = [&](int t0, int n) { return path ? n : min(n, count - t0); };
+  // Their rows into a buffer, as one group of copies.
   auto fetch = [&](const Unit& u, int t0, int n, int buf) {
-    const T* const from = (u.key ? k : v) + u.g * a.n_h + (lane - row_c * chunks) * (16 / (int)sizeof(T));
-    uint8_t* const to = held + buf * a.buffer + (lane - row_c * chunks) * 16;
-    for (int t = row_c; t < n && row_c < per_c; t += per_c) {
-      const int r = u.key && a.k_out ? t0 + t : source(t0 + t);
-      if (r >= 0) copy16(to + t * row_bytes, from + r * a.n_t);
+    const bool out = u.key && a.k_out;
+    const int m = row_c < per_c ? (out ? n : kept(t0, n)) : 0, col = lane - row_c * chunks;
+    const T* const from = (u.key ? k : v) + u.g * a.n_h + col * (16 / (int)sizeof(T));
+    uint32_t to = (uint32_t)__cvta_generic_to_shared(held + buf * a.buffer) + (uint32_t)(row_c * row_bytes + col * 16);
+    if (out || !path) {
+      const T* row = from + (t0 + row_c) * a.n_t;
+      const int64_t step = per_c * a.n_t;
+      for (int t = row_c; t < m; t += per_c, row += step, to += per_c * row_bytes) copy16(to, row);
+    } else {
+      for (int t = row_c; t < m; t += per_c, to += per_c * row_bytes)
+        if (const int r = source(t0 + t); r >= 0) copy16(to, from + r * a.n_t);
     }
     copies_issued();
   };
-  // Row t of a buffer, token t + t0, whose angles are the chunk's at c, turned.
-  auto values = [&](const Unit& u, const uint8_t* rows, int t, int c, float (&e)[VE], float (&o)[VE]) {
+  // A row of a buffer, turned by the cosines and sines at c and s.
+  auto values = [&](bool turned, const uint8_t* row, const float* c, const float* s, float (&e)[VE], float (&o)[VE]) {
     V x, y;
-    part.load(reinterpret_cast<const T*>(rows + t * row_bytes), x, y);
-    if (u.key && a.freqs) {
+    part.load(reinterpret_cast<const T*>(row), x, y);
+    if (turned) {
       typename P::Angles by;
-      part.load(cosines + c * a.half, sines + c * a.half, by);
+      part.load(c, s, by);
       part.turn(x, y, by, e, o);
     } else {
       P::unpack(x, e);
-      if (!INTER && part.o1 >= 0) P::unpack(y, o);
+      if (!INTER) P::unpack(y, o);
     }
   };
-  // The largest magnitude's bits, of the rows that go to the cache; turned keys to k_out.
+  // The largest magnitude's bits, of the rows that go to the cache; turned keys to k_out. c0: the chunk's first token.
   auto largest = [&](const Unit& u, int t0, int n, int c0, int buf) {
     float top = 0.f;
-    T* const k_out = static_cast<T*>(a.k_out) + (((int64_t)b * a.tokens + t0) * a.kv_heads + u.g) * a.d;
+    const bool out = u.key && a.k_out, turned = u.key && a.freqs;
+    const int nc = kept(t0, n), m = row0 < per ? (out ? n : nc) : 0;
     const int64_t k_row = (int64_t)a.kv_heads * a.d;
+    T* to = static_cast<T*>(a.k_out) + (((int64_t)b * a.tokens + t0 + row0) * a.kv_heads + u.g) * a.d;
+    const uint8_t* row = held + buf * a.buffer + row0 * row_bytes;
+    const float *c = cosines + (t0 + row0 - c0) * a.half, *s = c + (sines - cosines);
 #pragma unroll 2
-    for (int t = row0; t < n && row0 < per; t += per) {
-      const bool cached = source(t0 + t) >= 0, out = u.key && a.k_out;
-      if (!cached && !out) continue;  // not read
+    for (int t = row0; t < m; t += per, row += per * row_bytes, to += per * k_row, c += per * a.half, s += per * a.half) {
+      if (path && !out && source(t0 + t) < 0) continue;  // not read
       float e[VE], o[VE];
-      values(u, held + buf * a.buffer, t, t0 + t - c0, e, o);
-      if (out) part.store(k_out + t * k_row, e, o);
-      if (!cached) continue;
+      values(turned, row, c, s, e, o);
+      if (out) part.store(to, e, o);
+      float most = 0.f;
 #pragma unroll
       for (int z = 0; z < VE; ++z) {
-        top = max_nan(top, fabsf(e[z]));
-        if (!INTER && part.o1 >= 0) top = max_nan(top, fabsf(o[z]));
+        most = max_nan(most, fabsf(e[z]));
+        if (!INTER) most = max_nan(most, fabsf(o[z]));
       }
+      if (path ? source(t0 + t) >= 0 : t < nc) top = max_nan(top, most);
     }
     return __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   };
   auto write = [&](const Unit& u, int t0, int n, int c0, int buf, uint8_t* rows8, int code) {
     const float inv = code == kNanScale ? 0.f : power_of_two(127 - code);
-    uint8_t* const to0 = rows8 + (u.p0 % a.page + len + t0 - u.p0) * a.c_s;
+    const bool turned = u.key && a.freqs;
+    const int m = row0 < per ? kept(t0, n) : 0;
+    uint8_t* to = rows8 + (len + t0 - u.p0 + row0) * a.c_s;
+    const uint8_t* row = held + buf * a.buffer + row0 * row_bytes;
+    const float *c = cosines + (t0 + row0 - c0) * a.half, *s = c + (sines - cosines);
 #pragma unroll 2
-    for (int t = row0; t < n && row0 < per; t += per) {
-      if (source(t0 + t) < 0) continue;
+    for (int t = row0; t < m; t += per, row += per * row_bytes, to += per * a.c_s, c += per * a.half, s += per * a.half) {
+      if (path && source(t0 + t) < 0) continue;
       float e[VE], o[VE];
-      values(u, held + buf * a.buffer, t, t0 + t - c0, e, o);
-      uint8_t* const to = to0 + t * a.c_s;
+      values(turned, row, c, s, e, o);
       store_codes<VE>(to + part.o0, e, inv);
-      if (!INTER && part.o1 >= 0) store_codes<VE>(to + part.o1, o, inv);
+      if (!INTER) store_codes<VE>(to + part.o1, o, inv);
     }
   };
   // The block's power of two, given the largest magnitude that comes to it; rows that were in it
@@ -445,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
         const int words = a.d / 4;
         for (int z = lane; z < old * words; z += 32) {
           const int r = z / words, w = z - r * words;
-          uint32_t* const at = reinterpret_cast<uint32_t*>(rows8 + (u.p0 % a.page + r) * a.c_s) + w;
+          uint32_t* const at = reinterpret_cast<uint32_t*>(rows8 + r * a.c_s) + w;
           *at = round_again(*at, factor);
         }
       } else {
@@ -456,11 +470,18 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
     if (lane == 0) *scale = (uint8_t)code;
     return code;
   };
-  auto place = [&](const Unit& u, uint8_t*& rows8, uint8_t*& scale) {
-    const int p = page_of(u.p0);
-    rows8 = static_cast<uint8_t*>(u.key ? a.k_cache : a.v_cache) + layer * a.c_l + max(p, 0) * a.c_p + u.g * a.c_h;
-    scale = (u.key ? a.k_scales : a.v_scales) + (((int64_t)layer * a.pages + max(p, 0)) * a.kv_heads + u.g) * nb + (u.p0 % a.page) / a.block;
-    return p >= 0;
+  int placed = -1, page = -1, in_page = 0, in_scales = 0;  // the place of the last units' first position
+  auto place = [&](const Unit& u, uint8_t*& rows8, uint8_t*& scale) {  // of the block's first row
+    if (u.p0 != placed) {
+      placed = u.p0;
+      page = page_of(u.p0);
+      in_page = u.p0 % a.page;
+      in_scales = in_page / a.block;
+    }
+    const int p = max(page, 0);
+    rows8 = static_cast<uint8_t*>(u.key ? a.k_cache : a.v_cache) + layer * a.c_l + p * a.c_p + u.g * a.c_h + in_page * a.c_s;
+    scale = (u.key ? a.k_scales : a.v_scales) + (((int64_t)layer * a.pages + p) * a.kv_heads + u.g) * nb + in_scales;
+    return page >= 0;
   };
   // whether any row of the tokens [t0, t1) goes to the cache (an accepted path may leave rows out)
   auto any_row = [&](int t0, int t1) {
