@@ -4,7 +4,7 @@
 // a = position * freqs[i], pair i being the entries (i, i + r / 2) or, interleaved, (2 i, 2 i + 1):
 //   y1 = m (x1 cos a - x2 sin a)      y2 = m (x2 cos a + x1 sin a)
 // The rest of the head is copied. The gradient is the same turn by -a. Angles are products in 64
-// bits, taken modulo a full turn before they are rounded to 32, so that far positions lose
+// bits, taken modulo a full turn, as are their sines and cosines, so that far positions lose
 // nothing; freqs come from the caller, who may stretch them for long contexts.
 //
 //   rotary         x -> y
@@ -23,11 +23,13 @@
 // through all threads, each with two vectors at places half of r apart; a block of an 8-bit
 // cache is one warp's, which copies its rows to shared memory as they are, finds the largest magnitude of
 // the turned ones, and turns them again to round them (in fp32 they would not fit into registers; held there in
-// bf16 they were unpacked once for both, and spilled: a prompt of 4 x 4096 239 us, so 190).
+// bf16 they were unpacked once for both, and spilled: a prompt of 4 x 4096 239 us, so 190 at first; places looked up once a
+// block, rows gone through by pointers in loops that are not unrolled: 156). A warp has two buffers of rows where they are
+// of 4 KB or less (168 us with one); three thread blocks to an SM, with 85 registers to a thread, took 187 and more.
 //
 // Measured (6.57 TB/s is what a copy of memory reaches): x and its gradient, bf16, 4 x 4096 tokens of 64 heads of 128
-// 185 us (1.07 GB: 163 by bytes); q, k, v of 32 heads, turned, k and v to a cache in 8 bits, 4 x 4096 tokens 190 us
-// (808 MB: 123), bound by issue: unpacking, turning and rounding take 60 instructions for 16 entries. The smallest calls:
+// 186 us (1.07 GB: 163 by bytes; 183 with sines and cosines in 32 bits); q, k, v of 32 heads, turned, k and v to a cache in 8 bits, 4 x 4096 tokens 156 us
+// (808 MB: 123), bound by issue and by what a thread block's two phases (queries, then blocks) do not overlap. The smallest calls:
 // 2.5 us on the GPU for x alone, 5 to 6 with a cache (lengths -> tables -> rows), and 6 to 9 of the host's.
 #include <algorithm>
 #include <atomic>
@@ -210,6 +212,19 @@ __device__ __forceinline__ uint32_t round_again(uint32_t w, float factor) {
   return out;
 }
 
+// Of an angle given as a part of a turn, in [-1/2, 1/2]: the Taylor series in 64 bits, within an eighth of a turn of the
+// nearest quarter (first terms left out: 7e-12 and 5e-13). In 32 bits they would be off by up to two steps, which
+// brings more keys over the border between two e4m3 numbers than the products' roundings do.
+__device__ __forceinline__ void sine_cosine(double turns, double& sine, double& cosine) {
+  const double quarter = rint(4. * turns), x = (turns - 0.25 * quarter) * 6.283185307179586, z = x * x;
+  const double s = x + x * z * (-1. / 6 + z * (1. / 120 + z * (-1. / 5040 + z * (1. / 362880 - z * (1. / 39916800)))));
+  const double c = 1. + z * (-1. / 2 + z * (1. / 24 + z * (-1. / 720 + z * (1. / 40320 + z * (-1. / 3628800 + z * (1. / 479001600))))));
+  const int q = (int)quarter & 3;
+  const double u = q & 1 ? c : s, v = q & 1 ? s : c;
+  sine = q & 2 ? -u : u;
+  cosine = (q + 1) & 2 ? -v : v;
+}
+
 // Position below its sequence's first of token j: its depth in a tree of drafted tokens (0 for a
 // child of the last cached position, an absent token and a child of one, as in the attention).
 __device__ __forceinline__ int depth_of(const int* parents, int j) {
@@ -269,13 +284,10 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
       else at = a.per_token ? a.positions[(int64_t)b * a.tokens + t0 + t] : a.positions[b] + t0 + t;
       double turns = (double)at * a.freqs[f] * 0.15915494309189533577;  // 1 / (2 pi)
       turns -= rint(turns);
-      // what the rounding to 32 bits leaves of the angle, up to 1.9e-7, is put right to first order
-      const float near = (float)turns, rest = (float)(turns - (double)near) * 6.2831853f;
-      float s, c;
-      sincospif(2.f * near, &s, &c);
-      cosines[x] = fmaf(-s, rest, c) * a.magnitude;
-      const float sine = fmaf(c, rest, s) * a.magnitude;
-      sines[x] = a.inverse ? -sine : sine;
+      double sine, cosine;
+      sine_cosine(turns, sine, cosine);
+      cosines[x] = (float)(cosine * a.magnitude);
+      sines[x] = (float)((a.inverse ? -sine : sine) * a.magnitude);
     }
   };
   const T* const q = static_cast<const T*>(a.q) + b * a.q_b;
@@ -288,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
     const int h0 = (int)((int64_t)all * blockIdx.y / a.splits), h1 = (int)((int64_t)all * (blockIdx.y + 1) / a.splits);
     // A thread stays with its entries and with a token, whose cosines and sines it keeps, and goes from head to head.
     // (Counting rows through, with divisions for token and head and the cosines from shared memory for each: 29
-    // instructions to a pair, and 112 us for 4 x 4096 tokens of 64 heads of 128; so 85.)
+    // instructions to a pair, and 110 us for 4 x 4096 tokens of 64 heads of 128; so 92.)
     const int per = kThreads / items, row0 = tid / items;
     const int tokens = min(n, per), step = per / tokens;  // tokens of a pass, and its heads
     const int my_t = row0 % tokens, my_h = row0 / tokens;
@@ -413,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
     T* to = static_cast<T*>(a.k_out) + (((int64_t)b * a.tokens + t0 + row0) * a.kv_heads + u.g) * a.d;
     const uint8_t* row = held + buf * a.buffer + row0 * row_bytes;
     const float *c = cosines + (t0 + row0 - c0) * a.half, *s = c + (sines - cosines);
-#pragma unroll 2
+#pragma unroll 1
     for (int t = row0; t < m; t += per, row += per * row_bytes, to += per * k_row, c += per * a.half, s += per * a.half) {
       if (path && !out && source(t0 + t) < 0) continue;  // not read
       float e[VE], o[VE];
@@ -436,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
     uint8_t* to = rows8 + (len + t0 - u.p0 + row0) * a.c_s;
     const uint8_t* row = held + buf * a.buffer + row0 * row_bytes;
     const float *c = cosines + (t0 + row0 - c0) * a.half, *s = c + (sines - cosines);
-#pragma unroll 2
+#pragma unroll 1
     for (int t = row0; t < m; t += per, row += per * row_bytes, to += per * a.c_s, c += per * a.half, s += per * a.half) {
       if (path && source(t0 + t) < 0) continue;
       float e[VE], o[VE];
