@@ -684,6 +684,8 @@ Shape8 shape_8bit(int64_t rows) {
 
 // Blocks that share a sequence's keys, of at least two windows to a warp, as long as there are no
 // more than kRoom8 for each SM where all sequences are as long as the tables allow.
+// (bf16, 32 heads over 8 of 128: 8 to an SM, three of them at a time, took 123 us for 150 over 32 sequences of up to
+// 8192 positions, but 47 for 34 over 64 of about 700.)
 constexpr int kRoom8 = 4, kLeast8 = 2;
 int64_t splits_8bit(int64_t batch, int64_t kv_heads, int64_t rows, int64_t capacity) {
   const Shape8 s = shape_8bit(rows);
