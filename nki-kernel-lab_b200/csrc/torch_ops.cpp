@@ -515,6 +515,9 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits_in, const Tensor& uniform
   return {token, prob};
 }
 
+// Whether a forward derivative is on its way through t.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
 // The attention has no backward pass: with inputs that require a gradient, one through it raises.
 Tensor no_backward(Tensor out, const char* name, std::initializer_list<Tensor> inputs) {
   const std::vector<Tensor> in(inputs);
@@ -605,7 +608,13 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 
 Tensor rotary_autograd(const Tensor& x, const Tensor& positions, const Tensor& freqs, OptTensor parents,
                        bool interleaved, double magnitude, bool inverse) {
-  TORCH_CHECK(!torch::autograd::compute_requires_grad(freqs), "nkilab::rotary: freqs have no gradient");
+  TORCH_CHECK(!torch::autograd::compute_requires_grad(freqs) && !has_tangent(freqs), "nkilab::rotary: freqs have no gradient");
+  if (has_tangent(x)) {  // the turn is linear: the tangent turns as its x does
+    const Tensor tangent = rotary_op(x._fw_grad(0), positions, freqs, parents, interleaved, magnitude, inverse);
+    const Tensor out = rotary_autograd(x._fw_primal(0), positions, freqs, parents, interleaved, magnitude, inverse);
+    out._set_fw_grad(tangent, 0, /*is_inplace_op=*/false);
+    return out;
+  }
   if (!torch::autograd::compute_requires_grad(x)) {  // past the graph's bookkeeping: the smallest calls are bound by it
     at::AutoDispatchBelowADInplaceOrView below;
     return rotary_op(x, positions, freqs, parents, interleaved, magnitude, inverse);
