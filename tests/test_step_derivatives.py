@@ -49,12 +49,14 @@ def test_the_forward_derivative_is_the_same_turn(dtype):
 
     out, tangent = torch.func.jvp(call, (x,), (dx,))
     assert torch.equal(out, call(x)) and torch.equal(tangent, call(dx))
-    # forward over reverse: the gradient of (call(t) * y).sum() does not depend on t, that of its square does
-    def half_square(t):
-        return 0.5 * (call(t).float() ** 2).sum()
-
-    grad, moved = torch.func.jvp(torch.func.grad(half_square), (x,), (dx,))
-    assert torch.equal(grad, torch.func.grad(half_square)(x))
+    # forward over reverse: half the sum of squares has the gradient R^T R x, whose derivative along dx is R^T R dx
+    # (torch.func.grad does not take operators with a C++ gradient: it raises)
+    leaf = x.clone().requires_grad_()
+    with fwAD.dual_level():
+        loss = 0.5 * (call(fwAD.make_dual(leaf, dx)).float() ** 2).sum()
+        grad, moved = fwAD.unpack_dual(torch.autograd.grad(loss, leaf)[0])
+        grad, moved = grad.clone(), moved.clone()
+    assert torch.equal(grad, torch.autograd.grad(0.5 * (call(leaf).float() ** 2).sum(), leaf)[0])
     # The turn's transpose after the turn is the magnitude squared. With p = |x1| + |x2| of a pair, the turned entries are up
     # to 1.25 p, rounded by half a step each (bf16 2^-8), and the two turned back again bring 2 x 2^-8 x 1.25^2 p, the
     # last rounding 2^-8 x 1.25^2 p; in fp32 sines, products and sums are some sixteen roundings of 2^-24.
