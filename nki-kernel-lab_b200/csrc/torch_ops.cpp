@@ -518,6 +518,11 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits_in, const Tensor& uniform
 // Whether a forward derivative is on its way through t.
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 
+// An operator without derivatives refuses tangents at the call, before it writes anything.
+void no_tangent(const char* name, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs) TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), name, " has no forward derivative");
+}
+
 // The attention has no backward pass: with inputs that require a gradient, one through it raises.
 Tensor no_backward(Tensor out, const char* name, std::initializer_list<Tensor> inputs) {
   const std::vector<Tensor> in(inputs);
@@ -534,6 +539,7 @@ Tensor no_backward(Tensor out, const char* name, std::initializer_list<Tensor> i
 Tensor attention_tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_cache,
                                const Tensor& v_cache, const Tensor& tables, const Tensor& lens, OptTensor parents,
                                double scale) {
+  no_tangent("nkilab::attention_tree", {&q, &k, &v, &k_cache, &v_cache});
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("nkilab::attention_tree", "")
                              .typed<decltype(attention_tree_autograd)>();
@@ -549,6 +555,7 @@ Tensor attention_tree_autograd(const Tensor& q, const Tensor& k, const Tensor& v
 Tensor attention_tree_8bit_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_cache,
                                     const Tensor& v_cache, const Tensor& k_scales, const Tensor& v_scales,
                                     const Tensor& tables, const Tensor& lens, OptTensor parents, double scale) {
+  no_tangent("nkilab::attention_tree_8bit", {&q, &k, &v});
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("nkilab::attention_tree_8bit", "")
                              .typed<decltype(attention_tree_8bit_autograd)>();
@@ -564,6 +571,8 @@ Tensor attention_tree_8bit_autograd(const Tensor& q, const Tensor& k, const Tens
 std::tuple<Tensor, Tensor> sample_autograd(const Tensor& logits, const Tensor& uniforms, OptTensor temperatures,
                                            OptTensor top_ks, OptTensor top_ps, OptTensor min_ps, double temperature,
                                            int64_t top_k, double top_p, double min_p) {
+  const Tensor t = temperatures.value_or(Tensor());
+  no_tangent("nkilab::sample", {&logits, &t});
   static const auto op =
       c10::Dispatcher::singleton().findSchemaOrThrow("nkilab::sample", "").typed<decltype(sample)>();
   std::tuple<Tensor, Tensor> out;
@@ -571,7 +580,7 @@ std::tuple<Tensor, Tensor> sample_autograd(const Tensor& logits, const Tensor& u
     at::AutoDispatchBelowADInplaceOrView below;
     out = op.call(logits, uniforms, temperatures, top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p);
   }
-  if (torch::autograd::compute_requires_grad(logits)) no_backward(std::get<1>(out), "nkilab::sample", {logits});
+  if (torch::autograd::compute_requires_grad(logits, t)) no_backward(std::get<1>(out), "nkilab::sample", {logits, t});
   return out;
 }
 
@@ -629,6 +638,7 @@ std::tuple<Tensor, Tensor> rotary_append_autograd(const Tensor& q, const Tensor&
                                                   OptTensor v_scales, const Tensor& tables, const Tensor& lens,
                                                   const Tensor& freqs, OptTensor count, bool interleaved,
                                                   double magnitude) {
+  no_tangent("nkilab::rotary_append", {&q, &k, &v, &freqs});
   static const auto op = c10::Dispatcher::singleton()
                              .findSchemaOrThrow("nkilab::rotary_append", "")
                              .typed<decltype(rotary_append)>();

@@ -71,3 +71,36 @@ def test_the_forward_derivative_is_the_same_turn(dtype):
         out = fwAD.unpack_dual(call(fwAD.make_dual(leaf, dx)))
         assert torch.equal(out.tangent, call(dx))
         assert torch.equal(torch.autograd.grad((out.primal * y).sum(), leaf)[0], torch.autograd.grad((call(leaf) * y).sum(), leaf)[0])
+
+
+def others():
+    i32, e4m3, e8m0 = (lambda *s: m(*s, dtype=torch.int32)), m(20, HKV, 16, D, dtype=E4M3), m(20, HKV, 2, dtype=E8M0)
+    q, k, v, f = m(B, T, H, D), m(B, T, HKV, D), m(B, T, HKV, D), m(16, dtype=torch.float64)
+    cache, tables, lens = m(20, HKV, 16, D), i32(B, 3), i32(B)
+    out = []
+    for at in range(3):
+        def put(t, at=at):
+            return tuple(t if i == at else x for i, x in enumerate((q, k, v)))
+
+        x = (q, k, v)[at]
+        out += [(x, lambda t, p=put: ops.attention_tree(*p(t), cache, cache, tables, lens)),
+                (x, lambda t, p=put: ops.attention_tree(*p(t), e4m3, e4m3, tables, lens, None, None, e8m0, e8m0)),
+                (x, lambda t, p=put: ops.rotary_append(*p(t), cache, cache, tables, lens, f)[at % 2]),
+                (x, lambda t, p=put: ops.rotary_append(*p(t), e4m3, e4m3, tables, lens, f, k_scales=e8m0, v_scales=e8m0)[1])]
+    out.append((cache, lambda t: ops.attention_tree(q, k, v, t, cache, tables, lens)))
+    out.append((m(B, 50), lambda t: ops.sample(t, m(B))[1]))
+    out.append((m(B), lambda t: ops.sample(m(B, 50), m(B), t)[1]))
+    return out
+
+
+@pytest.mark.parametrize("at", range(len(others())))
+def test_the_others_raise(at):
+    x, call = others()[at]
+    with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward"):
+        call(fwAD.make_dual(x, torch.empty_like(x)))
+    with pytest.raises(NotImplementedError, match="forward"):
+        torch.func.jvp(call, (x,), (torch.empty_like(x),))
+    out = call(x.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="not implemented"):
+        out.sum().backward()
+    assert not call(x).requires_grad
