@@ -301,10 +301,35 @@ def _as_bf16(*caches):
     return tuple(c.view(torch.bfloat16) if c.dtype == torch.float8_e4m3fn else c for c in caches)
 
 
+def _check_scales(k_cache, v_cache, k_scales, v_scales):
+    """Before pages move: a cache in 8 bits has both scales, one for each block of a page and head, others none."""
+    if (k_scales is None) != (v_scales is None):
+        raise ValueError("scales: need both or none")
+    bits8 = k_scales is not None
+    for c in (k_cache, v_cache):
+        if (c.dtype == torch.float8_e4m3fn) != bits8:
+            raise TypeError(f"a {c.dtype} cache {'with' if bits8 else 'without'} scales")
+    if not bits8:
+        return
+    if k_scales.shape != v_scales.shape:
+        raise ValueError(f"scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}: need equal shapes")
+    for s in (k_scales, v_scales):
+        if s.dtype != torch.float8_e8m0fnu:
+            raise TypeError(f"scales must be float8_e8m0fnu, got {s.dtype}")
+        if s.device != k_cache.device:
+            raise RuntimeError(f"scales are on {s.device}, not on {k_cache.device}")
+        if (s.dim() != k_cache.dim() - 1 or s.shape[:-1] != k_cache.shape[:-2] or s.shape[-1] < 1 or
+                k_cache.shape[-2] % s.shape[-1]):
+            raise ValueError(f"scales {tuple(s.shape)}, cache {tuple(k_cache.shape)}: need one for each block of a page and head")
+        if not s.is_contiguous():
+            raise RuntimeError("scales must be contiguous")
+
+
 def cache_fork(k_cache, v_cache, tables, lens, refs, src, dst, k_scales=None, v_scales=None):
     """Slot dst[f] becomes a copy of slot src[f]: full pages are shared, the last, partly
     filled one is copied to a free page. Returns (tables, lens, refs, missing); with
-    missing [1] > 0 (too few free pages) nothing is forked. The scales of a cache in 8 bits go along."""
+    missing [1] > 0 (too few free pages) nothing is forked. A cache in 8 bits needs its scales, which go along."""
+    _check_scales(k_cache, v_cache, k_scales, v_scales)
     if k_cache.dim() == 4:  # one layer
         k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
         k_scales, v_scales = (t if t is None else t.unsqueeze(0) for t in (k_scales, v_scales))
@@ -336,8 +361,9 @@ def cache_free(tables, lens, refs, slots):
 
 
 def cache_compact(k_cache, v_cache, tables, refs, k_scales=None, v_scales=None):
-    """Moves the pages in use to the lowest indices. Returns (tables, refs). The scales of a cache in 8
-    bits go along."""
+    """Moves the pages in use to the lowest indices. Returns (tables, refs). A cache in 8 bits needs
+    its scales, which go along."""
+    _check_scales(k_cache, v_cache, k_scales, v_scales)
     if k_cache.dim() == 4:  # one layer
         k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
         k_scales, v_scales = (t if t is None else t.unsqueeze(0) for t in (k_scales, v_scales))

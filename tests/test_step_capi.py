@@ -202,3 +202,29 @@ def test_sample_numbers_out_of_range():
             ops.sample(x, u, **kw)
     with pytest.raises(NotImplementedError):
         ops.sample(torch.zeros(2, 10), torch.zeros(2))
+
+
+def test_page_operations_need_the_scales_of_a_cache_in_8_bits():
+    import torch
+
+    from nkilab import ops
+
+    def m(*shape, dtype=torch.int32):
+        return torch.empty(shape, dtype=dtype, device="meta")
+
+    e4m3, e8m0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+    tables, lens, refs = m(3, 4), m(3), m(20)
+    for lead in ((), (2,)):
+        c, s = m(*lead, 20, 2, 16, 64, dtype=e4m3), m(*lead, 20, 2, 2, dtype=e8m0)
+        plain = m(*lead, 20, 2, 16, 64, dtype=torch.bfloat16)
+        for call in (lambda kc, ks, vs: ops.cache_fork(kc, kc, tables, lens, refs, m(1), m(1), ks, vs),
+                     lambda kc, ks, vs: ops.cache_compact(kc, kc, tables, refs, ks, vs)):
+            assert call(c, s, s)[0].shape == (3, 4) and call(plain, None, None)[0].shape == (3, 4)
+            with pytest.raises(ValueError):
+                call(c, s, None)
+            with pytest.raises(ValueError):
+                call(c, None, s)
+            with pytest.raises(TypeError):
+                call(c, None, None)
+            with pytest.raises(TypeError):
+                call(plain, s, s)
