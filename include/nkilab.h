@@ -470,6 +470,20 @@ int nkl_cache_compact(void* k_cache, void* v_cache, const int64_t* cache_strides
                       size_t workspace_bytes, int64_t layers, int64_t batch, int64_t kv_heads, int64_t head_dim,
                       int64_t pages, int64_t page_size, int64_t max_pages, int dtype, void* stream);
 
+/* The same of a cache in 8 bits (above nkl_rotary_append), with the powers of two of the pages that are
+ * copied or moved; workspaces as theirs. */
+int nkl_cache_fork_8bit(void* k_cache, void* v_cache, const int64_t* cache_strides, void* k_scales, void* v_scales,
+                        const int32_t* tables, const int32_t* lens, const int32_t* refs, const int32_t* src,
+                        const int32_t* dst, int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* missing,
+                        void* workspace, size_t workspace_bytes, int64_t forks, int64_t layers, int64_t batch,
+                        int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages,
+                        int64_t block, void* stream);
+int nkl_cache_compact_8bit(void* k_cache, void* v_cache, const int64_t* cache_strides, void* k_scales, void* v_scales,
+                           const int32_t* tables, const int32_t* refs, int32_t* tables_out, int32_t* refs_out,
+                           void* workspace, size_t workspace_bytes, int64_t layers, int64_t batch, int64_t kv_heads,
+                           int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages, int64_t block,
+                           void* stream);
+
 /* Which drafted tokens the target accepts, and the token after them. probs [batch, drafted +
  * 1, vocab]: row 0 follows the last cached token, row i + 1 drafted token i. uniforms [batch,
  * drafted + 1] in [0, 1): number i tests token i, the last one draws the next token.

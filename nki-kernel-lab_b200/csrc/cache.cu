@@ -16,6 +16,7 @@
 //
 // Allocation takes free pages in ascending order, so every result is a function of the
 // inputs alone. The copies read each byte once and write it once; what bounds them is HBM.
+// A cache in 8 bits has powers of two besides (rotary.cu); a copied page's go with it.
 #include <algorithm>
 
 #include <atomic>
@@ -331,6 +332,34 @@ __device__ __forceinline__ void copy_pages(uint4* kc, uint4* vc, const CacheLayo
   if (runs) bulk.finish();
 }
 
+// The powers of two of a cache in 8 bits (C8): dense, `bytes` to a layer's page.
+struct PageScales {
+  uint8_t *k, *v;
+  int bytes;
+};
+
+// Where pages are copied to, their powers of two go too, by the warps that the copies of runs leave free.
+template <typename Pages>
+__device__ __forceinline__ void copy_scales(const PageScales& s, const CacheDims& d, int64_t copies, int first, Pages pages) {
+  constexpr int kOthers = kCopyThreads / 32 - 1;
+  const int warp = (int)(threadIdx.x >> 5) - 1, lane = threadIdx.x & 31;
+  if (warp < 0) return;
+  const bool vec = s.bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(s.k) | reinterpret_cast<uintptr_t>(s.v)) % 16 == 0;
+  const int64_t units = copies * d.layers * 2;
+  for (int64_t u = (int64_t)first * kOthers + warp; u < units; u += (int64_t)gridDim.x * kOthers) {
+    const int i = (int)(u / (d.layers * 2)), x = (int)(u - (int64_t)i * (d.layers * 2));
+    int from, to, rows;
+    if (!pages(i, from, to, rows)) continue;
+    uint8_t* const c = ((x & 1) ? s.v : s.k) + (int64_t)(x >> 1) * d.pages * s.bytes;
+    const uint8_t* const src = c + (int64_t)from * s.bytes;
+    uint8_t* const dst = c + (int64_t)to * s.bytes;
+    if (vec)
+      for (int e = 16 * lane; e < s.bytes; e += 512) *reinterpret_cast<uint4*>(dst + e) = *reinterpret_cast<const uint4*>(src + e);
+    else
+      for (int e = lane; e < s.bytes; e += 32) dst[e] = src[e];
+  }
+}
+
 // ------------------------------------------------------------------ reserve
 
 struct ReserveArgs {
@@ -403,6 +432,7 @@ struct ForkArgs {
   CacheLayout c;
   CacheDims d;
   int batch, forks, max_pages;
+  PageScales scales;
 };
 
 constexpr int kNoFork = 0x7fffffff;
@@ -469,16 +499,19 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, int b, int f, int fr
   if (write && lane == 0) a.lens_out[b] = f == kNoFork ? a.lens[b] : a.lens[s];
 }
 
-// The used rows of the forks' last pages.
+// The used rows of the forks' last pages, and these pages' powers of two.
+template <bool C8>
 __device__ __forceinline__ void fork_copies(const ForkArgs& a, const int* fresh, int first, uint8_t* ring, BulkRing& r) {
-  copy_pages(a.kc, a.vc, a.c, a.d, a.forks, first, ring, r, [&](int f, int& from, int& to, int& rows) {
+  auto pages = [&](int f, int& from, int& to, int& rows) {
     to = fresh[f];
     if (to < 0) return false;
     const int s = a.src[f], n = max(a.lens[s], 0), full = n / a.d.page;
     from = a.tables[(int64_t)s * a.max_pages + full];
     rows = n - full * a.d.page;
     return from >= 0 && from < a.d.pages;
-  });
+  };
+  if constexpr (C8) copy_scales(a.scales, a.d, a.forks, first, pages);
+  copy_pages(a.kc, a.vc, a.c, a.d, a.forks, first, ring, r, pages);
 }
 
 // Small caches: every block makes the whole plan for itself, in shared memory, which costs
@@ -490,6 +523,7 @@ __device__ __forceinline__ void fork_copies(const ForkArgs& a, const int* fresh,
 constexpr int kSmallForkPages = 4096, kSmallSlots = 512, kSmallForks = 256, kSmallEntries = 8192;
 constexpr int kSmallPages = 8192;
 
+template <bool C8>
 __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_fork_small_kernel(const __grid_constant__ ForkArgs a) {
   __shared__ u64 scratch[33];
   __shared__ int owner[kSmallSlots], fresh[kSmallForks], page_of[kSmallForks];
@@ -516,7 +550,7 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_fork_small_ke
   }
   for (int b = (int)blockIdx.x * kWarps + warp; b < a.batch; b += (int)gridDim.x * kWarps) row(b, true, [](int, int) {});
   // block 0 comes last: it has had the counts to do
-  fork_copies(a, fresh, (int)((blockIdx.x + gridDim.x - 1) % gridDim.x), ring, bulk);
+  fork_copies<C8>(a, fresh, (int)((blockIdx.x + gridDim.x - 1) % gridDim.x), ring, bulk);
 }
 
 __global__ void __launch_bounds__(kPlanThreads) cache_fork_plan_kernel(const __grid_constant__ ForkArgs a) {
@@ -526,6 +560,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_fork_plan_kernel(const __g
   if (threadIdx.x == 0) a.missing[0] = lacking;
 }
 
+template <bool C8>
 __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_fork_apply_kernel(const __grid_constant__ ForkArgs a) {
   __shared__ BulkRing bulk;
   extern __shared__ __align__(128) uint8_t ring[];
@@ -535,7 +570,7 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_fork_apply_ke
     const int f = a.owner[b];
     fork_row(a, b, f, f == kNoFork ? -1 : a.fresh[f], true, [&](int p, int by) { atomicAdd(&a.refs_out[p], by); });
   }
-  fork_copies(a, a.fresh, (int)blockIdx.x, ring, bulk);
+  fork_copies<C8>(a, a.fresh, (int)blockIdx.x, ring, bulk);
 }
 
 // ------------------------------------------------------------------ free
@@ -582,6 +617,7 @@ struct CompactArgs {
   CacheLayout c;
   CacheDims d;
   int64_t entries;
+  PageScales scales;
 };
 
 __global__ void __launch_bounds__(kPlanThreads) cache_compact_plan_kernel(const __grid_constant__ CompactArgs a) {
@@ -604,17 +640,20 @@ __global__ void __launch_bounds__(kPlanThreads) cache_compact_plan_kernel(const 
 }
 
 // Whole pages; `come` and `go` are indices, of 32 or 16 bits.
-template <typename I>
+template <bool C8, typename I>
 __device__ __forceinline__ void compact_copies(const CompactArgs& a, const I* come, const I* go, int moves, uint8_t* ring,
                                                BulkRing& r) {
-  copy_pages(a.kc, a.vc, a.c, a.d, moves, (int)blockIdx.x, ring, r, [&](int i, int& from, int& to, int& rows) {
+  auto pages = [&](int i, int& from, int& to, int& rows) {
     from = come[i];
     to = go[i];
     rows = a.d.page;
     return true;
-  });
+  };
+  if constexpr (C8) copy_scales(a.scales, a.d, moves, (int)blockIdx.x, pages);
+  copy_pages(a.kc, a.vc, a.c, a.d, moves, (int)blockIdx.x, ring, r, pages);
 }
 
+template <bool C8>
 __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_compact_apply_kernel(const __grid_constant__ CompactArgs a) {
   __shared__ BulkRing bulk;
   extern __shared__ __align__(128) uint8_t ring[];
@@ -623,11 +662,12 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_compact_apply
     const int p = a.tables[i];
     a.tables_out[i] = p >= 0 && p < a.d.pages ? a.place[p] : p;
   }
-  compact_copies(a, a.come, a.go, a.moves[0], ring, bulk);
+  compact_copies<C8>(a, a.come, a.go, a.moves[0], ring, bulk);
 }
 
 // As cache_fork_small_kernel: every block plans for itself. There are at most as many moves as
 // half of the pages, rounded down.
+template <bool C8>
 __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_compact_small_kernel(const __grid_constant__ CompactArgs a) {
   __shared__ u64 scratch[33];
   __shared__ uint16_t come[kSmallPages / 2], go[kSmallPages / 2], rank_of[kSmallPages];
@@ -651,7 +691,7 @@ __global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) cache_compact_small
     // a page in use from `live` on moves; a table entry for one that is not in use stays
     a.tables_out[i] = p >= live && p < a.d.pages && a.refs[p] > 0 ? go[rank_of[p]] : p;
   }
-  compact_copies(a, come, go, movers, ring, bulk);
+  compact_copies<C8>(a, come, go, movers, ring, bulk);
 }
 
 // ------------------------------------------------------------------ host
@@ -660,13 +700,15 @@ constexpr int64_t kMaxInt = 0x7fffffffLL;
 
 size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
 
+constexpr int kBytes = -1;  // beside the dtypes: a cache in 8 bits
+
 // Checks and converts the cache's description; strides (elements) are layer, page, head, slot.
 int cache_dims(const char* op, const void* kc, const void* vc, const int64_t* strides, int64_t layers, int64_t pages,
                int64_t kv_heads, int64_t page_size, int64_t head_dim, int dtype, CacheDims* d, CacheLayout* c) {
-  if (!valid_dtype(dtype)) return fail(NKL_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
+  if (dtype != kBytes && !valid_dtype(dtype)) return fail(NKL_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
   if (layers < 1 || pages < 1 || kv_heads < 1 || page_size < 1 || head_dim < 1)
     return fail(NKL_ERR_SHAPE, "%s: layers, pages, heads, page size and head_dim must be positive", op);
-  const int64_t per = 16 / (int64_t)dtype_size(dtype);
+  const int64_t per = dtype == kBytes ? 16 : 16 / (int64_t)dtype_size(dtype);
   if (head_dim % per)
     return fail(NKL_ERR_SHAPE, "%s: a row must be a multiple of 16 bytes (head_dim %lld)", op, (long long)head_dim);
   if (layers > 65535 || pages > kMaxInt / 4 || kv_heads > 65535 || page_size > 65536 || head_dim > 65536 ||
@@ -693,6 +735,17 @@ int cache_dims(const char* op, const void* kc, const void* vc, const int64_t* st
   return NKL_OK;
 }
 
+// The powers of two of a cache in 8 bits, given its checked dimensions.
+int page_scales(const char* op, void* k_scales, void* v_scales, int64_t block, const CacheDims& d, PageScales* s) {
+  if (block < 1 || d.page % block)
+    return fail(NKL_ERR_SHAPE, "%s: blocks of %lld positions do not divide pages of %d", op, (long long)block, d.page);
+  if (!k_scales || !v_scales) return fail(NKL_ERR_ARG, "%s: NULL pointer", op);
+  const int64_t bytes = d.heads * (d.page / block);
+  if (bytes > kMaxInt) return fail(NKL_ERR_SHAPE, "%s: size out of range", op);
+  *s = {static_cast<uint8_t*>(k_scales), static_cast<uint8_t*>(v_scales), (int)bytes};
+  return NKL_OK;
+}
+
 int check_table(const char* op, int64_t batch, int64_t max_pages) {
   if (batch < 0 || max_pages < 1) return fail(NKL_ERR_SHAPE, "%s: batch must not be negative, tables need a column", op);
   if (batch > kMaxInt / 4 || max_pages > kMaxInt / 4 || batch * max_pages > kMaxInt)
@@ -705,6 +758,7 @@ unsigned grid_for(int64_t blocks, int per_sm) {
 }
 
 // Allows the kernels that copy pages their ring, once per device.
+template <bool C8>
 int allow_ring(const char* op) {
   static std::atomic<bool> set[64] = {};  // idempotent
   int dev = 0;
@@ -714,10 +768,10 @@ int allow_ring(const char* op) {
   auto allow = [&](const void* kernel, int bytes) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   };
-  allow((const void*)cache_fork_small_kernel, kRing * kChunk + kSmallForkPages * 4);
-  allow((const void*)cache_fork_apply_kernel, kRing * kChunk);
-  allow((const void*)cache_compact_small_kernel, kRing * kChunk);
-  allow((const void*)cache_compact_apply_kernel, kRing * kChunk);
+  allow((const void*)cache_fork_small_kernel<C8>, kRing * kChunk + kSmallForkPages * 4);
+  allow((const void*)cache_fork_apply_kernel<C8>, kRing * kChunk);
+  allow((const void*)cache_compact_small_kernel<C8>, kRing * kChunk);
+  allow((const void*)cache_compact_apply_kernel<C8>, kRing * kChunk);
   if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
   if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
   return NKL_OK;
@@ -812,17 +866,20 @@ extern "C" size_t nkl_cache_fork_workspace_size(int64_t batch, int64_t forks) {
   return batch > 0 && forks >= 0 ? round256(((size_t)batch + 2 * (size_t)forks) * 4) : 0;
 }
 
-extern "C" int nkl_cache_fork(void* k_cache, void* v_cache, const int64_t* cache_strides, const int32_t* tables,
-                              const int32_t* lens, const int32_t* refs, const int32_t* src, const int32_t* dst,
-                              int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* missing,
-                              void* workspace, size_t workspace_bytes, int64_t forks, int64_t layers, int64_t batch,
-                              int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size,
-                              int64_t max_pages, int dtype, void* stream) {
-  const char* op = "nkl_cache_fork";
+namespace {
+
+// Both entry points; C8: with scales, of dtype kBytes.
+template <bool C8>
+int fork(const char* op, void* k_cache, void* v_cache, const int64_t* cache_strides, void* k_scales, void* v_scales,
+         const int32_t* tables, const int32_t* lens, const int32_t* refs, const int32_t* src, const int32_t* dst,
+         int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* missing, void* workspace,
+         size_t workspace_bytes, int64_t forks, int64_t layers, int64_t batch, int64_t kv_heads, int64_t head_dim,
+         int64_t pages, int64_t page_size, int64_t max_pages, int64_t block, int dtype, void* stream) {
   ForkArgs a = {};
   int rc = cache_dims(op, k_cache, v_cache, cache_strides, layers, pages, kv_heads, page_size, head_dim, dtype, &a.d,
                       &a.c);
   if (rc) return rc;
+  if (C8 && (rc = page_scales(op, k_scales, v_scales, block, a.d, &a.scales))) return rc;
   rc = check_table(op, batch, max_pages);
   if (rc) return rc;
   if (forks < 0 || forks > kMaxInt / 4) return fail(NKL_ERR_SHAPE, "%s: bad number of forks", op);
@@ -849,14 +906,40 @@ extern "C" int nkl_cache_fork(void* k_cache, void* v_cache, const int64_t* cache
   a.forks = (int)forks;
   a.max_pages = (int)max_pages;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int e = allow_ring(op)) return e;
+  if (int e = allow_ring<C8>(op)) return e;
   if (pages <= kSmallForkPages && batch <= kSmallSlots && forks <= kSmallForks && batch * max_pages <= kSmallEntries)
-    return launch_pdl(cache_fork_small_kernel, dim3(grid_for(std::max(batch / 8, forks * layers * 2), kCopyBlocks)),
+    return launch_pdl(cache_fork_small_kernel<C8>, dim3(grid_for(std::max(batch / 8, forks * layers * 2), kCopyBlocks)),
                       dim3(kCopyThreads), kRing * kChunk + (size_t)pages * 4, st, op, a);
   rc = launch_pdl(cache_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, op, a);
   if (rc) return rc;
-  return launch_pdl(cache_fork_apply_kernel, dim3(grid_for(std::max(batch / 8, forks * layers * 2), kCopyBlocks)), dim3(kCopyThreads),
+  return launch_pdl(cache_fork_apply_kernel<C8>, dim3(grid_for(std::max(batch / 8, forks * layers * 2), kCopyBlocks)), dim3(kCopyThreads),
                     kRing * kChunk, st, op, a);
+}
+
+}  // namespace
+
+extern "C" int nkl_cache_fork(void* k_cache, void* v_cache, const int64_t* cache_strides, const int32_t* tables,
+                              const int32_t* lens, const int32_t* refs, const int32_t* src, const int32_t* dst,
+                              int32_t* tables_out, int32_t* lens_out, int32_t* refs_out, int32_t* missing,
+                              void* workspace, size_t workspace_bytes, int64_t forks, int64_t layers, int64_t batch,
+                              int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size,
+                              int64_t max_pages, int dtype, void* stream) {
+  const char* op = "nkl_cache_fork";
+  if (!valid_dtype(dtype)) return fail(NKL_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
+  return fork<false>(op, k_cache, v_cache, cache_strides, nullptr, nullptr, tables, lens, refs, src, dst, tables_out, lens_out,
+              refs_out, missing, workspace, workspace_bytes, forks, layers, batch, kv_heads, head_dim, pages, page_size,
+              max_pages, 0, dtype, stream);
+}
+
+extern "C" int nkl_cache_fork_8bit(void* k_cache, void* v_cache, const int64_t* cache_strides, void* k_scales,
+                                   void* v_scales, const int32_t* tables, const int32_t* lens, const int32_t* refs,
+                                   const int32_t* src, const int32_t* dst, int32_t* tables_out, int32_t* lens_out,
+                                   int32_t* refs_out, int32_t* missing, void* workspace, size_t workspace_bytes,
+                                   int64_t forks, int64_t layers, int64_t batch, int64_t kv_heads, int64_t head_dim,
+                                   int64_t pages, int64_t page_size, int64_t max_pages, int64_t block, void* stream) {
+  return fork<true>("nkl_cache_fork_8bit", k_cache, v_cache, cache_strides, k_scales, v_scales, tables, lens, refs, src, dst,
+              tables_out, lens_out, refs_out, missing, workspace, workspace_bytes, forks, layers, batch, kv_heads, head_dim,
+              pages, page_size, max_pages, block, kBytes, stream);
 }
 
 extern "C" int nkl_cache_free(const int32_t* tables, const int32_t* lens, const int32_t* refs, const int32_t* slots,
@@ -897,16 +980,18 @@ extern "C" size_t nkl_cache_compact_workspace_size(int64_t pages) {
   return pages > 0 ? round256(((size_t)pages * 3 + 1) * 4) : 0;
 }
 
-extern "C" int nkl_cache_compact(void* k_cache, void* v_cache, const int64_t* cache_strides, const int32_t* tables,
-                                 const int32_t* refs, int32_t* tables_out, int32_t* refs_out, void* workspace,
-                                 size_t workspace_bytes, int64_t layers, int64_t batch, int64_t kv_heads,
-                                 int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages, int dtype,
-                                 void* stream) {
-  const char* op = "nkl_cache_compact";
+namespace {
+
+template <bool C8>
+int compact(const char* op, void* k_cache, void* v_cache, const int64_t* cache_strides, void* k_scales, void* v_scales,
+            const int32_t* tables, const int32_t* refs, int32_t* tables_out, int32_t* refs_out, void* workspace,
+            size_t workspace_bytes, int64_t layers, int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t pages,
+            int64_t page_size, int64_t max_pages, int64_t block, int dtype, void* stream) {
   CompactArgs a = {};
   int rc = cache_dims(op, k_cache, v_cache, cache_strides, layers, pages, kv_heads, page_size, head_dim, dtype, &a.d,
                       &a.c);
   if (rc) return rc;
+  if (C8 && (rc = page_scales(op, k_scales, v_scales, block, a.d, &a.scales))) return rc;
   rc = check_table(op, batch, max_pages);
   if (rc) return rc;
   if (!refs || !refs_out || (batch && (!tables || !tables_out))) return fail(NKL_ERR_ARG, "%s: NULL pointer", op);
@@ -924,14 +1009,37 @@ extern "C" int nkl_cache_compact(void* k_cache, void* v_cache, const int64_t* ca
   a.vc = static_cast<uint4*>(v_cache);
   a.entries = batch * max_pages;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int e = allow_ring(op)) return e;
+  if (int e = allow_ring<C8>(op)) return e;
   if (pages <= kSmallPages)
-    return launch_pdl(cache_compact_small_kernel,
+    return launch_pdl(cache_compact_small_kernel<C8>,
                       dim3(grid_for(std::max<int64_t>((a.entries + 255) / 256, pages * layers), kCopyBlocks)), dim3(kCopyThreads),
                       kRing * kChunk, st, op, a);
   rc = launch_pdl(cache_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, op, a);
   if (rc) return rc;
-  return launch_pdl(cache_compact_apply_kernel,
+  return launch_pdl(cache_compact_apply_kernel<C8>,
                     dim3(grid_for(std::max<int64_t>((a.entries + 255) / 256, pages * layers), kCopyBlocks)), dim3(kCopyThreads),
                     kRing * kChunk, st, op, a);
+}
+
+}  // namespace
+
+extern "C" int nkl_cache_compact(void* k_cache, void* v_cache, const int64_t* cache_strides, const int32_t* tables,
+                                 const int32_t* refs, int32_t* tables_out, int32_t* refs_out, void* workspace,
+                                 size_t workspace_bytes, int64_t layers, int64_t batch, int64_t kv_heads,
+                                 int64_t head_dim, int64_t pages, int64_t page_size, int64_t max_pages, int dtype,
+                                 void* stream) {
+  const char* op = "nkl_cache_compact";
+  if (!valid_dtype(dtype)) return fail(NKL_ERR_DTYPE, "%s: unsupported dtype %d", op, dtype);
+  return compact<false>(op, k_cache, v_cache, cache_strides, nullptr, nullptr, tables, refs, tables_out, refs_out, workspace,
+                 workspace_bytes, layers, batch, kv_heads, head_dim, pages, page_size, max_pages, 0, dtype, stream);
+}
+
+extern "C" int nkl_cache_compact_8bit(void* k_cache, void* v_cache, const int64_t* cache_strides, void* k_scales,
+                                      void* v_scales, const int32_t* tables, const int32_t* refs, int32_t* tables_out,
+                                      int32_t* refs_out, void* workspace, size_t workspace_bytes, int64_t layers,
+                                      int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                                      int64_t page_size, int64_t max_pages, int64_t block, void* stream) {
+  return compact<true>("nkl_cache_compact_8bit", k_cache, v_cache, cache_strides, k_scales, v_scales, tables, refs, tables_out,
+                 refs_out, workspace, workspace_bytes, layers, batch, kv_heads, head_dim, pages, page_size, max_pages, block,
+                 kBytes, stream);
 }

@@ -104,11 +104,12 @@ Scales check_scales(const Tensor& k_cache, const Tensor& v_cache, const Tensor& 
     TORCH_CHECK(c->device() == dev, "k and v caches on different devices");
   }
   TORCH_CHECK(k_cache.strides() == v_cache.strides() && k_cache.stride(-1) == 1, "caches need equal strides and contiguous rows");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "scales ", k.sizes(), " and ", v.sizes(), ": need equal shapes");
   for (const Tensor* s : {&k, &v}) {
     TORCH_CHECK_TYPE(s->scalar_type() == at::kFloat8_e8m0fnu, "scales must be float8_e8m0fnu, got ", s->scalar_type());
     TORCH_CHECK(s->device() == dev, "scales are on ", s->device(), ", not on ", dev);
     TORCH_CHECK_VALUE(s->dim() == dims - 1 && s->sizes().slice(0, dims - 2) == k_cache.sizes().slice(0, dims - 2) &&
-                          s->size(-1) >= 1 && s->sizes() == k.sizes() && k_cache.size(-2) % s->size(-1) == 0,
+                          s->size(-1) >= 1 && k_cache.size(-2) % s->size(-1) == 0,
                       "scales ", k.sizes(), " and ", v.sizes(), ", caches ", k_cache.sizes(),
                       ": need one for each block of a page and head, and whole blocks");
     TORCH_CHECK(s->is_contiguous(), "scales must be contiguous");
@@ -397,10 +398,14 @@ std::tuple<Tensor, Tensor, Tensor> cache_reserve(const Tensor& tables, const Ten
   return {tables_out, refs_out, missing};
 }
 
-std::tuple<Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_cache, const Tensor& v_cache, const Tensor& tables,
-                                                      const Tensor& lens, const Tensor& refs, const Tensor& src,
-                                                      const Tensor& dst) {
-  const int dt = check_caches(k_cache, v_cache, 5);
+// k_scales and v_scales: of a cache in 8 bits, else undefined.
+std::tuple<Tensor, Tensor, Tensor, Tensor> fork(const Tensor& k_cache, const Tensor& v_cache, const Tensor* k_scales,
+                                                const Tensor* v_scales, const Tensor& tables, const Tensor& lens,
+                                                const Tensor& refs, const Tensor& src, const Tensor& dst) {
+  Scales sc = {nullptr, nullptr, 0};
+  int dt = 0;
+  if (k_scales) sc = check_scales(k_cache, v_cache, *k_scales, *v_scales, 5);
+  else dt = check_caches(k_cache, v_cache, 5);
   const Table t = check_table(tables, lens, refs);
   TORCH_CHECK_VALUE(k_cache.size(1) == t.P, "the cache has ", k_cache.size(1), " pages, refs ", t.P);
   TORCH_CHECK(k_cache.device() == t.dev, "tensors on different devices: ", k_cache.device(), " vs ", t.dev);
@@ -414,11 +419,31 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_cache, con
          missing = new_ints({1}, t.dev);
   const size_t bytes = nkl_cache_fork_workspace_size(t.B, F);
   const Workspace ws = workspace(t.dev, st, bytes);
-  check("nkl_cache_fork",
-        nkl_cache_fork(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), t.tables, t.lens, t.refs, from,
-                       to, out_ints(tables_out), out_ints(lens_out), out_ints(refs_out), out_ints(missing), ws.data, bytes, F,
-                       k_cache.size(0), t.B, k_cache.size(2), k_cache.size(4), t.P, k_cache.size(3), t.M, dt, st));
+  const int64_t L = k_cache.size(0), Hkv = k_cache.size(2), page = k_cache.size(3), d = k_cache.size(4);
+  if (k_scales)
+    check("nkl_cache_fork_8bit",
+          nkl_cache_fork_8bit(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), sc.k, sc.v, t.tables, t.lens,
+                              t.refs, from, to, out_ints(tables_out), out_ints(lens_out), out_ints(refs_out),
+                              out_ints(missing), ws.data, bytes, F, L, t.B, Hkv, d, t.P, page, t.M, sc.block, st));
+  else
+    check("nkl_cache_fork",
+          nkl_cache_fork(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), t.tables, t.lens, t.refs, from, to,
+                         out_ints(tables_out), out_ints(lens_out), out_ints(refs_out), out_ints(missing), ws.data, bytes, F,
+                         L, t.B, Hkv, d, t.P, page, t.M, dt, st));
   return {tables_out, lens_out, refs_out, missing};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> cache_fork(const Tensor& k_cache, const Tensor& v_cache, const Tensor& tables,
+                                                      const Tensor& lens, const Tensor& refs, const Tensor& src,
+                                                      const Tensor& dst) {
+  return fork(k_cache, v_cache, nullptr, nullptr, tables, lens, refs, src, dst);
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> cache_fork_8bit(const Tensor& k_cache, const Tensor& v_cache,
+                                                           const Tensor& k_scales, const Tensor& v_scales,
+                                                           const Tensor& tables, const Tensor& lens, const Tensor& refs,
+                                                           const Tensor& src, const Tensor& dst) {
+  return fork(k_cache, v_cache, &k_scales, &v_scales, tables, lens, refs, src, dst);
 }
 
 std::tuple<Tensor, Tensor, Tensor> cache_free(const Tensor& tables, const Tensor& lens, const Tensor& refs,
@@ -434,9 +459,12 @@ std::tuple<Tensor, Tensor, Tensor> cache_free(const Tensor& tables, const Tensor
   return {tables_out, lens_out, refs_out};
 }
 
-std::tuple<Tensor, Tensor> cache_compact(const Tensor& k_cache, const Tensor& v_cache, const Tensor& tables,
-                                         const Tensor& refs) {
-  const int dt = check_caches(k_cache, v_cache, 5);
+std::tuple<Tensor, Tensor> compact(const Tensor& k_cache, const Tensor& v_cache, const Tensor* k_scales,
+                                   const Tensor* v_scales, const Tensor& tables, const Tensor& refs) {
+  Scales sc = {nullptr, nullptr, 0};
+  int dt = 0;
+  if (k_scales) sc = check_scales(k_cache, v_cache, *k_scales, *v_scales, 5);
+  else dt = check_caches(k_cache, v_cache, 5);
   const Table t = check_table(tables, std::nullopt, refs);
   TORCH_CHECK_VALUE(k_cache.size(1) == t.P, "the cache has ", k_cache.size(1), " pages, refs ", t.P);
   TORCH_CHECK(k_cache.device() == t.dev, "tensors on different devices: ", k_cache.device(), " vs ", t.dev);
@@ -445,11 +473,27 @@ std::tuple<Tensor, Tensor> cache_compact(const Tensor& k_cache, const Tensor& v_
   Tensor tables_out = new_ints({t.B, t.M}, t.dev), refs_out = new_ints({t.P}, t.dev);
   const size_t bytes = nkl_cache_compact_workspace_size(t.P);
   const Workspace ws = workspace(t.dev, st, bytes);
-  check("nkl_cache_compact",
-        nkl_cache_compact(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), t.tables, t.refs,
-                          out_ints(tables_out), out_ints(refs_out), ws.data, bytes, k_cache.size(0), t.B, k_cache.size(2),
-                          k_cache.size(4), t.P, k_cache.size(3), t.M, dt, st));
+  const int64_t L = k_cache.size(0), Hkv = k_cache.size(2), page = k_cache.size(3), d = k_cache.size(4);
+  if (k_scales)
+    check("nkl_cache_compact_8bit",
+          nkl_cache_compact_8bit(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), sc.k, sc.v, t.tables,
+                                 t.refs, out_ints(tables_out), out_ints(refs_out), ws.data, bytes, L, t.B, Hkv, d, t.P, page,
+                                 t.M, sc.block, st));
+  else
+    check("nkl_cache_compact",
+          nkl_cache_compact(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.strides().data(), t.tables, t.refs,
+                            out_ints(tables_out), out_ints(refs_out), ws.data, bytes, L, t.B, Hkv, d, t.P, page, t.M, dt, st));
   return {tables_out, refs_out};
+}
+
+std::tuple<Tensor, Tensor> cache_compact(const Tensor& k_cache, const Tensor& v_cache, const Tensor& tables,
+                                         const Tensor& refs) {
+  return compact(k_cache, v_cache, nullptr, nullptr, tables, refs);
+}
+
+std::tuple<Tensor, Tensor> cache_compact_8bit(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scales,
+                                              const Tensor& v_scales, const Tensor& tables, const Tensor& refs) {
+  return compact(k_cache, v_cache, &k_scales, &v_scales, tables, refs);
 }
 
 std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& probs_in, const Tensor& tokens, const Tensor& uniforms_in,
@@ -678,6 +722,10 @@ TORCH_LIBRARY_FRAGMENT(nkilab, m) {
         "Tensor dst) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("cache_free(Tensor tables, Tensor lens, Tensor refs, Tensor slots) -> (Tensor, Tensor, Tensor)");
   m.def("cache_compact(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor tables, Tensor refs) -> (Tensor, Tensor)");
+  m.def("cache_fork_8bit(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor tables, "
+        "Tensor lens, Tensor refs, Tensor src, Tensor dst) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("cache_compact_8bit(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, Tensor(d!) v_scales, Tensor tables, "
+        "Tensor refs) -> (Tensor, Tensor)");
   m.def("sample(Tensor logits, Tensor uniforms, Tensor? temperatures, Tensor? top_ks, Tensor? top_ps, Tensor? min_ps, "
         "float temperature, int top_k, float top_p, float min_p) -> (Tensor, Tensor)");
   m.def("verify_drafts(Tensor probs, Tensor tokens, Tensor uniforms, Tensor? parents, Tensor? draft_probs) "
@@ -695,6 +743,8 @@ TORCH_LIBRARY_IMPL(nkilab, CUDA, m) {
   m.impl("cache_fork", &cache_fork);
   m.impl("cache_free", &cache_free);
   m.impl("cache_compact", &cache_compact);
+  m.impl("cache_fork_8bit", &cache_fork_8bit);
+  m.impl("cache_compact_8bit", &cache_compact_8bit);
   m.impl("verify_drafts", &verify_drafts);
   m.impl("sample", &sample);
 }

@@ -93,6 +93,8 @@ SIGNATURES = {
     "nkl_cache_free": (_int, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "nkl_cache_compact_workspace_size": (_sz, [_i64]),
     "nkl_cache_compact": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p]),
+    "nkl_cache_fork_8bit": (_int, [_p] * 15 + [_sz] + [_i64] * 9 + [_p]),
+    "nkl_cache_compact_8bit": (_int, [_p] * 10 + [_sz] + [_i64] * 8 + [_p]),
     "nkl_verify_drafts": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _int, _p]),
     "nkl_sample": (_int, [_p, _i64, _p, _p, _p, _p, _p, _f, _int, _f, _f, _p, _p, _i64, _i64, _int, _p]),
     "nkl_attention_naive_workspace_size": (_sz, [_i64, _i64, _int]),

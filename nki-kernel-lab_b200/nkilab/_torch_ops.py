@@ -16,6 +16,7 @@ compose with streams and CUDA-graph capture like any torch op:
     torch.ops.nkilab.rotary_append(q, k, v, k_cache, v_cache, ...) -> nkl_rotary_append
     torch.ops.nkilab.cache_append_8bit(k, v, k_cache, v_cache, ...) -> nkl_cache_append_8bit
     torch.ops.nkilab.cache_{append,reserve,fork,free,compact}  -> nkl_cache_*
+    torch.ops.nkilab.cache_{fork,compact}_8bit(k_cache, v_cache, k_scales, v_scales, ...) -> nkl_cache_{fork,compact}_8bit
     torch.ops.nkilab.verify_drafts(probs, tokens, uniforms, parents, draft_probs) -> nkl_verify_drafts
     torch.ops.nkilab.sample(logits, uniforms, temperatures, top_ks, top_ps, min_ps, ...) -> nkl_sample
 
@@ -384,6 +385,10 @@ torch.library.register_fake("nkilab::cache_fork",
                             lambda k_cache, v_cache, tables, lens, refs, src, dst: _like(tables, lens, refs, refs[:1]))
 torch.library.register_fake("nkilab::cache_free", lambda tables, lens, refs, slots: _like(tables, lens, refs))
 torch.library.register_fake("nkilab::cache_compact", lambda k_cache, v_cache, tables, refs: _like(tables, refs))
+torch.library.register_fake("nkilab::cache_fork_8bit", lambda k_cache, v_cache, k_scales, v_scales, tables, lens, refs, src, dst:
+                            _like(tables, lens, refs, refs[:1]))
+torch.library.register_fake("nkilab::cache_compact_8bit", lambda k_cache, v_cache, k_scales, v_scales, tables, refs:
+                            _like(tables, refs))
 torch.library.register_fake("nkilab::verify_drafts", lambda probs, tokens, uniforms, parents, draft_probs:
                             (_like(tokens), tokens.new_empty(tokens.shape[0]), tokens.new_empty(tokens.shape[0])))
 torch.library.register_fake("nkilab::sample", lambda logits, uniforms, *_:

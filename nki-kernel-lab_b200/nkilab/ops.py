@@ -178,8 +178,9 @@ def _decode(name: str):
 _attention_tree, _cache_append, _cache_reserve, _cache_fork, _cache_free, _cache_compact, _verify_drafts = map(
     _decode, ("attention_tree", "cache_append", "cache_reserve", "cache_fork", "cache_free", "cache_compact",
               "verify_drafts"))
-_attention_tree_8bit, _cache_append_8bit, _rotary, _rotary_append, _sample = map(
-    _decode, ("attention_tree_8bit", "cache_append_8bit", "rotary", "rotary_append", "sample"))
+_attention_tree_8bit, _cache_append_8bit, _cache_fork_8bit, _cache_compact_8bit, _rotary, _rotary_append, _sample = map(
+    _decode, ("attention_tree_8bit", "cache_append_8bit", "cache_fork_8bit", "cache_compact_8bit", "rotary", "rotary_append",
+              "sample"))
 
 
 def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=None, k_scales=None, v_scales=None):
@@ -296,63 +297,27 @@ def cache_reserve(tables, lens, refs, extra, page_size):
     return _cache_reserve(tables, lens, refs, extra, int(page_size))
 
 
-def _as_bf16(*caches):
-    """Caches in 8 bits as pairs of bytes: what moves whole rows does not look into them."""
-    return tuple(c.view(torch.bfloat16) if c.dtype == torch.float8_e4m3fn else c for c in caches)
-
-
-def _check_scales(k_cache, v_cache, k_scales, v_scales):
-    """Before pages move: a cache in 8 bits has both scales, one for each block of a page and head, others none."""
+def _check_8bits(k_cache, v_cache, k_scales, v_scales):
+    """Caches in 8 bits have both scales, others none."""
     if (k_scales is None) != (v_scales is None):
         raise ValueError("scales: need both or none")
-    bits8 = k_scales is not None
     for c in (k_cache, v_cache):
-        if (c.dtype == torch.float8_e4m3fn) != bits8:
-            raise TypeError(f"a {c.dtype} cache {'with' if bits8 else 'without'} scales")
-    if not bits8:
-        return
-    if k_scales.shape != v_scales.shape:
-        raise ValueError(f"scales {tuple(k_scales.shape)} and {tuple(v_scales.shape)}: need equal shapes")
-    for s in (k_scales, v_scales):
-        if s.dtype != torch.float8_e8m0fnu:
-            raise TypeError(f"scales must be float8_e8m0fnu, got {s.dtype}")
-        if s.device != k_cache.device:
-            raise RuntimeError(f"scales are on {s.device}, not on {k_cache.device}")
-        if (s.dim() != k_cache.dim() - 1 or s.shape[:-1] != k_cache.shape[:-2] or s.shape[-1] < 1 or
-                k_cache.shape[-2] % s.shape[-1]):
-            raise ValueError(f"scales {tuple(s.shape)}, cache {tuple(k_cache.shape)}: need one for each block of a page and head")
-        if not s.is_contiguous():
-            raise RuntimeError("scales must be contiguous")
+        if (c.dtype == torch.float8_e4m3fn) != (k_scales is not None):
+            raise TypeError(f"a {c.dtype} cache {'without' if k_scales is None else 'with'} scales")
 
 
 def cache_fork(k_cache, v_cache, tables, lens, refs, src, dst, k_scales=None, v_scales=None):
     """Slot dst[f] becomes a copy of slot src[f]: full pages are shared, the last, partly
     filled one is copied to a free page. Returns (tables, lens, refs, missing); with
     missing [1] > 0 (too few free pages) nothing is forked. A cache in 8 bits needs its scales, which go along."""
-    _check_scales(k_cache, v_cache, k_scales, v_scales)
+    if k_scales is not None or v_scales is not None or k_cache.dtype == torch.float8_e4m3fn:
+        _check_8bits(k_cache, v_cache, k_scales, v_scales)
+        if k_cache.dim() == 4:  # one layer
+            k_cache, v_cache, k_scales, v_scales = (t.unsqueeze(0) for t in (k_cache, v_cache, k_scales, v_scales))
+        return _cache_fork_8bit(k_cache, v_cache, k_scales, v_scales, tables, lens, refs, src, dst)
     if k_cache.dim() == 4:  # one layer
         k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-        k_scales, v_scales = (t if t is None else t.unsqueeze(0) for t in (k_scales, v_scales))
-    out = _cache_fork(*_as_bf16(k_cache, v_cache), tables, lens, refs, src, dst)
-    if k_scales is not None:
-        # the copied page of each fork that was made, by the operator's rules; the others' turn is a live
-        # page that is written onto itself (a copied one was free)
-        B, M = tables.shape
-        s, t, each = src.long(), dst.long(), torch.arange(src.numel(), device=src.device)
-        good = (s >= 0) & (s < B) & (t >= 0) & (t < B) & (s != t)
-        again = ((t[:, None] == t) & good & (each < each[:, None])).any(1)
-        s, t = s.clamp(0, B - 1), t.clamp(0, B - 1)
-        page = k_cache.shape[3]
-        n = lens[s].clamp(0, M * page)
-        col = (n // page).clamp(max=M - 1).long()
-        come, go = tables[s, col].long(), out[0][t, col].long()
-        made = good & ~again & (n % page > 0) & (out[3] == 0) & (come >= 0) & (come < refs.numel()) & (go >= 0)
-        live = (refs > 0).int().argmax()
-        come, go = torch.where(made, come, live), torch.where(made, go, live)
-        for x in (k_scales, v_scales):
-            b = x.view(torch.uint8)
-            b[:, go] = b[:, come]
-    return out
+    return _cache_fork(k_cache, v_cache, tables, lens, refs, src, dst)
 
 
 def cache_free(tables, lens, refs, slots):
@@ -363,20 +328,14 @@ def cache_free(tables, lens, refs, slots):
 def cache_compact(k_cache, v_cache, tables, refs, k_scales=None, v_scales=None):
     """Moves the pages in use to the lowest indices. Returns (tables, refs). A cache in 8 bits needs
     its scales, which go along."""
-    _check_scales(k_cache, v_cache, k_scales, v_scales)
+    if k_scales is not None or v_scales is not None or k_cache.dtype == torch.float8_e4m3fn:
+        _check_8bits(k_cache, v_cache, k_scales, v_scales)
+        if k_cache.dim() == 4:  # one layer
+            k_cache, v_cache, k_scales, v_scales = (t.unsqueeze(0) for t in (k_cache, v_cache, k_scales, v_scales))
+        return _cache_compact_8bit(k_cache, v_cache, k_scales, v_scales, tables, refs)
     if k_cache.dim() == 4:  # one layer
         k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-        k_scales, v_scales = (t if t is None else t.unsqueeze(0) for t in (k_scales, v_scales))
-    out = _cache_compact(*_as_bf16(k_cache, v_cache), tables, refs)
-    if k_scales is not None:
-        P = refs.numel()
-        there = (tables >= 0) & (tables < P) & (out[0] >= 0)
-        come = torch.arange(P + 1, device=refs.device)  # where each page's contents were
-        come.scatter_(0, torch.where(there, out[0], P).flatten().long(), torch.where(there, tables, P).flatten().long())
-        for x in (k_scales, v_scales):
-            b = x.view(torch.uint8)
-            b.copy_(b[:, come[:P].clamp(max=P - 1)])
-    return out
+    return _cache_compact(k_cache, v_cache, tables, refs)
 
 
 def verify_drafts(probs, tokens, uniforms, parents=None, draft_probs=None):

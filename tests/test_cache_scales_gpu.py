@@ -56,6 +56,30 @@ def test_a_fork_takes_the_powers_of_its_last_page(L, P, Hkv, page, d, block, str
     assert torch.equal(now[0], codes) and torch.equal(now[1], powers)
 
 
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("L,P,Hkv,page,d,block", SHAPES)
+def test_a_compaction_takes_every_moved_page_s_powers(L, P, Hkv, page, d, block, strided):
+    """Pages move by `refs`: some in use are in none of the tables' rows (another table's, or held for later), and a row
+    may name a page that is not in use."""
+    r = np.random.RandomState(P + 1)
+    c = Cache8(L, P, Hkv, page, d, block, strided)
+    refs = (r.rand(P) < 0.4) * r.randint(1, 3, P)
+    tables = np.full((3, 5), -1)
+    used, free = np.flatnonzero(refs > 0), np.flatnonzero(refs == 0)
+    tables[0, :4], tables[1, :2], tables[2, :3] = used[-4:], used[:2], [free[0], P + 9, free[-1]]
+    live = len(used)
+    holes, movers = [p for p in range(live) if refs[p] == 0], [p for p in range(live, P) if refs[p] > 0]
+    codes, powers = (t.clone() for t in pages_of(c))
+    to, from_ = torch.tensor(holes, device=DEV), torch.tensor(movers, device=DEV)
+    codes[:, :, to], powers[:, :, to] = codes[:, :, from_], powers[:, :, from_]
+    place = dict(zip(movers, holes))
+    t, out = ops.cache_compact(c.k, c.v, i32(tables.tolist()), i32(refs.tolist()), c.ks, c.vs)
+    assert t.tolist() == [[place.get(p, p) for p in row] for row in tables.tolist()]
+    now = pages_of(c)
+    assert torch.equal(now[0][:, :, :live], codes[:, :, :live])
+    assert torch.equal(now[1][:, :, :live], powers[:, :, :live])
+
+
 def test_refusals_leave_the_cache_as_it_was():
     c = Cache8(1, 6, 2, 32, 32, 16)
     tables, lens, refs = i32([[0], [-1]]), i32([5, 0]), i32([1, 0, 0, 0, 0, 1])

@@ -228,3 +228,30 @@ def test_page_operations_need_the_scales_of_a_cache_in_8_bits():
                 call(c, None, None)
             with pytest.raises(TypeError):
                 call(plain, s, s)
+
+
+def test_page_operations_of_8_bits_refusals(N):
+    nf, nc = N.lib.nkl_cache_fork_workspace_size(4, 3), N.lib.nkl_cache_compact_workspace_size(10)
+
+    def fork(**kw):
+        a = dict(kc=FAKE, vc=FAKE, cs=None, ks=FAKE, vs=FAKE, tables=FAKE, lens=FAKE, refs=FAKE, src=FAKE, dst=FAKE, to=FAKE,
+                 lo=FAKE, ro=FAKE, missing=FAKE, ws=FAKE, wsb=nf, F=3, L=1, B=4, Hkv=2, d=64, P=10, page=16, M=4, block=8)
+        assert not set(kw) - set(a)
+        a.update(kw)
+        return N.lib.nkl_cache_fork_8bit(*a.values(), None)
+
+    def compact(**kw):
+        a = dict(kc=FAKE, vc=FAKE, cs=None, ks=FAKE, vs=FAKE, tables=FAKE, refs=FAKE, to=FAKE, ro=FAKE, ws=FAKE, wsb=nc, L=1,
+                 B=4, Hkv=2, d=64, P=10, page=16, M=4, block=8)
+        assert not set(kw) - set(a)
+        a.update(kw)
+        return N.lib.nkl_cache_compact_8bit(*a.values(), None)
+
+    for call in (fork, compact):
+        for kw in (dict(d=24), dict(d=0), dict(L=0), dict(Hkv=0), dict(P=0), dict(page=0), dict(M=0), dict(block=0), dict(block=5),
+                   dict(block=32), dict(B=-1)):
+            assert call(**kw) == N.ERR_SHAPE
+        for name in ("kc", "vc", "ks", "vs", "tables", "refs", "to", "ro", "ws"):
+            assert call(**{name: None}) == N.ERR_ARG
+        assert call(kc=ODD) == N.ERR_ALIGN and call(cs=strides(20480, 2048, 1024, 72)) == N.ERR_ALIGN
+        assert call(wsb=0) == N.ERR_ARG
