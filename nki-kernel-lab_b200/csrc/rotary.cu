@@ -180,15 +180,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN (0x7fffffff
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
-// e4m3 codes of VE values times 2^-e.
+// e4m3 codes of VE values times 2^-e; with `keep` 0 they are zeros, for a block whose power is NaN: 0 times a number that
+// is none would be e4m3's code for NaN, which the attention does not look for.
 template <int VE>
-__device__ __forceinline__ void store_codes(uint8_t* to, const float (&a)[VE], float inv) {
+__device__ __forceinline__ void store_codes(uint8_t* to, const float (&a)[VE], float inv, uint32_t keep) {
   uint32_t w[VE / 4];
 #pragma unroll
   for (int i = 0; i < VE / 4; ++i) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a[4 * i] * inv, a[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(a[4 * i + 2] * inv, a[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-    w[i] = lo | hi << 16;
+    w[i] = (lo | hi << 16) & keep;
   }
   if constexpr (VE == 8) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
   else *reinterpret_cast<uint32_t*>(to) = w[0];
@@ -443,6 +444,7 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
   };
   auto write = [&](const Unit& u, int t0, int n, int c0, int buf, uint8_t* rows8, int code) {
     const float inv = code == kNanScale ? 0.f : power_of_two(127 - code);
+    const uint32_t keep = code == kNanScale ? 0u : ~0u;
     const bool turned = u.key && a.freqs;
     const int m = row0 < per ? kept(t0, n) : 0;
     uint8_t* to = rows8 + (len + t0 - u.p0 + row0) * a.c_s;
@@ -453,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
       if (path && source(t0 + t) < 0) continue;
       float e[VE], o[VE];
       values(turned, row, c, s, e, o);
-      store_codes<VE>(to + part.o0, e, inv);
-      if (!INTER) store_codes<VE>(to + part.o1, o, inv);
+      store_codes<VE>(to + part.o0, e, inv, keep);
+      if (!INTER) store_codes<VE>(to + part.o1, o, inv, keep);
     }
   };
   // The block's power of two, given the largest magnitude that comes to it; rows that were in it
