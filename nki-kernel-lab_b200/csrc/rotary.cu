@@ -48,6 +48,8 @@ constexpr int kMaxHead = 256;
 constexpr int kMaxHead8 = 128;   // in 8 bits: as the attention
 constexpr int kLowest = -100;    // of the powers of two
 constexpr uint8_t kNanScale = 255;
+constexpr int kMostTokens = 1 << 24;  // of a call
+constexpr int kMostLen = 0x7fffffff - 2 * kMostTokens;
 
 constexpr int kMostSmem = 2 * kMaxTokens * (kMaxHead / 2) * 4 + kWarps * kHeld;
 
@@ -251,9 +253,10 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
   float* const sines = angles + a.chunk * a.half;
   const int items = P::items(a.d, a.half);
   const int capacity = a.max_pages * a.page;
-  const int len = KIND == kPlain ? 0 : min(max(a.lens[b], 0), capacity);
+  // (a length past the tables is a position all the same; what ends it keeps the sums below in 32 bits)
+  const int given = KIND == kPlain ? 0 : max(a.lens[b], 0), len = min(given, kMostLen);
   const int count = KIND == kPlain ? a.tokens : a.count ? min(max(a.count[b], 0), a.tokens) : a.tokens;
-  if (KIND == kBits8 && a.lens_out && layer == 0 && i == 0 && blockIdx.y == 0 && tid == 0) a.lens_out[b] = len + count;
+  if (KIND == kBits8 && a.lens_out && layer == 0 && i == 0 && blockIdx.y == 0 && tid == 0) a.lens_out[b] = given + count;
   // the group's tokens [j0, j1), of which those before `kept` go to the cache
   int j0, j1, first = 0;  // first: an 8-bit cache's position where the group begins
   if (KIND == kBits8) {
@@ -660,7 +663,7 @@ int take_strides(const char* op, const int64_t* given, int n, const int64_t* siz
 }
 
 bool rotary_sizes_ok(int64_t batch, int64_t tokens, int64_t heads, int64_t d, int64_t r) {
-  return batch >= 0 && batch <= 0x7fffffLL && tokens >= 0 && tokens <= (1LL << 24) && heads >= 1 && heads <= 65535 &&
+  return batch >= 0 && batch <= 0x7fffffLL && tokens >= 0 && tokens <= kMostTokens && heads >= 1 && heads <= 65535 &&
          d >= 8 && d <= kMaxHead && d % 8 == 0 && r >= 0 && r <= d && r % 8 == 0;
 }
 
