@@ -167,6 +167,8 @@ def extend(blocks: list[DecoderBlock], x: torch.Tensor, cache: PagedCache, rotar
 
         out.append(_through(blocks, part, attend))
         cache._grow(cache.lens + (n if now is None else now))
+    if not out:  # no token: nothing is kept
+        return x.new_empty(x.shape)
     return torch.cat(out, 1) if len(out) != 1 else out[0]
 
 
