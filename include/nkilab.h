@@ -415,9 +415,12 @@ int nkl_rotary_append(const void* q, const int64_t* q_strides, const void* k, co
                       int interleaved, float magnitude, int dtype, void* stream);
 
 /* nkl_attention_tree over one layer's cache in 8 bits; dtype is that of q, the drafted tokens' k_new and
- * v_new, and out. fp32 accumulation and softmax statistics, weights rounded to f16 (fp32: to 22
- * bits) for their product with v; the cache's values enter the products as they are. Of its
- * numbers, the appends never write e4m3's code for NaN, and it is not looked for. head_dim a multiple of 16 up to 128. */
+ * v_new, and out. fp32 accumulation and softmax statistics; the cache's values enter the products as they are.
+ * What the weights of cached positions are rounded to for their product with v goes by the call: fp32, 22 bits (two f16
+ * numbers; queries as well); bf16, f16; but bf16 with head_dim 64 or 128, pages of a multiple of 8 and 17 or more query
+ * rows (tokens x heads / kv_heads) to a key/value head, bf16, eight times coarser, and in two parts, 16 bits, in sequences of
+ * up to 1024 cached positions. Drafted tokens' weights: three bf16 parts (fp32), two, or as the cached ones' in that last case.
+ * The appends never write e4m3's code for NaN, and it is not looked for. head_dim a multiple of 16 up to 128. */
 size_t nkl_attention_tree_8bit_workspace_size(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads,
                                               int64_t head_dim, int64_t page_size, int64_t max_pages, int dtype);
 int nkl_attention_tree_8bit(const void* q, const int64_t* q_strides, const void* k_new, const void* v_new,
@@ -504,7 +507,7 @@ int nkl_verify_drafts(const void* probs, const void* draft_probs, const int32_t*
                       int64_t drafted, int64_t vocab, int dtype, void* stream);
 
 /* The next token of each row of logits [batch, vocab] (rows row_stride elements apart), from the uniform
- * numbers [batch] in [0, 1). With weights w = floor(2^31 exp((x - max) / T)), in order of the logits
+ * numbers [batch] in [0, 1). With weights w, whole numbers within one of floor(2^31 exp((x - max) / T)), in order of the logits
  * (of equal ones the lowest index first), what is drawn from is the longest beginning of that order that
  * has no more than top_k tokens, no more than it takes for the share top_p of the first top_k's
  * weights, and only weights of at least min_p 2^31; its first token is always in it. token [batch]: the

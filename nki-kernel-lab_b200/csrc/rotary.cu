@@ -29,7 +29,9 @@
 //
 // Measured (6.57 TB/s is what a copy of memory reaches): x and its gradient, bf16, 4 x 4096 tokens of 64 heads of 128
 // 186 us (1.07 GB: 163 by bytes; 183 with sines and cosines in 32 bits); q, k, v of 32 heads, turned, k and v to a cache in 8 bits, 4 x 4096 tokens 156 us
-// (808 MB: 123), bound by issue and by what a thread block's two phases (queries, then blocks) do not overlap. The smallest calls:
+// (808 MB: 123), bound by issue and by what a thread block's two phases (queries, then blocks) do not overlap. x alone, bf16, 4 x
+// 4096 tokens of 64 heads of 64 (269 MB: 41): whole heads in halves 50 us, interleaved 59, half of each head 65 (halves: entries that
+// stay are loaded and stored twice) and 59 (interleaved), where a thread has half as many bytes on their way. The smallest calls:
 // 2.5 us on the GPU for x alone, 5 to 6 with a cache (lengths -> tables -> rows), and 6 to 9 of the host's.
 #include <algorithm>
 #include <atomic>

@@ -2,7 +2,7 @@
 // uniform numbers.
 //
 // A row's tokens in order of their logits, of equal ones the lowest index first, have the weights
-//   w = floor(2^31 exp((x - max) / T))
+//   w = floor(2^31 exp((x - max) / T)), or one more or less
 // What is drawn from is the longest beginning of that order that every filter allows: top-k its k first
 // tokens; top-p the fewest whose weights come to the share p of the top-k's; min-p those of at least
 // p times the first one's weight. Of it the token is the first one, by index, with which

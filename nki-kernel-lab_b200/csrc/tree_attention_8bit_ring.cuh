@@ -19,11 +19,14 @@
 //   1 token, 64 sequences of about 700                     37 and 35 us (10 by bytes)
 //   4 tokens, 8 sequences of up to 4096                    34 and 47 us (6 by bytes)
 //   16 tokens, 4 sequences of up to 4096, 32 heads of 128  50 and 70 us (12 by bytes)
-// so every call that it can take goes here. What bounds it: on long rows the products' warps, 1130 cycles to a tile of 32
-// KB, of which the conversions from e4m3 to f16 alone take 820 (a conversion of 32 lanes issues every other cycle on an SM);
-// on short ones a piece's beginning and end (5000 cycles) and the start: plan, tables and the first tiles take 7000. More
-// than eight such warps do not fit: their sums are 64 or 128 registers each. The drafted tokens by one of the eight warps at
-// a piece's end instead of by warp 10: 32 sequences 117 us for 109, 203 positions 11.8 for 7.8 (at that time).
+// so every call that it can take goes here: only many short sequences lose by it, 2 us, and how long they are the host
+// does not know. What bounds it: on long rows the products' warps, 1130 cycles to a tile of 32 KB. The conversions from
+// e4m3 to f16 are 264 of them (measured alone: a scheduler takes one of 32 lanes every other cycle, the SM's four 512 to a
+// tile), with the loads and products around them some 380; the rest is the chain from the scores over the weights to the
+// transposed ones, with two warps to a scheduler, which issue in 43 % of the cycles. On short rows it is a piece's
+// beginning and end (5000 cycles) and the start: plan, tables and the first tiles take 7000. More than eight such warps do
+// not fit: their sums are 64 or 128 registers each. The drafted tokens by one of the eight warps at a piece's end instead
+// of by warp 10: 32 sequences 117 us for 109, 203 positions 11.8 for 7.8 (at that time).
 #pragma once
 
 namespace {

@@ -193,7 +193,7 @@ def attention_tree(q, k, v, k_cache, v_cache, tables, lens, parents=None, scale=
     each token follows the one before it, so T = 1 is plain decoding and T > 1 a chunk of a
     prompt. At most 128 tokens; scale defaults to 1/sqrt(d). d: a multiple of 8 up to 128
     (64 and 128 in bf16, with pages of a multiple of 8 positions, run on tcgen05). There is
-    no backward pass: one through it raises.
+    no backward pass: one through it raises, as does a forward derivative.
 
     With k_scales and v_scales the caches are in 8 bits, as cache_append writes them (d a multiple
     of 16); q, k and v are bf16 or fp32 all the same.
@@ -238,8 +238,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, scaling=None, factor=1.0, train
     "linear"  every frequency / factor (positions interpolated)
     "ntk"     base * factor^(r / (r - 2)), which divides the lowest frequency by factor
     "yarn"    frequencies that turn less than once in `trained` positions / factor, those that turn
-              over 32 times as they are, mixed linearly between; magnitude 0.1 ln(factor) + 1
-              (Peng et al., YaRN, 2023)
+              over 32 times as they are, mixed linearly between, by the number of turns; magnitude
+              0.1 ln(factor) + 1 (Peng et al., YaRN, 2023). Implementations that mix linearly by the pair's
+              index have other frequencies in between: a model trained with those needs its own `freqs`
     """
     r = int(rotary_dim)
     if r < 2 or r % 2:
@@ -273,7 +274,7 @@ def rotary(x, positions, freqs, parents=None, interleaved=False, magnitude=1.0):
 
     positions int32: [B, T], or [B], where token j is at positions[b] + j, or, in a tree (parents
     [B, T] as in attention_tree), as far behind as it is deep. Angles are reduced in 64 bits. x may
-    need a gradient, which turns the other way.
+    need a gradient, which turns the other way, or have a forward derivative, which turns along.
     """
     return _rotary(x, positions, freqs, parents, bool(interleaved), float(magnitude), False)
 
@@ -284,7 +285,7 @@ def rotary_append(q, k, v, k_cache, v_cache, tables, lens, freqs, count=None, in
     turned k and v written to those positions of one layer's cache (in 8 bits with scales, see
     cache_append; rounded once there). Returns (q, k). Rows from count[b] on stay out of
     the cache, as do rows without a page; lens stays as it is, for a step's layers share it. There
-    is no backward pass: one through it raises.
+    is no backward pass: one through it raises, as does a forward derivative.
     """
     return _rotary_append(q, k, v, k_cache, v_cache, k_scales, v_scales, tables, lens, freqs, count, bool(interleaved),
                           float(magnitude))
@@ -361,7 +362,8 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     0 takes the first one; top_k 0, top_p 1 and min_p 0 keep all. Each is a number, or one for each row: a
     tensor [B] on the GPU (top_k int32, the others float32), where NaN is off. Minus infinity and NaN are never
     drawn. Returns (token [B] int32, -1 if there is none; prob [B] float32, its share of what was kept).
-    Weights are whole multiples of 2^-31, so equal inputs give equal tokens on every launch. V up to 360448.
+    Weights are whole multiples of 2^-31 (the formula's, rounded down, to within one), so equal inputs give equal tokens on
+    every launch. V up to 360448. No derivative passes through it: one that is asked for raises.
     """
     numbers, rows = [], []
     for name, x, low, high in (("temperature", temperature, 0, math.inf), ("top_k", top_k, 0, 2 ** 31), ("top_p", top_p, 0, 1),

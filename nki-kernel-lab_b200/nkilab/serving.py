@@ -115,7 +115,8 @@ class PagedCache:
 
 class Rotary:
     """Rotary positions of a model: `rotary_dim` entries of each head (default: all) turn with
-    frequencies base^(-2i / rotary_dim), stretched for long contexts as ops.rotary_frequencies does."""
+    frequencies base^(-2i / rotary_dim), stretched for long contexts as ops.rotary_frequencies does. A model
+    with frequencies of its own sets `freqs` (float64 on the GPU) and `magnitude`."""
 
     def __init__(self, head_dim: int, rotary_dim: int | None = None, base: float = 10000.0, scaling: str | None = None,
                  factor: float = 1.0, trained: int | None = None, interleaved: bool = False, device=None):
@@ -213,7 +214,8 @@ def step(blocks: list[DecoderBlock], embedding: torch.Tensor, head: torch.Tensor
          uniforms: torch.Tensor, rotary: Rotary, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One token of every slot: `last` [slots], its latest token (not in the cache yet, for which a
     page has to be reserved), goes through the blocks and is kept, and the next one is drawn with the uniform
-    numbers [slots]. Returns (token, prob) as ops.sample does."""
+    numbers [slots]. Returns (token, prob) as ops.sample does. A slot without pages stays empty; one that has ended and
+    still has its pages goes on growing: free it, or extend with a count of 0 for it."""
     x = embedding[last.clamp(0, embedding.shape[0] - 1).long()][:, None]
     return next_token(extend(blocks, x, cache, rotary)[:, 0], head, uniforms, temperature, top_k, top_p, min_p)
 
