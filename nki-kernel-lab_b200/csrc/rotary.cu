@@ -593,15 +593,15 @@ __global__ void __launch_bounds__(kThreads, 2) rotary_kernel(const __grid_consta
 
 template <auto Kernel>
 int launch_kernel(const RotaryArgs& a, dim3 grid, size_t smem, cudaStream_t st, const char* op) {
-  if (smem > 48 * 1024) {
-    static std::atomic<bool> set[64] = {};  // per device: the shared memory attribute is set (idempotent)
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
-      const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
-      if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
-      if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
-    }
+  // per device: the shared memory attribute is set (idempotent), for every call: 48 KB without it are together with the
+  // kernel's own 2 KB
+  static std::atomic<bool> set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem);
+    if (e != cudaSuccess) return fail(NKL_ERR_CUDA, "%s: %s", op, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) set[dev].store(true, std::memory_order_release);
   }
   return launch_pdl(Kernel, grid, dim3(kThreads), smem, st, op, a);
 }
