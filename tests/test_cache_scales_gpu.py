@@ -108,3 +108,38 @@ def test_refusals_leave_the_cache_as_it_was():
         for x, y in zip(c.all, was):
             assert torch.equal(x, y)
         assert (plain == 0).all()
+
+
+def test_a_captured_fork_and_compaction_replay():
+    """Another stream, and a graph that is replayed on caches filled anew: the bytes of the eager calls."""
+    tables, lens, refs = i32([[7, 9, -1], [5, -1, -1], [-1, -1, -1]]), i32([21, 3, 0]), i32([0, 0, 0, 0, 0, 1, 0, 1, 0, 1])
+    src, dst = i32([0, 1]), i32([2, 0])
+    a, b = (Cache8(2, 10, 3, 16, 32, 4) for _ in range(2))
+    start = a.bytes()
+
+    def fill(c):
+        for x, y in zip(c.all, start):
+            x.copy_(y)
+
+    def call(c):
+        t, n, r, missing = ops.cache_fork(c.k, c.v, tables, lens, refs, src, dst, c.ks, c.vs)
+        return (n, missing, *ops.cache_compact(c.k, c.v, t, r, c.ks, c.vs))
+
+    want = call(a)
+    fill(b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert all(torch.equal(x, y) for x, y in zip(call(b), want))
+        fill(b)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = call(b)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(2):
+        fill(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        for x, y in zip(a.all, b.all):
+            assert torch.equal(x, y)
