@@ -24,6 +24,6 @@ for d, block, dtype in ((96, 16, torch.bfloat16), (64, 24, torch.bfloat16), (48,
 
 
 def test_appends_whose_rows_take_48_kilobytes():
-    """Eight warps' two buffers of 3072 bytes, rows of 96 in blocks of 16 among them, are 48 KB exactly."""
+    """The two buffers of each of eight warps are 48 KB exactly, with rows of 96 in blocks of 16 for instance."""
     out = subprocess.run([sys.executable, "-c", APPENDS], env=dict(os.environ, PYTHONPATH=PKG), capture_output=True, text=True, timeout=300)
     assert out.returncode == 0, out.stderr[-2000:]
