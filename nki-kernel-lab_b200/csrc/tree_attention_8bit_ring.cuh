@@ -14,7 +14,7 @@
 // Measured against the kernel of tree_attention_8bit.cuh on the same calls, GPU time with the join (32 heads over 8 of
 // 128 but where it says so):
 //   1 token, 203 positions                                7.2 and 11 us
-//   1 token, 32 sequences of up to 8192                    84 and 150 us (60 by bytes)
+//   1 token, 32 sequences of up to 8192                    85 and 150 us (60 by bytes)
 //   1 token, 65536 positions                               41 and 49 us (20 by bytes)
 //   1 token, 64 sequences of about 700                     37 and 35 us (10 by bytes)
 //   4 tokens, 8 sequences of up to 4096                    34 and 47 us (6 by bytes)
